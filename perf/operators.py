@@ -127,7 +127,7 @@ def _codes(w):
     tiles = wide.view(groups, nb, BLOCK, kb, BLOCK)
     scales = tiles.abs().amax(dim=(2, 4)).clamp(min=1e-20) / 448
     q = (tiles / scales[:, :, None, :, None]).clamp(-TOP, TOP).to(torch.float8_e4m3fn)
-    return q.view(groups, nb * BLOCK, kb * BLOCK)[:, :n, :inner].contiguous(), scales.transpose(1, 2).contiguous()
+    return q.view(groups, nb * BLOCK, kb * BLOCK)[:, :n, :inner].contiguous(), scales
 
 
 def prepare(case, seed):
@@ -228,8 +228,8 @@ def _blocks(x):
 
 
 def _weights(s):
-    q, scales = s["codes"], s["scales"].transpose(1, 2)
-    wide = scales.repeat_interleave(BLOCK, 1).repeat_interleave(BLOCK, 2)
+    q = s["codes"]
+    wide = s["scales"].repeat_interleave(BLOCK, 1).repeat_interleave(BLOCK, 2)
     return q.float() * wide[:, :q.shape[1], :q.shape[2]]
 
 
@@ -344,9 +344,9 @@ def _stored(x, dim):
 
 def _tile_values(s):
     w = s["codes"].double()
-    for b in range(s["scales"].shape[1]):
-        for a in range(s["scales"].shape[2]):
-            w[:, a * BLOCK:(a + 1) * BLOCK, b * BLOCK:(b + 1) * BLOCK] *= s["scales"][:, b, a, None, None].double()
+    for a in range(s["scales"].shape[1]):
+        for b in range(s["scales"].shape[2]):
+            w[:, a * BLOCK:(a + 1) * BLOCK, b * BLOCK:(b + 1) * BLOCK] *= s["scales"][:, a, b, None, None].double()
     return w
 
 
