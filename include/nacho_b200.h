@@ -346,6 +346,85 @@ int nb200_dcsr_mul_f32_into(const nb200_dcsr *a, const nb200_dcsr *b, nb200_dcsr
 int nb200_inner_prod_f32(const nb200_csf3 *a, const nb200_csf3 *b, float *z, void *stream);
 int nb200_inner_prod_coo_f32(const nb200_coo3 *a, const nb200_coo3 *b, float *z, void *stream);
 
+/* ---- around a router ---------------------------------------------------------------------- */
+
+/* A router's decision is a CSR matrix R of tokens x experts whose values are the gate weights. The entry points
+ * below bring dense rows (one per token) into the order of the experts, multiply every expert's rows with its
+ * weights in 8-bit floating point, and bring them back. They have no counterpart in the reference.
+ *   - Rows of R may be empty or hold any number of entries, in any order of experts (duplicates count twice).
+ *     An entry whose column lies outside [0, cols) is dropped: it has no slot and takes part in nothing.
+ *   - None of the calls waits for the device: all result lengths are known before. They can be captured in a
+ *     CUDA graph once a call of that size has been made on the stream (scratch arrays grow on first use).
+ *   - Sums are 32-bit, in a fixed order: the same call gives the same bits. */
+
+/* Dense rows in device memory: element (r, c) lies at data[r * stride + c]. */
+typedef enum nb200_type { NB200_F32 = 0, NB200_F16 = 1, NB200_BF16 = 2 } nb200_type;
+typedef struct nb200_dense {
+    int64_t rows, cols, stride;
+    int32_t type; /* nb200_type; data is aligned to the type's size */
+    void *data;
+} nb200_dense;
+
+/* The order of the experts: entries of R sorted by expert, entries of one expert in storage order. Kept entries take
+ * the slots 0 .. offsets[experts] - 1; the slots behind those belong to nobody. */
+typedef struct nb200_expert_order {
+    int32_t tokens, experts, entries;
+    int32_t *row_ptr; /* R's own, tokens + 1 */
+    int32_t *offsets; /* experts + 1: where each expert's slots begin */
+    int32_t *rows;    /* entries: the token of every slot, -1 for a slot of nobody */
+    int32_t *slots;   /* entries: the slot of every entry of R, -1 for a dropped one */
+} nb200_expert_order;
+
+#define NB200_MAX_EXPERTS 4096
+
+/* Matrices in 8-bit floating point (e4m3) with a 32-bit scale for every 128 columns of a row (tiled = 0; one group) or for
+ * every 128 x 128 (tiled = 1). With m the largest magnitude of a block, at least 2^-110: scale = m / 448, code =
+ * e4m3(x * (448 / m)), both quotients rounded to 32 bits; a block that holds a NaN or an infinity stands for NaNs.
+ * values: [group][column block][row, to a multiple of 8][128 codes], column blocks filled up with zeros. The 16-byte piece p of
+ *         a row's 128 codes lies at place p ^ (row % 8). 16-byte aligned.
+ * scales: tiled = 0: [column block][row, to a multiple of 8]; tiled = 1: [group][column block][row block]. */
+typedef struct nb200_fp8 {
+    int32_t groups, rows, cols, tiled;
+    uint8_t *values;
+    float *scales;
+} nb200_fp8;
+
+/* Lengths of the two arrays for the extents in `m`, -1 if those are not possible. */
+int64_t nb200_fp8_value_count(const nb200_fp8 *m);
+int64_t nb200_fp8_scale_count(const nb200_fp8 *m);
+
+/* order of R, and (where x is not NULL) xs[slot] = x[token], zeros for slots of nobody. order->row_ptr is set to R's. The
+ * other three arrays are the caller's. The form with fp8 rows quantises on the way. At most NB200_MAX_EXPERTS columns. */
+int nb200_expert_sort(const nb200_csr *r, const nb200_dense *x, nb200_expert_order *order, nb200_dense *xs, void *stream);
+int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert_order *order, nb200_fp8 *xs, void *stream);
+/* y[t] = sum over the kept entries e of token t of w[e] * z[slot(e)]; w = NULL stands for ones (the gradient of the sort). */
+int nb200_expert_unsort(const nb200_expert_order *order, const float *w, const nb200_dense *z, nb200_dense *y, void *stream);
+/* Its gradients: dz[slot(e)] = w[e] * dy[t] (zeros for slots of nobody), dw[e] = <dy[t], z[slot(e)]> (0 where dropped). */
+int nb200_expert_unsort_grad(const nb200_expert_order *order, const float *w, const nb200_dense *z, const nb200_dense *dy,
+                             nb200_dense *dz, float *dw, void *stream);
+
+/* Quantises. The rows of x are those of z, group after group. */
+int nb200_fp8_quantise(const nb200_dense *x, nb200_fp8 *z, void *stream);
+/* Takes over codes and scales that exist: codes [groups * rows][cols] one after another, scales [rows][column blocks]
+ * (tiled = 0) or [groups][row blocks][column blocks] (tiled = 1). */
+int nb200_fp8_pack(const uint8_t *codes, const float *scales, nb200_fp8 *z, void *stream);
+/* The 32-bit values that a matrix stands for, [groups * rows][cols] one after another. */
+int nb200_fp8_unpack(const nb200_fp8 *a, float *z, void *stream);
+/* Every group's transpose; tiled = 1 only. */
+int nb200_fp8_transpose(const nb200_fp8 *a, nb200_fp8 *z, void *stream);
+
+/* y[i] = a[i] * w[g]^T: rows a (tiled = 0), weights w (tiled = 1) with as many columns, y of a->rows x w->rows in any type. With
+ * `offsets` (w->groups + 1 of them, rising, in device memory) rows offsets[g] .. offsets[g + 1] - 1 take group g and rows
+ * in front of the first or behind the last are zeros; without it there is one group. Products of a block of 128 columns are summed on
+ * the tensor cores and the blocks, times their two scales, in 32 bits. */
+int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *offsets, nb200_dense *y, void *stream);
+/* The gradient for the weights: z[g] = sum over the rows i of group g of dy[i]^T x[i], z = [groups][dy->cols][x->cols] 32-bit. Both
+ * operands are quantised along the rows, a scale for every column and 128 rows counted from the group's first. */
+int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_t groups, const int32_t *offsets, float *z,
+                             void *scratch, int64_t scratch_bytes, void *stream);
+/* Bytes of scratch, 256-byte aligned device memory, that it needs: the quantised operands; -1 for impossible operands. */
+int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dense *x, int32_t groups);
+
 /* ---- self-test -------------------------------------------------------------------------- */
 
 /* Exercises the give-up path of the bounded device-side waits without faulting or hanging the

@@ -47,6 +47,23 @@ class DcsrStruct(C.Structure):
                 ("i_idx", C.c_void_p), ("j_ptr", C.c_void_p), ("j_idx", C.c_void_p), ("val", C.c_void_p)]
 
 
+class DenseStruct(C.Structure):
+    """``nb200_dense``."""
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("stride", C.c_int64), ("type", C.c_int32), ("data", C.c_void_p)]
+
+
+class ExpertOrderStruct(C.Structure):
+    """``nb200_expert_order``."""
+    _fields_ = [("tokens", C.c_int32), ("experts", C.c_int32), ("entries", C.c_int32),
+                ("row_ptr", C.c_void_p), ("offsets", C.c_void_p), ("rows", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class Fp8Struct(C.Structure):
+    """``nb200_fp8``."""
+    _fields_ = [("groups", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("tiled", C.c_int32),
+                ("values", C.c_void_p), ("scales", C.c_void_p)]
+
+
 OK, E_BADARG, E_CUDA, E_OVERFLOW, E_CAPACITY, E_TIMEOUT, E_NOMEM, E_UNSUPPORTED = range(8)
 
 # name -> (restype, argtypes); every symbol include/nacho_b200.h declares.
@@ -100,6 +117,19 @@ PROTOTYPES = {
     "nb200_dcsr_mul_f32_into": (C.c_int, [_P(DcsrStruct)] * 3 + [C.c_int64, C.c_int64, C.c_void_p]),
     "nb200_inner_prod_f32": (C.c_int, [_P(Csf3Struct)] * 2 + [C.c_void_p, C.c_void_p]),
     "nb200_inner_prod_coo_f32": (C.c_int, [_P(Coo3Struct)] * 2 + [C.c_void_p, C.c_void_p]),
+    "nb200_fp8_value_count": (C.c_int64, [_P(Fp8Struct)]),
+    "nb200_fp8_scale_count": (C.c_int64, [_P(Fp8Struct)]),
+    "nb200_expert_sort": (C.c_int, [_P(CsrStruct), _P(DenseStruct), _P(ExpertOrderStruct), _P(DenseStruct), C.c_void_p]),
+    "nb200_expert_sort_fp8": (C.c_int, [_P(CsrStruct), _P(DenseStruct), _P(ExpertOrderStruct), _P(Fp8Struct), C.c_void_p]),
+    "nb200_expert_unsort": (C.c_int, [_P(ExpertOrderStruct), C.c_void_p, _P(DenseStruct), _P(DenseStruct), C.c_void_p]),
+    "nb200_expert_unsort_grad": (C.c_int, [_P(ExpertOrderStruct), C.c_void_p] + [_P(DenseStruct)] * 3 + [C.c_void_p, C.c_void_p]),
+    "nb200_fp8_quantise": (C.c_int, [_P(DenseStruct), _P(Fp8Struct), C.c_void_p]),
+    "nb200_fp8_pack": (C.c_int, [C.c_void_p, C.c_void_p, _P(Fp8Struct), C.c_void_p]),
+    "nb200_fp8_unpack": (C.c_int, [_P(Fp8Struct), C.c_void_p, C.c_void_p]),
+    "nb200_fp8_transpose": (C.c_int, [_P(Fp8Struct), _P(Fp8Struct), C.c_void_p]),
+    "nb200_fp8_product": (C.c_int, [_P(Fp8Struct), _P(Fp8Struct), C.c_void_p, _P(DenseStruct), C.c_void_p]),
+    "nb200_fp8_product_grad_w": (C.c_int, [_P(DenseStruct)] * 2 + [C.c_int32] + [C.c_void_p] * 3 + [C.c_int64, C.c_void_p]),
+    "nb200_fp8_product_grad_w_scratch": (C.c_int64, [_P(DenseStruct)] * 2 + [C.c_int32]),
 }
 
 

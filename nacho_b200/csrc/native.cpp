@@ -26,12 +26,12 @@ namespace {
 
 // ---- what nacho_ext.py binds ---------------------------------------------------------------
 
-enum Kind { CSR = 0, COO = 1, DCSR = 2, COO3 = 3, CSF3 = 4, SCALAR = 5, KINDS = 6 };
-PyTypeObject *g_class[KINDS] = {};
+enum Kind { CSR = 0, COO = 1, DCSR = 2, COO3 = 3, CSF3 = 4, SCALAR = 5, KINDS = 6, ORDER = 6, FP8 = 7, ALL_KINDS = 8 };
+PyTypeObject *g_class[ALL_KINDS] = {};  // the first KINDS from nacho_ext.py, the others from experts.py
 PyObject *g_check = nullptr;  // check(status, where): raises on a non-zero status
-PyObject *g_name[9] = {};    // interned slot names
-enum Name { N_offsets, N_indices, N_values, N_dims, N_i, N_j, N_k, N_jp, N_kp, NAMES };
-const char *const NAME_TEXT[NAMES] = {"_offsets", "_indices", "_values", "_dims", "_i", "_j", "_k", "_jp", "_kp"};
+enum Name { N_offsets, N_indices, N_values, N_dims, N_i, N_j, N_k, N_jp, N_kp, N_rows, N_slots, N_token_offsets, N_scales, N_tiled, NAMES };
+PyObject *g_name[NAMES] = {};  // interned slot names
+const char *const NAME_TEXT[NAMES] = {"_offsets", "_indices", "_values", "_dims", "_i", "_j", "_k", "_jp", "_kp", "_rows", "_slots", "_token_offsets", "_scales", "_tiled"};
 
 struct PyFailure {};  // a Python exception is set
 
@@ -433,6 +433,310 @@ PyObject *inner(Kind kind, const char *what, const char *where, PyObject *const 
 PyObject *inner_prod(PyObject *const *args) { return inner(CSF3, "CSF3_gpu", "gpu_inner_prod_f32", args, view_csf3, nb200_inner_prod_f32); }
 PyObject *inner_prod_coo(PyObject *const *args) { return inner(COO3, "COO3_gpu", "gpu_inner_prod_coo_f32", args, view_coo3, nb200_inner_prod_coo_f32); }
 
+// ---- around a router -------------------------------------------------------------------------
+
+int type_of(const at::Tensor &t) { return t.scalar_type() == at::kFloat ? NB200_F32 : t.scalar_type() == at::kHalf ? NB200_F16 : t.scalar_type() == at::kBFloat16 ? NB200_BF16 : -1; }
+at::ScalarType scalar_of(int type) { return type == NB200_F32 ? at::kFloat : type == NB200_F16 ? at::kHalf : at::kBFloat16; }
+
+void refuse(PyObject *kind, const char *text, const char *where, const char *name) {
+    PyErr_Format(kind, text, where, name);
+    throw PyFailure();
+}
+
+// A 2-D CUDA tensor of floats whose rows are contiguous; any distance between rows. With `groups`, also a 3-D one whose groups follow one
+// another at that distance: it is seen as their rows.
+nb200_dense view_dense(PyObject *o, View &v, const char *where, const char *name, int64_t *groups = nullptr) {
+    if (!THPVariable_Check(o)) refuse(PyExc_TypeError, "%s: %s must be a torch tensor", where, name);
+    v.arrays[v.n] = THPVariable_Unpack(o);
+    const at::Tensor &t = v.arrays[v.n++];
+    const int type = type_of(t);
+    const bool three = groups && t.dim() == 3;
+    if (!t.is_cuda() || type < 0 || !(t.dim() == 2 || three)) refuse(PyExc_TypeError, "%s: %s must be a CUDA tensor of rows of float32, float16 or bfloat16", where, name);
+    const int64_t rows = t.size(-2), cols = t.size(-1);
+    if (rows > INT32_MAX || cols > INT32_MAX || (three && t.size(0) > INT32_MAX)) refuse(PyExc_ValueError, "%s: %s has an extent beyond int32", where, name);
+    if (cols > 1 && rows > 0 && t.stride(-1) != 1) refuse(PyExc_TypeError, "%s: the rows of %s must be contiguous", where, name);
+    int64_t all = rows, stride = rows > 1 ? t.stride(-2) : cols;
+    if (three) {
+        all = t.size(0) * rows;
+        if (rows == 1) stride = t.size(0) > 1 ? t.stride(0) : cols;
+        else if (t.size(0) > 1 && t.stride(0) != rows * stride) refuse(PyExc_TypeError, "%s: the groups of %s must follow one another", where, name);
+    }
+    if (groups) *groups = three ? t.size(0) : 1;
+    v.device = t.device();
+    return nb200_dense{all, cols, stride, type, t.data_ptr()};
+}
+
+nb200_expert_order view_order(PyObject *o, View &v) {
+    const at::Tensor &slots = v.array(o, N_slots);
+    int32_t d[2];
+    dims_of<2>(o, d);
+    v.device = slots.device();
+    return nb200_expert_order{d[0], d[1], (int32_t)slots.numel(), v.index(o, N_token_offsets), v.index(o, N_offsets), v.index(o, N_rows), ints(slots)};
+}
+
+nb200_fp8 view_fp8(PyObject *o, View &v) {
+    const at::Tensor &values = v.array(o, N_values), &scales = v.array(o, N_scales);
+    int32_t d[3];
+    dims_of<3>(o, d);
+    Ref tiled(PyObject_GetAttr(o, g_name[N_tiled]));
+    v.device = values.device();
+    return nb200_fp8{d[0], d[1], d[2], tiled.p == Py_True, static_cast<uint8_t *>(values.data_ptr()), floats(scales)};
+}
+
+at::Tensor matrix(int64_t rows, int64_t cols, int type, c10::Device dev) { return at::Tensor(at::detail::empty_cuda({rows, cols}, scalar_of(type), dev, std::nullopt)); }
+nb200_dense dense(const at::Tensor &t, int type) { return nb200_dense{t.size(0), t.size(1), t.size(1), type, t.data_ptr()}; }
+
+struct OrderResult {  // the arrays of an order of R, and the object that holds them
+    at::Tensor row_ptr, offsets, rows, slots;
+    nb200_expert_order order{};
+    int64_t entries;
+
+    OrderResult(PyObject *r, const nb200_csr &a, c10::Device dev)
+        : row_ptr(tensor_of(r, N_offsets)), offsets(int_array((int64_t)a.cols + 1, dev)), rows(int_array(a.nnz, dev)), slots(int_array(a.nnz, dev)), entries(a.nnz) {
+        order.offsets = ints(offsets), order.rows = ints(rows), order.slots = ints(slots);
+    }
+    PyObject *object() {
+        used(rows, entries), used(slots, entries);
+        Result r(ORDER);
+        r.set(N_offsets, offsets), r.set(N_rows, rows), r.set(N_slots, slots), r.set(N_token_offsets, row_ptr);
+        const int32_t d[2] = {order.tokens, order.experts};
+        r.dims<2>(d);
+        return r.obj.release();
+    }
+};
+
+struct Fp8Result {
+    at::Tensor values, scales;
+    nb200_fp8 m{};
+
+    Fp8Result(int64_t groups, int64_t rows, int64_t cols, bool tiled, c10::Device dev) {
+        m = nb200_fp8{(int32_t)groups, (int32_t)rows, (int32_t)cols, tiled, nullptr, nullptr};
+        const int64_t n = nb200_fp8_value_count(&m), s = nb200_fp8_scale_count(&m);
+        values = array(n, at::kByte, dev), scales = float_array(s, dev);
+        m.values = static_cast<uint8_t *>(values.data_ptr()), m.scales = floats(scales);
+        used(values, n), used(scales, s);
+    }
+    PyObject *object() {
+        Result r(FP8);
+        r.set(N_values, values), r.set(N_scales, scales);
+        if (PyObject_SetAttr(r.obj.p, g_name[N_tiled], m.tiled ? Py_True : Py_False) < 0) throw PyFailure();
+        const int32_t d[3] = {m.groups, m.rows, m.cols};
+        r.dims<3>(d);
+        return r.obj.release();
+    }
+};
+
+PyObject *two(PyObject *a, PyObject *b) {
+    Ref first(a), second(b);
+    return PyTuple_Pack(2, first.p, second.p);
+}
+PyObject *wrap(const at::Tensor &t) { return THPVariable_Wrap(t); }
+
+void extent(int64_t is, int64_t wanted, const char *where, const char *name, const char *what) {
+    if (is == wanted) return;
+    PyErr_Format(PyExc_ValueError, "%s: %s has %lld %s, %lld expected", where, name, (long long)is, what, (long long)wanted);
+    throw PyFailure();
+}
+void same_type(int a, int b, const char *where) {
+    if (a != b) refuse(PyExc_TypeError, "%s: operands differ in %s", where, "type");
+}
+
+PyObject *expert_order(PyObject *const *args) {
+    const char *where = "gpu_expert_order";
+    need_kind(args[0], CSR, where, "CSR_gpu");
+    View vr;
+    const nb200_csr r = view_csr(args[0], vr);
+    OrderResult z(args[0], r, vr.device);
+    launch({&vr}, where, [&](void *stream) { return nb200_expert_sort(&r, nullptr, &z.order, nullptr, stream); });
+    return z.object();
+}
+
+PyObject *expert_sort(PyObject *const *args) {
+    const char *where = "gpu_expert_sort";
+    need_kind(args[0], CSR, where, "(CSR_gpu, tensor)");
+    View vr, vx;
+    const nb200_csr r = view_csr(args[0], vr);
+    const nb200_dense x = view_dense(args[1], vx, where, "x");
+    same_device(vr, vx);
+    extent(x.rows, r.rows, where, "x", "rows");
+    OrderResult z(args[0], r, vr.device);
+    at::Tensor xs = matrix(r.nnz, x.cols, x.type, vr.device);
+    nb200_dense out = dense(xs, x.type);
+    launch({&vr, &vx}, where, [&](void *stream) { return nb200_expert_sort(&r, &x, &z.order, &out, stream); });
+    return two(z.object(), wrap(xs));
+}
+
+PyObject *expert_sort_fp8(PyObject *const *args) {
+    const char *where = "gpu_expert_sort_fp8";
+    need_kind(args[0], CSR, where, "(CSR_gpu, tensor)");
+    View vr, vx;
+    const nb200_csr r = view_csr(args[0], vr);
+    const nb200_dense x = view_dense(args[1], vx, where, "x");
+    same_device(vr, vx);
+    extent(x.rows, r.rows, where, "x", "rows");
+    OrderResult z(args[0], r, vr.device);
+    Fp8Result xs(1, r.nnz, x.cols, false, vr.device);
+    launch({&vr, &vx}, where, [&](void *stream) { return nb200_expert_sort_fp8(&r, &x, &z.order, &xs.m, stream); });
+    return two(z.object(), xs.object());
+}
+
+PyObject *expert_sort_grad(PyObject *const *args) {
+    const char *where = "gpu_expert_sort_grad";
+    need_kind(args[0], ORDER, where, "(ExpertOrder_gpu, tensor)");
+    View vo, vz;
+    const nb200_expert_order o = view_order(args[0], vo);
+    const nb200_dense z = view_dense(args[1], vz, where, "dxs");
+    same_device(vo, vz);
+    extent(z.rows, o.entries, where, "dxs", "rows");
+    at::Tensor y = matrix(o.tokens, z.cols, z.type, vo.device);
+    nb200_dense out = dense(y, z.type);
+    launch({&vo, &vz}, where, [&](void *stream) { return nb200_expert_unsort(&o, nullptr, &z, &out, stream); });
+    return wrap(y);
+}
+
+// R is read for its values only.
+nb200_csr routing_of(PyObject *r, PyObject *order, View &vr, View &vo, nb200_expert_order *o, const char *where) {
+    need_kind(r, CSR, where, "(CSR_gpu, ExpertOrder_gpu, tensors)");
+    need_kind(order, ORDER, where, "(CSR_gpu, ExpertOrder_gpu, tensors)");
+    const nb200_csr a = view_csr(r, vr);
+    *o = view_order(order, vo);
+    same_device(vr, vo);
+    extent(a.nnz, o->entries, where, "the routing", "entries");
+    extent(a.rows, o->tokens, where, "the routing", "rows");
+    return a;
+}
+
+PyObject *expert_unsort(PyObject *const *args) {
+    const char *where = "gpu_expert_unsort";
+    View vr, vo, vz;
+    nb200_expert_order o;
+    const nb200_csr r = routing_of(args[0], args[1], vr, vo, &o, where);
+    const nb200_dense z = view_dense(args[2], vz, where, "z");
+    same_device(vo, vz);
+    extent(z.rows, o.entries, where, "z", "rows");
+    at::Tensor y = matrix(o.tokens, z.cols, z.type, vo.device);
+    nb200_dense out = dense(y, z.type);
+    launch({&vr, &vo, &vz}, where, [&](void *stream) { return nb200_expert_unsort(&o, r.val, &z, &out, stream); });
+    return wrap(y);
+}
+
+PyObject *expert_unsort_grad(PyObject *const *args) {
+    const char *where = "gpu_expert_unsort_grad";
+    View vr, vo, vz, vd;
+    nb200_expert_order o;
+    const nb200_csr r = routing_of(args[0], args[1], vr, vo, &o, where);
+    const nb200_dense z = view_dense(args[2], vz, where, "z"), dy = view_dense(args[3], vd, where, "dy");
+    same_device(vo, vz);
+    same_device(vo, vd);
+    extent(z.rows, o.entries, where, "z", "rows");
+    extent(dy.rows, o.tokens, where, "dy", "rows");
+    extent(dy.cols, z.cols, where, "dy", "columns");
+    same_type(dy.type, z.type, where);
+    at::Tensor dz = matrix(o.entries, z.cols, z.type, vo.device), dw = float_array(o.entries, vo.device);
+    nb200_dense out = dense(dz, z.type);
+    launch({&vr, &vo, &vz, &vd}, where, [&](void *stream) { return nb200_expert_unsort_grad(&o, r.val, &z, &dy, &out, floats(dw), stream); });
+    used(dw, o.entries);
+    return two(wrap(dz), wrap(dw));
+}
+
+PyObject *fp8_quantised(PyObject *x, bool tiled, const char *where) {
+    View vx;
+    int64_t groups = 1;
+    const nb200_dense a = view_dense(x, vx, where, "x", tiled ? &groups : nullptr);
+    Fp8Result z(groups, vx.arrays[0].size(-2), a.cols, tiled, vx.device);
+    launch({&vx}, where, [&](void *stream) { return nb200_fp8_quantise(&a, &z.m, stream); });
+    return z.object();
+}
+PyObject *fp8_rows(PyObject *const *args) { return fp8_quantised(args[0], false, "to_fp8_rows"); }
+PyObject *fp8_tiles(PyObject *const *args) { return fp8_quantised(args[0], true, "to_fp8_tiles"); }
+
+// fp8_pack(codes as bytes, scales, tiled): codes of 2 dimensions, or 3 where tiled; both contiguous (the caller has checked)
+PyObject *fp8_pack(PyObject *const *args) {
+    const char *where = "to_fp8";
+    if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) refuse(PyExc_TypeError, "%s: %s must be torch tensors", where, "codes and scales");
+    View vc;
+    vc.arrays[vc.n++] = THPVariable_Unpack(args[0]);
+    vc.arrays[vc.n++] = THPVariable_Unpack(args[1]);
+    const at::Tensor &codes = vc.arrays[0], &scales = vc.arrays[1];
+    vc.device = codes.device();
+    const bool tiled = args[2] == Py_True;
+    const int64_t groups = codes.dim() == 3 ? codes.size(0) : 1;
+    Fp8Result z(groups, codes.size(-2), codes.size(-1), tiled, vc.device);
+    launch({&vc}, where, [&](void *stream) { return nb200_fp8_pack(static_cast<const uint8_t *>(codes.data_ptr()), floats(scales), &z.m, stream); });
+    return z.object();
+}
+
+PyObject *fp8_unpack(PyObject *const *args) {
+    const char *where = "to_dense";
+    need_kind(args[0], FP8, where, "FP8_gpu");
+    View va;
+    const nb200_fp8 a = view_fp8(args[0], va);
+    at::Tensor z = matrix((int64_t)a.groups * a.rows, a.cols, NB200_F32, va.device);
+    launch({&va}, where, [&](void *stream) { return nb200_fp8_unpack(&a, floats(z), stream); });
+    return wrap(z);
+}
+
+PyObject *fp8_transpose(PyObject *const *args) {
+    const char *where = "transposed";
+    need_kind(args[0], FP8, where, "FP8_gpu");
+    View va;
+    const nb200_fp8 a = view_fp8(args[0], va);
+    Fp8Result z(a.groups, a.cols, a.rows, true, va.device);
+    launch({&va}, where, [&](void *stream) { return nb200_fp8_transpose(&a, &z.m, stream); });
+    return z.object();
+}
+
+// Row ranges of the groups: an order's, or none for a single matrix.
+const int32_t *ranges_of(PyObject *order, View &vo, int64_t rows, int64_t groups, const char *where) {
+    if (order == Py_None) {
+        extent(groups, 1, where, "w without an order", "groups");
+        return nullptr;
+    }
+    need_kind(order, ORDER, where, "ExpertOrder_gpu (or None)");
+    const nb200_expert_order o = view_order(order, vo);
+    extent(rows, o.entries, where, "the left operand", "rows");
+    extent(groups, o.experts, where, "w", "groups");
+    return o.offsets;
+}
+
+// fp8_product(a, w, order or None, type)
+PyObject *fp8_product(PyObject *const *args) {
+    const char *where = "gpu_fp8_product";
+    for (int k = 0; k < 2; ++k) need_kind(args[k], FP8, where, "FP8_gpu");
+    View va, vw, vo;
+    const nb200_fp8 a = view_fp8(args[0], va), w = view_fp8(args[1], vw);
+    same_device(va, vw);
+    vo.device = va.device;
+    const int32_t *offsets = ranges_of(args[2], vo, a.rows, w.groups, where);
+    same_device(va, vo);
+    if (a.tiled || !w.tiled) refuse(PyExc_ValueError, "%s: %s", where, "the left operand has a scale per row (to_fp8_rows), the right one per tile (to_fp8_tiles)");
+    extent(a.cols, w.cols, where, "the left operand", "columns");
+    const int type = (int)PyLong_AsLong(args[3]);
+    at::Tensor y = matrix(a.rows, w.rows, type, va.device);
+    nb200_dense out = dense(y, type);
+    launch({&va, &vw, &vo}, where, [&](void *stream) { return nb200_fp8_product(&a, &w, offsets, &out, stream); });
+    return wrap(y);
+}
+
+// fp8_grad_w(dy, x, order or None, groups)
+PyObject *fp8_grad_w(PyObject *const *args) {
+    const char *where = "gpu_fp8_product_grad";
+    View vd, vx, vo;
+    const nb200_dense dy = view_dense(args[0], vd, where, "dy"), x = view_dense(args[1], vx, where, "x");
+    same_device(vd, vx);
+    same_type(dy.type, x.type, where);
+    extent(x.rows, dy.rows, where, "x", "rows");
+    const int64_t groups = PyLong_AsLongLong(args[3]);
+    vo.device = vd.device;
+    const int32_t *offsets = ranges_of(args[2], vo, dy.rows, groups, where);
+    same_device(vd, vo);
+    const int64_t bytes = nb200_fp8_product_grad_w_scratch(&dy, &x, (int32_t)groups);
+    if (bytes < 0) check(NB200_E_BADARG, where);
+    at::Tensor scratch = array(bytes, at::kByte, vd.device), z = at::Tensor(at::detail::empty_cuda({groups, dy.cols, x.cols}, at::kFloat, vd.device, std::nullopt));
+    launch({&vd, &vx, &vo}, where, [&](void *stream) { return nb200_fp8_product_grad_w(&dy, &x, (int32_t)groups, offsets, floats(z), scratch.data_ptr(), bytes, stream); });
+    return wrap(z);
+}
+
 // ---- module --------------------------------------------------------------------------------
 
 template <PyObject *(*OP)(PyObject *const *), int ARGS>
@@ -466,6 +770,17 @@ PyObject *bind(PyObject *, PyObject *args) {
     Py_RETURN_NONE;
 }
 
+// bind_experts((ExpertOrder_gpu, FP8_gpu))
+PyObject *bind_experts(PyObject *, PyObject *args) {
+    PyObject *classes[2];
+    if (!PyArg_ParseTuple(args, "(O!O!)", &PyType_Type, &classes[0], &PyType_Type, &classes[1])) return nullptr;
+    for (int k = 0; k < 2; ++k) {
+        Py_INCREF(classes[k]);
+        g_class[ORDER + k] = reinterpret_cast<PyTypeObject *>(classes[k]);
+    }
+    Py_RETURN_NONE;
+}
+
 // turn_of(device, stream handle): identity of the lock by which calls there take turns (for tests)
 PyObject *turn_of(PyObject *, PyObject *args) {
     int device;
@@ -485,6 +800,11 @@ PyMethodDef g_methods[] = {
     op<sssmm, 3>("sssmm"), op<coo3d_add, 2>("coo3d_add"), op<csf_add, 2>("csf_add"), op<coo_add, 2>("coo_add"),
     op<coo_mul, 2>("coo_mul"), op<coo_csr_add, 2>("coo_csr_add"), op<dcsr_add, 2>("dcsr_add"), op<dcsr_mul, 2>("dcsr_mul"),
     op<inner_prod, 2>("inner_prod"), op<inner_prod_coo, 2>("inner_prod_coo"),
+    {"bind_experts", bind_experts, METH_VARARGS, nullptr},
+    op<expert_order, 1>("expert_order"), op<expert_sort, 2>("expert_sort"), op<expert_sort_fp8, 2>("expert_sort_fp8"),
+    op<expert_sort_grad, 2>("expert_sort_grad"), op<expert_unsort, 3>("expert_unsort"), op<expert_unsort_grad, 4>("expert_unsort_grad"),
+    op<fp8_rows, 1>("fp8_rows"), op<fp8_tiles, 1>("fp8_tiles"), op<fp8_pack, 3>("fp8_pack"), op<fp8_unpack, 1>("fp8_unpack"),
+    op<fp8_transpose, 1>("fp8_transpose"), op<fp8_product, 4>("fp8_product"), op<fp8_grad_w, 4>("fp8_grad_w"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
