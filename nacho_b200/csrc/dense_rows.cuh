@@ -49,6 +49,15 @@ inline int word_bytes(std::initializer_list<const nb200_dense *> all) {
     return word;
 }
 
+inline int sm_count() {
+    static const int count = [] {
+        int dev = 0, n = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
+        return n;
+    }();
+    return count;
+}
+
 // Calls f(T{}) with the element type.
 template <typename F>
 int with_type(int type, F f) {

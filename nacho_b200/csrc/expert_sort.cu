@@ -347,15 +347,6 @@ int team_of(int64_t words) {
     return t;
 }
 
-int sm_count() {
-    static const int count = [] {
-        int dev = 0, n = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
-        return n;
-    }();
-    return count;
-}
-
 dim3 grid_of(int64_t teams, int tpr) {
     const int64_t ctas = (teams * tpr + NT - 1) / NT;
     return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, (int64_t)sm_count() * 64)));

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(NT) k_fp8_transpose(Blocks a, Blocks z) {
     if (threadIdx.x == 0) z.scales[(g * z.kb + n) * z.nb + b] = a.scales[(g * a.kb + b) * a.nb + n];
 }
 
-dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, 148 * 64))); }
+dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, sm_count() * 64ll))); }
 
 constexpr int64_t MAX_CTAS = (1ll << 31) - 1;
 

@@ -6,23 +6,281 @@
 #include <type_traits>
 
 #include "dense_rows.cuh"
+#include "tensor_core.cuh"
 
 namespace nb200 {
 namespace {
 
 constexpr int NT = 256;
 
-// An operand: [group][block][row][128 codes], and where the scale of (group, block, row) lies.
+// An operand: [group][block of 128][row][128 codes], and the scales of a block, one for every row or for every 128.
 struct Operand {
     const uint8_t *values;
     const float *scales;
-    int64_t blocks, pad;        // per group; rows to a multiple of 8
-    int64_t scale_pitch;        // scales per block
-    int scale_shift;            // rows per scale, as a power of two
+    int64_t blocks, pad;   // per group; rows to a multiple of 8
+    int64_t scale_pitch;   // scales per block
 
     __device__ const uint8_t *block(int64_t g, int64_t b) const { return values + (g * blocks + b) * pad * BLOCK8; }
-    __device__ float scale(int64_t g, int64_t b, int64_t r) const { return ld_late(scales + (g * blocks + b) * scale_pitch + (r >> scale_shift)); }
+    __device__ const float *scale(int64_t g, int64_t b) const { return scales + (g * blocks + b) * scale_pitch; }
 };
+
+// ---- tiles of 128 x 256 on the tensor cores ----------------------------------------------
+
+constexpr int BM = 128, BN = 256, STAGES = 4, STORE_WARPS = 8, THREADS = (STORE_WARPS + 4) * 32;
+// Registers a thread: 168 at launch (65536 / 384), then 232 for the two groups of four warps that hold sums and 40 for the third: 64512 as before.
+constexpr int REGS_SUMS = 232, REGS_OTHERS = 40;
+static_assert(256 * REGS_SUMS + 128 * REGS_OTHERS <= 168 * THREADS, "");
+constexpr int WAIT_LIMIT = 1 << 22;  // polls, after which a wait gives up: seconds, where microseconds are usual
+constexpr int PANEL = 16;            // tiles that share columns follow one another: 16 of rows, then the next columns
+
+// What a CTA has in shared memory; tiles and the stores' staging begin at 1024-byte boundaries.
+struct Shared {
+    uint8_t a[STAGES][BM * BLOCK8];
+    uint8_t b[STAGES][BN * BLOCK8];
+    uint8_t out[STORE_WARPS][32 * 128];
+    uint64_t full[STAGES], empty[STAGES];  // a stage's copies have landed; its matrix instructions are done
+    uint64_t sum_full[2], sum_empty[2];    // a block's sums lie in tensor memory; they have been read
+    uint64_t drained;
+    uint32_t tmem;
+    int failed;
+};
+constexpr size_t SHARED_BYTES = sizeof(Shared) + 1024;
+
+struct Tile {
+    int g;
+    int64_t row, from, to;  // first row, a multiple of 8; the group's rows
+    int64_t col;
+};
+
+// Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order.
+struct Walk {
+    const int32_t *offsets;
+    int groups;
+    int64_t rows, col_tiles;
+    int chunk = -32;
+    int64_t base = 0, incl = 0;  // tiles of the groups before this chunk; of this chunk's groups up to the lane's
+    int64_t from = 0, to = 0;
+
+    __device__ Walk(const int32_t *o, int g, int64_t r, int64_t c) : offsets(o), groups(g), rows(r), col_tiles(c) {}
+
+    __device__ static int64_t row_tiles(int64_t from, int64_t to) { return to > from ? (to - (from & ~int64_t(7)) + BM - 1) / BM : 0; }
+
+    __device__ bool find(int64_t tile, Tile &t) {
+        int64_t total;
+        while (total = __shfl_sync(FULL_MASK, incl, 31), tile >= base + total) {
+            base += total;
+            chunk += 32;
+            if (chunk >= groups) return false;
+            const int g = chunk + lane_id();
+            from = to = 0;
+            if (g < groups) {
+                from = offsets ? min(max((int64_t)ld_late(offsets + g), (int64_t)0), rows) : 0;
+                to = offsets ? min(max((int64_t)ld_late(offsets + g + 1), from), rows) : rows;
+            }
+            incl = row_tiles(from, to) * col_tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(FULL_MASK, incl, o);
+                if (lane_id() >= o) incl += v;
+            }
+        }
+        const int src = __ffs(__ballot_sync(FULL_MASK, base + incl > tile)) - 1;
+        t.g = chunk + src;
+        t.from = __shfl_sync(FULL_MASK, from, src);
+        t.to = __shfl_sync(FULL_MASK, to, src);
+        const int64_t high = row_tiles(t.from, t.to);
+        const int64_t within = tile - base - (__shfl_sync(FULL_MASK, incl, src) - high * col_tiles);
+        const int64_t panel = within / (PANEL * col_tiles), width = min((int64_t)PANEL, high - panel * PANEL), rest = within - panel * PANEL * col_tiles;
+        t.row = (t.from & ~int64_t(7)) + (panel * PANEL + rest % width) * BM;
+        t.col = rest / width * BN;
+        return true;
+    }
+};
+
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed) {
+    for (int i = 0; i < WAIT_LIMIT; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (i % 64 == 63 && *failed) return false;
+    }
+    *failed = 1;
+    return false;
+}
+
+// 32 rows of a warp, 128 columns from `col` on, from registers to memory: through shared memory, 128 bytes of every row at a time, so
+// that whole lines are written. WIDE: rows can be written in words of 16 bytes.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint8_t *buffer, T *y, int64_t stride, int64_t row, int64_t from, int64_t to, int64_t col, int64_t cols) {
+    constexpr int PER = 128 / sizeof(T), EACH = 16 / sizeof(T);  // columns at a time; in 16 bytes
+    const int lane = lane_id();
+#pragma unroll
+    for (int c = 0; c < 128; c += PER) {
+        if (col + c >= cols) break;
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            Vec<T, EACH> v;
+#pragma unroll
+            for (int j = 0; j < EACH; j += 2) {
+                const float2 f = parts(acc[(c + p * EACH + j) / 2]);
+                v.v[j] = from_float<T>(f.x), v.v[j + 1] = from_float<T>(f.y);
+            }
+            *reinterpret_cast<Vec<T, EACH> *>(buffer + piece_at(lane, p)) = v;
+        }
+        __syncwarp();
+        if constexpr (WIDE) {
+            const int p = lane & 7;
+            const bool there = col + c + p * EACH < cols;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const int r = i + lane / 8;
+                if (there && row + r >= from && row + r < to)
+                    *reinterpret_cast<uint4 *>(y + (row + r) * stride + col + c + p * EACH) = *reinterpret_cast<const uint4 *>(buffer + piece_at(r, p));
+            }
+        } else {
+            for (int r = 0; r < 32; ++r) {
+                if (row + r < from || row + r >= to) continue;
+#pragma unroll
+                for (int j = lane; j < PER; j += 32)
+                    if (col + c + j < cols) y[(row + r) * stride + col + c + j] = *reinterpret_cast<const T *>(buffer + piece_at(r, j / EACH) + j % EACH * sizeof(T));
+            }
+        }
+    }
+}
+
+// One CTA per SM, which takes every gridDim-th tile of 128 rows by 256 columns. One warp brings blocks of both operands into shared memory (plain
+// bulk copies: a tile of a block is consecutive memory), one issues the matrix instructions, whose sums of a block land in
+// one half of tensor memory, and eight multiply the other half's by their scales into registers, 128 columns of a row per thread: scales
+// differ from block to block, so the sums have to leave tensor memory every 128 columns. That takes the eight warps half of
+// the time that the matrix instructions of a block take.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
+                                                        unsigned long long *report) {
+    extern __shared__ uint8_t raw[];
+    Shared &sh = *reinterpret_cast<Shared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int warp = warp_id(), lane = lane_id();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < 2; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], STORE_WARPS);
+        mbar_init(&sh.drained, 1);
+        mbar_fence_init();
+        sh.failed = 0;
+    }
+    if (warp == STORE_WARPS) tmem_alloc(&sh.tmem, 512);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    volatile int *failed = &sh.failed;
+    trigger_dependents();
+    wait_for_previous();
+
+    const int blocks = (int)a.blocks;
+    if (warp < STORE_WARPS) {
+        // sums and stores: warps w and w + 4 have the lanes of tensor memory that every fourth warp can reach, and a half of the columns each
+        more_registers<REGS_SUMS>();
+        Walk walk(offsets, groups, rows, (cols + BN - 1) / BN);
+        Tile t;
+        const int lanes = warp & 3, half = warp >> 2;
+        uint32_t it = 0;
+        for (int64_t tile = blockIdx.x; !__any_sync(FULL_MASK, *failed) && walk.find(tile, t); tile += gridDim.x) {
+            uint64_t acc[64];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) acc[j] = 0;
+            const int64_t row = t.row + lanes * 32, col = t.col + half * 128;
+            const float *sa = a.scales + min(row + lane, a.pad - 1), *sw = w.scale(t.g, 0) + min(col / BLOCK8, w.scale_pitch - 1);
+            float next_a = blocks > 0 ? ld_late(sa) : 0.f, next_w = blocks > 0 ? ld_late(sw) : 0.f;
+            bool fine = true;
+            for (int b = 0; b < blocks; ++b, ++it) {
+                const int h = (int)(it & 1);
+                const uint64_t s = both(next_a * next_w);
+                if (b + 1 < blocks) next_a = ld_late(sa + (b + 1) * a.scale_pitch), next_w = ld_late(sw + (b + 1) * w.scale_pitch);
+                fine = wait_for(&sh.sum_full[h], (it / 2) & 1, failed);
+                if (!__all_sync(FULL_MASK, fine)) {
+                    fine = false;
+                    break;
+                }
+                tmem_fence_after();
+                const uint32_t at = tmem + ((uint32_t)(lanes * 32) << 16) + h * BN + half * 128;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t v[32];
+                    tmem_load32(at + q * 32, v);
+                    tmem_wait_loads(v);
+                    if (q == 3) {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.sum_empty[h]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) fma2(acc[q * 16 + j], v[2 * j], v[2 * j + 1], s);
+                }
+            }
+            if (!fine) break;
+            if (col < cols) store_rows<T, WIDE>(acc, sh.out[warp], y, stride, row, t.from, t.to, col, cols);
+        }
+        // rows of no group
+        if (offsets) {
+            const int64_t lo = min(max((int64_t)ld_late(offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(offsets + groups), lo), rows);
+            for (int64_t r = blockIdx.x * STORE_WARPS + warp; r < rows; r += (int64_t)gridDim.x * STORE_WARPS)
+                if (r < lo || r >= hi)
+                    for (int64_t c = lane; c < cols; c += 32) y[r * stride + c] = from_float<T>(0.f);
+        }
+    } else {
+        fewer_registers<REGS_OTHERS>();
+        Walk walk(offsets, groups, rows, (cols + BN - 1) / BN);
+        Tile t;
+        if (warp == STORE_WARPS + 1) {  // copies
+            uint32_t it = 0;
+            for (int64_t tile = blockIdx.x; !__any_sync(FULL_MASK, *failed) && walk.find(tile, t); tile += gridDim.x) {
+                if (lane == 0) {
+                    const uint32_t a_bytes = (uint32_t)min((int64_t)BM, a.pad - t.row) * BLOCK8, b_bytes = (uint32_t)min((int64_t)BN, w.pad - t.col) * BLOCK8;
+                    for (int b = 0; b < blocks; ++b, ++it) {
+                        const int s = (int)(it % STAGES);
+                        if (it >= STAGES && !wait_for(&sh.empty[s], (it / STAGES - 1) & 1, failed)) break;
+                        mbar_arrive_expect_tx(&sh.full[s], a_bytes + b_bytes);
+                        bulk_load(sh.a[s], a.block(0, b) + t.row * BLOCK8, a_bytes, &sh.full[s]);
+                        bulk_load(sh.b[s], w.block(t.g, b) + t.col * BLOCK8, b_bytes, &sh.full[s]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (lane == 0 && *failed)  // nothing may land in shared memory that is no longer this CTA's
+                for (uint32_t i = it - min(it, (uint32_t)STAGES); i != it; ++i) mbar_wait_bounded(&sh.full[i % STAGES], (i / STAGES) & 1, 1 << 16);
+        } else if (warp == STORE_WARPS) {  // matrix instructions
+            uint32_t it = 0;
+            for (int64_t tile = blockIdx.x; !__any_sync(FULL_MASK, *failed) && walk.find(tile, t); tile += gridDim.x) {
+                if (lane == 0) {
+                    for (int b = 0; b < blocks; ++b, ++it) {
+                        const int s = (int)(it % STAGES), h = (int)(it & 1);
+                        if (it >= 2 && !wait_for(&sh.sum_empty[h], (it / 2 - 1) & 1, failed)) break;
+                        if (!wait_for(&sh.full[s], (it / STAGES) & 1, failed)) break;
+                        tmem_fence_after();
+                        const uint64_t da = tile_descriptor(smem_u32(sh.a[s])), db = tile_descriptor(smem_u32(sh.b[s]));
+    #pragma unroll
+                        for (int k = 0; k < BLOCK8 / 32; ++k) mma_e4m3(tmem + h * BN, da + 2 * k, db + 2 * k, product_descriptor(BM, BN), k > 0);
+                        mma_commit(&sh.empty[s]);
+                        mma_commit(&sh.sum_full[h]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (lane == 0 && *failed) {
+                mma_commit(&sh.drained);
+                mbar_wait_bounded(&sh.drained, 0, 1 << 16);
+            }
+            __syncwarp();
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == STORE_WARPS) {
+        tmem_fence_after();
+        tmem_free(tmem, 512);
+        if (lane == 0 && *failed) publish_result_word(report, 1, blockIdx.x);
+    }
+}
+
+// ---- the gradient, an element per thread --------------------------------------------------
 
 __device__ __forceinline__ float2 pair_of(uint32_t two) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
@@ -45,26 +303,6 @@ __device__ float dot128(const uint8_t *a, int64_t ra, const uint8_t *b, int64_t 
     return sum;
 }
 
-// A thread per element of the result.
-template <typename T>
-__global__ void __launch_bounds__(NT) k_product_simple(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride) {
-    wait_for_previous();
-    trigger_dependents();
-    const int64_t all = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
-        const int64_t r = i / cols, n = i - r * cols;
-        int g = 0;
-        if (offsets) {
-            while (g < groups && ld_late(offsets + g + 1) <= r) ++g;
-            if (r < ld_late(offsets)) g = groups;
-        }
-        float sum = 0.f;
-        if (g < groups)
-            for (int64_t b = 0; b < a.blocks; ++b) sum = __fmaf_rn(a.scale(0, b, r) * w.scale(g, b, n), dot128(a.block(0, b), r, w.block(g, b), n), sum);
-        y[r * stride + n] = from_float<T>(sum);
-    }
-}
-
 __global__ void __launch_bounds__(NT) k_grad_w_simple(Operand d, Operand x, const int32_t *first_block, int groups, int64_t rows, int64_t cols, float *z) {
     wait_for_previous();
     trigger_dependents();
@@ -73,7 +311,7 @@ __global__ void __launch_bounds__(NT) k_grad_w_simple(Operand d, Operand x, cons
         const int64_t g = i / (rows * cols), n = i / cols % rows, k = i % cols;
         float sum = 0.f;
         for (int64_t b = ld_late(first_block + g); b < ld_late(first_block + g + 1); ++b)
-            sum = __fmaf_rn(d.scale(0, b, n) * x.scale(0, b, k), dot128(d.block(0, b), n, x.block(0, b), k), sum);
+            sum = __fmaf_rn(ld_late(d.scale(0, b) + n) * ld_late(x.scale(0, b) + k), dot128(d.block(0, b), n, x.block(0, b), k), sum);
         z[i] = sum;
     }
 }
@@ -151,7 +389,20 @@ __global__ void __launch_bounds__(NT) k_fp8_columns(const T *x, int64_t stride, 
 
 // ---- host ------------------------------------------------------------------------------
 
-dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, 148 * 64))); }
+dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, sm_count() * 64ll))); }
+
+// The word by which a product of this stream says that a wait gave up. The call does not wait for its kernel, so the next one on the stream
+// finds it and returns the error in its place.
+constexpr int PRODUCT_SLOT = 9;
+int report_of(cudaStream_t stream, Workspace **ws) {
+    int st;
+    if ((st = acquire_workspace(stream, 0, ws, PRODUCT_SLOT))) return st;
+    volatile unsigned long long *word = reinterpret_cast<volatile unsigned long long *>((*ws)->host) + 32;
+    const unsigned long long said = *word;
+    if (!(said & RW_VALID)) return NB200_OK;
+    *word = 0;
+    return note_timeout(3, (int)(said & RW_VALUE_MASK), "an earlier 8-bit product");
+}
 
 struct GradScratch {
     int32_t *first_block;
@@ -209,14 +460,24 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     if (w->groups > NB200_MAX_EXPERTS) return NB200_E_UNSUPPORTED;
     if (y->rows == 0 || y->cols == 0) return NB200_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), padded_rows(a->rows), 0};
-    const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows), 7};
+    const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), padded_rows(a->rows)};
+    const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows)};
+    Workspace *ws = nullptr;
+    int st;
+    if ((st = report_of(stream, &ws))) return st;
+    unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
+    // tiles at most: every group but one may begin and end inside tiles
+    const int64_t tiles = (blocks_of(y->rows) + 2 * (int64_t)w->groups) * ((y->cols + BN - 1) / BN);
     return with_type(y->type, [&](auto e) {
         using T = decltype(e);
-        LaunchScope scope("fp8_product", stream);
-        NB200_CUDA(launch_overlapped(k_product_simple<T>, grid_of((y->rows * y->cols + NT - 1) / NT), dim3(NT), 0, stream, oa, ow, offsets, w->groups, y->rows, y->cols,
-                                     static_cast<T *>(y->data), y->stride));
-        return (int)NB200_OK;
+        auto go = [&](auto kernel) -> int {
+            NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SHARED_BYTES));
+            LaunchScope scope("fp8_product", stream);
+            NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles, sm_count())), dim3(THREADS), SHARED_BYTES, stream, oa, ow, offsets, w->groups, y->rows,
+                                         y->cols, static_cast<T *>(y->data), y->stride, report));
+            return NB200_OK;
+        };
+        return word_bytes({y}) == 16 ? go(k_product<T, true>) : go(k_product<T, false>);
     });
 }
 
@@ -239,8 +500,8 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
     int st;
     if ((st = quantise_columns(dy, s.block, s.bound, s.d, s.ds, stream))) return st;
     if ((st = quantise_columns(x, s.block, s.bound, s.x, s.xs, stream))) return st;
-    const Operand od{s.d, s.ds, s.bound, padded_rows(dy->cols), padded_rows(dy->cols), 0};
-    const Operand ox{s.x, s.xs, s.bound, padded_rows(x->cols), padded_rows(x->cols), 0};
+    const Operand od{s.d, s.ds, s.bound, padded_rows(dy->cols), padded_rows(dy->cols)};
+    const Operand ox{s.x, s.xs, s.bound, padded_rows(x->cols), padded_rows(x->cols)};
     LaunchScope scope("fp8_grad_w", stream);
     NB200_CUDA(launch_overlapped(k_grad_w_simple, grid_of(((int64_t)groups * dy->cols * x->cols + NT - 1) / NT), dim3(NT), 0, stream, od, ox, s.first_block, groups, dy->cols,
                                  x->cols, z));

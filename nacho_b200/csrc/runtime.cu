@@ -70,8 +70,8 @@ int note_cuda_error(cudaError_t e, const char *what) {
 }
 
 int note_timeout(int site, int tile, const char *where) {
-    static const char *const names[] = {"?", "look-back over earlier tiles", "bulk copy into shared memory"};
-    std::snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s gave up at tile %d", where, names[site >= 1 && site <= 2 ? site : 0], tile);
+    static const char *const names[] = {"?", "look-back over earlier tiles", "bulk copy into shared memory", "matrix product pipeline"};
+    std::snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s gave up at tile %d", where, names[site >= 1 && site <= 3 ? site : 0], tile);
     return NB200_E_TIMEOUT;
 }
 
@@ -80,7 +80,10 @@ int acquire_workspace(cudaStream_t stream, size_t bytes, Workspace **out, int sl
     NB200_CUDA(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> g(g_ws_mutex);
     Workspace &ws = g_workspaces[{{dev, slot}, stream}];
-    if (!ws.host) NB200_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&ws.host), 64 * sizeof(int64_t), cudaHostAllocDefault));
+    if (!ws.host) {
+        NB200_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&ws.host), 64 * sizeof(int64_t), cudaHostAllocDefault));
+        std::memset(ws.host, 0, 64 * sizeof(int64_t));
+    }
     ++ws.generation;  // first of all: a block that fails to grow is gone too
     if (bytes > ws.dev_bytes) {
         if (ws.dev) {

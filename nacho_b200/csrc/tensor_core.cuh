@@ -1,0 +1,102 @@
+// Thin wrappers over the sm_100a tensor-core PTX that the 8-bit products use: tensor memory, descriptors of shared-memory tiles,
+// matrix instructions on e4m3 operands with 32-bit sums, and the barriers they complete on.
+#pragma once
+
+#include "tma.cuh"
+
+namespace nb200 {
+
+// ---- tensor memory ---------------------------------------------------------------------
+
+// One warp takes `columns` (a power of two from 32 to 512) of all 128 lanes and later gives them back. The address lands in shared memory.
+__device__ __forceinline__ void tmem_alloc(uint32_t *address, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(address)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns) : "memory");
+}
+
+// 32 columns of this warp's 32 lanes: thread i gets lane i's. The words are there after tmem_wait_loads, which names them so that
+// nothing uses them before.
+__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+          "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(address)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_loads(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :
+                 : "memory");
+}
+
+// Orders tensor-memory accesses with the barrier operations of other threads.
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// ---- operands --------------------------------------------------------------------------
+
+// A tile of rows of 128 bytes, one after another from a 1024-byte boundary on, whose 16-byte pieces are turned by row % 8 (the 128-byte
+// swizzle): start address and distance of 8 rows in units of 16 bytes, version 1, swizzle code 2. A step of 32 bytes along the rows adds 2.
+__device__ __forceinline__ uint64_t tile_descriptor(uint32_t smem_address) {
+    return (uint64_t)((smem_address >> 4) & 0x3fff) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// e4m3 times e4m3, sums in 32 bits, both operands by rows along the summed axis.
+__host__ __device__ constexpr uint32_t product_descriptor(int m, int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24; }
+
+// d (+)= a b^T over 32 columns of the operands. One thread issues it.
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+        : "memory");
+}
+
+// The barrier gets an arrival when all matrix instructions that this thread has issued so far are done.
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ---- registers -------------------------------------------------------------------------
+
+// Four neighbouring warps together change how many registers each of their threads has. What the warps of a block end up with must not be
+// more than the block was launched with.
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ---- sums ------------------------------------------------------------------------------
+
+// Two sums at a time: acc = v * s + acc, each rounded once.
+__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t v0, uint32_t v1, uint64_t s) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
+}
+__device__ __forceinline__ uint64_t both(float s) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(s));
+    return v;
+}
+__device__ __forceinline__ float2 parts(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+
+}  // namespace nb200
