@@ -382,7 +382,7 @@ typedef struct nb200_expert_order {
  * e4m3(x * (448 / m)), both quotients rounded to 32 bits; a block that holds a NaN or an infinity stands for NaNs.
  * values: [group][column block][row, to a multiple of 8][128 codes], column blocks filled up with zeros. The 16-byte piece p of
  *         a row's 128 codes lies at place p ^ (row % 8). 16-byte aligned.
- * scales: tiled = 0: [column block][row, to a multiple of 8]; tiled = 1: [group][column block][row block]. */
+ * scales: tiled = 0: [column block][row, to a multiple of 8]; tiled = 1: [group][row block][column block]. 16-byte aligned. */
 typedef struct nb200_fp8 {
     int32_t groups, rows, cols, tiled;
     uint8_t *values;

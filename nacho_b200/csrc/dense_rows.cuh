@@ -109,7 +109,7 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
 
 inline bool fp8_ok(const nb200_fp8 *m) {
     return m && nb200_fp8_value_count(m) >= 0 && (nb200_fp8_value_count(m) == 0 || (m->values && m->scales)) &&
-           reinterpret_cast<uintptr_t>(m->values) % 16 == 0;
+           reinterpret_cast<uintptr_t>(m->values) % 16 == 0 && reinterpret_cast<uintptr_t>(m->scales) % 16 == 0;
 }
 
 // Eight neighbouring elements of a row from column c on, zeros from column `cols` on. V: what one load brings.

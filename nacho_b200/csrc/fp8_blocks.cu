@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(NT) k_fp8_tiles(Blocks z, const T *x, int64_t 
             *reinterpret_cast<uint2 *>(z.block(g, b) + piece_at(r, sub >> 1) + (sub & 1) * 8) =
                 make_uint2(codes4(v[i][0], v[i][1], v[i][2], v[i][3], f.inverse), codes4(v[i][4], v[i][5], v[i][6], v[i][7], f.inverse));
     }
-    if (threadIdx.x == 0) z.scales[(g * z.kb + b) * z.nb + n] = f.scale;
+    if (threadIdx.x == 0) z.scales[(g * z.nb + n) * z.kb + b] = f.scale;
 }
 
 // Eight threads have a row's block: 16 codes each. `wide`: the rows of the given codes can be read in words of 16.
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(NT) k_fp8_pack(Blocks z, const uint8_t *codes,
         }
         *reinterpret_cast<uint4 *>(z.block(g, b) + piece_at(r, p)) = q;
         if (tiled) {
-            if (p == 0 && r % BLOCK8 == 0) z.scales[(g * z.kb + b) * z.nb + r / BLOCK8] = scales[(g * z.nb + r / BLOCK8) * z.kb + b];
+            if (p == 0 && r % BLOCK8 == 0) z.scales[(g * z.nb + r / BLOCK8) * z.kb + b] = scales[(g * z.nb + r / BLOCK8) * z.kb + b];
         } else if (p == 0) {
             z.scales[b * z.pad + r] = scales[r * z.kb + b];
         }
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(NT) k_fp8_unpack(Blocks a, bool tiled, float *
         const int64_t r = row - (int64_t)g * a.rows;
         __nv_fp8_e4m3 q;
         q.__x = a.block(g, b)[piece_at(r, at / 16) + at % 16];
-        z[i] = float(q) * (tiled ? a.scales[(g * a.kb + b) * a.nb + r / BLOCK8] : a.scales[b * a.pad + r]);
+        z[i] = float(q) * (tiled ? a.scales[(g * a.nb + r / BLOCK8) * a.kb + b] : a.scales[b * a.pad + r]);
     }
 }
 
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(NT) k_fp8_transpose(Blocks a, Blocks z) {
             w[j] = tile[p * 16 + j * 4][c] | tile[p * 16 + j * 4 + 1][c] << 8 | tile[p * 16 + j * 4 + 2][c] << 16 | (uint32_t)tile[p * 16 + j * 4 + 3][c] << 24;
         *reinterpret_cast<uint4 *>(z.block(g, n) + piece_at(row, p)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (threadIdx.x == 0) z.scales[(g * z.kb + n) * z.nb + b] = a.scales[(g * a.kb + b) * a.nb + n];
+    if (threadIdx.x == 0) z.scales[(g * z.nb + b) * z.kb + n] = a.scales[(g * a.nb + n) * a.kb + b];
 }
 
 dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, sm_count() * 64ll))); }

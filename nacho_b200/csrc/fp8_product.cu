@@ -13,38 +13,62 @@ namespace {
 
 constexpr int NT = 256;
 
-// An operand: [group][block of 128][row][128 codes], and the scales of a block, one for every row or for every 128.
+// An operand, [group][block of 128][row][128 codes], with its scales: of a row per block [block][row], or per 128 x 128 [group][row block][block].
 struct Operand {
     const uint8_t *values;
     const float *scales;
-    int64_t blocks, pad;   // per group; rows to a multiple of 8
-    int64_t scale_pitch;   // scales per block
+    int64_t blocks, pad;  // per group; rows to a multiple of 8
+    int64_t row_blocks;
 
     __device__ const uint8_t *block(int64_t g, int64_t b) const { return values + (g * blocks + b) * pad * BLOCK8; }
-    __device__ const float *scale(int64_t g, int64_t b) const { return scales + (g * blocks + b) * scale_pitch; }
+    __device__ const float *row_scales(int64_t b) const { return scales + b * pad; }
+    __device__ const float *tile_scales(int64_t g, int64_t n) const { return scales + (g * row_blocks + min(n, row_blocks - 1)) * blocks; }
 };
 
-// ---- tiles of 128 x 256 on the tensor cores ----------------------------------------------
+// ---- tiles on the tensor cores -------------------------------------------------------------
 
-constexpr int BM = 128, BN = 256, STAGES = 4, STORE_WARPS = 8, THREADS = (STORE_WARPS + 4) * 32;
-// Registers a thread: 168 at launch (65536 / 384), then 232 for the two groups of four warps that hold sums and 40 for the third: 64512 as before.
-constexpr int REGS_SUMS = 232, REGS_OTHERS = 40;
+constexpr int STORE_WARPS = 8, THREADS = (STORE_WARPS + 4) * 32;
+// Registers a thread: 168 at launch (65536 / 384), then 224 for the two groups of four warps that hold sums and 56 for the third: 64512 as before.
+constexpr int REGS_SUMS = 224, REGS_OTHERS = 56;
 static_assert(256 * REGS_SUMS + 128 * REGS_OTHERS <= 168 * THREADS, "");
 constexpr int WAIT_LIMIT = 1 << 22;  // polls, after which a wait gives up: seconds, where microseconds are usual
-constexpr int PANEL = 16;            // tiles that share columns follow one another: 16 of rows, then the next columns
 
-// What a CTA has in shared memory; tiles and the stores' staging begin at 1024-byte boundaries.
-struct Shared {
-    uint8_t a[STAGES][BM * BLOCK8];
-    uint8_t b[STAGES][BN * BLOCK8];
-    uint8_t out[STORE_WARPS][32 * 128];
-    uint64_t full[STAGES], empty[STAGES];  // a stage's copies have landed; its matrix instructions are done
-    uint64_t sum_full[2], sum_empty[2];    // a block's sums lie in tensor memory; they have been read
-    uint64_t drained;
-    uint32_t tmem;
-    int failed;
+// A CTA has 128 rows of the result and 128 columns, in a pair 256. Both CTAs of a pair have the same columns, each brings half of their codes.
+template <bool PAIR>
+struct Shape {
+    static constexpr int CTAS = PAIR ? 2 : 1, BM = 128 * CTAS, BN = 128 * CTAS;  // a tile of the result
+    static constexpr int A_ROWS = 128, B_ROWS = 128;                             // what a CTA brings per block
+    static constexpr int STAGES = 5, SUMS = 512 / BN;                            // blocks under way; places for their sums in tensor memory
+    // Scales are written into a place STAGES + SUMS blocks after it was used before: by then their matrix instructions, and with them those of
+    // STAGES blocks earlier, are done, which had to wait until the sums of SUMS blocks earlier had been read.
+    static constexpr int SCALES = STAGES + SUMS;
+    static constexpr int PANEL = PAIR ? 8 : 16;  // tiles that share columns follow one another: 2048 rows, then the next columns
+
+    // What a CTA has in shared memory; tiles and the stores' staging begin at 1024-byte boundaries.
+    struct Shared {
+        uint8_t a[STAGES][A_ROWS * BLOCK8];
+        uint8_t b[STAGES][B_ROWS * BLOCK8];
+        uint8_t out[STORE_WARPS][32 * 128];
+        float scale[SCALES][A_ROWS];
+        uint64_t full[STAGES], empty[STAGES];      // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
+        uint64_t sum_full[SUMS], sum_empty[SUMS];  // a block's sums lie in tensor memory; they have been read
+        uint64_t drained;
+        uint32_t tmem;
+        int failed;
+    };
+    static constexpr size_t SHARED_BYTES = sizeof(Shared) + 1024;
+    static_assert(SHARED_BYTES <= 227 * 1024, "");
 };
-constexpr size_t SHARED_BYTES = sizeof(Shared) + 1024;
+
+// Which of N places is next, and in which phase of its barriers.
+template <int N>
+struct Ring {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ void next() {
+        if (++at == N) at = 0, phase ^= 1;
+    }
+};
 
 struct Tile {
     int g;
@@ -53,6 +77,7 @@ struct Tile {
 };
 
 // Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order.
+template <int BM, int BN, int PANEL>
 struct Walk {
     const int32_t *offsets;
     int groups;
@@ -97,33 +122,31 @@ struct Walk {
     }
 };
 
+// For a whole warp; false for all of it once one of its threads, or another warp of the CTA, has given up.
 __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed) {
     for (int i = 0; i < WAIT_LIMIT; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (i % 64 == 63 && *failed) return false;
+        if (__all_sync(FULL_MASK, mbar_try_wait(bar, parity))) return true;
+        if (i % 64 == 63 && __any_sync(FULL_MASK, *failed)) return false;
     }
     *failed = 1;
     return false;
 }
 
-// 32 rows of a warp, 128 columns from `col` on, from registers to memory: through shared memory, 128 bytes of every row at a time, so
+// 32 rows of a warp, N columns from `col` on, from registers to memory: through shared memory, 128 bytes of every row at a time, so
 // that whole lines are written. WIDE: rows can be written in words of 16 bytes.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint8_t *buffer, T *y, int64_t stride, int64_t row, int64_t from, int64_t to, int64_t col, int64_t cols) {
+template <typename T, bool WIDE, int N>
+__device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t *buffer, T *y, int64_t stride, int64_t row, int64_t from, int64_t to, int64_t col, int64_t cols) {
     constexpr int PER = 128 / sizeof(T), EACH = 16 / sizeof(T);  // columns at a time; in 16 bytes
     const int lane = lane_id();
 #pragma unroll
-    for (int c = 0; c < 128; c += PER) {
+    for (int c = 0; c < N; c += PER) {
         if (col + c >= cols) break;
         __syncwarp();
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
             Vec<T, EACH> v;
 #pragma unroll
-            for (int j = 0; j < EACH; j += 2) {
-                const float2 f = parts(acc[(c + p * EACH + j) / 2]);
-                v.v[j] = from_float<T>(f.x), v.v[j + 1] = from_float<T>(f.y);
-            }
+            for (int j = 0; j < EACH; ++j) v.v[j] = from_float<T>(acc[c + p * EACH + j]);
             *reinterpret_cast<Vec<T, EACH> *>(buffer + piece_at(lane, p)) = v;
         }
         __syncwarp();
@@ -147,27 +170,30 @@ __device__ __forceinline__ void store_rows(const uint64_t (&acc)[64], uint8_t *b
     }
 }
 
-// One CTA per SM, which takes every gridDim-th tile of 128 rows by 256 columns. One warp brings blocks of both operands into shared memory (plain
-// bulk copies: a tile of a block is consecutive memory), one issues the matrix instructions, whose sums of a block land in
-// one half of tensor memory, and eight multiply the other half's by their scales into registers, 128 columns of a row per thread: scales
-// differ from block to block, so the sums have to leave tensor memory every 128 columns. That takes the eight warps half of
-// the time that the matrix instructions of a block take.
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
-                                                        unsigned long long *report) {
+// One CTA per SM; they take tiles of 128 x 128 (a pair of them 256 x 256) in turn. One warp brings blocks of both operands into shared
+// memory (plain bulk copies: a tile of a block is consecutive memory), one issues the matrix instructions, whose sums of a block land in
+// tensor memory, and eight multiply the sums of earlier blocks by their scales into registers, half of a tile's columns of a row per thread: scales
+// differ from block to block, so the sums have to leave tensor memory every 128 columns.
+template <typename T, bool WIDE, bool PAIR>
+__device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
+                                        unsigned long long *report) {
+    using S = Shape<PAIR>;
+    constexpr int STAGES = S::STAGES, SUMS = S::SUMS, BN = S::BN, N = BN / 2;
     extern __shared__ uint8_t raw[];
-    Shared &sh = *reinterpret_cast<Shared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    typename S::Shared &sh = *reinterpret_cast<typename S::Shared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = warp_id(), lane = lane_id();
+    const int rank = PAIR ? (int)cluster_rank() : 0;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1);
-        for (int s = 0; s < 2; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], STORE_WARPS);
+        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[s], PAIR && rank == 0 ? 2 : 1), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < SUMS; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], STORE_WARPS * S::CTAS);
         mbar_init(&sh.drained, 1);
         mbar_fence_init();
         sh.failed = 0;
     }
-    if (warp == STORE_WARPS) tmem_alloc(&sh.tmem, 512);
+    if (warp == STORE_WARPS) tmem_alloc<PAIR>(&sh.tmem, 512);
     tmem_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // nobody arrives at a barrier that is not there yet
     tmem_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     volatile int *failed = &sh.failed;
@@ -175,48 +201,58 @@ __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, co
     wait_for_previous();
 
     const int blocks = (int)a.blocks;
+    const int64_t first = blockIdx.x / S::CTAS, step = gridDim.x / S::CTAS;
+    using Tiles = Walk<S::BM, BN, S::PANEL>;
     if (warp < STORE_WARPS) {
         // sums and stores: warps w and w + 4 have the lanes of tensor memory that every fourth warp can reach, and a half of the columns each
         more_registers<REGS_SUMS>();
-        Walk walk(offsets, groups, rows, (cols + BN - 1) / BN);
+        Tiles walk(offsets, groups, rows, (cols + BN - 1) / BN);
         Tile t;
         const int lanes = warp & 3, half = warp >> 2;
-        uint32_t it = 0;
-        for (int64_t tile = blockIdx.x; !__any_sync(FULL_MASK, *failed) && walk.find(tile, t); tile += gridDim.x) {
-            uint64_t acc[64];
+        Ring<SUMS> sums;
+        Ring<S::SCALES> place;
+        const uint32_t base = tmem + ((uint32_t)(lanes * 32) << 16) + half * N;
+        for (int64_t tile = first; walk.find(tile, t); tile += step) {
+            float acc[N];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) acc[j] = 0;
-            const int64_t row = t.row + lanes * 32, col = t.col + half * 128;
-            const float *sa = a.scales + min(row + lane, a.pad - 1), *sw = w.scale(t.g, 0) + min(col / BLOCK8, w.scale_pitch - 1);
-            float next_a = blocks > 0 ? ld_late(sa) : 0.f, next_w = blocks > 0 ? ld_late(sw) : 0.f;
+            for (int j = 0; j < N; ++j) acc[j] = 0.f;
+            const int64_t row = t.row + rank * 128 + lanes * 32, col = t.col + half * N;
+            // The scales of the columns' tiles: each lane has a block's, of 32 blocks, and asks for those of the next 32. The scales of rows come with
+            // the copies, which the matrix instructions have waited for and this warp waits for those.
+            const float *sw = w.tile_scales(t.g, col / BLOCK8);
+            float tile_scale = 0.f, next_scale = lane < blocks ? ld_late(sw + lane) : 0.f;
             bool fine = true;
-            for (int b = 0; b < blocks; ++b, ++it) {
-                const int h = (int)(it & 1);
-                const uint64_t s = both(next_a * next_w);
-                if (b + 1 < blocks) next_a = ld_late(sa + (b + 1) * a.scale_pitch), next_w = ld_late(sw + (b + 1) * w.scale_pitch);
-                fine = wait_for(&sh.sum_full[h], (it / 2) & 1, failed);
-                if (!__all_sync(FULL_MASK, fine)) {
-                    fine = false;
-                    break;
+            for (int b = 0; b < blocks; ++b, sums.next(), place.next()) {
+                if (b % 32 == 0) {
+                    tile_scale = next_scale;
+                    next_scale = b + 32 + lane < blocks ? ld_late(sw + b + 32 + lane) : 0.f;
                 }
+                if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
                 tmem_fence_after();
-                const uint32_t at = tmem + ((uint32_t)(lanes * 32) << 16) + h * BN + half * 128;
+                const uint32_t at = base + sums.at * BN;
+                // 32 columns are on their way while 32 others are added
+                uint32_t v[N / 32][32];
+                tmem_load32(at, v[0]);
+                const float s = __shfl_sync(FULL_MASK, tile_scale, b % 32) * sh.scale[place.at][lanes * 32 + lane];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t v[32];
-                    tmem_load32(at + q * 32, v);
-                    tmem_wait_loads(v);
-                    if (q == 3) {
+                for (int q = 0; q < N / 32; ++q) {
+                    tmem_wait_loads(v[q]);
+                    if (q + 1 < N / 32) {
+                        tmem_load32(at + (q + 1) * 32, v[q + 1]);
+                    } else {
                         tmem_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.sum_empty[h]);
+                        if (lane == 0) {
+                            if constexpr (PAIR) mbar_arrive_leader(&sh.sum_empty[sums.at]);
+                            else mbar_arrive(&sh.sum_empty[sums.at]);
+                        }
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) fma2(acc[q * 16 + j], v[2 * j], v[2 * j + 1], s);
+                    for (int j = 0; j < 32; ++j) acc[q * 32 + j] = __fmaf_rn(__uint_as_float(v[q][j]), s, acc[q * 32 + j]);
                 }
             }
             if (!fine) break;
-            if (col < cols) store_rows<T, WIDE>(acc, sh.out[warp], y, stride, row, t.from, t.to, col, cols);
+            if (col < cols) store_rows<T, WIDE, N>(acc, sh.out[warp], y, stride, row, t.from, t.to, col, cols);
         }
         // rows of no group
         if (offsets) {
@@ -227,57 +263,87 @@ __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, co
         }
     } else {
         fewer_registers<REGS_OTHERS>();
-        Walk walk(offsets, groups, rows, (cols + BN - 1) / BN);
+        Tiles walk(offsets, groups, rows, (cols + BN - 1) / BN);
         Tile t;
+        Ring<STAGES> stage;
+        Ring<S::SCALES> place;
+        bool fine = true;
         if (warp == STORE_WARPS + 1) {  // copies
-            uint32_t it = 0;
-            for (int64_t tile = blockIdx.x; !__any_sync(FULL_MASK, *failed) && walk.find(tile, t); tile += gridDim.x) {
-                if (lane == 0) {
-                    const uint32_t a_bytes = (uint32_t)min((int64_t)BM, a.pad - t.row) * BLOCK8, b_bytes = (uint32_t)min((int64_t)BN, w.pad - t.col) * BLOCK8;
-                    for (int b = 0; b < blocks; ++b, ++it) {
-                        const int s = (int)(it % STAGES);
-                        if (it >= STAGES && !wait_for(&sh.empty[s], (it / STAGES - 1) & 1, failed)) break;
-                        mbar_arrive_expect_tx(&sh.full[s], a_bytes + b_bytes);
-                        bulk_load(sh.a[s], a.block(0, b) + t.row * BLOCK8, a_bytes, &sh.full[s]);
-                        bulk_load(sh.b[s], w.block(t.g, b) + t.col * BLOCK8, b_bytes, &sh.full[s]);
+            for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
+                const int64_t row = t.row + rank * S::A_ROWS, col = t.col + rank * S::B_ROWS;
+                const uint32_t a_bytes = (uint32_t)min((int64_t)S::A_ROWS, max(a.pad - row, (int64_t)0)) * BLOCK8;
+                const uint32_t b_bytes = (uint32_t)min((int64_t)S::B_ROWS, max(w.pad - col, (int64_t)0)) * BLOCK8;
+                const uint32_t scale_bytes = a_bytes / BLOCK8 * sizeof(float);
+                const float *from_scales = a.row_scales(0) + row;
+                const uint8_t *from_a = a.block(0, 0) + row * BLOCK8, *from_b = w.block(t.g, 0) + col * BLOCK8;
+                for (int b = 0; b < blocks; ++b, stage.next(), place.next()) {
+                    if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
+                    if (elected()) {
+                        mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + b_bytes + scale_bytes);
+                        if (a_bytes) {
+                            bulk_load(sh.a[stage.at], from_a, a_bytes, &sh.full[stage.at]);
+                            bulk_load(sh.scale[place.at], from_scales, scale_bytes, &sh.full[stage.at]);
+                        }
+                        if (b_bytes) bulk_load(sh.b[stage.at], from_b, b_bytes, &sh.full[stage.at]);
                     }
+                    __syncwarp();
+                    from_a += a.pad * BLOCK8, from_b += w.pad * BLOCK8, from_scales += a.pad;
                 }
-                __syncwarp();
             }
-            if (lane == 0 && *failed)  // nothing may land in shared memory that is no longer this CTA's
-                for (uint32_t i = it - min(it, (uint32_t)STAGES); i != it; ++i) mbar_wait_bounded(&sh.full[i % STAGES], (i / STAGES) & 1, 1 << 16);
-        } else if (warp == STORE_WARPS) {  // matrix instructions
-            uint32_t it = 0;
-            for (int64_t tile = blockIdx.x; !__any_sync(FULL_MASK, *failed) && walk.find(tile, t); tile += gridDim.x) {
-                if (lane == 0) {
-                    for (int b = 0; b < blocks; ++b, ++it) {
-                        const int s = (int)(it % STAGES), h = (int)(it & 1);
-                        if (it >= 2 && !wait_for(&sh.sum_empty[h], (it / 2 - 1) & 1, failed)) break;
-                        if (!wait_for(&sh.full[s], (it / STAGES) & 1, failed)) break;
-                        tmem_fence_after();
-                        const uint64_t da = tile_descriptor(smem_u32(sh.a[s])), db = tile_descriptor(smem_u32(sh.b[s]));
-    #pragma unroll
-                        for (int k = 0; k < BLOCK8 / 32; ++k) mma_e4m3(tmem + h * BN, da + 2 * k, db + 2 * k, product_descriptor(BM, BN), k > 0);
-                        mma_commit(&sh.empty[s]);
-                        mma_commit(&sh.sum_full[h]);
+            if (!fine)  // nothing may land in shared memory that is no longer this CTA's
+                for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1, 1 << 16);
+        } else if (warp == STORE_WARPS && rank == 0) {  // matrix instructions
+            const uint64_t tile_a = tile_descriptor(smem_u32(sh.a[0])), tile_b = tile_descriptor(smem_u32(sh.b[0]));
+            Ring<SUMS> sums;
+            for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
+                for (int b = 0; b < blocks; ++b, stage.next(), sums.next()) {
+                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                    tmem_fence_after();
+                    if (elected()) {
+                        const uint64_t da = tile_a + (uint64_t)(stage.at * (S::A_ROWS * BLOCK8 >> 4)), db = tile_b + (uint64_t)(stage.at * (S::B_ROWS * BLOCK8 >> 4));
+#pragma unroll
+                        for (int k = 0; k < BLOCK8 / 32; ++k) mma_e4m3<PAIR>(tmem + sums.at * BN, da + 2 * k, db + 2 * k, product_descriptor(S::BM, BN), k > 0);
+                        mma_commit<PAIR>(&sh.empty[stage.at]);
+                        mma_commit<PAIR>(&sh.sum_full[sums.at]);
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-            if (lane == 0 && *failed) {
-                mma_commit(&sh.drained);
+            if (!fine) {
+                if (elected()) mma_commit<PAIR>(&sh.drained);
+                __syncwarp();
                 mbar_wait_bounded(&sh.drained, 0, 1 << 16);
             }
-            __syncwarp();
+        } else if (PAIR && warp == STORE_WARPS) {  // tells the leader of the copies that have landed here
+            for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
+                for (int b = 0; b < blocks; ++b, stage.next()) {
+                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (elected()) mbar_arrive_leader(&sh.full[stage.at]);
+                    __syncwarp();
+                }
+            }
         }
     }
     tmem_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // no arrival is on its way to a CTA that is gone
     if (warp == STORE_WARPS) {
         tmem_fence_after();
-        tmem_free(tmem, 512);
+        tmem_free<PAIR>(tmem, 512);
         if (lane == 0 && *failed) publish_result_word(report, 1, blockIdx.x);
     }
+}
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
+                                                        unsigned long long *report) {
+    product<T, WIDE, false>(a, w, offsets, groups, rows, cols, y, stride, report);
+}
+template <typename T, bool WIDE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_product_pair(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y,
+                                                                                       int64_t stride, unsigned long long *report) {
+    product<T, WIDE, true>(a, w, offsets, groups, rows, cols, y, stride, report);
 }
 
 // ---- the gradient, an element per thread --------------------------------------------------
@@ -311,7 +377,7 @@ __global__ void __launch_bounds__(NT) k_grad_w_simple(Operand d, Operand x, cons
         const int64_t g = i / (rows * cols), n = i / cols % rows, k = i % cols;
         float sum = 0.f;
         for (int64_t b = ld_late(first_block + g); b < ld_late(first_block + g + 1); ++b)
-            sum = __fmaf_rn(ld_late(d.scale(0, b) + n) * ld_late(x.scale(0, b) + k), dot128(d.block(0, b), n, x.block(0, b), k), sum);
+            sum = __fmaf_rn(ld_late(d.row_scales(b) + n) * ld_late(x.row_scales(b) + k), dot128(d.block(0, b), n, x.block(0, b), k), sum);
         z[i] = sum;
     }
 }
@@ -460,24 +526,28 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     if (w->groups > NB200_MAX_EXPERTS) return NB200_E_UNSUPPORTED;
     if (y->rows == 0 || y->cols == 0) return NB200_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), padded_rows(a->rows)};
+    const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), 0};
     const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows)};
     Workspace *ws = nullptr;
     int st;
     if ((st = report_of(stream, &ws))) return st;
     unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
-    // tiles at most: every group but one may begin and end inside tiles
-    const int64_t tiles = (blocks_of(y->rows) + 2 * (int64_t)w->groups) * ((y->cols + BN - 1) / BN);
+    // tiles at most: a group may begin and end inside tiles
+    const bool pair = y->rows >= (int64_t)w->groups * 192;
+    const int ctas = pair ? 2 : 1;
+    const int64_t tiles = ((y->rows + 128 * ctas - 1) / (128 * ctas) + 2 * (int64_t)w->groups) * ((y->cols + 128 * ctas - 1) / (128 * ctas));
     return with_type(y->type, [&](auto e) {
         using T = decltype(e);
-        auto go = [&](auto kernel) -> int {
-            NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SHARED_BYTES));
+        auto go = [&](auto kernel, size_t smem) -> int {
+            NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             LaunchScope scope("fp8_product", stream);
-            NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles, sm_count())), dim3(THREADS), SHARED_BYTES, stream, oa, ow, offsets, w->groups, y->rows,
-                                         y->cols, static_cast<T *>(y->data), y->stride, report));
+            NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles * ctas, sm_count() / ctas * ctas)), dim3(THREADS), smem, stream, oa, ow, offsets, w->groups,
+                                         y->rows, y->cols, static_cast<T *>(y->data), y->stride, report));
             return NB200_OK;
         };
-        return word_bytes({y}) == 16 ? go(k_product<T, true>) : go(k_product<T, false>);
+        const bool wide = word_bytes({y}) == 16;
+        if (pair) return wide ? go(k_product_pair<T, true>, Shape<true>::SHARED_BYTES) : go(k_product_pair<T, false>, Shape<true>::SHARED_BYTES);
+        return wide ? go(k_product<T, true>, Shape<false>::SHARED_BYTES) : go(k_product<T, false>, Shape<false>::SHARED_BYTES);
     });
 }
 
@@ -500,8 +570,8 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
     int st;
     if ((st = quantise_columns(dy, s.block, s.bound, s.d, s.ds, stream))) return st;
     if ((st = quantise_columns(x, s.block, s.bound, s.x, s.xs, stream))) return st;
-    const Operand od{s.d, s.ds, s.bound, padded_rows(dy->cols), padded_rows(dy->cols)};
-    const Operand ox{s.x, s.xs, s.bound, padded_rows(x->cols), padded_rows(x->cols)};
+    const Operand od{s.d, s.ds, s.bound, padded_rows(dy->cols), 0};
+    const Operand ox{s.x, s.xs, s.bound, padded_rows(x->cols), 0};
     LaunchScope scope("fp8_grad_w", stream);
     NB200_CUDA(launch_overlapped(k_grad_w_simple, grid_of(((int64_t)groups * dy->cols * x->cols + NT - 1) / NT), dim3(NT), 0, stream, od, ox, s.first_block, groups, dy->cols,
                                  x->cols, z));
