@@ -49,7 +49,7 @@ struct Shape {
         uint8_t a[STAGES][A_ROWS * BLOCK8];
         uint8_t b[STAGES][B_ROWS * BLOCK8];
         uint8_t out[STORE_WARPS][32 * 128];
-        float scale[SCALES][A_ROWS];
+        float scale[SCALES][A_ROWS], col_scale[SCALES][BN];  // the latter for the gradient
         uint64_t full[STAGES], empty[STAGES];      // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
         uint64_t sum_full[SUMS], sum_empty[SUMS];  // a block's sums lie in tensor memory; they have been read
         uint64_t drained;
@@ -70,23 +70,32 @@ struct Ring {
     }
 };
 
+// A tile of the result: its group, first row (a multiple of 8) and column, the rows that count, and the blocks that are summed.
 struct Tile {
     int g;
-    int64_t row, from, to;  // first row, a multiple of 8; the group's rows
-    int64_t col;
+    int64_t row, from, to, col;
+    int first_block, blocks;
 };
+
+// The order of the tiles of `high` x `wide`: panels of rows, column by column.
+template <int PANEL>
+__device__ __forceinline__ void place_tile(int64_t within, int64_t high, int64_t wide, int64_t *row, int64_t *col) {
+    const int64_t panel = within / (PANEL * wide), width = min((int64_t)PANEL, high - panel * PANEL), rest = within - panel * PANEL * wide;
+    *row = panel * PANEL + rest % width;
+    *col = rest / width;
+}
 
 // Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order.
 template <int BM, int BN, int PANEL>
 struct Walk {
     const int32_t *offsets;
-    int groups;
+    int groups, blocks;
     int64_t rows, col_tiles;
     int chunk = -32;
     int64_t base = 0, incl = 0;  // tiles of the groups before this chunk; of this chunk's groups up to the lane's
     int64_t from = 0, to = 0;
 
-    __device__ Walk(const int32_t *o, int g, int64_t r, int64_t c) : offsets(o), groups(g), rows(r), col_tiles(c) {}
+    __device__ Walk(const int32_t *o, int g, int b, int64_t r, int64_t c) : offsets(o), groups(g), blocks(b), rows(r), col_tiles((c + BN - 1) / BN) {}
 
     __device__ static int64_t row_tiles(int64_t from, int64_t to) { return to > from ? (to - (from & ~int64_t(7)) + BM - 1) / BM : 0; }
 
@@ -115,9 +124,29 @@ struct Walk {
         t.to = __shfl_sync(FULL_MASK, to, src);
         const int64_t high = row_tiles(t.from, t.to);
         const int64_t within = tile - base - (__shfl_sync(FULL_MASK, incl, src) - high * col_tiles);
-        const int64_t panel = within / (PANEL * col_tiles), width = min((int64_t)PANEL, high - panel * PANEL), rest = within - panel * PANEL * col_tiles;
-        t.row = (t.from & ~int64_t(7)) + (panel * PANEL + rest % width) * BM;
-        t.col = rest / width * BN;
+        place_tile<PANEL>(within, high, col_tiles, &t.row, &t.col);
+        t.row = (t.from & ~int64_t(7)) + t.row * BM;
+        t.col *= BN;
+        t.first_block = 0, t.blocks = blocks;
+        return true;
+    }
+};
+
+// The same for the gradient, whose groups have a result each, all of one size, and blocks of their own.
+template <int BM, int BN, int PANEL>
+struct GradWalk {
+    const int32_t *first_block;
+    int groups;
+    int64_t rows, cols;
+
+    __device__ bool find(int64_t tile, Tile &t) {
+        const int64_t high = (rows + BM - 1) / BM, wide = (cols + BN - 1) / BN;
+        t.g = (int)min(tile / (high * wide), (int64_t)groups);
+        if (t.g == groups) return false;
+        place_tile<PANEL>(tile - t.g * high * wide, high, wide, &t.row, &t.col);
+        t.row *= BM, t.col *= BN, t.from = 0, t.to = rows;
+        t.first_block = ld_late(first_block + t.g);
+        t.blocks = ld_late(first_block + t.g + 1) - t.first_block;
         return true;
     }
 };
@@ -174,7 +203,10 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t *buffe
 // memory (plain bulk copies: a tile of a block is consecutive memory), one issues the matrix instructions, whose sums of a block land in
 // tensor memory, and eight multiply the sums of earlier blocks by their scales into registers, half of a tile's columns of a row per thread: scales
 // differ from block to block, so the sums have to leave tensor memory every 128 columns.
-template <typename T, bool WIDE, bool PAIR>
+//
+// GRAD: the sums run over a group's blocks of rows of dy and x, `offsets` says where those begin, and columns have a scale each. The scales of
+// both are multiplied for every element, which is as much arithmetic again.
+template <typename T, bool WIDE, bool PAIR, bool GRAD>
 __device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                         unsigned long long *report) {
     using S = Shape<PAIR>;
@@ -200,13 +232,15 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
     trigger_dependents();
     wait_for_previous();
 
-    const int blocks = (int)a.blocks;
     const int64_t first = blockIdx.x / S::CTAS, step = gridDim.x / S::CTAS;
-    using Tiles = Walk<S::BM, BN, S::PANEL>;
+    auto tiles = [&] {
+        if constexpr (GRAD) return GradWalk<S::BM, BN, S::PANEL>{offsets, groups, rows, cols};
+        else return Walk<S::BM, BN, S::PANEL>(offsets, groups, (int)a.blocks, rows, cols);
+    };
     if (warp < STORE_WARPS) {
         // sums and stores: warps w and w + 4 have the lanes of tensor memory that every fourth warp can reach, and a half of the columns each
         more_registers<REGS_SUMS>();
-        Tiles walk(offsets, groups, rows, (cols + BN - 1) / BN);
+        auto walk = tiles();
         Tile t;
         const int lanes = warp & 3, half = warp >> 2;
         Ring<SUMS> sums;
@@ -217,15 +251,15 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] = 0.f;
             const int64_t row = t.row + rank * 128 + lanes * 32, col = t.col + half * N;
-            // The scales of the columns' tiles: each lane has a block's, of 32 blocks, and asks for those of the next 32. The scales of rows come with
-            // the copies, which the matrix instructions have waited for and this warp waits for those.
-            const float *sw = w.tile_scales(t.g, col / BLOCK8);
-            float tile_scale = 0.f, next_scale = lane < blocks ? ld_late(sw + lane) : 0.f;
+            // The scales of the columns' tiles: each lane has a block's, of 32 blocks, and asks for those of the next 32. The scales of rows (for the
+            // gradient, of columns too) come with the copies, which the matrix instructions have waited for and this warp waits for those.
+            const float *sw = GRAD ? nullptr : w.tile_scales(t.g, col / BLOCK8);
+            float tile_scale = 0.f, next_scale = !GRAD && lane < t.blocks ? ld_late(sw + lane) : 0.f;
             bool fine = true;
-            for (int b = 0; b < blocks; ++b, sums.next(), place.next()) {
-                if (b % 32 == 0) {
+            for (int b = 0; b < t.blocks; ++b, sums.next(), place.next()) {
+                if (!GRAD && b % 32 == 0) {
                     tile_scale = next_scale;
-                    next_scale = b + 32 + lane < blocks ? ld_late(sw + b + 32 + lane) : 0.f;
+                    next_scale = b + 32 + lane < t.blocks ? ld_late(sw + b + 32 + lane) : 0.f;
                 }
                 if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
                 tmem_fence_after();
@@ -233,7 +267,8 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 // 32 columns are on their way while 32 others are added
                 uint32_t v[N / 32][32];
                 tmem_load32(at, v[0]);
-                const float s = __shfl_sync(FULL_MASK, tile_scale, b % 32) * sh.scale[place.at][lanes * 32 + lane];
+                float s = sh.scale[place.at][lanes * 32 + lane];
+                if constexpr (!GRAD) s *= __shfl_sync(FULL_MASK, tile_scale, b % 32);
 #pragma unroll
                 for (int q = 0; q < N / 32; ++q) {
                     tmem_wait_loads(v[q]);
@@ -247,15 +282,27 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                             else mbar_arrive(&sh.sum_empty[sums.at]);
                         }
                     }
+                    if constexpr (GRAD) {
+                        const float4 *columns = reinterpret_cast<const float4 *>(&sh.col_scale[place.at][half * N + q * 32]);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[q * 32 + j] = __fmaf_rn(__uint_as_float(v[q][j]), s, acc[q * 32 + j]);
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 c = columns[j / 4];
+                            acc[q * 32 + j] = __fmaf_rn(__uint_as_float(v[q][j]), s * c.x, acc[q * 32 + j]);
+                            acc[q * 32 + j + 1] = __fmaf_rn(__uint_as_float(v[q][j + 1]), s * c.y, acc[q * 32 + j + 1]);
+                            acc[q * 32 + j + 2] = __fmaf_rn(__uint_as_float(v[q][j + 2]), s * c.z, acc[q * 32 + j + 2]);
+                            acc[q * 32 + j + 3] = __fmaf_rn(__uint_as_float(v[q][j + 3]), s * c.w, acc[q * 32 + j + 3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) acc[q * 32 + j] = __fmaf_rn(__uint_as_float(v[q][j]), s, acc[q * 32 + j]);
+                    }
                 }
             }
             if (!fine) break;
-            if (col < cols) store_rows<T, WIDE, N>(acc, sh.out[warp], y, stride, row, t.from, t.to, col, cols);
+            if (col < cols) store_rows<T, WIDE, N>(acc, sh.out[warp], GRAD ? y + t.g * rows * stride : y, stride, row, t.from, t.to, col, cols);
         }
         // rows of no group
-        if (offsets) {
+        if (!GRAD && offsets) {
             const int64_t lo = min(max((int64_t)ld_late(offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(offsets + groups), lo), rows);
             for (int64_t r = blockIdx.x * STORE_WARPS + warp; r < rows; r += (int64_t)gridDim.x * STORE_WARPS)
                 if (r < lo || r >= hi)
@@ -263,7 +310,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
         }
     } else {
         fewer_registers<REGS_OTHERS>();
-        Tiles walk(offsets, groups, rows, (cols + BN - 1) / BN);
+        auto walk = tiles();
         Tile t;
         Ring<STAGES> stage;
         Ring<S::SCALES> place;
@@ -274,20 +321,22 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 const uint32_t a_bytes = (uint32_t)min((int64_t)S::A_ROWS, max(a.pad - row, (int64_t)0)) * BLOCK8;
                 const uint32_t b_bytes = (uint32_t)min((int64_t)S::B_ROWS, max(w.pad - col, (int64_t)0)) * BLOCK8;
                 const uint32_t scale_bytes = a_bytes / BLOCK8 * sizeof(float);
-                const float *from_scales = a.row_scales(0) + row;
-                const uint8_t *from_a = a.block(0, 0) + row * BLOCK8, *from_b = w.block(t.g, 0) + col * BLOCK8;
-                for (int b = 0; b < blocks; ++b, stage.next(), place.next()) {
+                const uint32_t col_bytes = GRAD ? (uint32_t)min((int64_t)BN, w.pad - t.col) * sizeof(float) : 0;
+                const float *from_scales = a.row_scales(t.first_block) + row, *from_col_scales = w.row_scales(t.first_block) + t.col;
+                const uint8_t *from_a = a.block(0, t.first_block) + row * BLOCK8, *from_b = w.block(GRAD ? 0 : t.g, t.first_block) + col * BLOCK8;
+                for (int b = 0; b < t.blocks; ++b, stage.next(), place.next()) {
                     if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
                     if (elected()) {
-                        mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + b_bytes + scale_bytes);
+                        mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + b_bytes + scale_bytes + col_bytes);
                         if (a_bytes) {
                             bulk_load(sh.a[stage.at], from_a, a_bytes, &sh.full[stage.at]);
                             bulk_load(sh.scale[place.at], from_scales, scale_bytes, &sh.full[stage.at]);
                         }
+                        if (GRAD) bulk_load(sh.col_scale[place.at], from_col_scales, col_bytes, &sh.full[stage.at]);
                         if (b_bytes) bulk_load(sh.b[stage.at], from_b, b_bytes, &sh.full[stage.at]);
                     }
                     __syncwarp();
-                    from_a += a.pad * BLOCK8, from_b += w.pad * BLOCK8, from_scales += a.pad;
+                    from_a += a.pad * BLOCK8, from_b += w.pad * BLOCK8, from_scales += a.pad, from_col_scales += w.pad;
                 }
             }
             if (!fine)  // nothing may land in shared memory that is no longer this CTA's
@@ -296,7 +345,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
             const uint64_t tile_a = tile_descriptor(smem_u32(sh.a[0])), tile_b = tile_descriptor(smem_u32(sh.b[0]));
             Ring<SUMS> sums;
             for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
-                for (int b = 0; b < blocks; ++b, stage.next(), sums.next()) {
+                for (int b = 0; b < t.blocks; ++b, stage.next(), sums.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
                     tmem_fence_after();
@@ -317,7 +366,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
             }
         } else if (PAIR && warp == STORE_WARPS) {  // tells the leader of the copies that have landed here
             for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
-                for (int b = 0; b < blocks; ++b, stage.next()) {
+                for (int b = 0; b < t.blocks; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     if (elected()) mbar_arrive_leader(&sh.full[stage.at]);
                     __syncwarp();
@@ -335,51 +384,15 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
     }
 }
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                                         unsigned long long *report) {
-    product<T, WIDE, false>(a, w, offsets, groups, rows, cols, y, stride, report);
+    product<T, WIDE, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report);
 }
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, bool GRAD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_product_pair(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y,
                                                                                        int64_t stride, unsigned long long *report) {
-    product<T, WIDE, true>(a, w, offsets, groups, rows, cols, y, stride, report);
-}
-
-// ---- the gradient, an element per thread --------------------------------------------------
-
-__device__ __forceinline__ float2 pair_of(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffff), __NV_E4M3);
-    return __half22float2(__half2(h));
-}
-
-// Sum over one block of 128.
-__device__ float dot128(const uint8_t *a, int64_t ra, const uint8_t *b, int64_t rb) {
-    float sum = 0.f;
-    for (int p = 0; p < 8; ++p) {
-        const uint4 qa = *reinterpret_cast<const uint4 *>(a + piece_at(ra, p)), qb = *reinterpret_cast<const uint4 *>(b + piece_at(rb, p));
-        const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 u = pair_of(wa[j / 2] >> (j % 2 * 16)), v = pair_of(wb[j / 2] >> (j % 2 * 16));
-            sum = __fmaf_rn(u.x, v.x, sum);
-            sum = __fmaf_rn(u.y, v.y, sum);
-        }
-    }
-    return sum;
-}
-
-__global__ void __launch_bounds__(NT) k_grad_w_simple(Operand d, Operand x, const int32_t *first_block, int groups, int64_t rows, int64_t cols, float *z) {
-    wait_for_previous();
-    trigger_dependents();
-    const int64_t all = groups * rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
-        const int64_t g = i / (rows * cols), n = i / cols % rows, k = i % cols;
-        float sum = 0.f;
-        for (int64_t b = ld_late(first_block + g); b < ld_late(first_block + g + 1); ++b)
-            sum = __fmaf_rn(ld_late(d.row_scales(b) + n) * ld_late(x.row_scales(b) + k), dot128(d.block(0, b), n, x.block(0, b), k), sum);
-        z[i] = sum;
-    }
+    product<T, WIDE, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report);
 }
 
 // ---- operands of the gradient ------------------------------------------------------------
@@ -470,6 +483,25 @@ int report_of(cudaStream_t stream, Workspace **ws) {
     return note_timeout(3, (int)(said & RW_VALUE_MASK), "an earlier 8-bit product");
 }
 
+// `tiles` of the shape that `pair` selects, at most.
+template <typename T, bool GRAD>
+int launch_product(const char *name, bool pair, int64_t tiles, const Operand &a, const Operand &w, const int32_t *offsets, int groups, const nb200_dense &y, cudaStream_t stream) {
+    Workspace *ws = nullptr;
+    int st;
+    if ((st = report_of(stream, &ws))) return st;
+    unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
+    auto go = [&](auto kernel, size_t smem, int ctas) -> int {
+        NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        LaunchScope scope(name, stream);
+        NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles * ctas, sm_count() / ctas * ctas)), dim3(THREADS), smem, stream, a, w, offsets, groups,
+                                     GRAD ? y.rows / groups : y.rows, y.cols, static_cast<T *>(y.data), y.stride, report));
+        return NB200_OK;
+    };
+    const bool wide = word_bytes({&y}) == 16;
+    if (pair) return wide ? go(k_product_pair<T, true, GRAD>, Shape<true>::SHARED_BYTES, 2) : go(k_product_pair<T, false, GRAD>, Shape<true>::SHARED_BYTES, 2);
+    return wide ? go(k_product<T, true, GRAD>, Shape<false>::SHARED_BYTES, 1) : go(k_product<T, false, GRAD>, Shape<false>::SHARED_BYTES, 1);
+}
+
 struct GradScratch {
     int32_t *first_block;
     int2 *block;
@@ -528,27 +560,10 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), 0};
     const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows)};
-    Workspace *ws = nullptr;
-    int st;
-    if ((st = report_of(stream, &ws))) return st;
-    unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
     // tiles at most: a group may begin and end inside tiles
     const bool pair = y->rows >= (int64_t)w->groups * 192;
-    const int ctas = pair ? 2 : 1;
-    const int64_t tiles = ((y->rows + 128 * ctas - 1) / (128 * ctas) + 2 * (int64_t)w->groups) * ((y->cols + 128 * ctas - 1) / (128 * ctas));
-    return with_type(y->type, [&](auto e) {
-        using T = decltype(e);
-        auto go = [&](auto kernel, size_t smem) -> int {
-            NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            LaunchScope scope("fp8_product", stream);
-            NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles * ctas, sm_count() / ctas * ctas)), dim3(THREADS), smem, stream, oa, ow, offsets, w->groups,
-                                         y->rows, y->cols, static_cast<T *>(y->data), y->stride, report));
-            return NB200_OK;
-        };
-        const bool wide = word_bytes({y}) == 16;
-        if (pair) return wide ? go(k_product_pair<T, true>, Shape<true>::SHARED_BYTES) : go(k_product_pair<T, false>, Shape<true>::SHARED_BYTES);
-        return wide ? go(k_product<T, true>, Shape<false>::SHARED_BYTES) : go(k_product<T, false>, Shape<false>::SHARED_BYTES);
-    });
+    const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * (int64_t)w->groups) * ((y->cols + side - 1) / side);
+    return with_type(y->type, [&](auto e) { return launch_product<decltype(e), false>("fp8_product", pair, tiles, oa, ow, offsets, w->groups, *y, stream); });
 }
 
 int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dense *x, int32_t groups) {
@@ -572,10 +587,10 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
     if ((st = quantise_columns(x, s.block, s.bound, s.x, s.xs, stream))) return st;
     const Operand od{s.d, s.ds, s.bound, padded_rows(dy->cols), 0};
     const Operand ox{s.x, s.xs, s.bound, padded_rows(x->cols), 0};
-    LaunchScope scope("fp8_grad_w", stream);
-    NB200_CUDA(launch_overlapped(k_grad_w_simple, grid_of(((int64_t)groups * dy->cols * x->cols + NT - 1) / NT), dim3(NT), 0, stream, od, ox, s.first_block, groups, dy->cols,
-                                 x->cols, z));
-    return NB200_OK;
+    const nb200_dense result{(int64_t)groups * dy->cols, x->cols, x->cols, NB200_F32, z};
+    const bool pair = dy->cols > 128 && x->cols > 128;
+    const int64_t side = pair ? 256 : 128, tiles = groups * ((dy->cols + side - 1) / side) * ((x->cols + side - 1) / side);
+    return launch_product<float, true>("fp8_grad_w", pair, tiles, od, ox, s.first_block, groups, result, stream);
 }
 
 }  // extern "C"
