@@ -30,6 +30,29 @@ struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
 
+// 16 bytes of a row as a thread handles them: words of V elements, `pitch` elements apart (neighbouring threads have neighbouring words), so that
+// rows of any alignment keep as much on its way per thread.
+template <typename T, int V>
+struct Chunk {
+    static constexpr int WORDS = 16 / (int)sizeof(T) / V, N = WORDS * V;
+    Vec<T, V> w[WORDS];
+
+    __device__ __forceinline__ void load(const T *row, int64_t c, int64_t pitch, int64_t cols) {
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u)
+            if (u == 0 || c + u * pitch < cols) w[u] = *reinterpret_cast<const Vec<T, V> *>(row + c + u * pitch);
+    }
+    __device__ __forceinline__ void store(T *row, int64_t c, int64_t pitch, int64_t cols) const {
+#pragma unroll
+        for (int u = 0; u < WORDS; ++u)
+            if (u == 0 || c + u * pitch < cols) *reinterpret_cast<Vec<T, V> *>(row + c + u * pitch) = w[u];
+    }
+    __device__ __forceinline__ float get(int i) const { return to_float(w[i / V].v[i % V]); }
+    __device__ __forceinline__ void set(int i, float f) { w[i / V].v[i % V] = from_float<T>(f); }
+    // Whether element i lies in the row.
+    __device__ __forceinline__ static bool there(int i, int64_t c, int64_t pitch, int64_t cols) { return i < V || c + i / V * pitch < cols; }
+};
+
 inline size_t type_size(int type) { return type == NB200_F32 ? 4 : 2; }
 
 inline bool dense_ok(const nb200_dense *x) {
@@ -114,20 +137,51 @@ inline bool fp8_ok(const nb200_fp8 *m) {
 
 // Eight neighbouring elements of a row from column c on, zeros from column `cols` on. V: what one load brings.
 template <typename T, int V>
-__device__ __forceinline__ void load8(const T *row, int64_t c, int64_t cols, float (&out)[8]) {
+__device__ __forceinline__ Vec<T, 8> load8(const T *row, int64_t c, int64_t cols) {
+    Vec<T, 8> out;
 #pragma unroll
-    for (int i = 0; i < 8; i += V < 8 ? V : 8) {
-        if constexpr (V <= 8) {
-            if (c + i < cols) {
-                const Vec<T, V> w = *reinterpret_cast<const Vec<T, V> *>(row + c + i);
+    for (int i = 0; i < 8; i += V) {
+        Vec<T, V> w;
+        if (c + i < cols) {
+            w = *reinterpret_cast<const Vec<T, V> *>(row + c + i);
+        } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) out[i + j] = to_float(w.v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) out[i + j] = 0.f;
-            }
+            for (int j = 0; j < V; ++j) w.v[j] = from_float<T>(0.f);
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) out.v[i + j] = w.v[j];
     }
+    return out;
+}
+
+// The factors of U blocks (a power of two) of 16 threads, which all have their largest magnitudes: every thread divides for one of them, a division
+// being as much as a dozen other instructions.
+template <int U>
+__device__ __forceinline__ void share_factors(unsigned threads, const uint32_t (&m)[U], Factors (&f)[U]) {
+    const int lane = lane_id();
+    uint32_t mine = m[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) mine = (lane & (U - 1)) == u ? m[u] : mine;
+    const Factors own = factors_of(mine);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        f[u].scale = __shfl_sync(threads, own.scale, (lane & 16) + u);
+        f[u].inverse = __shfl_sync(threads, own.inverse, (lane & 16) + u);
+    }
+}
+
+// Eight neighbouring codes, and the largest magnitude of eight elements.
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const Vec<T, 8> &v, float inverse) {
+    return make_uint2(codes4(to_float(v.v[0]), to_float(v.v[1]), to_float(v.v[2]), to_float(v.v[3]), inverse),
+                      codes4(to_float(v.v[4]), to_float(v.v[5]), to_float(v.v[6]), to_float(v.v[7]), inverse));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude8(const Vec<T, 8> &v) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, magnitude(to_float(v.v[j])));
+    return m;
 }
 
 }  // namespace nb200

@@ -132,6 +132,8 @@ struct Team {
 template <typename T, int V>
 __device__ __forceinline__ void copy_rows(const Order &o, const Team &team, int t, const T *x, int64_t stride, int64_t cols, T *xs) {
     constexpr int U = 4;
+    using C = Chunk<T, V>;
+    const int64_t pitch = (int64_t)team.size * V;
     const int e0 = o.entry_of(t), e1 = o.entry_of(t + 1);
     if (team.lane == 0)
         for (int e = e0; e < e1; ++e) {
@@ -139,21 +141,17 @@ __device__ __forceinline__ void copy_rows(const Order &o, const Team &team, int 
             if (s >= 0) o.rows[s] = t;
         }
     if (e0 >= e1) return;
-    for (int64_t c = team.lane * V; c < cols; c += (int64_t)team.size * V * U) {
-        Vec<T, V> v[U];
+    for (int64_t c = team.lane * V; c < cols; c += pitch * C::WORDS * U) {
+        C v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t at = c + (int64_t)u * team.size * V;
-            if (at < cols) v[u] = *reinterpret_cast<const Vec<T, V> *>(x + t * stride + at);
-        }
+        for (int u = 0; u < U; ++u)
+            if (c + u * C::WORDS * pitch < cols) v[u].load(x + t * stride, c + u * C::WORDS * pitch, pitch, cols);
         for (int e = e0; e < e1; ++e) {
             const int s = o.slot(e);
             if (s < 0) continue;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t at = c + (int64_t)u * team.size * V;
-                if (at < cols) *reinterpret_cast<Vec<T, V> *>(xs + s * cols + at) = v[u];
-            }
+            for (int u = 0; u < U; ++u)
+                if (c + u * C::WORDS * pitch < cols) v[u].store(xs + s * cols, c + u * C::WORDS * pitch, pitch, cols);
         }
     }
 }
@@ -180,44 +178,104 @@ __global__ void __launch_bounds__(NT) k_sort_rows(Order o, int tpr, const T *x, 
     clear_rows<T, V>(o, team, cols, xs);
 }
 
-// The same into 8-bit rows: 16 threads have a block of 128 columns, quantise it once and write it to all of the token's slots.
-template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_sort_rows_fp8(Order o, int tpr, const T *x, int64_t stride, int64_t cols, uint8_t *codes, float *scales) {
-    wait_for_previous();
-    trigger_dependents();
-    const Team team(tpr);
-    const int sub = team.lane & 15;
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
-    const int64_t pad = padded_rows(o.entries), kb = blocks_of(cols);
-    for (int t = team.first; t < o.tokens; t += team.step) {
-        const int e0 = o.entry_of(t), e1 = o.entry_of(t + 1);
-        if (team.lane == 0)
-            for (int e = e0; e < e1; ++e) {
-                const int s = o.slot(e);
-                if (s >= 0) o.rows[s] = t;
-            }
-        if (e0 >= e1) continue;
-        for (int64_t b = team.lane >> 4; b < kb; b += team.size >> 4) {
-            float v[8];
-            load8<T, V>(x + t * stride, b * BLOCK8 + sub * 8, cols, v);
-            uint32_t m = 0;
+// The entries of the tokens a team works on, asked for early: row offsets two tokens ahead, the slots (and weights) of up to N entries one
+// ahead, so that a token's rows can be asked for at once. Nothing here looks at a loaded word before the token's turn.
+template <int N>
+struct Entries {
+    const Order &o;
+    const float *w;
+    int t, step;
+    int e0, e1, next0, next1, slot[N], raw[N];
+    float weight[N], raw_weight[N];
+
+    __device__ Entries(const Order &order, const float *weights, int first, int distance) : o(order), w(weights), t(first - distance), step(distance) {
+        next0 = o.entry_of(min(first, o.tokens)), next1 = o.entry_of(min(first + 1, o.tokens));
+        ask();
+    }
+    __device__ void ask() {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, magnitude(v[j]));
-#pragma unroll
-            for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(half, m, d));
-            const Factors f = factors_of(m);
-            const uint2 q = make_uint2(codes4(v[0], v[1], v[2], v[3], f.inverse), codes4(v[4], v[5], v[6], v[7], f.inverse));
-            for (int e = e0; e < e1; ++e) {
-                const int s = o.slot(e);
-                if (s < 0) continue;
-                *reinterpret_cast<uint2 *>(codes + b * pad * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = q;
-                if (sub == 0) scales[b * pad + s] = f.scale;
+        for (int i = 0; i < N; ++i) {
+            raw[i] = -1, raw_weight[i] = 1.f;
+            if (next0 + i < next1) {
+                raw[i] = ld_late(o.slots + next0 + i);
+                if (w) raw_weight[i] = ld_late(w + next0 + i);
             }
         }
     }
+    __device__ int clamped(int s) const { return s < o.entries ? s : -1; }
+    // The next token, if there is one.
+    __device__ bool advance() {
+        t += step;
+        if (t >= o.tokens) return false;
+        const int64_t after = min((int64_t)t + step, (int64_t)o.tokens);
+        e0 = next0, e1 = next1;
+        next0 = ld_late(o.row_ptr + after), next1 = ld_late(o.row_ptr + min(after + 1, (int64_t)o.tokens));
+#pragma unroll
+        for (int i = 0; i < N; ++i) slot[i] = clamped(raw[i]), weight[i] = raw_weight[i];
+        return true;
+    }
+    // To be called when the rows of this token are on their way.
+    __device__ void ask_next() {
+        next0 = min(max(next0, 0), o.entries), next1 = min(max(next1, 0), o.entries);
+        ask();
+    }
+};
+
+// The same into 8-bit rows: 16 threads have a block of 128 columns, quantise it once and write it to all of the token's slots.
+template <typename T, int V>
+__global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const T *x, int64_t stride, int64_t cols, uint8_t *codes, float *scales) {
+    constexpr int N = 8, U = 2;
+    wait_for_previous();
+    trigger_dependents();
+    const Team team(tpr);
+    const int sub = team.lane & 15, mine = team.lane >> 4, blocks = team.size >> 4;
+    const unsigned half = 0xffffu << (threadIdx.x & 16);
+    const int64_t pad = padded_rows(o.entries);
+    const int kb = (int)blocks_of(cols);
+    Entries<N> at(o, nullptr, team.first, team.step);
+    while (at.advance()) {
+        const T *row = x + at.t * stride;
+        for (int b = mine; b < kb; b += blocks * U) {
+            Vec<T, 8> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = load8<T, V>(row, (int64_t)(b + u * blocks) * BLOCK8 + sub * 8, cols);
+            if (b == mine) {
+                if (team.lane == 0)
+                    for (int e = at.e0; e < at.e1; ++e) {
+                        const int s = o.slot(e);
+                        if (s >= 0) o.rows[s] = at.t;
+                    }
+                at.ask_next();
+            }
+            uint32_t m[U];
+            Factors f[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                m[u] = magnitude8(v[u]);
+#pragma unroll
+                for (int d = 8; d; d >>= 1) m[u] = max(m[u], __shfl_xor_sync(half, m[u], d));
+            }
+            share_factors<U>(half, m, f);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (b + u * blocks >= kb) break;
+                const int64_t block = (int64_t)(b + u * blocks) * pad;
+                const uint2 q = codes8(v[u], f[u].inverse);
+                auto put = [&](int s) {
+                    if (s < 0) return;
+                    *reinterpret_cast<uint2 *>(codes + block * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = q;
+                    if (sub == 0) scales[block + s] = f[u].scale;
+                };
+#pragma unroll
+                for (int i = 0; i < N; ++i) put(at.slot[i]);
+                for (int e = at.e0 + N; e < at.e1; ++e) put(o.slot(e));
+            }
+        }
+        if (mine >= kb) at.ask_next();
+    }
     for (int s = o.kept() + team.first; s < o.entries; s += team.step) {
         if (team.lane == 0) o.rows[s] = -1;
-        for (int64_t b = team.lane >> 4; b < kb; b += team.size >> 4) {
+        for (int64_t b = mine; b < kb; b += blocks) {
             *reinterpret_cast<uint2 *>(codes + b * pad * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = make_uint2(0, 0);
             if (sub == 0) scales[b * pad + s] = 0.f;
         }
@@ -225,109 +283,114 @@ __global__ void __launch_bounds__(NT) k_sort_rows_fp8(Order o, int tpr, const T 
 }
 
 // y[t] = sum of w[e] * z[slot(e)]. The rows of up to N entries are on their way together.
-template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_unsort_rows(Order o, int tpr, const float *w, const T *z, int64_t stride, T *y, int64_t y_stride, int64_t cols) {
-    constexpr int N = 4;
+template <typename T, int V, int N>
+__global__ void __launch_bounds__(NT, N == 8 ? 2 : 4) k_unsort_rows(Order o, int tpr, const float *w, const T *z, int64_t stride, T *y, int64_t y_stride, int64_t cols) {
     wait_for_previous();
     trigger_dependents();
     const Team team(tpr);
-    for (int t = team.first; t < o.tokens; t += team.step) {
-        const int e0 = o.entry_of(t), e1 = o.entry_of(t + 1);
-        for (int64_t c = team.lane * V; c < cols; c += team.size * V) {
-            float sum[V];
+    using C = Chunk<T, V>;
+    const int64_t pitch = (int64_t)team.size * V;
+    Entries<N> at(o, w, team.first, team.step);
+    while (at.advance()) {
+        bool asked = false;
+        for (int64_t c = team.lane * V; c < cols; c += pitch * C::WORDS) {
+            float sum[C::N];
+            C v[N];
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] = 0.f;
-            for (int e = e0; e < e1; e += N) {
-                Vec<T, V> v[N];
-                int s[N];
-                float g[N];
+            for (int i = 0; i < N; ++i)
+                if (at.slot[i] >= 0) v[i].load(z + at.slot[i] * stride, c, pitch, cols);
+            if (!asked) at.ask_next(), asked = true;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    s[i] = e + i < e1 ? o.slot(e + i) : -1;
-                    g[i] = s[i] >= 0 && w ? ld_late(w + e + i) : 1.f;
+            for (int j = 0; j < C::N; ++j) sum[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (at.slot[i] >= 0) {
+#pragma unroll
+                    for (int j = 0; j < C::N; ++j) sum[j] = __fmaf_rn(at.weight[i], v[i].get(j), sum[j]);
                 }
+            for (int e = at.e0 + N; e < at.e1; ++e) {
+                const int s = o.slot(e);
+                if (s < 0) continue;
+                C more;
+                more.load(z + s * stride, c, pitch, cols);
+                const float g = w ? ld_late(w + e) : 1.f;
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (s[i] >= 0) v[i] = *reinterpret_cast<const Vec<T, V> *>(z + s[i] * stride + c);
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (s[i] >= 0) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) sum[j] = __fmaf_rn(g[i], to_float(v[i].v[j]), sum[j]);
-                    }
+                for (int j = 0; j < C::N; ++j) sum[j] = __fmaf_rn(g, more.get(j), sum[j]);
             }
-            Vec<T, V> out;
+            C out;
 #pragma unroll
-            for (int j = 0; j < V; ++j) out.v[j] = from_float<T>(sum[j]);
-            *reinterpret_cast<Vec<T, V> *>(y + t * y_stride + c) = out;
+            for (int j = 0; j < C::N; ++j) out.set(j, sum[j]);
+            out.store(y + at.t * y_stride, c, pitch, cols);
         }
+        if (!asked) at.ask_next();
     }
 }
 
 // dz[slot(e)] = w[e] * dy[t] and dw[e] = <dy[t], z[slot(e)]>, N entries of a token at a time. Sums over the columns: every thread its own,
-// then the team's, in a fixed order.
-template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_unsort_grad(Order o, int tpr, const float *w, const T *z, int64_t z_stride, const T *dy, int64_t dy_stride, T *dz, float *dw,
+// then the warp's by exchanges, then the team's warps' in order, in shared memory that two batches in turn have.
+template <typename T, int V, int N>
+__global__ void __launch_bounds__(NT, N == 8 ? 2 : 3) k_unsort_grad(Order o, int tpr, const float *w, const T *z, int64_t z_stride, const T *dy, int64_t dy_stride, T *dz, float *dw,
                                                     int64_t cols) {
-    constexpr int N = 4;
-    __shared__ float part[NT / 32][N];
+    __shared__ float part[2][NT / 32][N];
     wait_for_previous();
     trigger_dependents();
     const Team team(tpr);
-    // All threads of a CTA take the same number of rounds, since teams of several warps meet at barriers.
-    for (int t0 = team.first - (int)threadIdx.x / tpr; t0 < o.tokens; t0 += team.step) {
-        const int t = t0 + (int)threadIdx.x / tpr;
-        const bool there = t < o.tokens;
-        const int e0 = there ? o.entry_of(t) : 0, e1 = there ? o.entry_of(t + 1) : 0;
-        for (int e = e0; __syncthreads_or(e < e1); e += N) {
-            float dot[N];
-            int s[N];
-            float g[N];
+    using C = Chunk<T, V>;
+    const int64_t pitch = (int64_t)team.size * V;
+    const int warps = tpr / 32, name = 1 + threadIdx.x / tpr;
+    int turn = 0;
+    Entries<N> at(o, w, team.first, team.step);
+    while (at.advance()) {
+        bool asked = false;
+        for (int e = at.e0; e < at.e1; e += N, turn ^= 1) {
+            if (e > at.e0)  // more than N entries: these were not asked for early
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                dot[i] = 0.f;
-                s[i] = e + i < e1 ? o.slot(e + i) : -1;
-                g[i] = s[i] >= 0 ? ld_late(w + e + i) : 0.f;
-            }
-            if (e < e1)
-                for (int64_t c = team.lane * V; c < cols; c += team.size * V) {
-                    const Vec<T, V> d = *reinterpret_cast<const Vec<T, V> *>(dy + t * dy_stride + c);
-                    Vec<T, V> v[N];
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (s[i] >= 0) v[i] = *reinterpret_cast<const Vec<T, V> *>(z + s[i] * z_stride + c);
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (s[i] >= 0) {
-                            Vec<T, V> out;
-#pragma unroll
-                            for (int j = 0; j < V; ++j) {
-                                dot[i] = __fmaf_rn(to_float(d.v[j]), to_float(v[i].v[j]), dot[i]);
-                                out.v[j] = from_float<T>(g[i] * to_float(d.v[j]));
-                            }
-                            *reinterpret_cast<Vec<T, V> *>(dz + s[i] * cols + c) = out;
-                        }
+                for (int i = 0; i < N; ++i) {
+                    at.slot[i] = e + i < at.e1 ? o.slot(e + i) : -1;
+                    at.weight[i] = at.slot[i] >= 0 ? ld_late(w + e + i) : 0.f;
                 }
+            float dot[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot[i] = 0.f;
+            for (int64_t c = team.lane * V; c < cols; c += pitch * C::WORDS) {
+                C d, v[N];
+                d.load(dy + at.t * dy_stride, c, pitch, cols);
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (at.slot[i] >= 0) v[i].load(z + at.slot[i] * z_stride, c, pitch, cols);
+                if (!asked) at.ask_next(), asked = true;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (at.slot[i] >= 0) {
+                        C out;
+#pragma unroll
+                        for (int j = 0; j < C::N; ++j) {
+                            if (C::there(j, c, pitch, cols)) dot[i] = __fmaf_rn(d.get(j), v[i].get(j), dot[i]);
+                            out.set(j, at.weight[i] * d.get(j));
+                        }
+                        out.store(dz + at.slot[i] * cols, c, pitch, cols);
+                    }
+            }
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 for (int d = 16; d; d >>= 1) dot[i] += __shfl_xor_sync(FULL_MASK, dot[i], d);
-            if (tpr > 32) {
+            if (warps > 1) {
                 if (lane_id() == 0)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) part[warp_id()][i] = dot[i];
-                __syncthreads();
-                if (team.lane == 0)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        dot[i] = 0.f;
-                        for (int v = 0; v < tpr / 32; ++v) dot[i] += part[warp_id() + v][i];
-                    }
-            }
-            if (team.lane == 0)
+                    for (int i = 0; i < N; ++i) part[turn][warp_id()][i] = dot[i];
+                asm volatile("bar.sync %0, %1;" ::"r"(name), "r"(tpr) : "memory");
+                if (team.lane < N) {
+                    float sum = 0.f;
+                    for (int v = 0; v < warps; ++v) sum += part[turn][warp_id() + v][team.lane];
+                    if (e + team.lane < at.e1) dw[e + team.lane] = o.slot(e + team.lane) >= 0 ? sum : 0.f;
+                }
+            } else if (team.lane == 0) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (e + i < e1) dw[e + i] = s[i] >= 0 ? dot[i] : 0.f;
+                    if (e + i < at.e1) dw[e + i] = at.slot[i] >= 0 ? dot[i] : 0.f;
+            }
         }
+        if (!asked) at.ask_next();
     }
     Order tail = o;
     tail.rows = nullptr;
@@ -340,10 +403,10 @@ __global__ void __launch_bounds__(NT) k_unsort_grad(Order o, int tpr, const floa
 
 // ---- host ------------------------------------------------------------------------------
 
-// Threads per token for rows of `words` loads: one load each, whole warps from 32 on.
-int team_of(int64_t words) {
+// Threads per token for rows that take `loads` of 16 bytes: one each.
+int team_of(int64_t loads) {
     int t = 32;
-    while (t < NT && t < words) t *= 2;
+    while (t < NT && t < loads) t *= 2;
     return t;
 }
 
@@ -351,6 +414,18 @@ dim3 grid_of(int64_t teams, int tpr) {
     const int64_t ctas = (teams * tpr + NT - 1) / NT;
     return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, (int64_t)sm_count() * 64)));
 }
+
+// As many CTAs as can be at work at once, or fewer where there are fewer teams' worth of tokens.
+template <typename... P>
+dim3 resident_grid(void (*kernel)(P...), int64_t teams, int tpr) {
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, NT, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+    const int64_t ctas = (teams * tpr + NT - 1) / NT;
+    return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, (int64_t)sm_count() * per_sm)));
+}
+
+// Entries per token that kernels hold at a time: what an average token has, 4 or 8.
+bool many_entries(const Order &o) { return (int64_t)o.entries > 4 * (int64_t)o.tokens; }
 
 int check_order(const nb200_expert_order *o, bool slots_given) {
     if (!o || o->tokens < 0 || o->experts < 0 || o->entries < 0 || !o->row_ptr || !o->offsets) return NB200_E_BADARG;
@@ -405,7 +480,7 @@ int nb200_expert_sort(const nb200_csr *r, const nb200_dense *x, nb200_expert_ord
     if ((st = make_order(o, stream))) return st;
     const nb200_dense none{r->rows, 0, 0, NB200_F32, nullptr};
     if (!x) x = &none, xs = const_cast<nb200_dense *>(&none);
-    const int word = word_bytes({x, xs}), tpr = team_of(x->cols * type_size(x->type) / word / 4);
+    const int word = word_bytes({x, xs}), tpr = team_of((x->cols * type_size(x->type) + 15) / 16 / 4);
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
@@ -424,13 +499,14 @@ int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, r->col);
     if ((st = make_order(o, stream))) return st;
-    const int word = word_bytes({x}), tpr = team_of(blocks_of(x->cols) * 16);
+    const int word = word_bytes({x}), tpr = team_of(blocks_of(x->cols) * 8);
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
+            auto kernel = k_sort_rows_fp8<T, decltype(v)::value>;
             LaunchScope scope("sort_rows_fp8", stream);
-            NB200_CUDA(launch_overlapped(k_sort_rows_fp8<T, decltype(v)::value>, grid_of(o.tokens, tpr), dim3(NT), 0, stream, o, tpr, static_cast<const T *>(x->data), x->stride,
-                                         x->cols, xs->values, xs->scales));
+            NB200_CUDA(launch_overlapped(kernel, resident_grid(kernel, o.tokens, tpr), dim3(NT), 0, stream, o, tpr, static_cast<const T *>(x->data), x->stride, x->cols, xs->values,
+                                         xs->scales));
             return (int)NB200_OK;
         });
     });
@@ -443,12 +519,13 @@ int nb200_expert_unsort(const nb200_expert_order *order, const float *w, const n
     if (y->rows == 0 || y->cols == 0) return NB200_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, nullptr);
-    const int word = word_bytes({z, y}), tpr = team_of(z->cols * type_size(z->type) / word);
+    const int word = word_bytes({z, y}), tpr = team_of((z->cols * type_size(z->type) + 15) / 16);
     return with_type(z->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
+            auto kernel = many_entries(o) ? k_unsort_rows<T, decltype(v)::value, 8> : k_unsort_rows<T, decltype(v)::value, 4>;
             LaunchScope scope("unsort_rows", stream);
-            NB200_CUDA(launch_overlapped(k_unsort_rows<T, decltype(v)::value>, grid_of(o.tokens, tpr), dim3(NT), 0, stream, o, tpr, w, static_cast<const T *>(z->data), z->stride,
+            NB200_CUDA(launch_overlapped(kernel, resident_grid(kernel, o.tokens, tpr), dim3(NT), 0, stream, o, tpr, w, static_cast<const T *>(z->data), z->stride,
                                          static_cast<T *>(y->data), y->stride, z->cols));
             return (int)NB200_OK;
         });
@@ -464,12 +541,13 @@ int nb200_expert_unsort_grad(const nb200_expert_order *order, const float *w, co
     if (order->entries == 0) return NB200_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, nullptr);
-    const int word = word_bytes({z, dy, dz}), tpr = team_of(z->cols * type_size(z->type) / word);
+    const int word = word_bytes({z, dy, dz}), tpr = team_of((z->cols * type_size(z->type) + 15) / 16);
     return with_type(z->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
+            auto kernel = many_entries(o) ? k_unsort_grad<T, decltype(v)::value, 8> : k_unsort_grad<T, decltype(v)::value, 4>;
             LaunchScope scope("unsort_grad", stream);
-            NB200_CUDA(launch_overlapped(k_unsort_grad<T, decltype(v)::value>, grid_of(std::max<int64_t>(o.tokens, 1), tpr), dim3(NT), 0, stream, o, tpr, w,
+            NB200_CUDA(launch_overlapped(kernel, resident_grid(kernel, std::max<int64_t>(o.tokens, 1), tpr), dim3(NT), 0, stream, o, tpr, w,
                                          static_cast<const T *>(z->data), z->stride, static_cast<const T *>(dy->data), dy->stride, static_cast<T *>(dz->data), dw, z->cols));
             return (int)NB200_OK;
         });

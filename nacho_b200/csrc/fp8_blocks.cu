@@ -22,27 +22,37 @@ struct Blocks {
 
 Blocks blocks(const nb200_fp8 *m) { return {m->rows, m->cols, m->groups, blocks_of(m->cols), padded_rows(m->rows), blocks_of(m->rows), m->values, m->scales}; }
 
-// 16 threads have a row's block of 128 columns: a load of eight elements each, the largest magnitude by four exchanges, eight codes each.
+// A CTA has 16 rows by four blocks: 16 threads a row's block of 128 columns, a load of eight elements of each block each, the largest magnitude by
+// four exchanges, eight codes each. So a block's 16 rows of codes are written as one stretch, and so are their scales.
+constexpr int ROWS8 = 16, BLOCKS8 = 4;
+
 template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_fp8_rows(Blocks z, const T *x, int64_t stride) {
+__global__ void __launch_bounds__(NT) k_fp8_rows(Blocks z, int chunks, const T *x, int64_t stride) {
     wait_for_previous();
     trigger_dependents();
     const int sub = threadIdx.x & 15;
     const unsigned half = 0xffffu << (threadIdx.x & 16);
-    const int64_t all = (int64_t)z.rows * z.kb;
-    for (int64_t i = (int64_t)blockIdx.x * (NT / 16) + threadIdx.x / 16; i < all; i += (int64_t)gridDim.x * (NT / 16)) {
-        const int64_t r = i / z.kb, b = i - r * z.kb;
-        float v[8];
-        load8<T, V>(x + r * stride, b * BLOCK8 + sub * 8, z.cols, v);
-        uint32_t m = 0;
+    const int64_t r = (int64_t)(blockIdx.x / chunks) * ROWS8 + threadIdx.x / 16;
+    const int64_t b0 = (int64_t)(blockIdx.x % chunks) * BLOCKS8;
+    if (r >= z.rows) return;
+    Vec<T, 8> v[BLOCKS8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, magnitude(v[j]));
+    for (int u = 0; u < BLOCKS8; ++u) v[u] = load8<T, V>(x + r * stride, (b0 + u) * BLOCK8 + sub * 8, z.cols);
+    uint32_t m[BLOCKS8];
+    Factors f[BLOCKS8];
 #pragma unroll
-        for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(half, m, d));
-        const Factors f = factors_of(m);
-        *reinterpret_cast<uint2 *>(z.block(0, b) + piece_at(r, sub >> 1) + (sub & 1) * 8) =
-            make_uint2(codes4(v[0], v[1], v[2], v[3], f.inverse), codes4(v[4], v[5], v[6], v[7], f.inverse));
-        if (sub == 0) z.scales[b * z.pad + r] = f.scale;
+    for (int u = 0; u < BLOCKS8; ++u) {
+        m[u] = magnitude8(v[u]);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) m[u] = max(m[u], __shfl_xor_sync(half, m[u], d));
+    }
+    share_factors<BLOCKS8>(half, m, f);
+#pragma unroll
+    for (int u = 0; u < BLOCKS8; ++u) {
+        const int64_t b = b0 + u;
+        if (b >= z.kb) break;
+        *reinterpret_cast<uint2 *>(z.block(0, b) + piece_at(r, sub >> 1) + (sub & 1) * 8) = codes8(v[u], f[u].inverse);
+        if (sub == 0) z.scales[b * z.pad + r] = f[u].scale;
     }
 }
 
@@ -58,15 +68,15 @@ __global__ void __launch_bounds__(NT) k_fp8_tiles(Blocks z, const T *x, int64_t 
     const int64_t b = blockIdx.x % per_group / z.nb, n = blockIdx.x % z.nb;
     if (threadIdx.x == 0) top = 0;
     __syncthreads();
-    float v[8][8];
+    Vec<T, 8> v[8];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = n * BLOCK8 + i * 16 + threadIdx.x / 16;
-        load8<T, V>(x + ((int64_t)g * z.rows + min(r, (int64_t)z.rows - 1)) * stride, b * BLOCK8 + sub * 8, r < z.rows ? z.cols : 0, v[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, magnitude(v[i][j]));
+        v[i] = load8<T, V>(x + ((int64_t)g * z.rows + min(r, (int64_t)z.rows - 1)) * stride, b * BLOCK8 + sub * 8, r < z.rows ? z.cols : 0);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, magnitude8(v[i]));
     m = __reduce_max_sync(FULL_MASK, m);
     if (lane_id() == 0) atomicMax(&top, m);
     __syncthreads();
@@ -75,8 +85,7 @@ __global__ void __launch_bounds__(NT) k_fp8_tiles(Blocks z, const T *x, int64_t 
     for (int i = 0; i < 8; ++i) {
         const int64_t r = n * BLOCK8 + i * 16 + threadIdx.x / 16;
         if (r < z.rows)
-            *reinterpret_cast<uint2 *>(z.block(g, b) + piece_at(r, sub >> 1) + (sub & 1) * 8) =
-                make_uint2(codes4(v[i][0], v[i][1], v[i][2], v[i][3], f.inverse), codes4(v[i][4], v[i][5], v[i][6], v[i][7], f.inverse));
+            *reinterpret_cast<uint2 *>(z.block(g, b) + piece_at(r, sub >> 1) + (sub & 1) * 8) = codes8(v[i], f.inverse);
     }
     if (threadIdx.x == 0) z.scales[(g * z.nb + n) * z.kb + b] = f.scale;
 }
@@ -125,31 +134,41 @@ __global__ void __launch_bounds__(NT) k_fp8_unpack(Blocks a, bool tiled, float *
     }
 }
 
-// A CTA per tile: read by rows, turned in shared memory, written by rows of the transpose.
+// A CTA per tile: read by rows into shared memory, words of four codes turned four by four, written by rows of the transpose. Word w of row r lies at
+// place w ^ (r / 4), so that a warp reads a column of words without conflicts.
 __global__ void __launch_bounds__(NT) k_fp8_transpose(Blocks a, Blocks z) {
-    __shared__ uint8_t tile[BLOCK8][BLOCK8 + 4];
+    __shared__ uint32_t tile[BLOCK8][32];
     wait_for_previous();
     trigger_dependents();
-    const int64_t per_group = a.kb * a.nb;
-    const int g = (int)(blockIdx.x / per_group);
-    const int64_t b = blockIdx.x % per_group / a.nb, n = blockIdx.x % a.nb;
-    for (int i = threadIdx.x; i < BLOCK8 * 8; i += NT) {
-        const int r = i / 8, p = i % 8;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (n * BLOCK8 + r < a.rows) q = *reinterpret_cast<const uint4 *>(a.block(g, b) + piece_at(n * BLOCK8 + r, p));
-        uint32_t *to = reinterpret_cast<uint32_t *>(&tile[r][p * 16]);
-        to[0] = q.x, to[1] = q.y, to[2] = q.z, to[3] = q.w;
+    const int per_group = (int)(a.kb * a.nb), g = blockIdx.x / per_group, b = blockIdx.x % per_group / (int)a.nb, n = blockIdx.x % (int)a.nb;
+    uint4 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + threadIdx.x / 8;
+        q[i] = make_uint4(0, 0, 0, 0);
+        if ((int64_t)n * BLOCK8 + r < a.rows) q[i] = *reinterpret_cast<const uint4 *>(a.block(g, b) + piece_at((int64_t)n * BLOCK8 + r, threadIdx.x & 7));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + threadIdx.x / 8, w = (threadIdx.x & 7) * 4, turn = r / 4;
+        tile[r][w ^ turn] = q[i].x, tile[r][(w + 1) ^ turn] = q[i].y, tile[r][(w + 2) ^ turn] = q[i].z, tile[r][(w + 3) ^ turn] = q[i].w;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < BLOCK8 * 8; i += NT) {
-        const int c = i % BLOCK8, p = i / BLOCK8;  // row c of the transpose; its 16 codes from rows p * 16 on
-        const int64_t row = b * BLOCK8 + c;
-        if (row >= z.rows) continue;
-        uint32_t w[4];
+    const int lane = lane_id();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            w[j] = tile[p * 16 + j * 4][c] | tile[p * 16 + j * 4 + 1][c] << 8 | tile[p * 16 + j * 4 + 2][c] << 16 | (uint32_t)tile[p * 16 + j * 4 + 3][c] << 24;
-        *reinterpret_cast<uint4 *>(z.block(g, n) + piece_at(row, p)) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; ++i) {
+        const int w = i * 8 + warp_id();  // rows 4w .. 4w + 3 of the transpose, their codes 4 lane .. 4 lane + 3
+        uint32_t r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = tile[lane * 4 + k][w ^ lane];
+        const uint32_t lo01 = __byte_perm(r[0], r[1], 0x5140), lo23 = __byte_perm(r[2], r[3], 0x5140), hi01 = __byte_perm(r[0], r[1], 0x7362),
+                       hi23 = __byte_perm(r[2], r[3], 0x7362);
+        const uint32_t turned[4] = {__byte_perm(lo01, lo23, 0x5410), __byte_perm(lo01, lo23, 0x7632), __byte_perm(hi01, hi23, 0x5410), __byte_perm(hi01, hi23, 0x7632)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t row = (int64_t)b * BLOCK8 + w * 4 + k;
+            if (row < z.rows) *reinterpret_cast<uint32_t *>(z.block(g, n) + piece_at(row, lane / 4) + lane % 4 * 4) = turned[k];
+        }
     }
     if (threadIdx.x == 0) z.scales[(g * z.nb + b) * z.kb + n] = a.scales[(g * a.nb + n) * a.kb + b];
 }
@@ -180,7 +199,8 @@ int nb200_fp8_quantise(const nb200_dense *x, nb200_fp8 *z, void *stream_) {
     if (x->rows == 0 || x->cols == 0) return NB200_OK;
     const Blocks m = blocks(z);
     const int64_t tiles = m.groups * m.kb * m.nb;
-    if (z->tiled && tiles > MAX_CTAS) return NB200_E_UNSUPPORTED;
+    const int64_t chunks = (m.kb + BLOCKS8 - 1) / BLOCKS8, row_ctas = (m.rows + ROWS8 - 1) / ROWS8 * chunks;
+    if ((z->tiled ? tiles : row_ctas) > MAX_CTAS) return NB200_E_UNSUPPORTED;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
@@ -192,7 +212,7 @@ int nb200_fp8_quantise(const nb200_dense *x, nb200_fp8 *z, void *stream_) {
                 NB200_CUDA(launch_overlapped(k_fp8_tiles<T, V>, dim3((unsigned)tiles), dim3(NT), 0, stream, m, data, x->stride));
             } else {
                 LaunchScope scope("fp8_rows", stream);
-                NB200_CUDA(launch_overlapped(k_fp8_rows<T, V>, grid_of((m.rows * m.kb + NT / 16 - 1) / (NT / 16)), dim3(NT), 0, stream, m, data, x->stride));
+                NB200_CUDA(launch_overlapped(k_fp8_rows<T, V>, dim3((unsigned)row_ctas), dim3(NT), 0, stream, m, (int)chunks, data, x->stride));
             }
             return (int)NB200_OK;
         });

@@ -422,48 +422,62 @@ __global__ void __launch_bounds__(1024) k_group_blocks(const int32_t *offsets, i
     for (int b = base + threadIdx.x; b < bound; b += 1024) block[b] = make_int2(0, 0);
 }
 
-// x by blocks of rows: column c becomes row c of the result, a scale for it per block. A CTA per block and 128 columns.
+// x by blocks of rows: column c becomes row c of the result, a scale for it per block. A CTA per block and 128 columns: a thread has eight columns of
+// eight rows, the largest magnitude of a column comes from 16 threads by way of shared memory, and the codes go through shared memory to whole
+// lines. There the eight codes of a column and eight rows p lie at place p ^ (column / 8) of the column's, which spreads a warp over the banks.
 template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_fp8_columns(const T *x, int64_t stride, int64_t cols, const int2 *block, uint8_t *values, float *scales) {
-    extern __shared__ unsigned char raw[];
-    constexpr int PITCH = BLOCK8 + 4 / sizeof(T);  // a word more: both directions without conflicts
-    T *tile = reinterpret_cast<T *>(raw);
+__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(const T *x, int64_t stride, int64_t cols, const int2 *block, uint8_t *values, float *scales) {
+    __shared__ uint32_t top[NT / 32][BLOCK8];
+    __shared__ alignas(16) float inverse[BLOCK8];
+    __shared__ alignas(16) uint2 codes[BLOCK8][16];
     wait_for_previous();
     trigger_dependents();
     const int64_t chunks = blocks_of(cols), b = blockIdx.x / chunks, c0 = blockIdx.x % chunks * BLOCK8, pad = padded_rows(cols);
     const int2 rows = *(block + b);
     if (rows.y == 0) return;
-    for (int i = threadIdx.x; i < BLOCK8 * (BLOCK8 / V); i += NT) {
-        const int r = i / (BLOCK8 / V), c = i % (BLOCK8 / V) * V;
-        Vec<T, V> v;
-        if (r < rows.y && c0 + c < cols) {
-            v = *reinterpret_cast<const Vec<T, V> *>(x + (int64_t)(rows.x + r) * stride + c0 + c);
-        } else {
+    const int sub = threadIdx.x & 15, part = threadIdx.x / 16;
+    Vec<T, 8> v[8];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v.v[j] = from_float<T>(0.f);
-        }
+    for (int i = 0; i < 8; ++i) {
+        const int r = part * 8 + i;
+        v[i] = load8<T, V>(x + (int64_t)(rows.x + min(r, rows.y - 1)) * stride, c0 + sub * 8, r < rows.y ? cols : 0);
+    }
+    uint32_t m[8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) tile[r * PITCH + c + j] = v.v[j];
+    for (int j = 0; j < 8; ++j) {
+        m[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[j] = max(m[j], magnitude(to_float(v[i].v[j])));
+        m[j] = max(m[j], __shfl_xor_sync(FULL_MASK, m[j], 16));
+    }
+    if (lane_id() < 16) {
+        *reinterpret_cast<uint4 *>(&top[warp_id()][sub * 8]) = make_uint4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<uint4 *>(&top[warp_id()][sub * 8 + 4]) = make_uint4(m[4], m[5], m[6], m[7]);
     }
     __syncthreads();
-    // two threads per column, 64 rows each, in different halves of a warp's pairs
-    const int c = threadIdx.x / 2, part = threadIdx.x & 1;
-    uint32_t m = 0;
-    for (int r = 0; r < 64; ++r) m = max(m, magnitude(to_float(tile[(part * 64 + r) * PITCH + c])));
-    m = max(m, __shfl_xor_sync(FULL_MASK, m, 1));
-    const Factors f = factors_of(m);
-    if (c0 + c >= cols) return;
-    uint8_t *to = values + b * pad * BLOCK8;
-    for (int p = 0; p < 4; ++p) {
-        uint32_t w[4];
+    if (threadIdx.x < BLOCK8) {
+        uint32_t all = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const T *at = tile + (part * 64 + p * 16 + j * 4) * PITCH + c;
-            w[j] = codes4(to_float(at[0]), to_float(at[PITCH]), to_float(at[2 * PITCH]), to_float(at[3 * PITCH]), f.inverse);
-        }
-        *reinterpret_cast<uint4 *>(to + piece_at(c0 + c, part * 4 + p)) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int w = 0; w < NT / 32; ++w) all = max(all, top[w][threadIdx.x]);
+        const Factors f = factors_of(all);
+        inverse[threadIdx.x] = f.inverse;
+        if (c0 + threadIdx.x < cols) scales[b * pad + c0 + threadIdx.x] = f.scale;
     }
-    if (part == 0) scales[b * pad + c0 + c] = f.scale;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float f = inverse[sub * 8 + j];
+        codes[sub * 8 + j][part ^ sub] = make_uint2(codes4(to_float(v[0].v[j]), to_float(v[1].v[j]), to_float(v[2].v[j]), to_float(v[3].v[j]), f),
+                                                    codes4(to_float(v[4].v[j]), to_float(v[5].v[j]), to_float(v[6].v[j]), to_float(v[7].v[j]), f));
+    }
+    __syncthreads();
+    uint8_t *to = values + b * pad * BLOCK8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = i * 32 + threadIdx.x / 8, p = threadIdx.x & 7, turn = c / 8;
+        const uint4 q = *reinterpret_cast<const uint4 *>(&codes[c][(p ^ (turn >> 1)) * 2]);
+        if (c0 + c < cols) *reinterpret_cast<uint4 *>(to + piece_at(c0 + c, p)) = turn & 1 ? make_uint4(q.z, q.w, q.x, q.y) : q;
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -535,10 +549,8 @@ int quantise_columns(const nb200_dense *x, const int2 *block, int64_t bound, uin
         using T = decltype(e);
         return with_vector<T>(word_bytes({x}), [&](auto v) {
             constexpr int V = decltype(v)::value;
-            const size_t smem = sizeof(T) * BLOCK8 * (BLOCK8 + 4 / sizeof(T));
-            if (smem > 48 * 1024) NB200_CUDA(cudaFuncSetAttribute(k_fp8_columns<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             LaunchScope scope("fp8_columns", stream);
-            NB200_CUDA(launch_overlapped(k_fp8_columns<T, V>, dim3((unsigned)ctas), dim3(NT), smem, stream, static_cast<const T *>(x->data), x->stride, x->cols, block, values,
+            NB200_CUDA(launch_overlapped(k_fp8_columns<T, V>, dim3((unsigned)ctas), dim3(NT), 0, stream, static_cast<const T *>(x->data), x->stride, x->cols, block, values,
                                          scales));
             return (int)NB200_OK;
         });
