@@ -144,6 +144,24 @@ cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+// The same for clusters of `ctas` along x.
+template <typename... P, typename... A>
+cudaError_t launch_overlapped_clusters(int ctas, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute how[2] = {};
+    how[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    how[0].val.programmaticStreamSerializationAllowed = 1;
+    how[1].id = cudaLaunchAttributeClusterDimension;
+    how[1].val.clusterDim.x = ctas, how[1].val.clusterDim.y = how[1].val.clusterDim.z = 1;
+    cfg.attrs = how;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Error word shared by kernels with bounded waits: 0 = fine, otherwise a site code.
 struct DeviceStatus {
     int error;

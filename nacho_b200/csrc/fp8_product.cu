@@ -266,14 +266,14 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 const uint32_t at = base + sums.at * BN;
                 // 32 columns are on their way while 32 others are added
                 uint32_t v[N / 32][32];
-                tmem_load32(at, v[0]);
+                tmem_load(at, v[0]);
                 float s = sh.scale[place.at][lanes * 32 + lane];
                 if constexpr (!GRAD) s *= __shfl_sync(FULL_MASK, tile_scale, b % 32);
 #pragma unroll
                 for (int q = 0; q < N / 32; ++q) {
                     tmem_wait_loads(v[q]);
                     if (q + 1 < N / 32) {
-                        tmem_load32(at + (q + 1) * 32, v[q + 1]);
+                        tmem_load(at + (q + 1) * 32, v[q + 1]);
                     } else {
                         tmem_fence_before();
                         __syncwarp();
@@ -395,6 +395,167 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_produc
     product<T, WIDE, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report);
 }
 
+// ---- few rows per group ------------------------------------------------------------------
+
+// The operands change sides: 128 rows of weights against NB rows, 16 to 64, of a group, so that a CTA brings hardly more than the weights, which is all
+// that such a product takes: one CTA per group and 128 columns of the result, several to an SM. Where there are not enough of them, the CTAs of
+// a cluster have a part of the blocks each (SPLIT) and add their sums, in order, through one another's shared memory. A group of more than NB rows
+// takes several turns over its weights.
+template <int NB, bool SPLIT>
+struct FewShape {
+    static constexpr int STAGES = 4, SUMS = 4, SCALES = STAGES + SUMS, COLUMNS = SUMS * NB;  // of tensor memory
+    struct Shared {
+        uint8_t w[STAGES][128 * BLOCK8];
+        uint8_t a[STAGES][NB * BLOCK8];
+        float scale[SCALES][NB];
+        float part[SPLIT ? NB : 1][128];
+        uint64_t full[STAGES], empty[STAGES], sum_full[SUMS], sum_empty[SUMS], drained;
+        uint32_t tmem;
+        int failed;
+    };
+    static constexpr size_t SHARED_BYTES = sizeof(Shared) + 1024;
+};
+constexpr int FEW_THREADS = 6 * 32;
+
+template <typename T, int NB, bool SPLIT>
+__global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : 2) k_product_few(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
+                                                             unsigned long long *report) {
+    using S = FewShape<NB, SPLIT>;
+    constexpr int STAGES = S::STAGES, SUMS = S::SUMS, W = NB < 32 ? 16 : 32;
+    extern __shared__ uint8_t raw[];
+    typename S::Shared &sh = *reinterpret_cast<typename S::Shared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int warp = warp_id(), lane = lane_id();
+    const int slices = SPLIT ? (int)cluster_size() : 1, slice = SPLIT ? (int)cluster_rank() : 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < SUMS; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], 4);
+        mbar_init(&sh.drained, 1);
+        mbar_fence_init();
+        sh.failed = 0;
+    }
+    if (warp == 4) tmem_alloc<false>(&sh.tmem, S::COLUMNS);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    volatile int *failed = &sh.failed;
+    trigger_dependents();
+    wait_for_previous();
+
+    const int g = blockIdx.y;
+    const int64_t col = (int64_t)(blockIdx.x / slices) * 128;
+    const int64_t from = offsets ? min(max((int64_t)ld_late(offsets + g), (int64_t)0), rows) : 0;
+    const int64_t to = offsets ? min(max((int64_t)ld_late(offsets + g + 1), from), rows) : rows;
+    const int first = (int)(a.blocks * slice / slices), blocks = (int)(a.blocks * (slice + 1) / slices) - first;
+    Ring<STAGES> stage;
+    Ring<SUMS> sums;
+    Ring<S::SCALES> place;
+    bool fine = true;
+    for (int64_t row = from & ~int64_t(7); row < to; row += NB) {
+        if (warp == 5) {  // copies
+            const uint32_t a_bytes = (uint32_t)min((int64_t)NB, a.pad - row) * BLOCK8, w_bytes = (uint32_t)min((int64_t)128, w.pad - col) * BLOCK8;
+            const uint32_t scale_bytes = a_bytes / BLOCK8 * sizeof(float);
+            for (int b = first; fine && b < first + blocks; ++b, stage.next(), place.next()) {
+                if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
+                if (elected()) {
+                    mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + w_bytes + scale_bytes);
+                    bulk_load(sh.w[stage.at], w.block(g, b) + col * BLOCK8, w_bytes, &sh.full[stage.at]);
+                    bulk_load(sh.a[stage.at], a.block(0, b) + row * BLOCK8, a_bytes, &sh.full[stage.at]);
+                    bulk_load(sh.scale[place.at], a.row_scales(b) + row, scale_bytes, &sh.full[stage.at]);
+                }
+                __syncwarp();
+            }
+        } else if (warp == 4) {  // matrix instructions
+            const uint64_t tile_w = tile_descriptor(smem_u32(sh.w[0])), tile_a = tile_descriptor(smem_u32(sh.a[0]));
+            for (int b = 0; fine && b < blocks; ++b, stage.next(), sums.next()) {
+                if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                tmem_fence_after();
+                if (elected()) {
+                    const uint64_t dw = tile_w + (uint64_t)(stage.at * (128 * BLOCK8 >> 4)), da = tile_a + (uint64_t)(stage.at * (NB * BLOCK8 >> 4));
+#pragma unroll
+                    for (int k = 0; k < BLOCK8 / 32; ++k) mma_e4m3<false>(tmem + sums.at * NB, dw + 2 * k, da + 2 * k, product_descriptor(128, NB), k > 0);
+                    mma_commit<false>(&sh.empty[stage.at]);
+                    mma_commit<false>(&sh.sum_full[sums.at]);
+                }
+                __syncwarp();
+            }
+        } else {  // sums and stores: a thread has a column of the result
+            float acc[NB];
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[j] = 0.f;
+            const float *sw = w.tile_scales(g, col / BLOCK8) + first;
+            float tile_scale = 0.f, next_scale = lane < blocks ? ld_late(sw + lane) : 0.f;
+            for (int b = 0; fine && b < blocks; ++b, sums.next(), place.next()) {
+                if (b % 32 == 0) {
+                    tile_scale = next_scale;
+                    next_scale = b + 32 + lane < blocks ? ld_late(sw + b + 32 + lane) : 0.f;
+                }
+                const float s = __shfl_sync(FULL_MASK, tile_scale, b % 32);
+                if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
+                tmem_fence_after();
+                uint32_t v[NB / W][W];
+#pragma unroll
+                for (int q = 0; q < NB / W; ++q) tmem_load(tmem + ((uint32_t)(warp * 32) << 16) + sums.at * NB + q * W, v[q]);
+#pragma unroll
+                for (int q = 0; q < NB / W; ++q) tmem_wait_loads(v[q]);
+                float row_scale[NB];
+#pragma unroll
+                for (int j = 0; j < NB; j += 4) *reinterpret_cast<float4 *>(row_scale + j) = *reinterpret_cast<const float4 *>(&sh.scale[place.at][j]);
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.sum_empty[sums.at]);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[j] = __fmaf_rn(__uint_as_float(v[j / W][j % W]), s * row_scale[j], acc[j]);
+            }
+            const int64_t n = col + threadIdx.x;
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int j = 0; j < NB; ++j) sh.part[j][threadIdx.x] = acc[j];
+            } else if (fine && n < cols) {
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    if (row + j >= from && row + j < to) y[(row + j) * stride + n] = from_float<T>(acc[j]);
+            }
+        }
+        if constexpr (SPLIT) {
+            cluster_sync();
+            if (threadIdx.x < 128 && fine && col + threadIdx.x < cols)
+                for (int j = slice; j < NB; j += slices)
+                    if (row + j >= from && row + j < to) {
+                        float sum = 0.f;
+                        for (int r = 0; r < slices; ++r) sum += load_remote(&sh.part[j][threadIdx.x], r);
+                        y[(row + j) * stride + col + threadIdx.x] = from_float<T>(sum);
+                    }
+            cluster_sync();  // the parts have been read, also those of a CTA that ends here
+        }
+    }
+    if (offsets && warp < 4) {  // rows of no group
+        const int64_t lo = min(max((int64_t)ld_late(offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(offsets + groups), lo), rows);
+        const int64_t cta = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, ctas = (int64_t)gridDim.x * gridDim.y;
+        auto clear = [&](int64_t begin, int64_t end) {
+            for (int64_t r = begin + cta; r < end; r += ctas)
+                for (int64_t c = threadIdx.x; c < cols; c += 128) y[r * stride + c] = from_float<T>(0.f);
+        };
+        clear(0, lo);
+        clear(hi, rows);
+    }
+    if (!fine && warp == 5)
+        for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1, 1 << 16);
+    if (!fine && warp == 4) {
+        if (elected()) mma_commit<false>(&sh.drained);
+        __syncwarp();
+        mbar_wait_bounded(&sh.drained, 0, 1 << 16);
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tmem_fence_after();
+        tmem_free<false>(tmem, S::COLUMNS);
+        if (lane == 0 && *failed) publish_result_word(report, 1, blockIdx.x);
+    }
+}
+
 // ---- operands of the gradient ------------------------------------------------------------
 
 // Blocks of 128 rows, counted from each group's first: where a group's blocks begin, and every block's rows {first, how many}. One CTA.
@@ -497,6 +658,31 @@ int report_of(cudaStream_t stream, Workspace **ws) {
     return note_timeout(3, (int)(said & RW_VALUE_MASK), "an earlier 8-bit product");
 }
 
+// Slices of the summed axis, CTAs of a cluster, for `tiles` CTAs' worth of work: as many as fill the SMs, eight at most, of four blocks at least.
+int slices_of(int64_t tiles, int64_t blocks) {
+    int s = 1;
+    while (s < 8 && tiles * s < 2 * sm_count() && blocks >= 8 * s) s *= 2;
+    return s;
+}
+
+template <typename T, int NB>
+int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int groups, const nb200_dense &y, cudaStream_t stream) {
+    Workspace *ws = nullptr;
+    int st;
+    if ((st = report_of(stream, &ws))) return st;
+    unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
+    const int64_t wide = blocks_of(y.cols);
+    const int slices = slices_of(wide * std::min<int64_t>(groups, y.rows), a.blocks);
+    if (wide * slices > INT32_MAX) return NB200_E_UNSUPPORTED;
+    auto kernel = slices > 1 ? k_product_few<T, NB, true> : k_product_few<T, NB, false>;
+    const size_t smem = slices > 1 ? FewShape<NB, true>::SHARED_BYTES : FewShape<NB, false>::SHARED_BYTES;
+    NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    LaunchScope scope("fp8_product_few", stream);
+    NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)(wide * slices), (unsigned)groups), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
+                                          static_cast<T *>(y.data), y.stride, report));
+    return NB200_OK;
+}
+
 // `tiles` of the shape that `pair` selects, at most.
 template <typename T, bool GRAD>
 int launch_product(const char *name, bool pair, int64_t tiles, const Operand &a, const Operand &w, const int32_t *offsets, int groups, const nb200_dense &y, cudaStream_t stream) {
@@ -575,7 +761,13 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     // tiles at most: a group may begin and end inside tiles
     const bool pair = y->rows >= (int64_t)w->groups * 192;
     const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * (int64_t)w->groups) * ((y->cols + side - 1) / side);
-    return with_type(y->type, [&](auto e) { return launch_product<decltype(e), false>("fp8_product", pair, tiles, oa, ow, offsets, w->groups, *y, stream); });
+    return with_type(y->type, [&](auto e) {
+        using T = decltype(e);
+        if (y->rows <= 6 * (int64_t)w->groups) return launch_few<T, 16>(oa, ow, offsets, w->groups, *y, stream);
+        if (y->rows <= 16 * (int64_t)w->groups) return launch_few<T, 32>(oa, ow, offsets, w->groups, *y, stream);
+        if (y->rows <= 64 * (int64_t)w->groups) return launch_few<T, 64>(oa, ow, offsets, w->groups, *y, stream);
+        return launch_product<T, false>("fp8_product", pair, tiles, oa, ow, offsets, w->groups, *y, stream);
+    });
 }
 
 int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dense *x, int32_t groups) {
