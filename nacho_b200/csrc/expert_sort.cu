@@ -37,8 +37,8 @@ struct Order {
 
 constexpr int MAX_TILES = 256;
 
-// How often each key occurs in this CTA's tile of entries: counts[key][tile].
-__global__ void __launch_bounds__(NT) k_order_count(Order o, int tile, int tiles, int32_t *counts) {
+// How often each key occurs in this CTA's tile of entries: counts[tile][key].
+__global__ void __launch_bounds__(NT) k_order_count(Order o, int tile, int32_t *counts) {
     extern __shared__ int32_t hist[];
     wait_for_previous();
     trigger_dependents();
@@ -51,15 +51,15 @@ __global__ void __launch_bounds__(NT) k_order_count(Order o, int tile, int tiles
         if (k < o.experts) atomicAdd(&hist[k], 1);
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < o.experts; k += NT) counts[(int64_t)k * tiles + blockIdx.x] = hist[k];
+    for (int k = threadIdx.x; k < o.experts; k += NT) counts[(int64_t)blockIdx.x * o.experts + k] = hist[k];
 }
 
 // Slots of a tile's entries. Every warp has a stretch of the tile and a counter per expert, which starts at the slots in front of its stretch:
 // those of all smaller experts, of this expert's entries in the tiles before, and of the warps before.
 __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles, const int32_t *counts) {
-    extern __shared__ int32_t next[];  // [warp][expert], then the experts' totals
+    extern __shared__ int32_t next[];  // [warp][expert], then the experts' totals and their entries in the tiles before
     __shared__ int tmp[33];
-    int32_t *total = next + (NT / 32) * o.experts;
+    int32_t *total = next + (NT / 32) * o.experts, *before = total + o.experts;
     wait_for_previous();
     trigger_dependents();
     const int w = warp_id(), lane = lane_id();
@@ -74,25 +74,21 @@ __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles
         const int k = key_of(e);
         if (k < o.experts) atomicAdd(&mine[k], 1);
     }
-    // this expert's entries in all tiles and in the tiles before, a warp per expert
+    // an expert's entries in all tiles and in the tiles before, all threads over all counts, eight of them on their way at a time
+    for (int k = threadIdx.x; k < 2 * o.experts; k += NT) total[k] = 0;
     __syncthreads();
-    for (int k = w; k < o.experts; k += NT / 32) {
-        int all = 0, before = 0;
-        for (int j = lane; j < tiles; j += 32) {
-            const int c = ld_late(counts + (int64_t)k * tiles + j);
-            all += c;
-            before += j < (int)blockIdx.x ? c : 0;
-        }
-        all = __reduce_add_sync(FULL_MASK, all);
-        before = __reduce_add_sync(FULL_MASK, before);
-        if (lane == 0) {
-            total[k] = all;
-            for (int v = 0; v < NT / 32; ++v) {
-                const int c = next[v * o.experts + k];
-                next[v * o.experts + k] = before;
-                before += c;
+    const int64_t all = (int64_t)tiles * o.experts, mine_too = (int64_t)blockIdx.x * o.experts;
+    for (int64_t i0 = threadIdx.x; i0 < all; i0 += 8 * NT) {
+        int c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c[u] = i0 + u * NT < all ? ld_late(counts + i0 + u * NT) : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (c[u]) {
+                const int k = (int)((i0 + u * NT) % o.experts);
+                atomicAdd(&total[k], c[u]);
+                if (i0 + u * NT < mine_too) atomicAdd(&before[k], c[u]);
             }
-        }
     }
     __syncthreads();
     int base = 0;
@@ -102,7 +98,12 @@ __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles
         const int at = base + block_excl_sum<NT>(k < o.experts ? total[k] : 0, tmp, sum);
         if (k < o.experts) {
             if (blockIdx.x == 0) o.offsets[k] = at;
-            for (int v = 0; v < NT / 32; ++v) next[v * o.experts + k] += at;
+            int from = at + before[k];
+            for (int v = 0; v < NT / 32; ++v) {
+                const int c = next[v * o.experts + k];
+                next[v * o.experts + k] = from;
+                from += c;
+            }
         }
         base += sum;
     }
@@ -157,8 +158,8 @@ __device__ __forceinline__ void copy_rows(const Order &o, const Team &team, int 
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void clear_rows(const Order &o, const Team &team, int64_t cols, T *xs) {
-    for (int s = o.kept() + team.first; s < o.entries; s += team.step) {
+__device__ __forceinline__ void clear_rows(const Order &o, int kept, const Team &team, int64_t cols, T *xs) {
+    for (int s = kept + team.first; s < o.entries; s += team.step) {
         if (o.rows && team.lane == 0) o.rows[s] = -1;
         for (int64_t c = team.lane * V; c < cols; c += team.size * V) {
             Vec<T, V> zero;
@@ -175,7 +176,19 @@ __global__ void __launch_bounds__(NT) k_sort_rows(Order o, int tpr, const T *x, 
     trigger_dependents();
     const Team team(tpr);
     for (int t = team.first; t < o.tokens; t += team.step) copy_rows<T, V>(o, team, t, x, stride, cols, xs);
-    clear_rows<T, V>(o, team, cols, xs);
+    clear_rows<T, V>(o, o.kept(), team, cols, xs);
+}
+
+__device__ __forceinline__ void clear_rows8(const Order &o, int kept, const Team &team, int64_t kb, uint8_t *codes, float *scales) {
+    const int sub = team.lane & 15;
+    const int64_t pad = padded_rows(o.entries);
+    for (int s = kept + team.first; s < o.entries; s += team.step) {
+        if (team.lane == 0) o.rows[s] = -1;
+        for (int64_t b = team.lane >> 4; b < kb; b += team.size >> 4) {
+            *reinterpret_cast<uint2 *>(codes + b * pad * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = make_uint2(0, 0);
+            if (sub == 0) scales[b * pad + s] = 0.f;
+        }
+    }
 }
 
 // The entries of the tokens a team works on, asked for early: row offsets two tokens ahead, the slots (and weights) of up to N entries one
@@ -273,13 +286,7 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
         }
         if (mine >= kb) at.ask_next();
     }
-    for (int s = o.kept() + team.first; s < o.entries; s += team.step) {
-        if (team.lane == 0) o.rows[s] = -1;
-        for (int64_t b = mine; b < kb; b += blocks) {
-            *reinterpret_cast<uint2 *>(codes + b * pad * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = make_uint2(0, 0);
-            if (sub == 0) scales[b * pad + s] = 0.f;
-        }
-    }
+    clear_rows8(o, o.kept(), team, kb, codes, scales);
 }
 
 // y[t] = sum of w[e] * z[slot(e)]. The rows of up to N entries are on their way together.
@@ -394,11 +401,114 @@ __global__ void __launch_bounds__(NT, N == 8 ? 2 : 3) k_unsort_grad(Order o, int
     }
     Order tail = o;
     tail.rows = nullptr;
-    clear_rows<T, V>(tail, team, cols, dz);
+    clear_rows<T, V>(tail, o.kept(), team, cols, dz);
     // entries of no row: views into larger arrays
     const int lo = o.entry_of(0), hi = o.entry_of(o.tokens);
     for (int e = blockIdx.x * NT + threadIdx.x; e < o.entries; e += gridDim.x * NT)
         if (e < lo || e >= hi) dw[e] = 0.f;
+}
+
+// ---- few entries: all in one launch ------------------------------------------------------
+
+// Up to this many entries, every CTA counts all of them: that takes less than a launch. Its own tokens' entries follow from the totals and
+// from the counts of those in front of them. 4096 entries, 1024 tokens of 2048: 8.3 us where two launches for the order in front take 14.7.
+constexpr int FEW_ENTRIES = 4096;
+
+// Slots of the entries of tokens t0 .. t1 - 1, the offsets, and how many entries are kept (returned). counts: two words per expert.
+__device__ int place_few(const Order &o, int t0, int t1, int32_t *counts) {
+    __shared__ int tmp[33];
+    int32_t *total = counts, *next = counts + o.experts;
+    const int lane = lane_id();
+    const int lo = o.entry_of(0), hi = o.entry_of(o.tokens), e0 = o.entry_of(t0), e1 = o.entry_of(t1);
+    for (int k = threadIdx.x; k < 2 * o.experts; k += NT) counts[k] = 0;
+    __syncthreads();
+    for (int e = lo + (int)threadIdx.x; e - lane < hi; e += NT) {
+        const int k = e < hi ? o.key(e) : o.experts;
+        const unsigned same = __match_any_sync(FULL_MASK, k);
+        const unsigned before = __ballot_sync(FULL_MASK, e < e0);
+        if (k < o.experts && (same & ((1u << lane) - 1)) == 0) {
+            atomicAdd(&total[k], __popc(same));
+            if (same & before) atomicAdd(&next[k], __popc(same & before));
+        }
+    }
+    __syncthreads();
+    int kept = 0;
+    for (int k0 = 0; k0 < o.experts; k0 += NT) {
+        const int k = k0 + threadIdx.x;
+        int sum;
+        const int at = kept + block_excl_sum<NT>(k < o.experts ? total[k] : 0, tmp, sum);
+        if (k < o.experts) {
+            next[k] += at;
+            if (blockIdx.x == 0) o.offsets[k] = at;
+        }
+        kept += sum;
+    }
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) o.offsets[o.experts] = kept;
+        for (int e = threadIdx.x; e < o.entries; e += NT)
+            if (e < lo || e >= hi) o.slots[e] = -1;  // entries of no row
+    }
+    __syncthreads();
+    if (warp_id() == 0)
+        for (int e = e0 + lane; e - lane < e1; e += 32) {
+            const int k = e < e1 ? o.key(e) : o.experts;
+            const unsigned same = __match_any_sync(FULL_MASK, k);
+            const int rank = __popc(same & ((1u << lane) - 1));
+            const int slot = k < o.experts ? next[k] + rank : -1;
+            __syncwarp();
+            if (k < o.experts && rank == 0) next[k] += __popc(same);
+            __syncwarp();
+            if (e < e1) o.slots[e] = slot;
+        }
+    __syncthreads();
+    return kept;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(NT) k_sort_few(Order o, int per_cta, int tpr, const T *x, int64_t stride, int64_t cols, T *xs) {
+    extern __shared__ int32_t counts[];
+    wait_for_previous();
+    trigger_dependents();
+    const int t0 = min((int)blockIdx.x * per_cta, o.tokens), t1 = min(t0 + per_cta, o.tokens);
+    const int kept = place_few(o, t0, t1, counts);
+    Team team(tpr);
+    for (int t = t0 + (int)threadIdx.x / tpr; t < t1; t += NT / tpr) copy_rows<T, V>(o, team, t, x, stride, cols, xs);
+    clear_rows<T, V>(o, kept, team, cols, xs);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(NT) k_sort_few_fp8(Order o, int per_cta, int tpr, const T *x, int64_t stride, int64_t cols, uint8_t *codes, float *scales) {
+    extern __shared__ int32_t counts[];
+    wait_for_previous();
+    trigger_dependents();
+    const int t0 = min((int)blockIdx.x * per_cta, o.tokens), t1 = min(t0 + per_cta, o.tokens);
+    const int kept = place_few(o, t0, t1, counts);
+    const Team team(tpr);
+    const int sub = team.lane & 15;
+    const unsigned half = 0xffffu << (threadIdx.x & 16);
+    const int64_t pad = padded_rows(o.entries), kb = blocks_of(cols);
+    for (int t = t0 + (int)threadIdx.x / tpr; t < t1; t += NT / tpr) {
+        const int e0 = o.entry_of(t), e1 = o.entry_of(t + 1);
+        for (int e = e0 + team.lane; e < e1; e += tpr) {
+            const int s = o.slot(e);
+            if (s >= 0) o.rows[s] = t;
+        }
+        for (int64_t b = team.lane >> 4; b < kb; b += team.size >> 4) {
+            const Vec<T, 8> v = load8<T, V>(x + t * stride, b * BLOCK8 + sub * 8, cols);
+            uint32_t m = magnitude8(v);
+#pragma unroll
+            for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(half, m, d));
+            const Factors f = factors_of(m);
+            const uint2 q = codes8(v, f.inverse);
+            for (int e = e0; e < e1; ++e) {
+                const int s = o.slot(e);
+                if (s < 0) continue;
+                *reinterpret_cast<uint2 *>(codes + b * pad * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = q;
+                if (sub == 0) scales[b * pad + s] = f.scale;
+            }
+        }
+    }
+    clear_rows8(o, kept, team, kb, codes, scales);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -444,6 +554,19 @@ int check_routing(const nb200_csr *r, nb200_expert_order *order) {
     return check_order(order, false);
 }
 
+// The launch for few entries: two CTAs to an SM at most, since each counts all entries.
+struct Few {
+    int per_cta;
+    dim3 grid;
+    size_t smem;
+    Few(const Order &o, int tpr) {
+        const int teams = NT / tpr, most = 2 * sm_count();
+        per_cta = std::max(teams, (o.tokens + most - 1) / most);
+        grid = dim3((unsigned)std::max(1, (o.tokens + per_cta - 1) / per_cta));
+        smem = sizeof(int32_t) * 2 * o.experts;
+    }
+};
+
 int make_order(const Order &o, cudaStream_t stream) {
     int tile = 2048;  // a multiple of the warps' 32 each
     while ((o.entries + (int64_t)tile - 1) / tile > MAX_TILES) tile *= 2;
@@ -452,11 +575,11 @@ int make_order(const Order &o, cudaStream_t stream) {
     int st;
     if ((st = acquire_workspace(stream, sizeof(int32_t) * (size_t)tiles * std::max(o.experts, 1), &ws, ORDER_SLOT))) return st;
     int32_t *counts = static_cast<int32_t *>(ws->dev);
-    const size_t count_smem = sizeof(int32_t) * o.experts, place_smem = sizeof(int32_t) * o.experts * (NT / 32 + 1);
+    const size_t count_smem = sizeof(int32_t) * o.experts, place_smem = sizeof(int32_t) * o.experts * (NT / 32 + 2);
     if (place_smem > 48 * 1024) NB200_CUDA(cudaFuncSetAttribute(k_order_place, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem));
     {
         LaunchScope scope("order_count", stream);
-        NB200_CUDA(launch_overlapped(k_order_count, dim3(tiles), dim3(NT), count_smem, stream, o, tile, tiles, counts));
+        NB200_CUDA(launch_overlapped(k_order_count, dim3(tiles), dim3(NT), count_smem, stream, o, tile, counts));
     }
     LaunchScope scope("order_place", stream);
     NB200_CUDA(launch_overlapped(k_order_place, dim3(tiles), dim3(NT), place_smem, stream, o, tile, tiles, counts));
@@ -477,13 +600,20 @@ int nb200_expert_sort(const nb200_csr *r, const nb200_dense *x, nb200_expert_ord
         return NB200_E_BADARG;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, r->col);
-    if ((st = make_order(o, stream))) return st;
     const nb200_dense none{r->rows, 0, 0, NB200_F32, nullptr};
     if (!x) x = &none, xs = const_cast<nb200_dense *>(&none);
+    if (o.entries > FEW_ENTRIES && (st = make_order(o, stream))) return st;
     const int word = word_bytes({x, xs}), tpr = team_of((x->cols * type_size(x->type) + 15) / 16 / 4);
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
+            if (o.entries <= FEW_ENTRIES) {
+                const Few few(o, tpr);
+                LaunchScope scope("sort_few", stream);
+                NB200_CUDA(launch_overlapped(k_sort_few<T, decltype(v)::value>, few.grid, dim3(NT), few.smem, stream, o, few.per_cta, tpr, static_cast<const T *>(x->data),
+                                             x->stride, x->cols, static_cast<T *>(xs->data)));
+                return (int)NB200_OK;
+            }
             LaunchScope scope("sort_rows", stream);
             NB200_CUDA(launch_overlapped(k_sort_rows<T, decltype(v)::value>, grid_of(o.tokens, tpr), dim3(NT), 0, stream, o, tpr, static_cast<const T *>(x->data), x->stride, x->cols,
                                          static_cast<T *>(xs->data)));
@@ -498,11 +628,19 @@ int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert
     if (!dense_ok(x) || !fp8_ok(xs) || x->rows != r->rows || xs->groups != 1 || xs->tiled || xs->rows != r->nnz || xs->cols != x->cols) return NB200_E_BADARG;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, r->col);
-    if ((st = make_order(o, stream))) return st;
-    const int word = word_bytes({x}), tpr = team_of(blocks_of(x->cols) * 8);
+    const bool all_in_one = o.entries <= FEW_ENTRIES;
+    if (!all_in_one && (st = make_order(o, stream))) return st;
+    const int word = word_bytes({x}), tpr = team_of(blocks_of(x->cols) * (all_in_one ? 16 : 8));
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
+            if (all_in_one) {
+                const Few few(o, tpr);
+                LaunchScope scope("sort_few_fp8", stream);
+                NB200_CUDA(launch_overlapped(k_sort_few_fp8<T, decltype(v)::value>, few.grid, dim3(NT), few.smem, stream, o, few.per_cta, tpr, static_cast<const T *>(x->data),
+                                             x->stride, x->cols, xs->values, xs->scales));
+                return (int)NB200_OK;
+            }
             auto kernel = k_sort_rows_fp8<T, decltype(v)::value>;
             LaunchScope scope("sort_rows_fp8", stream);
             NB200_CUDA(launch_overlapped(kernel, resident_grid(kernel, o.tokens, tpr), dim3(NT), 0, stream, o, tpr, static_cast<const T *>(x->data), x->stride, x->cols, xs->values,

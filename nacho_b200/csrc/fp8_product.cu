@@ -72,35 +72,33 @@ struct Ring {
 
 // A tile of the result: its group, first row (a multiple of 8) and column, the rows that count, and the blocks that are summed.
 struct Tile {
-    int g;
-    int64_t row, from, to, col;
+    int g, row, from, to, col;
     int first_block, blocks;
 };
 
 // The order of the tiles of `high` x `wide`: panels of rows, column by column.
 template <int PANEL>
-__device__ __forceinline__ void place_tile(int64_t within, int64_t high, int64_t wide, int64_t *row, int64_t *col) {
-    const int64_t panel = within / (PANEL * wide), width = min((int64_t)PANEL, high - panel * PANEL), rest = within - panel * PANEL * wide;
-    *row = panel * PANEL + rest % width;
-    *col = rest / width;
+__device__ __forceinline__ void place_tile(int within, int high, int wide, int *row, int *col) {
+    const unsigned panel = (unsigned)within / (unsigned)(PANEL * wide), width = min((unsigned)PANEL, (unsigned)high - panel * PANEL);
+    const unsigned rest = (unsigned)within - panel * PANEL * wide, column = rest / width;
+    *row = (int)(panel * PANEL + rest - column * width);
+    *col = (int)column;
 }
 
 // Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order.
 template <int BM, int BN, int PANEL>
 struct Walk {
     const int32_t *offsets;
-    int groups, blocks;
-    int64_t rows, col_tiles;
-    int chunk = -32;
-    int64_t base = 0, incl = 0;  // tiles of the groups before this chunk; of this chunk's groups up to the lane's
-    int64_t from = 0, to = 0;
+    int groups, blocks, rows, col_tiles;
+    int chunk = -32, base = 0, incl = 0;  // tiles of the groups before this chunk; of this chunk's groups up to the lane's
+    int from = 0, to = 0;
 
-    __device__ Walk(const int32_t *o, int g, int b, int64_t r, int64_t c) : offsets(o), groups(g), blocks(b), rows(r), col_tiles((c + BN - 1) / BN) {}
+    __device__ Walk(const int32_t *o, int g, int b, int r, int c) : offsets(o), groups(g), blocks(b), rows(r), col_tiles((c + BN - 1) / BN) {}
 
-    __device__ static int64_t row_tiles(int64_t from, int64_t to) { return to > from ? (to - (from & ~int64_t(7)) + BM - 1) / BM : 0; }
+    __device__ static int row_tiles(int from, int to) { return to > from ? (to - (from & ~7) + BM - 1) / BM : 0; }
 
-    __device__ bool find(int64_t tile, Tile &t) {
-        int64_t total;
+    __device__ bool find(int tile, Tile &t) {
+        int total;
         while (total = __shfl_sync(FULL_MASK, incl, 31), tile >= base + total) {
             base += total;
             chunk += 32;
@@ -108,24 +106,18 @@ struct Walk {
             const int g = chunk + lane_id();
             from = to = 0;
             if (g < groups) {
-                from = offsets ? min(max((int64_t)ld_late(offsets + g), (int64_t)0), rows) : 0;
-                to = offsets ? min(max((int64_t)ld_late(offsets + g + 1), from), rows) : rows;
+                from = offsets ? min(max(ld_late(offsets + g), 0), rows) : 0;
+                to = offsets ? min(max(ld_late(offsets + g + 1), from), rows) : rows;
             }
-            incl = row_tiles(from, to) * col_tiles;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(FULL_MASK, incl, o);
-                if (lane_id() >= o) incl += v;
-            }
+            incl = warp_incl_sum(row_tiles(from, to) * col_tiles);
         }
         const int src = __ffs(__ballot_sync(FULL_MASK, base + incl > tile)) - 1;
         t.g = chunk + src;
         t.from = __shfl_sync(FULL_MASK, from, src);
         t.to = __shfl_sync(FULL_MASK, to, src);
-        const int64_t high = row_tiles(t.from, t.to);
-        const int64_t within = tile - base - (__shfl_sync(FULL_MASK, incl, src) - high * col_tiles);
-        place_tile<PANEL>(within, high, col_tiles, &t.row, &t.col);
-        t.row = (t.from & ~int64_t(7)) + t.row * BM;
+        const int high = row_tiles(t.from, t.to);
+        place_tile<PANEL>(tile - base - (__shfl_sync(FULL_MASK, incl, src) - high * col_tiles), high, col_tiles, &t.row, &t.col);
+        t.row = (t.from & ~7) + t.row * BM;
         t.col *= BN;
         t.first_block = 0, t.blocks = blocks;
         return true;
@@ -136,13 +128,12 @@ struct Walk {
 template <int BM, int BN, int PANEL>
 struct GradWalk {
     const int32_t *first_block;
-    int groups;
-    int64_t rows, cols;
+    int groups, rows, cols;
 
-    __device__ bool find(int64_t tile, Tile &t) {
-        const int64_t high = (rows + BM - 1) / BM, wide = (cols + BN - 1) / BN;
-        t.g = (int)min(tile / (high * wide), (int64_t)groups);
-        if (t.g == groups) return false;
+    __device__ bool find(int tile, Tile &t) {
+        const int high = (rows + BM - 1) / BM, wide = (cols + BN - 1) / BN;
+        t.g = (int)((unsigned)tile / (unsigned)(high * wide));
+        if (t.g >= groups) return false;
         place_tile<PANEL>(tile - t.g * high * wide, high, wide, &t.row, &t.col);
         t.row *= BM, t.col *= BN, t.from = 0, t.to = rows;
         t.first_block = ld_late(first_block + t.g);
@@ -232,10 +223,10 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
     trigger_dependents();
     wait_for_previous();
 
-    const int64_t first = blockIdx.x / S::CTAS, step = gridDim.x / S::CTAS;
+    const int first = blockIdx.x / S::CTAS, step = gridDim.x / S::CTAS;
     auto tiles = [&] {
-        if constexpr (GRAD) return GradWalk<S::BM, BN, S::PANEL>{offsets, groups, rows, cols};
-        else return Walk<S::BM, BN, S::PANEL>(offsets, groups, (int)a.blocks, rows, cols);
+        if constexpr (GRAD) return GradWalk<S::BM, BN, S::PANEL>{offsets, groups, (int)rows, (int)cols};
+        else return Walk<S::BM, BN, S::PANEL>(offsets, groups, (int)a.blocks, (int)rows, (int)cols);
     };
     if (warp < STORE_WARPS) {
         // sums and stores: warps w and w + 4 have the lanes of tensor memory that every fourth warp can reach, and a half of the columns each
@@ -246,7 +237,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
         Ring<SUMS> sums;
         Ring<S::SCALES> place;
         const uint32_t base = tmem + ((uint32_t)(lanes * 32) << 16) + half * N;
-        for (int64_t tile = first; walk.find(tile, t); tile += step) {
+        for (int tile = first; walk.find(tile, t); tile += step) {
             float acc[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] = 0.f;
@@ -316,7 +307,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
         Ring<S::SCALES> place;
         bool fine = true;
         if (warp == STORE_WARPS + 1) {  // copies
-            for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
+            for (int tile = first; fine && walk.find(tile, t); tile += step) {
                 const int64_t row = t.row + rank * S::A_ROWS, col = t.col + rank * S::B_ROWS;
                 const uint32_t a_bytes = (uint32_t)min((int64_t)S::A_ROWS, max(a.pad - row, (int64_t)0)) * BLOCK8;
                 const uint32_t b_bytes = (uint32_t)min((int64_t)S::B_ROWS, max(w.pad - col, (int64_t)0)) * BLOCK8;
@@ -344,7 +335,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
         } else if (warp == STORE_WARPS && rank == 0) {  // matrix instructions
             const uint64_t tile_a = tile_descriptor(smem_u32(sh.a[0])), tile_b = tile_descriptor(smem_u32(sh.b[0]));
             Ring<SUMS> sums;
-            for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
+            for (int tile = first; fine && walk.find(tile, t); tile += step) {
                 for (int b = 0; b < t.blocks; ++b, stage.next(), sums.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
@@ -365,7 +356,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 mbar_wait_bounded(&sh.drained, 0, 1 << 16);
             }
         } else if (PAIR && warp == STORE_WARPS) {  // tells the leader of the copies that have landed here
-            for (int64_t tile = first; fine && walk.find(tile, t); tile += step) {
+            for (int tile = first; fine && walk.find(tile, t); tile += step) {
                 for (int b = 0; b < t.blocks; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     if (elected()) mbar_arrive_leader(&sh.full[stage.at]);
@@ -397,10 +388,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_produc
 
 // ---- few rows per group ------------------------------------------------------------------
 
-// The operands change sides: 128 rows of weights against NB rows, 16 to 64, of a group, so that a CTA brings hardly more than the weights, which is all
-// that such a product takes: one CTA per group and 128 columns of the result, several to an SM. Where there are not enough of them, the CTAs of
-// a cluster have a part of the blocks each (SPLIT) and add their sums, in order, through one another's shared memory. A group of more than NB rows
-// takes several turns over its weights.
+// The operands change sides: 128 rows of weights against NB rows, 16 to 128, of a group, so that a CTA brings hardly more than the weights, which is
+// all that a product of few rows takes: one CTA per group and 128 columns of the result, several to an SM. Where there are not enough of them, the
+// CTAs of a cluster have a part of the blocks each (SPLIT) and add their sums, in order, through one another's shared memory. A group of more rows
+// than NB (than NB times the grid's third extent) takes several turns over its weights.
 template <int NB, bool SPLIT>
 struct FewShape {
     static constexpr int STAGES = 4, SUMS = 4, SCALES = STAGES + SUMS, COLUMNS = SUMS * NB;  // of tensor memory
@@ -418,7 +409,7 @@ struct FewShape {
 constexpr int FEW_THREADS = 6 * 32;
 
 template <typename T, int NB, bool SPLIT>
-__global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : 2) k_product_few(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
+__global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : NB == 128 ? 1 : 2) k_product_few(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                                              unsigned long long *report) {
     using S = FewShape<NB, SPLIT>;
     constexpr int STAGES = S::STAGES, SUMS = S::SUMS, W = NB < 32 ? 16 : 32;
@@ -451,7 +442,7 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : 2) k_product_few(O
     Ring<SUMS> sums;
     Ring<S::SCALES> place;
     bool fine = true;
-    for (int64_t row = from & ~int64_t(7); row < to; row += NB) {
+    for (int64_t row = (from & ~int64_t(7)) + (int64_t)blockIdx.z * NB; row < to; row += (int64_t)gridDim.z * NB) {
         if (warp == 5) {  // copies
             const uint32_t a_bytes = (uint32_t)min((int64_t)NB, a.pad - row) * BLOCK8, w_bytes = (uint32_t)min((int64_t)128, w.pad - col) * BLOCK8;
             const uint32_t scale_bytes = a_bytes / BLOCK8 * sizeof(float);
@@ -494,19 +485,25 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : 2) k_product_few(O
                 const float s = __shfl_sync(FULL_MASK, tile_scale, b % 32);
                 if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
                 tmem_fence_after();
+                const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + sums.at * NB;
                 uint32_t v[NB / W][W];
+                tmem_load(at, v[0]);
 #pragma unroll
-                for (int q = 0; q < NB / W; ++q) tmem_load(tmem + ((uint32_t)(warp * 32) << 16) + sums.at * NB + q * W, v[q]);
+                for (int q = 0; q < NB / W; ++q) {
+                    float row_scale[W];
 #pragma unroll
-                for (int q = 0; q < NB / W; ++q) tmem_wait_loads(v[q]);
-                float row_scale[NB];
+                    for (int j = 0; j < W; j += 4) *reinterpret_cast<float4 *>(row_scale + j) = *reinterpret_cast<const float4 *>(&sh.scale[place.at][q * W + j]);
+                    tmem_wait_loads(v[q]);
+                    if (q + 1 < NB / W) {
+                        tmem_load(at + (q + 1) * W, v[q + 1]);
+                    } else {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.sum_empty[sums.at]);
+                    }
 #pragma unroll
-                for (int j = 0; j < NB; j += 4) *reinterpret_cast<float4 *>(row_scale + j) = *reinterpret_cast<const float4 *>(&sh.scale[place.at][j]);
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.sum_empty[sums.at]);
-#pragma unroll
-                for (int j = 0; j < NB; ++j) acc[j] = __fmaf_rn(__uint_as_float(v[j / W][j % W]), s * row_scale[j], acc[j]);
+                    for (int j = 0; j < W; ++j) acc[q * W + j] = __fmaf_rn(__uint_as_float(v[q][j]), s * row_scale[j], acc[q * W + j]);
+                }
             }
             const int64_t n = col + threadIdx.x;
             if constexpr (SPLIT) {
@@ -520,19 +517,23 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : 2) k_product_few(O
         }
         if constexpr (SPLIT) {
             cluster_sync();
+            // Eight loads of the others' parts are on their way at a time: one by one they took longer than the product.
             if (threadIdx.x < 128 && fine && col + threadIdx.x < cols)
-                for (int j = slice; j < NB; j += slices)
-                    if (row + j >= from && row + j < to) {
-                        float sum = 0.f;
-                        for (int r = 0; r < slices; ++r) sum += load_remote(&sh.part[j][threadIdx.x], r);
-                        y[(row + j) * stride + col + threadIdx.x] = from_float<T>(sum);
-                    }
+                for (int j = slice; j < NB; j += slices) {
+                    if (row + j < from || row + j >= to) continue;
+                    float part[8], sum = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) part[r] = r < slices ? load_remote(&sh.part[j][threadIdx.x], r) : 0.f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) sum += part[r];
+                    y[(row + j) * stride + col + threadIdx.x] = from_float<T>(sum);
+                }
             cluster_sync();  // the parts have been read, also those of a CTA that ends here
         }
     }
     if (offsets && warp < 4) {  // rows of no group
         const int64_t lo = min(max((int64_t)ld_late(offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(offsets + groups), lo), rows);
-        const int64_t cta = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, ctas = (int64_t)gridDim.x * gridDim.y;
+        const int64_t cta = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, ctas = (int64_t)gridDim.x * gridDim.y * gridDim.z;
         auto clear = [&](int64_t begin, int64_t end) {
             for (int64_t r = begin + cta; r < end; r += ctas)
                 for (int64_t c = threadIdx.x; c < cols; c += 128) y[r * stride + c] = from_float<T>(0.f);
@@ -658,10 +659,11 @@ int report_of(cudaStream_t stream, Workspace **ws) {
     return note_timeout(3, (int)(said & RW_VALUE_MASK), "an earlier 8-bit product");
 }
 
-// Slices of the summed axis, CTAs of a cluster, for `tiles` CTAs' worth of work: as many as fill the SMs, eight at most, of four blocks at least.
-int slices_of(int64_t tiles, int64_t blocks) {
+// Slices of the summed axis, CTAs of a cluster, for `tiles` CTAs' worth of work: more while the SMs are not all busy (where one CTA fills an SM: while
+// they would not be more than the SMs), eight at most, of four blocks at least. 256 tiles of 8 blocks take 17 us in two slices each, 13 in one.
+int slices_of(int64_t tiles, int64_t blocks, bool one_per_sm) {
     int s = 1;
-    while (s < 8 && tiles * s < 2 * sm_count() && blocks >= 8 * s) s *= 2;
+    while (s < 8 && (one_per_sm ? 2 : 1) * tiles * s < sm_count() && blocks >= 8 * s) s *= 2;
     return s;
 }
 
@@ -672,13 +674,14 @@ int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int g
     if ((st = report_of(stream, &ws))) return st;
     unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
     const int64_t wide = blocks_of(y.cols);
-    const int slices = slices_of(wide * std::min<int64_t>(groups, y.rows), a.blocks);
-    if (wide * slices > INT32_MAX) return NB200_E_UNSUPPORTED;
+    const int64_t turns = groups == 1 ? (y.rows + NB - 1) / NB : 1;
+    const int slices = slices_of(wide * std::min<int64_t>(groups, y.rows) * turns, a.blocks, NB >= 64);
+    if (wide * slices > INT32_MAX || turns > 65535) return NB200_E_UNSUPPORTED;
     auto kernel = slices > 1 ? k_product_few<T, NB, true> : k_product_few<T, NB, false>;
     const size_t smem = slices > 1 ? FewShape<NB, true>::SHARED_BYTES : FewShape<NB, false>::SHARED_BYTES;
     NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     LaunchScope scope("fp8_product_few", stream);
-    NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)(wide * slices), (unsigned)groups), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
+    NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)(wide * slices), (unsigned)groups, (unsigned)turns), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
                                           static_cast<T *>(y.data), y.stride, report));
     return NB200_OK;
 }
@@ -758,14 +761,24 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), 0};
     const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows)};
+    // Which kernel, by the rows of a group and the work there is (us on a B200, n x inner):
+    //   - few rows: with groups while NB rows are three times the mean, so that hardly a group takes two turns (32 groups of 2048 x 2048: 28 against
+    //     34 with 16 rows each, 35 against 34 with 24); one group up to 32 rows (4096 x 4096: 7 to 8 against 17), and where the sums are long enough
+    //     to be worth sharing, up to 64 (4096 x 4096: 12 against 17; 1024 x 2048: 10 either way; 2048 x 1024: 13 against 7) and beyond, while
+    //     tiles leave half of the SMs idle (128 rows, 1024 x 8192: 13 against 30; 4096 x 4096: 17 either way);
+    //   - pairs of CTAs from where single ones have a second tile (4096 x 4096, 512 rows: 19 against 18; 768 rows: 20 against 31) and groups fill
+    //     most of 128 rows (32 groups of 2048 x 2048 with 96 rows: 41 against 36, with 128 rows: 42 against 50).
     // tiles at most: a group may begin and end inside tiles
-    const bool pair = y->rows >= (int64_t)w->groups * 192;
-    const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * (int64_t)w->groups) * ((y->cols + side - 1) / side);
+    const int64_t groups = w->groups, mean = (y->rows + groups - 1) / groups, singles = blocks_of(y->rows) * blocks_of(y->cols);
+    const bool one = groups == 1, idle = 2 * singles <= sm_count(), pair = mean >= 112 && singles > sm_count();
+    const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * groups) * ((y->cols + side - 1) / side);
+    if (tiles > INT32_MAX / 2 || y->rows > INT32_MAX - 1024 || y->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     return with_type(y->type, [&](auto e) {
         using T = decltype(e);
-        if (y->rows <= 6 * (int64_t)w->groups) return launch_few<T, 16>(oa, ow, offsets, w->groups, *y, stream);
-        if (y->rows <= 16 * (int64_t)w->groups) return launch_few<T, 32>(oa, ow, offsets, w->groups, *y, stream);
-        if (y->rows <= 64 * (int64_t)w->groups) return launch_few<T, 64>(oa, ow, offsets, w->groups, *y, stream);
+        if (mean <= (one ? 16 : 5)) return launch_few<T, 16>(oa, ow, offsets, w->groups, *y, stream);
+        if (mean <= (one ? 32 : 20)) return launch_few<T, 32>(oa, ow, offsets, w->groups, *y, stream);
+        if (one && idle && mean <= 64 && oa.blocks >= 24) return launch_few<T, 64>(oa, ow, offsets, 1, *y, stream);
+        if (one && idle && oa.blocks >= 48) return launch_few<T, 128>(oa, ow, offsets, 1, *y, stream);
         return launch_product<T, false>("fp8_product", pair, tiles, oa, ow, offsets, w->groups, *y, stream);
     });
 }
@@ -794,6 +807,7 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
     const nb200_dense result{(int64_t)groups * dy->cols, x->cols, x->cols, NB200_F32, z};
     const bool pair = dy->cols > 128 && x->cols > 128;
     const int64_t side = pair ? 256 : 128, tiles = groups * ((dy->cols + side - 1) / side) * ((x->cols + side - 1) / side);
+    if (tiles > INT32_MAX / 2 || dy->cols > INT32_MAX - 1024 || x->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     return launch_product<float, true>("fp8_grad_w", pair, tiles, od, ox, s.first_block, groups, result, stream);
 }
 
