@@ -278,10 +278,8 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 c = columns[j / 4];
-                            acc[q * 32 + j] = __fmaf_rn(__uint_as_float(v[q][j]), s * c.x, acc[q * 32 + j]);
-                            acc[q * 32 + j + 1] = __fmaf_rn(__uint_as_float(v[q][j + 1]), s * c.y, acc[q * 32 + j + 1]);
-                            acc[q * 32 + j + 2] = __fmaf_rn(__uint_as_float(v[q][j + 2]), s * c.z, acc[q * 32 + j + 2]);
-                            acc[q * 32 + j + 3] = __fmaf_rn(__uint_as_float(v[q][j + 3]), s * c.w, acc[q * 32 + j + 3]);
+                            add_scaled(acc[q * 32 + j], acc[q * 32 + j + 1], v[q][j], v[q][j + 1], s, c.x, c.y);
+                            add_scaled(acc[q * 32 + j + 2], acc[q * 32 + j + 3], v[q][j + 2], v[q][j + 3], s, c.z, c.w);
                         }
                     } else {
 #pragma unroll

@@ -150,6 +150,22 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// ---- sums ------------------------------------------------------------------------------
+
+// a += v * (s * c) for two neighbours at once: half the instructions where every element has factors of its own.
+__device__ __forceinline__ void add_scaled(float &a0, float &a1, uint32_t v0, uint32_t v1, float s, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, v, s, c;\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "mov.b64 v, {%2, %3};\n\t"
+        "mov.b64 s, {%4, %4};\n\t"
+        "mov.b64 c, {%5, %6};\n\t"
+        "mul.rn.f32x2 c, s, c;\n\t"
+        "fma.rn.f32x2 a, v, c, a;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "r"(v0), "r"(v1), "f"(s), "f"(c0), "f"(c1));
+}
+
 // ---- registers -------------------------------------------------------------------------
 
 // Four neighbouring warps together change how many registers each of their threads has. What the warps of a block end up with must not be
