@@ -6,6 +6,9 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <initializer_list>
+#include <type_traits>
+
 #include "block_utils.cuh"
 
 namespace nb200 {
@@ -112,8 +115,73 @@ __host__ __device__ __forceinline__ int64_t padded_rows(int64_t rows) { return (
 // the tensor cores' shared-memory tiles has it, so that a tile is a plain copy of consecutive memory.
 __device__ __forceinline__ int64_t piece_at(int64_t r, int p) { return r * BLOCK8 + ((p ^ (int)(r & 7)) << 4); }
 
-// Magnitudes are compared as integers, in which a NaN is above everything.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// Eight neighbouring elements of a row as the words they lie in (kept whole: element by element the compiler takes them apart and puts them
+// together again, which was most of what quantising did).
+template <typename T>
+struct Eight {
+    static constexpr int WORDS = sizeof(T) * 2;
+    uint32_t w[WORDS];
+
+    // From column c on, zeros from column `cols` on. V: what one load brings.
+    template <int V>
+    __device__ __forceinline__ void load(const T *row, int64_t c, int64_t cols) {
+        constexpr int BYTES = V * sizeof(T);
+        if constexpr (BYTES >= 4) {
+            constexpr int EACH = BYTES / 4;
+#pragma unroll
+            for (int i = 0; i < WORDS; i += EACH) {
+                Vec<uint32_t, EACH> in{};
+                if (c + i * (4 / (int)sizeof(T)) < cols) in = *reinterpret_cast<const Vec<uint32_t, EACH> *>(row + c + i * (4 / (int)sizeof(T)));
+#pragma unroll
+                for (int j = 0; j < EACH; ++j) w[i + j] = in.v[j];
+            }
+        } else {
+            const uint16_t *from = reinterpret_cast<const uint16_t *>(row + c);
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+                const uint32_t lo = c + 2 * i < cols ? from[2 * i] : 0, hi = c + 2 * i + 1 < cols ? from[2 * i + 1] : 0;
+                w[i] = lo | hi << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+        else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+
+// Largest magnitudes. They are compared as integers, in which a NaN is above everything; those of 16-bit types two at a time, since what
+// quantises is bound by its instructions. `bits` is the larger one as a 32-bit number's.
+template <typename T>
+struct Top {
+    uint32_t v = 0;
+
+    __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t m;
+            asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+            return m;
+        } else {
+            return max(a, b);
+        }
+    }
+    __device__ __forceinline__ void add(uint32_t word) { v = larger(v, word & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu)); }
+    __device__ __forceinline__ void add(const Eight<T> &x) {
+#pragma unroll
+        for (int i = 0; i < Eight<T>::WORDS; ++i) add(x.w[i]);
+    }
+    // With that of the thread `distance` lanes away.
+    __device__ __forceinline__ void join(unsigned threads, int distance) { v = larger(v, __shfl_xor_sync(threads, v, distance)); }
+    __device__ __forceinline__ static uint32_t as_float(uint32_t half) {
+        if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)half)));
+        else return half << 16;
+    }
+    __device__ __forceinline__ uint32_t bits() const {
+        if constexpr (sizeof(T) == 2) return as_float(max(v & 0xffffu, v >> 16));
+        else return v;
+    }
+};
 
 // The two factors of a block whose largest magnitude is m.
 struct Factors {
@@ -125,33 +193,19 @@ __device__ __forceinline__ Factors factors_of(uint32_t m) {
 }
 
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inverse) {
-    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inverse, b * inverse), __NV_SATFINITE, __NV_E4M3);
-    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inverse, d * inverse), __NV_SATFINITE, __NV_E4M3);
-    return (uint32_t)lo | (uint32_t)hi << 16;
+    uint32_t q;
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(q)
+        : "f"(a * inverse), "f"(b * inverse), "f"(c * inverse), "f"(d * inverse));
+    return q;
 }
 
 inline bool fp8_ok(const nb200_fp8 *m) {
     return m && nb200_fp8_value_count(m) >= 0 && (nb200_fp8_value_count(m) == 0 || (m->values && m->scales)) &&
            reinterpret_cast<uintptr_t>(m->values) % 16 == 0 && reinterpret_cast<uintptr_t>(m->scales) % 16 == 0;
-}
-
-// Eight neighbouring elements of a row from column c on, zeros from column `cols` on. V: what one load brings.
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, 8> load8(const T *row, int64_t c, int64_t cols) {
-    Vec<T, 8> out;
-#pragma unroll
-    for (int i = 0; i < 8; i += V) {
-        Vec<T, V> w;
-        if (c + i < cols) {
-            w = *reinterpret_cast<const Vec<T, V> *>(row + c + i);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) w.v[j] = from_float<T>(0.f);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) out.v[i + j] = w.v[j];
-    }
-    return out;
 }
 
 // The factors of U blocks (a power of two) of 16 threads, which all have their largest magnitudes: every thread divides for one of them, a division
@@ -170,18 +224,10 @@ __device__ __forceinline__ void share_factors(unsigned threads, const uint32_t (
     }
 }
 
-// Eight neighbouring codes, and the largest magnitude of eight elements.
+// Eight neighbouring codes.
 template <typename T>
-__device__ __forceinline__ uint2 codes8(const Vec<T, 8> &v, float inverse) {
-    return make_uint2(codes4(to_float(v.v[0]), to_float(v.v[1]), to_float(v.v[2]), to_float(v.v[3]), inverse),
-                      codes4(to_float(v.v[4]), to_float(v.v[5]), to_float(v.v[6]), to_float(v.v[7]), inverse));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t magnitude8(const Vec<T, 8> &v) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, magnitude(to_float(v.v[j])));
-    return m;
+__device__ __forceinline__ uint2 codes8(const Eight<T> &v, float inverse) {
+    return make_uint2(codes4(v.get(0), v.get(1), v.get(2), v.get(3), inverse), codes4(v.get(4), v.get(5), v.get(6), v.get(7), inverse));
 }
 
 }  // namespace nb200

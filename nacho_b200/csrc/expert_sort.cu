@@ -249,9 +249,9 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
     while (at.advance()) {
         const T *row = x + at.t * stride;
         for (int b = mine; b < kb; b += blocks * U) {
-            Vec<T, 8> v[U];
+            Eight<T> v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load8<T, V>(row, (int64_t)(b + u * blocks) * BLOCK8 + sub * 8, cols);
+            for (int u = 0; u < U; ++u) v[u].template load<V>(row, (int64_t)(b + u * blocks) * BLOCK8 + sub * 8, cols);
             if (b == mine) {
                 if (team.lane == 0)
                     for (int e = at.e0; e < at.e1; ++e) {
@@ -264,9 +264,11 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
             Factors f[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                m[u] = magnitude8(v[u]);
+                Top<T> top;
+                top.add(v[u]);
 #pragma unroll
-                for (int d = 8; d; d >>= 1) m[u] = max(m[u], __shfl_xor_sync(half, m[u], d));
+                for (int d = 8; d; d >>= 1) top.join(half, d);
+                m[u] = top.bits();
             }
             share_factors<U>(half, m, f);
 #pragma unroll
@@ -494,11 +496,13 @@ __global__ void __launch_bounds__(NT) k_sort_few_fp8(Order o, int per_cta, int t
             if (s >= 0) o.rows[s] = t;
         }
         for (int64_t b = team.lane >> 4; b < kb; b += team.size >> 4) {
-            const Vec<T, 8> v = load8<T, V>(x + t * stride, b * BLOCK8 + sub * 8, cols);
-            uint32_t m = magnitude8(v);
+            Eight<T> v;
+            v.template load<V>(x + t * stride, b * BLOCK8 + sub * 8, cols);
+            Top<T> top;
+            top.add(v);
 #pragma unroll
-            for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(half, m, d));
-            const Factors f = factors_of(m);
+            for (int d = 8; d; d >>= 1) top.join(half, d);
+            const Factors f = factors_of(top.bits());
             const uint2 q = codes8(v, f.inverse);
             for (int e = e0; e < e1; ++e) {
                 const int s = o.slot(e);

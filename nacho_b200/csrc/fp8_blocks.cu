@@ -35,16 +35,18 @@ __global__ void __launch_bounds__(NT) k_fp8_rows(Blocks z, int chunks, const T *
     const int64_t r = (int64_t)(blockIdx.x / chunks) * ROWS8 + threadIdx.x / 16;
     const int64_t b0 = (int64_t)(blockIdx.x % chunks) * BLOCKS8;
     if (r >= z.rows) return;
-    Vec<T, 8> v[BLOCKS8];
+    Eight<T> v[BLOCKS8];
 #pragma unroll
-    for (int u = 0; u < BLOCKS8; ++u) v[u] = load8<T, V>(x + r * stride, (b0 + u) * BLOCK8 + sub * 8, z.cols);
+    for (int u = 0; u < BLOCKS8; ++u) v[u].template load<V>(x + r * stride, (b0 + u) * BLOCK8 + sub * 8, z.cols);
     uint32_t m[BLOCKS8];
     Factors f[BLOCKS8];
 #pragma unroll
     for (int u = 0; u < BLOCKS8; ++u) {
-        m[u] = magnitude8(v[u]);
+        Top<T> top;
+        top.add(v[u]);
 #pragma unroll
-        for (int d = 8; d; d >>= 1) m[u] = max(m[u], __shfl_xor_sync(half, m[u], d));
+        for (int d = 8; d; d >>= 1) top.join(half, d);
+        m[u] = top.bits();
     }
     share_factors<BLOCKS8>(half, m, f);
 #pragma unroll
@@ -68,16 +70,16 @@ __global__ void __launch_bounds__(NT) k_fp8_tiles(Blocks z, const T *x, int64_t 
     const int64_t b = blockIdx.x % per_group / z.nb, n = blockIdx.x % z.nb;
     if (threadIdx.x == 0) top = 0;
     __syncthreads();
-    Vec<T, 8> v[8];
-    uint32_t m = 0;
+    Eight<T> v[8];
+    Top<T> mine;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = n * BLOCK8 + i * 16 + threadIdx.x / 16;
-        v[i] = load8<T, V>(x + ((int64_t)g * z.rows + min(r, (int64_t)z.rows - 1)) * stride, b * BLOCK8 + sub * 8, r < z.rows ? z.cols : 0);
+        v[i].template load<V>(x + ((int64_t)g * z.rows + min(r, (int64_t)z.rows - 1)) * stride, b * BLOCK8 + sub * 8, r < z.rows ? z.cols : 0);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, magnitude8(v[i]));
-    m = __reduce_max_sync(FULL_MASK, m);
+    for (int i = 0; i < 8; ++i) mine.add(v[i]);
+    const uint32_t m = __reduce_max_sync(FULL_MASK, mine.bits());
     if (lane_id() == 0) atomicMax(&top, m);
     __syncthreads();
     const Factors f = factors_of(top);

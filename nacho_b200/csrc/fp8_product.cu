@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(1024) k_group_blocks(const int32_t *offsets, i
 // lines. There the eight codes of a column and eight rows p lie at place p ^ (column / 8) of the column's, which spreads a warp over the banks.
 template <typename T, int V>
 __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(const T *x, int64_t stride, int64_t cols, const int2 *block, uint8_t *values, float *scales) {
-    __shared__ uint32_t top[NT / 32][BLOCK8];
+    __shared__ uint32_t top[NT / 32][BLOCK8];  // words
     __shared__ alignas(16) float inverse[BLOCK8];
     __shared__ alignas(16) uint2 codes[BLOCK8][16];
     wait_for_previous();
@@ -596,29 +596,30 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(cons
     const int2 rows = *(block + b);
     if (rows.y == 0) return;
     const int sub = threadIdx.x & 15, part = threadIdx.x / 16;
-    Vec<T, 8> v[8];
+    Eight<T> v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int r = part * 8 + i;
-        v[i] = load8<T, V>(x + (int64_t)(rows.x + min(r, rows.y - 1)) * stride, c0 + sub * 8, r < rows.y ? cols : 0);
+        v[i].template load<V>(x + (int64_t)(rows.x + min(r, rows.y - 1)) * stride, c0 + sub * 8, r < rows.y ? cols : 0);
     }
-    uint32_t m[8];
+    // words of a row: a column each, or two neighbours
+    constexpr int WORDS = Eight<T>::WORDS, EACH = 4 / sizeof(T);
+    Top<T> m[WORDS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        m[j] = 0;
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m[j] = max(m[j], magnitude(to_float(v[i].v[j])));
-        m[j] = max(m[j], __shfl_xor_sync(FULL_MASK, m[j], 16));
-    }
-    if (lane_id() < 16) {
-        *reinterpret_cast<uint4 *>(&top[warp_id()][sub * 8]) = make_uint4(m[0], m[1], m[2], m[3]);
-        *reinterpret_cast<uint4 *>(&top[warp_id()][sub * 8 + 4]) = make_uint4(m[4], m[5], m[6], m[7]);
+        for (int j = 0; j < WORDS; ++j) m[j].add(v[i].w[j]);
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) {
+        m[j].join(FULL_MASK, 16);
+        if (lane_id() < 16) top[warp_id()][sub * WORDS + j] = m[j].v;
     }
     __syncthreads();
     if (threadIdx.x < BLOCK8) {
-        uint32_t all = 0;
+        Top<T> column;
 #pragma unroll
-        for (int w = 0; w < NT / 32; ++w) all = max(all, top[w][threadIdx.x]);
+        for (int w = 0; w < NT / 32; ++w) column.add(top[w][threadIdx.x / EACH]);
+        const uint32_t all = sizeof(T) == 2 ? Top<T>::as_float(threadIdx.x & 1 ? column.v >> 16 : column.v & 0xffffu) : column.v;
         const Factors f = factors_of(all);
         inverse[threadIdx.x] = f.inverse;
         if (c0 + threadIdx.x < cols) scales[b * pad + c0 + threadIdx.x] = f.scale;
@@ -627,8 +628,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(cons
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float f = inverse[sub * 8 + j];
-        codes[sub * 8 + j][part ^ sub] = make_uint2(codes4(to_float(v[0].v[j]), to_float(v[1].v[j]), to_float(v[2].v[j]), to_float(v[3].v[j]), f),
-                                                    codes4(to_float(v[4].v[j]), to_float(v[5].v[j]), to_float(v[6].v[j]), to_float(v[7].v[j]), f));
+        codes[sub * 8 + j][part ^ sub] =
+            make_uint2(codes4(v[0].get(j), v[1].get(j), v[2].get(j), v[3].get(j), f), codes4(v[4].get(j), v[5].get(j), v[6].get(j), v[7].get(j), f));
     }
     __syncthreads();
     uint8_t *to = values + b * pad * BLOCK8;
