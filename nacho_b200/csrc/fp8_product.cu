@@ -28,8 +28,8 @@ struct Operand {
 // ---- tiles on the tensor cores -------------------------------------------------------------
 
 constexpr int STORE_WARPS = 8, THREADS = (STORE_WARPS + 4) * 32;
-// Registers a thread: 168 at launch (65536 / 384), then 224 for the two groups of four warps that hold sums and 56 for the third: 64512 as before.
-constexpr int REGS_SUMS = 224, REGS_OTHERS = 56;
+// Registers a thread: 168 at launch (65536 / 384), then 216 for the two groups of four warps that hold sums and 72 for the third: 64512 as before.
+constexpr int REGS_SUMS = 216, REGS_OTHERS = 72;
 static_assert(256 * REGS_SUMS + 128 * REGS_OTHERS <= 168 * THREADS, "");
 constexpr int WAIT_LIMIT = 1 << 22;  // polls, after which a wait gives up: seconds, where microseconds are usual
 
@@ -201,7 +201,7 @@ template <typename T, bool WIDE, bool PAIR, bool GRAD>
 __device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                         unsigned long long *report) {
     using S = Shape<PAIR>;
-    constexpr int STAGES = S::STAGES, SUMS = S::SUMS, BN = S::BN, N = BN / 2;
+    constexpr int STAGES = S::STAGES, SUMS = S::SUMS, BN = S::BN, N = BN / 2, W = 16;
     extern __shared__ uint8_t raw[];
     typename S::Shared &sh = *reinterpret_cast<typename S::Shared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = warp_id(), lane = lane_id();
@@ -255,16 +255,16 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
                 tmem_fence_after();
                 const uint32_t at = base + sums.at * BN;
-                // 32 columns are on their way while 32 others are added
-                uint32_t v[N / 32][32];
+                // W columns are on their way while W others are added: with 32 the registers are short (8192^3 490 us, with 16 468)
+                uint32_t v[N / W][W];
                 tmem_load(at, v[0]);
                 float s = sh.scale[place.at][lanes * 32 + lane];
                 if constexpr (!GRAD) s *= __shfl_sync(FULL_MASK, tile_scale, b % 32);
 #pragma unroll
-                for (int q = 0; q < N / 32; ++q) {
+                for (int q = 0; q < N / W; ++q) {
                     tmem_wait_loads(v[q]);
-                    if (q + 1 < N / 32) {
-                        tmem_load(at + (q + 1) * 32, v[q + 1]);
+                    if (q + 1 < N / W) {
+                        tmem_load(at + (q + 1) * W, v[q + 1]);
                     } else {
                         tmem_fence_before();
                         __syncwarp();
@@ -274,16 +274,16 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                         }
                     }
                     if constexpr (GRAD) {
-                        const float4 *columns = reinterpret_cast<const float4 *>(&sh.col_scale[place.at][half * N + q * 32]);
+                        const float4 *columns = reinterpret_cast<const float4 *>(&sh.col_scale[place.at][half * N + q * W]);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
+                        for (int j = 0; j < W; j += 4) {
                             const float4 c = columns[j / 4];
-                            add_scaled(acc[q * 32 + j], acc[q * 32 + j + 1], v[q][j], v[q][j + 1], s, c.x, c.y);
-                            add_scaled(acc[q * 32 + j + 2], acc[q * 32 + j + 3], v[q][j + 2], v[q][j + 3], s, c.z, c.w);
+                            add_scaled(acc[q * W + j], acc[q * W + j + 1], v[q][j], v[q][j + 1], s, c.x, c.y);
+                            add_scaled(acc[q * W + j + 2], acc[q * W + j + 3], v[q][j + 2], v[q][j + 3], s, c.z, c.w);
                         }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) acc[q * 32 + j] = __fmaf_rn(__uint_as_float(v[q][j]), s, acc[q * 32 + j]);
+                        for (int j = 0; j < W; ++j) acc[q * W + j] = __fmaf_rn(__uint_as_float(v[q][j]), s, acc[q * W + j]);
                     }
                 }
             }
