@@ -413,7 +413,10 @@ int nb200_fp8_unpack(const nb200_fp8 *a, float *z, void *stream);
 /* Every group's transpose; tiled = 1 only. */
 int nb200_fp8_transpose(const nb200_fp8 *a, nb200_fp8 *z, void *stream);
 
-/* y[i] = a[i] * w[g]^T: rows a (tiled = 0), weights w (tiled = 1) with as many columns, y of a->rows x w->rows in any type. With
+/* The products' waits for copies and matrix instructions are bounded (two seconds, where microseconds are usual). One that gave up is reported by
+ * the next product on the stream, which returns NB200_E_TIMEOUT and does nothing.
+ *
+ * y[i] = a[i] * w[g]^T: rows a (tiled = 0), weights w (tiled = 1) with as many columns, y of a->rows x w->rows in any type. With
  * `offsets` (w->groups + 1 of them, rising, in device memory) rows offsets[g] .. offsets[g + 1] - 1 take group g and rows
  * in front of the first or behind the last are zeros; without it there is one group. Products of a block of 128 columns are summed on
  * the tensor cores and the blocks, times their two scales, in 32 bits. */
@@ -450,6 +453,11 @@ int nb200_selftest_chain_timeout(const nb200_csr *a, const nb200_csr *b, const n
                                  int64_t capacity, int32_t polls, void *stream);
 int nb200_selftest_levels_timeout(const nb200_csf3 *a, const nb200_csf3 *b, nb200_csf3 *z, int64_t cap_i, int64_t cap_j,
                                   int64_t cap_k, int32_t polls, void *stream);
+
+/* For the 8-bit products, whose calls do not wait for their kernels: a product that is never given its first block, so that every wait in it gives
+ * up after 20 ms. It writes nothing and returns NB200_OK; once it has ended, the NEXT product on the stream returns NB200_E_TIMEOUT in its
+ * place, and the one after that works. y is 32-bit. */
+int nb200_selftest_product_timeout(const nb200_fp8 *a, const nb200_fp8 *w, nb200_dense *y, void *stream);
 
 #ifdef __cplusplus
 }

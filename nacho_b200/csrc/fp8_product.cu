@@ -31,7 +31,7 @@ constexpr int STORE_WARPS = 8, THREADS = (STORE_WARPS + 4) * 32;
 // Registers a thread: 168 at launch (65536 / 384), then 216 for the two groups of four warps that hold sums and 72 for the third: 64512 as before.
 constexpr int REGS_SUMS = 216, REGS_OTHERS = 72;
 static_assert(256 * REGS_SUMS + 128 * REGS_OTHERS <= 168 * THREADS, "");
-constexpr int WAIT_LIMIT = 1 << 22;  // polls, after which a wait gives up: seconds, where microseconds are usual
+constexpr uint64_t PATIENCE = 2000000000, SHORT_PATIENCE = 20000000;  // ns, after which a wait gives up (microseconds are usual); the self-test's
 
 // A CTA has 128 rows of the result and 128 columns, in a pair 256. Both CTAs of a pair have the same columns, each brings half of their codes.
 template <bool PAIR>
@@ -142,14 +142,30 @@ struct GradWalk {
     }
 };
 
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+
 // For a whole warp; false for all of it once one of its threads, or another warp of the CTA, has given up.
+template <bool SELFTEST = false>
 __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed) {
-    for (int i = 0; i < WAIT_LIMIT; ++i) {
+    uint64_t start = 0;
+    for (int i = 1;; ++i) {
         if (__all_sync(FULL_MASK, mbar_try_wait(bar, parity))) return true;
-        if (i % 64 == 63 && __any_sync(FULL_MASK, *failed)) return false;
+        if (i % 64) continue;
+        if (__any_sync(FULL_MASK, *failed)) return false;
+        if (!start) start = now_ns();
+        if (__any_sync(FULL_MASK, now_ns() - start > (SELFTEST ? SHORT_PATIENCE : PATIENCE))) break;
     }
     *failed = 1;
     return false;
+}
+
+// After a give-up: what is still on its way lands first, or never will.
+__device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
+    for (const uint64_t start = now_ns(); now_ns() - start < SHORT_PATIENCE && !mbar_try_wait(bar, parity);) {}
 }
 
 // 32 rows of a warp, N columns from `col` on, from registers to memory: through shared memory, 128 bytes of every row at a time, so
@@ -197,7 +213,8 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t *buffe
 //
 // GRAD: the sums run over a group's blocks of rows of dy and x, `offsets` says where those begin, and columns have a scale each. The scales of
 // both are multiplied for every element, which is as much arithmetic again.
-template <typename T, bool WIDE, bool PAIR, bool GRAD>
+// SELFTEST: the first block's copies are left out, so that every warp's wait runs out.
+template <typename T, bool WIDE, bool PAIR, bool GRAD, bool SELFTEST = false>
 __device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                         unsigned long long *report) {
     using S = Shape<PAIR>;
@@ -252,7 +269,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                     tile_scale = next_scale;
                     next_scale = b + 32 + lane < t.blocks ? ld_late(sw + b + 32 + lane) : 0.f;
                 }
-                if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
+                if (!(fine = wait_for<SELFTEST>(&sh.sum_full[sums.at], sums.phase, failed))) break;
                 tmem_fence_after();
                 const uint32_t at = base + sums.at * BN;
                 // W columns are on their way while W others are added: with 32 the registers are short (8192^3 490 us, with 16 468)
@@ -314,8 +331,8 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 const float *from_scales = a.row_scales(t.first_block) + row, *from_col_scales = w.row_scales(t.first_block) + t.col;
                 const uint8_t *from_a = a.block(0, t.first_block) + row * BLOCK8, *from_b = w.block(GRAD ? 0 : t.g, t.first_block) + col * BLOCK8;
                 for (int b = 0; b < t.blocks; ++b, stage.next(), place.next()) {
-                    if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
-                    if (elected()) {
+                    if (!(fine = wait_for<SELFTEST>(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
+                    if (elected() && !(SELFTEST && b == 0)) {
                         mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + b_bytes + scale_bytes + col_bytes);
                         if (a_bytes) {
                             bulk_load(sh.a[stage.at], from_a, a_bytes, &sh.full[stage.at]);
@@ -329,14 +346,14 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 }
             }
             if (!fine)  // nothing may land in shared memory that is no longer this CTA's
-                for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1, 1 << 16);
+                for (int s = 0; s < STAGES; ++s) drain(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1);
         } else if (warp == STORE_WARPS && rank == 0) {  // matrix instructions
             const uint64_t tile_a = tile_descriptor(smem_u32(sh.a[0])), tile_b = tile_descriptor(smem_u32(sh.b[0]));
             Ring<SUMS> sums;
             for (int tile = first; fine && walk.find(tile, t); tile += step) {
                 for (int b = 0; b < t.blocks; ++b, stage.next(), sums.next()) {
-                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
-                    if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                    if (!(fine = wait_for<SELFTEST>(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (!(fine = wait_for<SELFTEST>(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
                     tmem_fence_after();
                     if (elected()) {
                         const uint64_t da = tile_a + (uint64_t)(stage.at * (S::A_ROWS * BLOCK8 >> 4)), db = tile_b + (uint64_t)(stage.at * (S::B_ROWS * BLOCK8 >> 4));
@@ -351,12 +368,12 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
             if (!fine) {
                 if (elected()) mma_commit<PAIR>(&sh.drained);
                 __syncwarp();
-                mbar_wait_bounded(&sh.drained, 0, 1 << 16);
+                drain(&sh.drained, 0);
             }
         } else if (PAIR && warp == STORE_WARPS) {  // tells the leader of the copies that have landed here
             for (int tile = first; fine && walk.find(tile, t); tile += step) {
                 for (int b = 0; b < t.blocks; ++b, stage.next()) {
-                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (!(fine = wait_for<SELFTEST>(&sh.full[stage.at], stage.phase, failed))) break;
                     if (elected()) mbar_arrive_leader(&sh.full[stage.at]);
                     __syncwarp();
                 }
@@ -377,6 +394,10 @@ template <typename T, bool WIDE, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                                         unsigned long long *report) {
     product<T, WIDE, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report);
+}
+__global__ void __launch_bounds__(THREADS, 1) k_product_selftest(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, float *y, int64_t stride,
+                                                                 unsigned long long *report) {
+    product<float, false, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, report);
 }
 template <typename T, bool WIDE, bool GRAD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_product_pair(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y,
@@ -540,11 +561,11 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : NB == 128 ? 1 : 2)
         clear(hi, rows);
     }
     if (!fine && warp == 5)
-        for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1, 1 << 16);
+        for (int s = 0; s < STAGES; ++s) drain(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1);
     if (!fine && warp == 4) {
         if (elected()) mma_commit<false>(&sh.drained);
         __syncwarp();
-        mbar_wait_bounded(&sh.drained, 0, 1 << 16);
+        drain(&sh.drained, 0);
     }
     tmem_fence_before();
     __syncthreads();
@@ -780,6 +801,23 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
         if (one && idle && oa.blocks >= 48) return launch_few<T, 128>(oa, ow, offsets, 1, *y, stream);
         return launch_product<T, false>("fp8_product", pair, tiles, oa, ow, offsets, w->groups, *y, stream);
     });
+}
+
+int nb200_selftest_product_timeout(const nb200_fp8 *a, const nb200_fp8 *w, nb200_dense *y, void *stream_) {
+    if (!fp8_ok(a) || !fp8_ok(w) || !dense_ok(y) || a->tiled || !w->tiled || w->groups != 1 || a->cols != w->cols || y->rows != a->rows || y->cols != w->rows ||
+        y->type != NB200_F32 || y->rows == 0 || y->cols == 0 || a->cols == 0)
+        return NB200_E_BADARG;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    Workspace *ws = nullptr;
+    int st;
+    if ((st = report_of(stream, &ws))) return st;
+    const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), 0};
+    const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows)};
+    NB200_CUDA(cudaFuncSetAttribute(k_product_selftest, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<false>::SHARED_BYTES));
+    LaunchScope scope("fp8_product_selftest", stream);
+    NB200_CUDA(launch_overlapped(k_product_selftest, dim3(1), dim3(THREADS), Shape<false>::SHARED_BYTES, stream, oa, ow, (const int32_t *)nullptr, 1, y->rows, y->cols,
+                                 static_cast<float *>(y->data), y->stride, reinterpret_cast<unsigned long long *>(ws->host) + 32));
+    return NB200_OK;
 }
 
 int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dense *x, int32_t groups) {

@@ -513,3 +513,21 @@ def test_example_learns():
     spec.loader.exec_module(example)
     losses, dx = example.descend(tokens=257, experts=6, best=2, width=130, hidden=200)
     assert all(b < a for a, b in zip(losses, losses[1:])) and dx.shape == (257, 130) and not torch.isnan(dx).any()
+
+
+def test_a_wait_that_gives_up_is_reported_by_the_next_product():
+    import ctypes as C
+    from nacho_b200 import _capi
+    n = nacho()
+    a, w = n.to_fp8_rows(normal((300, 700), torch.float32, 1)), n.to_fp8_tiles(normal((200, 700), torch.float32, 2))
+    want = n.gpu_fp8_product(a, w, dtype=torch.float32)
+    y = torch.full((300, 200), 7.0, device="cuda")
+    struct = lambda m: _capi.Fp8Struct(*m._dims, int(m.tiled), m._values.data_ptr(), m._scales.data_ptr())
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    status = _capi.lib.nb200_selftest_product_timeout(C.byref(struct(a)), C.byref(struct(w)), C.byref(_capi.DenseStruct(300, 200, 200, 0, y.data_ptr())), stream)
+    assert status == _capi.OK
+    torch.cuda.synchronize()
+    assert torch.all(y == 7.0)
+    with pytest.raises(RuntimeError, match="earlier 8-bit product: matrix product pipeline gave up"):
+        n.gpu_fp8_product(a, w)
+    assert torch.equal(n.gpu_fp8_product(a, w, dtype=torch.float32), want)
