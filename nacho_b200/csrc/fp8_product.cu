@@ -3,6 +3,7 @@
 // all rows by one matrix or every group of rows by its own, and the gradient for the weights of the latter,
 //     z[g][n, k] = sum_b sd[n, b] sx[k, b] sum_{i in block b} dy[i, n] x[i, k],   b over blocks of 128 rows of group g.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "dense_rows.cuh"
@@ -38,7 +39,7 @@ template <bool PAIR>
 struct Shape {
     static constexpr int CTAS = PAIR ? 2 : 1, BM = 128 * CTAS, BN = 128 * CTAS;  // a tile of the result
     static constexpr int A_ROWS = 128, B_ROWS = 128;                             // what a CTA brings per block
-    static constexpr int STAGES = 5, SUMS = 512 / BN;                            // blocks under way; places for their sums in tensor memory
+    static constexpr int STAGES = 4, SUMS = 512 / BN;                            // blocks under way; places for their sums in tensor memory
     // Scales are written into a place STAGES + SUMS blocks after it was used before: by then their matrix instructions, and with them those of
     // STAGES blocks earlier, are done, which had to wait until the sums of SUMS blocks earlier had been read.
     static constexpr int SCALES = STAGES + SUMS;
@@ -48,7 +49,7 @@ struct Shape {
     struct Shared {
         uint8_t a[STAGES][A_ROWS * BLOCK8];
         uint8_t b[STAGES][B_ROWS * BLOCK8];
-        uint8_t out[STORE_WARPS][32 * 128];
+        uint8_t out[STORE_WARPS][2][32 * 128];
         float scale[SCALES][A_ROWS], col_scale[SCALES][BN];  // the latter for the gradient
         uint64_t full[STAGES], empty[STAGES];      // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
         uint64_t sum_full[SUMS], sum_empty[SUMS];  // a block's sums lie in tensor memory; they have been read
@@ -168,41 +169,55 @@ __device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
     for (const uint64_t start = now_ns(); now_ns() - start < SHORT_PATIENCE && !mbar_try_wait(bar, parity);) {}
 }
 
-// 32 rows of a warp, N columns from `col` on, from registers to memory: through shared memory, 128 bytes of every row at a time, so
-// that whole lines are written. WIDE: rows can be written in words of 16 bytes.
+// 32 rows of a warp, N columns from `col` on, from registers to memory, through two places in shared memory of 128 bytes of every row. WIDE: rows
+// can be written in words of 16 bytes. Then the copy engine stores a place while the next one is filled, for which all 32 rows have to count (`base`: the
+// row of the matrix at which the group's rows begin; `last`: there are no rows behind the group's). Otherwise the warp reads the place again and writes
+// whole lines: 8192 x 32768 x 2048 521 us that way for all rows, 610 without shared memory.
 template <typename T, bool WIDE, int N>
-__device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t *buffer, T *y, int64_t stride, int64_t row, int64_t from, int64_t to, int64_t col, int64_t cols) {
+__device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t (*places)[32 * 128], int &turn, const CUtensorMap *matrix, int base, bool last, T *y, int64_t stride,
+                                           int row, int from, int to, int col, int cols) {
     constexpr int PER = 128 / sizeof(T), EACH = 16 / sizeof(T);  // columns at a time; in 16 bytes
     const int lane = lane_id();
+    if (row + 32 <= from || row >= to) return;
+    const bool whole = WIDE && row >= from && (row + 32 <= to || last);
 #pragma unroll
     for (int c = 0; c < N; c += PER) {
         if (col + c >= cols) break;
+        uint8_t *place = places[turn];
+        turn ^= 1;
+        if (WIDE && elected()) stores_read_but<1>();
         __syncwarp();
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
             Vec<T, EACH> v;
 #pragma unroll
             for (int j = 0; j < EACH; ++j) v.v[j] = from_float<T>(acc[c + p * EACH + j]);
-            *reinterpret_cast<Vec<T, EACH> *>(buffer + piece_at(lane, p)) = v;
+            *reinterpret_cast<Vec<T, EACH> *>(place + piece_at(lane, p)) = v;
         }
-        __syncwarp();
-        if constexpr (WIDE) {
+        if (whole) {
+            fence_async_shared();
+            __syncwarp();
+            if (elected()) store_tile(matrix, place, col + c, base + row);
+        } else if constexpr (WIDE) {
+            __syncwarp();
             const int p = lane & 7;
             const bool there = col + c + p * EACH < cols;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 const int r = i + lane / 8;
                 if (there && row + r >= from && row + r < to)
-                    *reinterpret_cast<uint4 *>(y + (row + r) * stride + col + c + p * EACH) = *reinterpret_cast<const uint4 *>(buffer + piece_at(r, p));
+                    *reinterpret_cast<uint4 *>(y + (int64_t)(row + r) * stride + col + c + p * EACH) = *reinterpret_cast<const uint4 *>(place + piece_at(r, p));
             }
         } else {
+            __syncwarp();
             for (int r = 0; r < 32; ++r) {
                 if (row + r < from || row + r >= to) continue;
 #pragma unroll
                 for (int j = lane; j < PER; j += 32)
-                    if (col + c + j < cols) y[(row + r) * stride + col + c + j] = *reinterpret_cast<const T *>(buffer + piece_at(r, j / EACH) + j % EACH * sizeof(T));
+                    if (col + c + j < cols) y[(int64_t)(row + r) * stride + col + c + j] = *reinterpret_cast<const T *>(place + piece_at(r, j / EACH) + j % EACH * sizeof(T));
             }
         }
+        if (WIDE && elected()) close_stores();  // an empty group where the warp has written itself
     }
 }
 
@@ -216,7 +231,7 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t *buffe
 // SELFTEST: the first block's copies are left out, so that every warp's wait runs out.
 template <typename T, bool WIDE, bool PAIR, bool GRAD, bool SELFTEST = false>
 __device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
-                                        unsigned long long *report) {
+                                        unsigned long long *report, const CUtensorMap *matrix) {
     using S = Shape<PAIR>;
     constexpr int STAGES = S::STAGES, SUMS = S::SUMS, BN = S::BN, N = BN / 2, W = 16;
     extern __shared__ uint8_t raw[];
@@ -251,6 +266,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
         auto walk = tiles();
         Tile t;
         const int lanes = warp & 3, half = warp >> 2;
+        int turn = 0;
         Ring<SUMS> sums;
         Ring<S::SCALES> place;
         const uint32_t base = tmem + ((uint32_t)(lanes * 32) << 16) + half * N;
@@ -305,8 +321,12 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
                 }
             }
             if (!fine) break;
-            if (col < cols) store_rows<T, WIDE, N>(acc, sh.out[warp], GRAD ? y + t.g * rows * stride : y, stride, row, t.from, t.to, col, cols);
+            if (col < cols)
+                store_rows<T, WIDE, N>(acc, sh.out[warp], turn, matrix, GRAD ? t.g * (int)rows : 0, GRAD ? t.g == groups - 1 : t.to == rows, GRAD ? y + t.g * rows * stride : y,
+                                       stride, (int)row, t.from, t.to, (int)col, (int)cols);
         }
+        if (WIDE && elected()) stores_done();
+        __syncwarp();
         // rows of no group
         if (!GRAD && offsets) {
             const int64_t lo = min(max((int64_t)ld_late(offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(offsets + groups), lo), rows);
@@ -392,17 +412,17 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
 
 template <typename T, bool WIDE, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
-                                                        unsigned long long *report) {
-    product<T, WIDE, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report);
+                                                        unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
+    product<T, WIDE, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
 }
 __global__ void __launch_bounds__(THREADS, 1) k_product_selftest(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, float *y, int64_t stride,
                                                                  unsigned long long *report) {
-    product<float, false, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, report);
+    product<float, false, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, report, nullptr);
 }
 template <typename T, bool WIDE, bool GRAD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_product_pair(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y,
-                                                                                       int64_t stride, unsigned long long *report) {
-    product<T, WIDE, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report);
+                                                                                       int64_t stride, unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
+    product<T, WIDE, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
 }
 
 // ---- few rows per group ------------------------------------------------------------------
@@ -706,6 +726,31 @@ int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int g
     return NB200_OK;
 }
 
+// The result as the copy engine sees it: boxes of 32 rows by 128 bytes.
+int describe(const nb200_dense &y, CUtensorMap *map) {
+    typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::atomic<encode_fn> known{nullptr};
+    encode_fn encode = known.load(std::memory_order_acquire);
+    if (!encode) {
+        void *found = nullptr;
+        cudaDriverEntryPointQueryResult how = cudaDriverEntryPointSymbolNotFound;
+        NB200_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault, &how));
+        if (how != cudaDriverEntryPointSuccess || !found) return note_cuda_error(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
+        encode = reinterpret_cast<encode_fn>(found);
+        known.store(encode, std::memory_order_release);
+    }
+    const CUtensorMapDataType type = y.type == NB200_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : y.type == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t extents[2] = {(cuuint64_t)y.cols, (cuuint64_t)y.rows}, pitch[1] = {(cuuint64_t)(y.rows > 1 ? y.stride : y.cols) * type_size(y.type)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / type_size(y.type)), 32}, steps[2] = {1, 1};
+    if (encode(map, type, 2, y.data, extents, pitch, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return note_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    return NB200_OK;
+}
+
 // `tiles` of the shape that `pair` selects, at most.
 template <typename T, bool GRAD>
 int launch_product(const char *name, bool pair, int64_t tiles, const Operand &a, const Operand &w, const int32_t *offsets, int groups, const nb200_dense &y, cudaStream_t stream) {
@@ -713,14 +758,17 @@ int launch_product(const char *name, bool pair, int64_t tiles, const Operand &a,
     int st;
     if ((st = report_of(stream, &ws))) return st;
     unsigned long long *report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
+    // As far as the copy engine counts a matrix (2^40 bytes from row to row); a result beyond that is written in words of its elements.
+    const bool wide = word_bytes({&y}) == 16 && y.stride < int64_t(1) << 36 && y.rows < int64_t(1) << 31;
+    CUtensorMap matrix{};
+    if (wide && (st = describe(y, &matrix))) return st;
     auto go = [&](auto kernel, size_t smem, int ctas) -> int {
         NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         LaunchScope scope(name, stream);
         NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles * ctas, sm_count() / ctas * ctas)), dim3(THREADS), smem, stream, a, w, offsets, groups,
-                                     GRAD ? y.rows / groups : y.rows, y.cols, static_cast<T *>(y.data), y.stride, report));
+                                     GRAD ? y.rows / groups : y.rows, y.cols, static_cast<T *>(y.data), y.stride, report, matrix));
         return NB200_OK;
     };
-    const bool wide = word_bytes({&y}) == 16;
     if (pair) return wide ? go(k_product_pair<T, true, GRAD>, Shape<true>::SHARED_BYTES, 2) : go(k_product_pair<T, false, GRAD>, Shape<true>::SHARED_BYTES, 2);
     return wide ? go(k_product<T, true, GRAD>, Shape<false>::SHARED_BYTES, 1) : go(k_product<T, false, GRAD>, Shape<false>::SHARED_BYTES, 1);
 }

@@ -2,6 +2,8 @@
 // matrix instructions on e4m3 operands with 32-bit sums, and the barriers they complete on.
 #pragma once
 
+#include <cuda.h>
+
 #include "tma.cuh"
 
 namespace nb200 {
@@ -106,6 +108,18 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
     else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+
+// ---- stores of tiles -------------------------------------------------------------------
+
+// A tile of rows of 128 bytes from shared memory, laid out as above, to the place (x, y) of a matrix; what lies beyond the matrix is left out. The
+// thread that starts such stores also closes them into groups and waits until all but its last N groups have been read (or written).
+__device__ __forceinline__ void store_tile(const CUtensorMap *matrix, const void *smem, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(matrix), "r"(smem_u32(smem)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void close_stores() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void stores_read_but() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ---- barriers within a cluster -----------------------------------------------------------
 
