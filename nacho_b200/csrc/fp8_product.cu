@@ -210,11 +210,15 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t (*plac
             }
         } else {
             __syncwarp();
+#pragma unroll 8
             for (int r = 0; r < 32; ++r) {
-                if (row + r < from || row + r >= to) continue;
+                const bool there = row + r >= from && row + r < to;
 #pragma unroll
-                for (int j = lane; j < PER; j += 32)
-                    if (col + c + j < cols) y[(int64_t)(row + r) * stride + col + c + j] = *reinterpret_cast<const T *>(place + piece_at(r, j / EACH) + j % EACH * sizeof(T));
+                for (int i = 0; i < PER; i += 32) {
+                    const int j = i + lane;
+                    if (there && col + c + j < cols)
+                        y[(int64_t)(row + r) * stride + col + c + j] = *reinterpret_cast<const T *>(place + piece_at(r, j / EACH) + j % EACH * sizeof(T));
+                }
             }
         }
         if (WIDE && elected()) close_stores();  // an empty group where the warp has written itself
@@ -449,7 +453,7 @@ constexpr int FEW_THREADS = 6 * 32;
 
 template <typename T, int NB, bool SPLIT>
 __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : NB == 128 ? 1 : 2) k_product_few(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
-                                                             unsigned long long *report) {
+                                                             int tiles_each, unsigned long long *report) {
     using S = FewShape<NB, SPLIT>;
     constexpr int STAGES = S::STAGES, SUMS = S::SUMS, W = NB < 32 ? 16 : 32;
     extern __shared__ uint8_t raw[];
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : NB == 128 ? 1 : 2)
     wait_for_previous();
 
     const int g = blockIdx.y;
-    const int64_t col = (int64_t)(blockIdx.x / slices) * 128;
+    const int64_t first_col = (int64_t)(blockIdx.x / slices) * tiles_each * 128, end_col = min(first_col + (int64_t)tiles_each * 128, cols);
     const int64_t from = offsets ? min(max((int64_t)ld_late(offsets + g), (int64_t)0), rows) : 0;
     const int64_t to = offsets ? min(max((int64_t)ld_late(offsets + g + 1), from), rows) : rows;
     const int first = (int)(a.blocks * slice / slices), blocks = (int)(a.blocks * (slice + 1) / slices) - first;
@@ -481,93 +485,95 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : NB == 128 ? 1 : 2)
     Ring<SUMS> sums;
     Ring<S::SCALES> place;
     bool fine = true;
-    for (int64_t row = (from & ~int64_t(7)) + (int64_t)blockIdx.z * NB; row < to; row += (int64_t)gridDim.z * NB) {
-        if (warp == 5) {  // copies
-            const uint32_t a_bytes = (uint32_t)min((int64_t)NB, a.pad - row) * BLOCK8, w_bytes = (uint32_t)min((int64_t)128, w.pad - col) * BLOCK8;
-            const uint32_t scale_bytes = a_bytes / BLOCK8 * sizeof(float);
-            for (int b = first; fine && b < first + blocks; ++b, stage.next(), place.next()) {
-                if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
-                if (elected()) {
-                    mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + w_bytes + scale_bytes);
-                    bulk_load(sh.w[stage.at], w.block(g, b) + col * BLOCK8, w_bytes, &sh.full[stage.at]);
-                    bulk_load(sh.a[stage.at], a.block(0, b) + row * BLOCK8, a_bytes, &sh.full[stage.at]);
-                    bulk_load(sh.scale[place.at], a.row_scales(b) + row, scale_bytes, &sh.full[stage.at]);
-                }
-                __syncwarp();
-            }
-        } else if (warp == 4) {  // matrix instructions
-            const uint64_t tile_w = tile_descriptor(smem_u32(sh.w[0])), tile_a = tile_descriptor(smem_u32(sh.a[0]));
-            for (int b = 0; fine && b < blocks; ++b, stage.next(), sums.next()) {
-                if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
-                if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
-                tmem_fence_after();
-                if (elected()) {
-                    const uint64_t dw = tile_w + (uint64_t)(stage.at * (128 * BLOCK8 >> 4)), da = tile_a + (uint64_t)(stage.at * (NB * BLOCK8 >> 4));
-#pragma unroll
-                    for (int k = 0; k < BLOCK8 / 32; ++k) mma_e4m3<false>(tmem + sums.at * NB, dw + 2 * k, da + 2 * k, product_descriptor(128, NB), k > 0);
-                    mma_commit<false>(&sh.empty[stage.at]);
-                    mma_commit<false>(&sh.sum_full[sums.at]);
-                }
-                __syncwarp();
-            }
-        } else {  // sums and stores: a thread has a column of the result
-            float acc[NB];
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[j] = 0.f;
-            const float *sw = w.tile_scales(g, col / BLOCK8) + first;
-            float tile_scale = 0.f, next_scale = lane < blocks ? ld_late(sw + lane) : 0.f;
-            for (int b = 0; fine && b < blocks; ++b, sums.next(), place.next()) {
-                if (b % 32 == 0) {
-                    tile_scale = next_scale;
-                    next_scale = b + 32 + lane < blocks ? ld_late(sw + b + 32 + lane) : 0.f;
-                }
-                const float s = __shfl_sync(FULL_MASK, tile_scale, b % 32);
-                if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
-                tmem_fence_after();
-                const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + sums.at * NB;
-                uint32_t v[NB / W][W];
-                tmem_load(at, v[0]);
-#pragma unroll
-                for (int q = 0; q < NB / W; ++q) {
-                    float row_scale[W];
-#pragma unroll
-                    for (int j = 0; j < W; j += 4) *reinterpret_cast<float4 *>(row_scale + j) = *reinterpret_cast<const float4 *>(&sh.scale[place.at][q * W + j]);
-                    tmem_wait_loads(v[q]);
-                    if (q + 1 < NB / W) {
-                        tmem_load(at + (q + 1) * W, v[q + 1]);
-                    } else {
-                        tmem_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.sum_empty[sums.at]);
+    for (int64_t col = first_col; col < end_col; col += 128) {
+        for (int64_t row = (from & ~int64_t(7)) + (int64_t)blockIdx.z * NB; row < to; row += (int64_t)gridDim.z * NB) {
+            if (warp == 5) {  // copies
+                const uint32_t a_bytes = (uint32_t)min((int64_t)NB, a.pad - row) * BLOCK8, w_bytes = (uint32_t)min((int64_t)128, w.pad - col) * BLOCK8;
+                const uint32_t scale_bytes = a_bytes / BLOCK8 * sizeof(float);
+                for (int b = first; fine && b < first + blocks; ++b, stage.next(), place.next()) {
+                    if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
+                    if (elected()) {
+                        mbar_arrive_expect_tx(&sh.full[stage.at], a_bytes + w_bytes + scale_bytes);
+                        bulk_load(sh.w[stage.at], w.block(g, b) + col * BLOCK8, w_bytes, &sh.full[stage.at]);
+                        bulk_load(sh.a[stage.at], a.block(0, b) + row * BLOCK8, a_bytes, &sh.full[stage.at]);
+                        bulk_load(sh.scale[place.at], a.row_scales(b) + row, scale_bytes, &sh.full[stage.at]);
                     }
-#pragma unroll
-                    for (int j = 0; j < W; ++j) acc[q * W + j] = __fmaf_rn(__uint_as_float(v[q][j]), s * row_scale[j], acc[q * W + j]);
+                    __syncwarp();
+                }
+            } else if (warp == 4) {  // matrix instructions
+                const uint64_t tile_w = tile_descriptor(smem_u32(sh.w[0])), tile_a = tile_descriptor(smem_u32(sh.a[0]));
+                for (int b = 0; fine && b < blocks; ++b, stage.next(), sums.next()) {
+                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                    tmem_fence_after();
+                    if (elected()) {
+                        const uint64_t dw = tile_w + (uint64_t)(stage.at * (128 * BLOCK8 >> 4)), da = tile_a + (uint64_t)(stage.at * (NB * BLOCK8 >> 4));
+    #pragma unroll
+                        for (int k = 0; k < BLOCK8 / 32; ++k) mma_e4m3<false>(tmem + sums.at * NB, dw + 2 * k, da + 2 * k, product_descriptor(128, NB), k > 0);
+                        mma_commit<false>(&sh.empty[stage.at]);
+                        mma_commit<false>(&sh.sum_full[sums.at]);
+                    }
+                    __syncwarp();
+                }
+            } else {  // sums and stores: a thread has a column of the result
+                float acc[NB];
+    #pragma unroll
+                for (int j = 0; j < NB; ++j) acc[j] = 0.f;
+                const float *sw = w.tile_scales(g, col / BLOCK8) + first;
+                float tile_scale = 0.f, next_scale = lane < blocks ? ld_late(sw + lane) : 0.f;
+                for (int b = 0; fine && b < blocks; ++b, sums.next(), place.next()) {
+                    if (b % 32 == 0) {
+                        tile_scale = next_scale;
+                        next_scale = b + 32 + lane < blocks ? ld_late(sw + b + 32 + lane) : 0.f;
+                    }
+                    const float s = __shfl_sync(FULL_MASK, tile_scale, b % 32);
+                    if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
+                    tmem_fence_after();
+                    const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + sums.at * NB;
+                    uint32_t v[NB / W][W];
+                    tmem_load(at, v[0]);
+    #pragma unroll
+                    for (int q = 0; q < NB / W; ++q) {
+                        float row_scale[W];
+    #pragma unroll
+                        for (int j = 0; j < W; j += 4) *reinterpret_cast<float4 *>(row_scale + j) = *reinterpret_cast<const float4 *>(&sh.scale[place.at][q * W + j]);
+                        tmem_wait_loads(v[q]);
+                        if (q + 1 < NB / W) {
+                            tmem_load(at + (q + 1) * W, v[q + 1]);
+                        } else {
+                            tmem_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh.sum_empty[sums.at]);
+                        }
+    #pragma unroll
+                        for (int j = 0; j < W; ++j) acc[q * W + j] = __fmaf_rn(__uint_as_float(v[q][j]), s * row_scale[j], acc[q * W + j]);
+                    }
+                }
+                const int64_t n = col + threadIdx.x;
+                if constexpr (SPLIT) {
+    #pragma unroll
+                    for (int j = 0; j < NB; ++j) sh.part[j][threadIdx.x] = acc[j];
+                } else if (fine && n < cols) {
+    #pragma unroll
+                    for (int j = 0; j < NB; ++j)
+                        if (row + j >= from && row + j < to) y[(row + j) * stride + n] = from_float<T>(acc[j]);
                 }
             }
-            const int64_t n = col + threadIdx.x;
             if constexpr (SPLIT) {
-#pragma unroll
-                for (int j = 0; j < NB; ++j) sh.part[j][threadIdx.x] = acc[j];
-            } else if (fine && n < cols) {
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-                    if (row + j >= from && row + j < to) y[(row + j) * stride + n] = from_float<T>(acc[j]);
+                cluster_sync();
+                // Eight loads of the others' parts are on their way at a time: one by one they took longer than the product.
+                if (threadIdx.x < 128 && fine && col + threadIdx.x < cols)
+                    for (int j = slice; j < NB; j += slices) {
+                        if (row + j < from || row + j >= to) continue;
+                        float part[8], sum = 0.f;
+    #pragma unroll
+                        for (int r = 0; r < 8; ++r) part[r] = r < slices ? load_remote(&sh.part[j][threadIdx.x], r) : 0.f;
+    #pragma unroll
+                        for (int r = 0; r < 8; ++r) sum += part[r];
+                        y[(row + j) * stride + col + threadIdx.x] = from_float<T>(sum);
+                    }
+                cluster_sync();  // the parts have been read, also those of a CTA that ends here
             }
-        }
-        if constexpr (SPLIT) {
-            cluster_sync();
-            // Eight loads of the others' parts are on their way at a time: one by one they took longer than the product.
-            if (threadIdx.x < 128 && fine && col + threadIdx.x < cols)
-                for (int j = slice; j < NB; j += slices) {
-                    if (row + j < from || row + j >= to) continue;
-                    float part[8], sum = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) part[r] = r < slices ? load_remote(&sh.part[j][threadIdx.x], r) : 0.f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) sum += part[r];
-                    y[(row + j) * stride + col + threadIdx.x] = from_float<T>(sum);
-                }
-            cluster_sync();  // the parts have been read, also those of a CTA that ends here
         }
     }
     if (offsets && warp < 4) {  // rows of no group
@@ -716,13 +722,17 @@ int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int g
     const int64_t wide = blocks_of(y.cols);
     const int64_t turns = groups == 1 ? (y.rows + NB - 1) / NB : 1;
     const int slices = slices_of(wide * std::min<int64_t>(groups, y.rows) * turns, a.blocks, NB >= 64);
+    // Short sums: a CTA takes several tiles of columns, one after another, while that leaves four CTAs for every SM. (Its copies run ahead from tile to tile,
+    // where a CTA's first take a microsecond or two.)
+    int each = 1;
+    while (slices == 1 && each < 8 && a.blocks * each <= 8 && wide * std::min<int64_t>(groups, y.rows) * turns >= (int64_t)8 * each * sm_count()) each *= 2;
     if (wide * slices > INT32_MAX || turns > 65535) return NB200_E_UNSUPPORTED;
     auto kernel = slices > 1 ? k_product_few<T, NB, true> : k_product_few<T, NB, false>;
     const size_t smem = slices > 1 ? FewShape<NB, true>::SHARED_BYTES : FewShape<NB, false>::SHARED_BYTES;
     NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     LaunchScope scope("fp8_product_few", stream);
-    NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)(wide * slices), (unsigned)groups, (unsigned)turns), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
-                                          static_cast<T *>(y.data), y.stride, report));
+    NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)((wide + each - 1) / each * slices), (unsigned)groups, (unsigned)turns), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
+                                          static_cast<T *>(y.data), y.stride, each, report));
     return NB200_OK;
 }
 
