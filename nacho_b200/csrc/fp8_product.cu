@@ -169,13 +169,14 @@ __device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
     for (const uint64_t start = now_ns(); now_ns() - start < SHORT_PATIENCE && !mbar_try_wait(bar, parity);) {}
 }
 
-// 32 rows of a warp, N columns from `col` on, from registers to memory, through two places in shared memory of 128 bytes of every row. WIDE: rows
-// can be written in words of 16 bytes. Then the copy engine stores a place while the next one is filled, for which all 32 rows have to count (`base`: the
+// 32 rows of a warp, N columns from `col` on, from registers to memory, through two places in shared memory of 128 bytes of every row. WORD: rows
+// can be written in words of so many bytes. With 16 the copy engine stores a place while the next one is filled, for which all 32 rows have to count (`base`: the
 // row of the matrix at which the group's rows begin; `last`: there are no rows behind the group's). Otherwise the warp reads the place again and writes
 // whole lines: 8192 x 32768 x 2048 521 us that way for all rows, 610 without shared memory.
-template <typename T, bool WIDE, int N>
+template <typename T, int WORD, int N>
 __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t (*places)[32 * 128], int &turn, const CUtensorMap *matrix, int base, bool last, T *y, int64_t stride,
                                            int row, int from, int to, int col, int cols) {
+    constexpr bool WIDE = WORD == 16;
     constexpr int PER = 128 / sizeof(T), EACH = 16 / sizeof(T);  // columns at a time; in 16 bytes
     const int lane = lane_id();
     if (row + 32 <= from || row >= to) return;
@@ -209,15 +210,17 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t (*plac
                     *reinterpret_cast<uint4 *>(y + (int64_t)(row + r) * stride + col + c + p * EACH) = *reinterpret_cast<const uint4 *>(place + piece_at(r, p));
             }
         } else {
+            constexpr int IN_WORD = WORD / sizeof(T);
             __syncwarp();
 #pragma unroll 8
             for (int r = 0; r < 32; ++r) {
                 const bool there = row + r >= from && row + r < to;
 #pragma unroll
-                for (int i = 0; i < PER; i += 32) {
-                    const int j = i + lane;
+                for (int i = 0; i < PER; i += 32 * IN_WORD) {
+                    const int j = i + lane * IN_WORD;
                     if (there && col + c + j < cols)
-                        y[(int64_t)(row + r) * stride + col + c + j] = *reinterpret_cast<const T *>(place + piece_at(r, j / EACH) + j % EACH * sizeof(T));
+                        *reinterpret_cast<Vec<T, IN_WORD> *>(y + (int64_t)(row + r) * stride + col + c + j) =
+                            *reinterpret_cast<const Vec<T, IN_WORD> *>(place + piece_at(r, j / EACH) + j % EACH * sizeof(T));
                 }
             }
         }
@@ -233,10 +236,11 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t (*plac
 // GRAD: the sums run over a group's blocks of rows of dy and x, `offsets` says where those begin, and columns have a scale each. The scales of
 // both are multiplied for every element, which is as much arithmetic again.
 // SELFTEST: the first block's copies are left out, so that every warp's wait runs out.
-template <typename T, bool WIDE, bool PAIR, bool GRAD, bool SELFTEST = false>
+template <typename T, int WORD, bool PAIR, bool GRAD, bool SELFTEST = false>
 __device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                         unsigned long long *report, const CUtensorMap *matrix) {
     using S = Shape<PAIR>;
+    constexpr bool WIDE = WORD == 16;
     constexpr int STAGES = S::STAGES, SUMS = S::SUMS, BN = S::BN, N = BN / 2, W = 16;
     extern __shared__ uint8_t raw[];
     typename S::Shared &sh = *reinterpret_cast<typename S::Shared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -326,7 +330,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
             }
             if (!fine) break;
             if (col < cols)
-                store_rows<T, WIDE, N>(acc, sh.out[warp], turn, matrix, GRAD ? t.g * (int)rows : 0, GRAD ? t.g == groups - 1 : t.to == rows, GRAD ? y + t.g * rows * stride : y,
+                store_rows<T, WORD, N>(acc, sh.out[warp], turn, matrix, GRAD ? t.g * (int)rows : 0, GRAD ? t.g == groups - 1 : t.to == rows, GRAD ? y + t.g * rows * stride : y,
                                        stride, (int)row, t.from, t.to, (int)col, (int)cols);
         }
         if (WIDE && elected()) stores_done();
@@ -414,19 +418,19 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
     }
 }
 
-template <typename T, bool WIDE, bool GRAD>
+template <typename T, int WORD, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
                                                         unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
-    product<T, WIDE, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
+    product<T, WORD, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
 }
 __global__ void __launch_bounds__(THREADS, 1) k_product_selftest(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, float *y, int64_t stride,
                                                                  unsigned long long *report) {
-    product<float, false, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, report, nullptr);
+    product<float, 4, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, report, nullptr);
 }
-template <typename T, bool WIDE, bool GRAD>
+template <typename T, int WORD, bool GRAD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_product_pair(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y,
                                                                                        int64_t stride, unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
-    product<T, WIDE, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
+    product<T, WORD, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
 }
 
 // ---- few rows per group ------------------------------------------------------------------
@@ -782,8 +786,15 @@ int launch_product(const char *name, bool pair, int64_t tiles, const Operand &a,
                                      GRAD ? y.rows / groups : y.rows, y.cols, static_cast<T *>(y.data), y.stride, report, matrix));
         return NB200_OK;
     };
-    if (pair) return wide ? go(k_product_pair<T, true, GRAD>, Shape<true>::SHARED_BYTES, 2) : go(k_product_pair<T, false, GRAD>, Shape<true>::SHARED_BYTES, 2);
-    return wide ? go(k_product<T, true, GRAD>, Shape<false>::SHARED_BYTES, 1) : go(k_product<T, false, GRAD>, Shape<false>::SHARED_BYTES, 1);
+    const int word = wide ? 16 : std::min(word_bytes({&y}), 4);
+    auto sized = [&](auto bytes) {
+        constexpr int WORD = decltype(bytes)::value;
+        return pair ? go(k_product_pair<T, WORD, GRAD>, Shape<true>::SHARED_BYTES, 2) : go(k_product<T, WORD, GRAD>, Shape<false>::SHARED_BYTES, 1);
+    };
+    if (word == 16) return sized(std::integral_constant<int, 16>{});
+    if constexpr (sizeof(T) == 2)
+        if (word == 2) return sized(std::integral_constant<int, 2>{});
+    return sized(std::integral_constant<int, 4>{});
 }
 
 struct GradScratch {
