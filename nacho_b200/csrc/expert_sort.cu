@@ -35,7 +35,7 @@ struct Order {
 
 // ---- the order -------------------------------------------------------------------------
 
-constexpr int MAX_TILES = 256;
+constexpr int MAX_TILES = 256, AT_ONCE = 8;  // entries per thread that are on their way together
 
 // How often each key occurs in this CTA's tile of entries: counts[tile][key].
 __global__ void __launch_bounds__(NT) k_order_count(Order o, int tile, int32_t *counts) {
@@ -70,9 +70,13 @@ __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles
     const int64_t end = min(begin + tile / (NT / 32), (int64_t)o.entries);
     const int lo = o.entry_of(0), hi = o.entry_of(o.tokens);
     auto key_of = [&](int64_t e) { return e < end && e >= lo && e < hi ? o.key((int)e) : o.experts; };
-    for (int64_t e = begin + lane; e - lane < end; e += 32) {
-        const int k = key_of(e);
-        if (k < o.experts) atomicAdd(&mine[k], 1);
+    for (int64_t e0 = begin + lane; e0 - lane < end; e0 += 32 * AT_ONCE) {
+        int key[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) key[u] = key_of(e0 + 32 * u);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            if (key[u] < o.experts) atomicAdd(&mine[key[u]], 1);
     }
     // an expert's entries in all tiles and in the tiles before, all threads over all counts, eight of them on their way at a time
     for (int k = threadIdx.x; k < 2 * o.experts; k += NT) total[k] = 0;
@@ -109,16 +113,22 @@ __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) o.offsets[o.experts] = base;
     __syncthreads();
-    for (int64_t e = begin + lane; e - lane < end; e += 32) {
-        const int k = key_of(e);
-        const unsigned same = __match_any_sync(FULL_MASK, k);
-        const int rank = __popc(same & ((1u << lane) - 1));
-        int slot = -1;
-        if (k < o.experts) slot = mine[k] + rank;
-        __syncwarp();
-        if (k < o.experts && rank == 0) mine[k] += __popc(same);
-        __syncwarp();
-        if (e < end) o.slots[e] = slot;
+    for (int64_t e0 = begin + lane; e0 - lane < end; e0 += 32 * AT_ONCE) {
+        int key[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) key[u] = key_of(e0 + 32 * u);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int k = key[u];
+            const unsigned same = __match_any_sync(FULL_MASK, k);
+            const int rank = __popc(same & ((1u << lane) - 1));
+            int slot = -1;
+            if (k < o.experts) slot = mine[k] + rank;
+            __syncwarp();
+            if (k < o.experts && rank == 0) mine[k] += __popc(same);
+            __syncwarp();
+            if (e0 + 32 * u < end) o.slots[e0 + 32 * u] = slot;
+        }
     }
 }
 
@@ -235,10 +245,11 @@ struct Entries {
     }
 };
 
-// The same into 8-bit rows: 16 threads have a block of 128 columns, quantise it once and write it to all of the token's slots.
-template <typename T, int V>
+// The same into 8-bit rows: 16 threads have a block of 128 columns, quantise it once and write it to all of the token's slots. Bound by its
+// instructions: 65536 rows of 4096 from 16384 tokens take 69 % of the issue slots.
+template <typename T, int V, int N>
 __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const T *x, int64_t stride, int64_t cols, uint8_t *codes, float *scales) {
-    constexpr int N = 8, U = 2;
+    constexpr int U = 2;
     wait_for_previous();
     trigger_dependents();
     const Team team(tpr);
@@ -246,9 +257,15 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
     const unsigned half = 0xffffu << (threadIdx.x & 16);
     const int64_t pad = padded_rows(o.entries);
     const int kb = (int)blocks_of(cols);
+    auto place_of = [&](int s) { return codes + piece_at(s, sub >> 1) + (sub & 1) * 8; };
     Entries<N> at(o, nullptr, team.first, team.step);
     while (at.advance()) {
         const T *row = x + at.t * stride;
+        uint8_t *place[N];  // kept where registers last
+        if constexpr (N == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) place[i] = place_of(at.slot[i]);
+        }
         for (int b = mine; b < kb; b += blocks * U) {
             Eight<T> v[U];
 #pragma unroll
@@ -277,14 +294,17 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
                 if (b + u * blocks >= kb) break;
                 const int64_t block = (int64_t)(b + u * blocks) * pad;
                 const uint2 q = codes8(v[u], f[u].inverse);
-                auto put = [&](int s) {
+                auto put = [&](uint8_t *to, int s) {
                     if (s < 0) return;
-                    *reinterpret_cast<uint2 *>(codes + block * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = q;
+                    *reinterpret_cast<uint2 *>(to + block * BLOCK8) = q;
                     if (sub == 0) scales[block + s] = f[u].scale;
                 };
 #pragma unroll
-                for (int i = 0; i < N; ++i) put(at.slot[i]);
-                for (int e = at.e0 + N; e < at.e1; ++e) put(o.slot(e));
+                for (int i = 0; i < N; ++i) put(N == 4 ? place[i] : place_of(at.slot[i]), at.slot[i]);
+                for (int e = at.e0 + N; e < at.e1; ++e) {
+                    const int s = o.slot(e);
+                    put(place_of(s), s);
+                }
             }
         }
         if (mine >= kb) at.ask_next();
@@ -647,7 +667,7 @@ int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert
                                              x->stride, x->cols, xs->values, xs->scales));
                 return (int)NB200_OK;
             }
-            auto kernel = k_sort_rows_fp8<T, decltype(v)::value>;
+            auto kernel = many_entries(o) ? k_sort_rows_fp8<T, decltype(v)::value, 8> : k_sort_rows_fp8<T, decltype(v)::value, 4>;
             LaunchScope scope("sort_rows_fp8", stream);
             NB200_CUDA(launch_overlapped(kernel, resident_grid(kernel, o.tokens, tpr), dim3(NT), 0, stream, o, tpr, static_cast<const T *>(x->data), x->stride, x->cols, xs->values,
                                          xs->scales));
