@@ -435,8 +435,9 @@ __global__ void __launch_bounds__(NT, N == 8 ? 2 : 3) k_unsort_grad(Order o, int
 // ---- few entries: all in one launch ------------------------------------------------------
 
 // Up to this many entries, every CTA counts all of them: that takes less than a launch. Its own tokens' entries follow from the totals and
-// from the counts of those in front of them. 4096 entries, 1024 tokens of 2048: 8.3 us where two launches for the order in front take 14.7.
-constexpr int FEW_ENTRIES = 4096;
+// from the counts of those in front of them. Order and rows of 2048 16-bit elements, us, by 8 / 64 / 256 experts: 2048 entries 7.6 / 9.8 / 10.4 where
+// two launches for the order in front take 11.5 / 11.3 / 11.4; 4096 entries 10.8 / 14.5 / 15.5 against 11.5 / 11.6 / 12.2.
+constexpr int FEW_ENTRIES = 2560;
 
 // Slots of the entries of tokens t0 .. t1 - 1, the offsets, and how many entries are kept (returned). counts: two words per expert.
 __device__ int place_few(const Order &o, int t0, int t1, int32_t *counts) {

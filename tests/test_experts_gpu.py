@@ -70,6 +70,7 @@ ROUTINGS = {
     "one_expert": dict(tokens=500, experts=1, k=2), "most_experts": dict(tokens=700, experts=4096, k=8, ragged=True, drop=0.1),
     "part": dict(tokens=60, experts=7, k=4, ragged=True, drop=0.1, lead=37, tail=1030), "long_row": dict(tokens=2, experts=6, k=5000, drop=0.05),
     "tiles": dict(tokens=30011, experts=61, k=7, ragged=True, drop=0.02), "many_tiles": dict(tokens=200003, experts=300, k=6, ragged=True, drop=0.1, lead=5, tail=9),
+    "edge_2559": dict(tokens=2559, experts=64, k=1), "edge_2560": dict(tokens=512, experts=300, k=5), "edge_2561": dict(tokens=2561, experts=64, k=1),
     "edge_8191": dict(tokens=8191, experts=64, k=1), "edge_8192": dict(tokens=1024, experts=64, k=8), "edge_8193": dict(tokens=8193, experts=64, k=1),
 }
 
