@@ -84,6 +84,13 @@ inline int sm_count() {
     return count;
 }
 
+// What the runtime is asked once per device and kernel (a microsecond each time): a limit of dynamic shared memory that has been raised, and how
+// many CTAs of so many threads an SM holds.
+int allow_shared_memory(const void *kernel, size_t bytes);
+int resident_ctas(const void *kernel, int threads);
+template <typename... P>
+int allow_shared(void (*kernel)(P...), size_t bytes) { return allow_shared_memory(reinterpret_cast<const void *>(kernel), bytes); }
+
 // Calls f(T{}) with the element type.
 template <typename F>
 int with_type(int type, F f) {

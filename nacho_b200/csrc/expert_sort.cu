@@ -555,8 +555,7 @@ dim3 grid_of(int64_t teams, int tpr) {
 // As many CTAs as can be at work at once, or fewer where there are fewer teams' worth of tokens.
 template <typename... P>
 dim3 resident_grid(void (*kernel)(P...), int64_t teams, int tpr) {
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, NT, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+    const int per_sm = resident_ctas(reinterpret_cast<const void *>(kernel), NT);
     const int64_t ctas = (teams * tpr + NT - 1) / NT;
     return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, (int64_t)sm_count() * per_sm)));
 }
@@ -603,7 +602,7 @@ int make_order(const Order &o, cudaStream_t stream) {
     if ((st = acquire_workspace(stream, sizeof(int32_t) * (size_t)tiles * std::max(o.experts, 1), &ws, ORDER_SLOT))) return st;
     int32_t *counts = static_cast<int32_t *>(ws->dev);
     const size_t count_smem = sizeof(int32_t) * o.experts, place_smem = sizeof(int32_t) * o.experts * (NT / 32 + 2);
-    if (place_smem > 48 * 1024) NB200_CUDA(cudaFuncSetAttribute(k_order_place, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem));
+    if (place_smem > 48 * 1024 && (st = allow_shared(k_order_place, place_smem))) return st;
     {
         LaunchScope scope("order_count", stream);
         NB200_CUDA(launch_overlapped(k_order_count, dim3(tiles), dim3(NT), count_smem, stream, o, tile, counts));

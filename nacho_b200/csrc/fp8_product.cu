@@ -86,19 +86,21 @@ __device__ __forceinline__ void place_tile(int within, int high, int wide, int *
     *col = (int)column;
 }
 
-// Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order.
+// Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order. `most`: as many as there
+// are with offsets that rise; others end there.
 template <int BM, int BN, int PANEL>
 struct Walk {
     const int32_t *offsets;
-    int groups, blocks, rows, col_tiles;
+    int groups, blocks, rows, col_tiles, most;
     int chunk = -32, base = 0, incl = 0;  // tiles of the groups before this chunk; of this chunk's groups up to the lane's
     int from = 0, to = 0;
 
-    __device__ Walk(const int32_t *o, int g, int b, int r, int c) : offsets(o), groups(g), blocks(b), rows(r), col_tiles((c + BN - 1) / BN) {}
+    __device__ Walk(const int32_t *o, int g, int b, int r, int c, int m) : offsets(o), groups(g), blocks(b), rows(r), col_tiles((c + BN - 1) / BN), most(m) {}
 
     __device__ static int row_tiles(int from, int to) { return to > from ? (to - (from & ~7) + BM - 1) / BM : 0; }
 
     __device__ bool find(int tile, Tile &t) {
+        if (tile >= most) return false;
         int total;
         while (total = __shfl_sync(FULL_MASK, incl, 31), tile >= base + total) {
             base += total;
@@ -110,7 +112,7 @@ struct Walk {
                 from = offsets ? min(max(ld_late(offsets + g), 0), rows) : 0;
                 to = offsets ? min(max(ld_late(offsets + g + 1), from), rows) : rows;
             }
-            incl = warp_incl_sum(row_tiles(from, to) * col_tiles);
+            incl = warp_incl_sum(min(row_tiles(from, to) * col_tiles, most));
         }
         const int src = __ffs(__ballot_sync(FULL_MASK, base + incl > tile)) - 1;
         t.g = chunk + src;
@@ -238,7 +240,7 @@ __device__ __forceinline__ void store_rows(const float (&acc)[N], uint8_t (*plac
 // SELFTEST: the first block's copies are left out, so that every warp's wait runs out.
 template <typename T, int WORD, bool PAIR, bool GRAD, bool SELFTEST = false>
 __device__ __forceinline__ void product(const Operand &a, const Operand &w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
-                                        unsigned long long *report, const CUtensorMap *matrix) {
+                                        int most, unsigned long long *report, const CUtensorMap *matrix) {
     using S = Shape<PAIR>;
     constexpr bool WIDE = WORD == 16;
     constexpr int STAGES = S::STAGES, SUMS = S::SUMS, BN = S::BN, N = BN / 2, W = 16;
@@ -266,7 +268,7 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
     const int first = blockIdx.x / S::CTAS, step = gridDim.x / S::CTAS;
     auto tiles = [&] {
         if constexpr (GRAD) return GradWalk<S::BM, BN, S::PANEL>{offsets, groups, (int)rows, (int)cols};
-        else return Walk<S::BM, BN, S::PANEL>(offsets, groups, (int)a.blocks, (int)rows, (int)cols);
+        else return Walk<S::BM, BN, S::PANEL>(offsets, groups, (int)a.blocks, (int)rows, (int)cols, most);
     };
     if (warp < STORE_WARPS) {
         // sums and stores: warps w and w + 4 have the lanes of tensor memory that every fourth warp can reach, and a half of the columns each
@@ -420,17 +422,17 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &w, cons
 
 template <typename T, int WORD, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 1) k_product(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y, int64_t stride,
-                                                        unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
-    product<T, WORD, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
+                                                        int most, unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
+    product<T, WORD, false, GRAD>(a, w, offsets, groups, rows, cols, y, stride, most, report, &matrix);
 }
 __global__ void __launch_bounds__(THREADS, 1) k_product_selftest(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, float *y, int64_t stride,
                                                                  unsigned long long *report) {
-    product<float, 4, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, report, nullptr);
+    product<float, 4, false, false, true>(a, w, offsets, groups, rows, cols, y, stride, 1 << 20, report, nullptr);
 }
 template <typename T, int WORD, bool GRAD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) k_product_pair(Operand a, Operand w, const int32_t *offsets, int groups, int64_t rows, int64_t cols, T *y,
-                                                                                       int64_t stride, unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
-    product<T, WORD, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, report, &matrix);
+                                                                                       int64_t stride, int most, unsigned long long *report, const __grid_constant__ CUtensorMap matrix) {
+    product<T, WORD, true, GRAD>(a, w, offsets, groups, rows, cols, y, stride, most, report, &matrix);
 }
 
 // ---- few rows per group ------------------------------------------------------------------
@@ -737,7 +739,7 @@ int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int g
     if (wide * slices > INT32_MAX || turns > 65535) return NB200_E_UNSUPPORTED;
     auto kernel = slices > 1 ? k_product_few<T, NB, true> : k_product_few<T, NB, false>;
     const size_t smem = slices > 1 ? FewShape<NB, true>::SHARED_BYTES : FewShape<NB, false>::SHARED_BYTES;
-    NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if ((st = allow_shared(kernel, smem))) return st;
     LaunchScope scope("fp8_product_few", stream);
     NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)((wide + each - 1) / each * slices), (unsigned)groups, (unsigned)turns), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
                                           static_cast<T *>(y.data), y.stride, each, report));
@@ -781,10 +783,10 @@ int launch_product(const char *name, bool pair, int64_t tiles, const Operand &a,
     CUtensorMap matrix{};
     if (wide && (st = describe(y, &matrix))) return st;
     auto go = [&](auto kernel, size_t smem, int ctas) -> int {
-        NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if ((st = allow_shared(kernel, smem))) return st;
         LaunchScope scope(name, stream);
         NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)std::min<int64_t>(tiles * ctas, sm_count() / ctas * ctas)), dim3(THREADS), smem, stream, a, w, offsets, groups,
-                                     GRAD ? y.rows / groups : y.rows, y.cols, static_cast<T *>(y.data), y.stride, report, matrix));
+                                     GRAD ? y.rows / groups : y.rows, y.cols, static_cast<T *>(y.data), y.stride, (int)tiles, report, matrix));
         return NB200_OK;
     };
     const int word = wide ? 16 : std::min(word_bytes({&y}), 4);
@@ -865,7 +867,7 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     const int64_t groups = w->groups, mean = (y->rows + groups - 1) / groups, singles = blocks_of(y->rows) * blocks_of(y->cols);
     const bool one = groups == 1, idle = 2 * singles <= sm_count(), pair = mean >= 112 && singles > sm_count();
     const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * groups) * ((y->cols + side - 1) / side);
-    if (tiles > INT32_MAX / 2 || y->rows > INT32_MAX - 1024 || y->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
+    if (tiles > INT32_MAX / 64 || y->rows > INT32_MAX - 1024 || y->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     return with_type(y->type, [&](auto e) {
         using T = decltype(e);
         if (mean <= (one ? 16 : 5)) return launch_few<T, 16>(oa, ow, offsets, w->groups, *y, stream);
@@ -886,7 +888,7 @@ int nb200_selftest_product_timeout(const nb200_fp8 *a, const nb200_fp8 *w, nb200
     if ((st = report_of(stream, &ws))) return st;
     const Operand oa{a->values, a->scales, blocks_of(a->cols), padded_rows(a->rows), 0};
     const Operand ow{w->values, w->scales, blocks_of(w->cols), padded_rows(w->rows), blocks_of(w->rows)};
-    NB200_CUDA(cudaFuncSetAttribute(k_product_selftest, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<false>::SHARED_BYTES));
+    if ((st = allow_shared(k_product_selftest, Shape<false>::SHARED_BYTES))) return st;
     LaunchScope scope("fp8_product_selftest", stream);
     NB200_CUDA(launch_overlapped(k_product_selftest, dim3(1), dim3(THREADS), Shape<false>::SHARED_BYTES, stream, oa, ow, (const int32_t *)nullptr, 1, y->rows, y->cols,
                                  static_cast<float *>(y->data), y->stride, reinterpret_cast<unsigned long long *>(ws->host) + 32));
@@ -917,7 +919,7 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
     const nb200_dense result{(int64_t)groups * dy->cols, x->cols, x->cols, NB200_F32, z};
     const bool pair = dy->cols > 128 && x->cols > 128;
     const int64_t side = pair ? 256 : 128, tiles = groups * ((dy->cols + side - 1) / side) * ((x->cols + side - 1) / side);
-    if (tiles > INT32_MAX / 2 || dy->cols > INT32_MAX - 1024 || x->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
+    if (tiles > INT32_MAX / 64 || dy->cols > INT32_MAX - 1024 || x->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     return launch_product<float, true>("fp8_grad_w", pair, tiles, od, ox, s.first_block, groups, result, stream);
 }
 

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "dense_rows.cuh"
 
 namespace nb200 {
 
@@ -175,6 +176,36 @@ int wait_result_word(const unsigned long long *word, cudaStream_t stream, int64_
     if (*device_status != 0) spoil_tagged(stream);
     *value = (int64_t)(v & RW_VALUE_MASK);
     return NB200_OK;
+}
+
+namespace {
+// Per device and kernel: the shared memory allowed so far, and the CTAs per SM (0: not asked yet).
+struct KernelFacts {
+    size_t shared = 48 * 1024;
+    int resident = 0;
+};
+std::mutex g_facts_mutex;
+std::map<std::pair<int, const void *>, KernelFacts> g_facts;
+}  // namespace
+
+int allow_shared_memory(const void *kernel, size_t bytes) {
+    int dev = 0;
+    NB200_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> g(g_facts_mutex);
+    KernelFacts &f = g_facts[{dev, kernel}];
+    if (bytes <= f.shared) return NB200_OK;
+    NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    f.shared = bytes;
+    return NB200_OK;
+}
+
+int resident_ctas(const void *kernel, int threads) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    std::lock_guard<std::mutex> g(g_facts_mutex);
+    KernelFacts &f = g_facts[{dev, kernel}];
+    if (!f.resident && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&f.resident, kernel, threads, 0) != cudaSuccess || f.resident < 1)) f.resident = 1;
+    return f.resident;
 }
 
 uint64_t workspace_epoch() { return g_ws_epoch.load(std::memory_order_acquire); }

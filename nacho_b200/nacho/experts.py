@@ -169,8 +169,8 @@ def gpu_fp8_product_grad(dy: torch.Tensor, x: torch.Tensor, w: FP8_gpu, order: E
     if not isinstance(w, FP8_gpu) or not w.tiled:
         raise TypeError("gpu_fp8_product_grad: w must be an FP8_gpu with a scale per tile")
     dx_type = _TYPES.get(getattr(dy, "dtype", None))
-    if dx_type is None:
-        raise TypeError("gpu_fp8_product_grad: dy must be a CUDA tensor of rows of float32, float16 or bfloat16")
+    if dx_type is None or not isinstance(x, torch.Tensor):
+        raise TypeError("gpu_fp8_product_grad: dy and x must be CUDA tensors of rows of float32, float16 or bfloat16")
     groups, n, inner = w._dims
     if dy.dim() != 2 or dy.shape[1] != n or x.dim() != 2 or x.shape[1] != inner:
         raise ValueError(f"gpu_fp8_product_grad: dy and x must have {n} and {inner} columns")

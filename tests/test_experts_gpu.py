@@ -532,3 +532,20 @@ def test_a_wait_that_gives_up_is_reported_by_the_next_product():
     with pytest.raises(RuntimeError, match="earlier 8-bit product: matrix product pipeline gave up"):
         n.gpu_fp8_product(a, w)
     assert torch.equal(n.gpu_fp8_product(a, w, dtype=torch.float32), want)
+
+
+def test_offsets_that_fall_end():
+    """Offsets that rise and fall again and again stand for more tiles than a matrix has: the product ends after as many as rising ones have."""
+    n = nacho()
+    rows, groups = 60000, 400
+    zigzag = torch.arange(groups + 1, device="cuda", dtype=torch.int32) % 2 * rows
+    nobody = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    order = n.ExpertOrder_gpu(zigzag, nobody, nobody, torch.zeros(1, dtype=torch.int32, device="cuda"), (0, groups))
+    a, w = n.to_fp8_rows(normal((rows, 128), torch.bfloat16, 1)), n.to_fp8_tiles(normal((groups, 256, 128), torch.bfloat16, 2))
+    start, stop = torch.cuda.Event(True), torch.cuda.Event(True)
+    n.gpu_fp8_product(a, w, order)
+    start.record()
+    n.gpu_fp8_product(a, w, order)
+    stop.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(stop) < 20  # ms; all of its tiles would be 200 products of the matrix
