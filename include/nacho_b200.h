@@ -422,9 +422,11 @@ int nb200_fp8_transpose(const nb200_fp8 *a, nb200_fp8 *z, void *stream);
  * the tensor cores and the blocks, times their two scales, in 32 bits. */
 int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *offsets, nb200_dense *y, void *stream);
 /* The gradient for the weights: z[g] = sum over the rows i of group g of dy[i]^T x[i], z = [groups][dy->cols][x->cols] 32-bit. Both
- * operands are quantised along the rows, a scale for every column and 128 rows counted from the group's first. */
+ * operands are quantised along the rows, a scale for every column and 128 rows counted from the group's first. With
+ * `dy_rows` (or NULL), the rows of dy that belong to a group are quantised into it as nb200_fp8_quantise would, in the same pass: the left operand of
+ * the gradient for x, dy * w, whose right one is nb200_fp8_transpose of w. Rows of no group are left as they are. */
 int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_t groups, const int32_t *offsets, float *z,
-                             void *scratch, int64_t scratch_bytes, void *stream);
+                             nb200_fp8 *dy_rows, void *scratch, int64_t scratch_bytes, void *stream);
 /* Bytes of scratch, 256-byte aligned device memory, that it needs: the quantised operands; -1 for impossible operands. */
 int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dense *x, int32_t groups);
 

@@ -128,7 +128,7 @@ PROTOTYPES = {
     "nb200_fp8_unpack": (C.c_int, [_P(Fp8Struct), C.c_void_p, C.c_void_p]),
     "nb200_fp8_transpose": (C.c_int, [_P(Fp8Struct), _P(Fp8Struct), C.c_void_p]),
     "nb200_fp8_product": (C.c_int, [_P(Fp8Struct), _P(Fp8Struct), C.c_void_p, _P(DenseStruct), C.c_void_p]),
-    "nb200_fp8_product_grad_w": (C.c_int, [_P(DenseStruct)] * 2 + [C.c_int32] + [C.c_void_p] * 3 + [C.c_int64, C.c_void_p]),
+    "nb200_fp8_product_grad_w": (C.c_int, [_P(DenseStruct)] * 2 + [C.c_int32, C.c_void_p, C.c_void_p, _P(Fp8Struct), C.c_void_p, C.c_int64, C.c_void_p]),
     "nb200_selftest_product_timeout": (C.c_int, [_P(Fp8Struct)] * 2 + [_P(DenseStruct), C.c_void_p]),
     "nb200_fp8_product_grad_w_scratch": (C.c_int64, [_P(DenseStruct)] * 2 + [C.c_int32]),
 }

@@ -638,8 +638,10 @@ __global__ void __launch_bounds__(1024) k_group_blocks(const int32_t *offsets, i
 // x by blocks of rows: column c becomes row c of the result, a scale for it per block. A CTA per block and 128 columns: a thread has eight columns of
 // eight rows, the largest magnitude of a column comes from 16 threads by way of shared memory, and the codes go through shared memory to whole
 // lines. There the eight codes of a column and eight rows p lie at place p ^ (column / 8) of the column's, which spreads a warp over the banks.
-template <typename T, int V>
-__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(const T *x, int64_t stride, int64_t cols, const int2 *block, uint8_t *values, float *scales) {
+// ROWS: the same elements quantised along the columns too, which reads them once for both: the 16 threads of a row have its block of 128.
+template <typename T, int V, bool ROWS>
+__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(const T *x, int64_t stride, int64_t cols, const int2 *block, uint8_t *values, float *scales,
+                                                                              uint8_t *row_values, float *row_scales, int64_t row_pad) {
     __shared__ uint32_t top[NT / 32][BLOCK8];  // words
     __shared__ alignas(16) float inverse[BLOCK8];
     __shared__ alignas(16) uint2 codes[BLOCK8][16];
@@ -654,6 +656,28 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(cons
     for (int i = 0; i < 8; ++i) {
         const int r = part * 8 + i;
         v[i].template load<V>(x + (int64_t)(rows.x + min(r, rows.y - 1)) * stride, c0 + sub * 8, r < rows.y ? cols : 0);
+    }
+    if constexpr (ROWS) {
+        const unsigned half = 0xffffu << (threadIdx.x & 16);
+        uint32_t top_of[8];
+        Factors f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            Top<T> row;
+            row.add(v[i]);
+#pragma unroll
+            for (int d = 8; d; d >>= 1) row.join(half, d);
+            top_of[i] = row.bits();
+        }
+        share_factors<8>(half, top_of, f);
+        const int64_t at = c0 / BLOCK8 * row_pad + rows.x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = part * 8 + i;
+            if (r >= rows.y) break;
+            *reinterpret_cast<uint2 *>(row_values + c0 / BLOCK8 * row_pad * BLOCK8 + piece_at(rows.x + r, sub >> 1) + (sub & 1) * 8) = codes8(v[i], f[i].inverse);
+            if (sub == 0) row_scales[at + r] = f[i].scale;
+        }
     }
     // words of a row: a column each, or two neighbours
     constexpr int WORDS = Eight<T>::WORDS, EACH = 4 / sizeof(T);
@@ -825,7 +849,8 @@ bool grad_ok(const nb200_dense *dy, const nb200_dense *x, int32_t groups) {
     return dense_ok(dy) && dense_ok(x) && dy->rows == x->rows && dy->type == x->type && groups >= 0 && dy->rows <= INT32_MAX - BLOCK8 && dy->cols <= INT32_MAX && x->cols <= INT32_MAX;
 }
 
-int quantise_columns(const nb200_dense *x, const int2 *block, int64_t bound, uint8_t *values, float *scales, cudaStream_t stream) {
+// `rows`: x quantised by rows too, or none.
+int quantise_columns(const nb200_dense *x, const int2 *block, int64_t bound, uint8_t *values, float *scales, const nb200_fp8 *rows, cudaStream_t stream) {
     const int64_t ctas = bound * blocks_of(x->cols);
     if (ctas == 0) return NB200_OK;
     if (ctas > INT32_MAX) return NB200_E_UNSUPPORTED;
@@ -833,9 +858,10 @@ int quantise_columns(const nb200_dense *x, const int2 *block, int64_t bound, uin
         using T = decltype(e);
         return with_vector<T>(word_bytes({x}), [&](auto v) {
             constexpr int V = decltype(v)::value;
-            LaunchScope scope("fp8_columns", stream);
-            NB200_CUDA(launch_overlapped(k_fp8_columns<T, V>, dim3((unsigned)ctas), dim3(NT), 0, stream, static_cast<const T *>(x->data), x->stride, x->cols, block, values,
-                                         scales));
+            auto kernel = rows ? k_fp8_columns<T, V, true> : k_fp8_columns<T, V, false>;
+            LaunchScope scope(rows ? "fp8_columns_rows" : "fp8_columns", stream);
+            NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(NT), 0, stream, static_cast<const T *>(x->data), x->stride, x->cols, block, values, scales,
+                                         rows ? rows->values : nullptr, rows ? rows->scales : nullptr, padded_rows(x->rows)));
             return (int)NB200_OK;
         });
     });
@@ -899,12 +925,14 @@ int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dens
     return grad_ok(dy, x, groups) ? (int64_t)GradScratch(nullptr, dy, x, groups).bytes : -1;
 }
 
-int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_t groups, const int32_t *offsets, float *z, void *scratch, int64_t scratch_bytes, void *stream_) {
+int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_t groups, const int32_t *offsets, float *z, nb200_fp8 *dy_rows, void *scratch,
+                             int64_t scratch_bytes, void *stream_) {
     if (!grad_ok(dy, x, groups) || (!offsets && groups != 1)) return NB200_E_BADARG;
+    if (dy_rows && (!fp8_ok(dy_rows) || dy_rows->tiled || dy_rows->groups != 1 || dy_rows->rows != dy->rows || dy_rows->cols != dy->cols)) return NB200_E_BADARG;
     if (groups > NB200_MAX_EXPERTS) return NB200_E_UNSUPPORTED;
-    if (groups == 0 || dy->cols == 0 || x->cols == 0) return NB200_OK;
+    if (groups == 0 || dy->cols == 0 || (x->cols == 0 && !dy_rows)) return NB200_OK;
     const GradScratch s(scratch, dy, x, groups);
-    if (!z || !scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return NB200_E_BADARG;
+    if ((!z && x->cols > 0) || !scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return NB200_E_BADARG;
     if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     {
@@ -912,8 +940,9 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
         NB200_CUDA(launch_overlapped(k_group_blocks, dim3(1), dim3(1024), 0, stream, offsets, groups, (int)dy->rows, (int)s.bound, s.first_block, s.block));
     }
     int st;
-    if ((st = quantise_columns(dy, s.block, s.bound, s.d, s.ds, stream))) return st;
-    if ((st = quantise_columns(x, s.block, s.bound, s.x, s.xs, stream))) return st;
+    if ((st = quantise_columns(dy, s.block, s.bound, s.d, s.ds, dy_rows, stream))) return st;
+    if (x->cols == 0) return NB200_OK;
+    if ((st = quantise_columns(x, s.block, s.bound, s.x, s.xs, nullptr, stream))) return st;
     const Operand od{s.d, s.ds, s.bound, padded_rows(dy->cols), 0};
     const Operand ox{s.x, s.xs, s.bound, padded_rows(x->cols), 0};
     const nb200_dense result{(int64_t)groups * dy->cols, x->cols, x->cols, NB200_F32, z};

@@ -718,7 +718,7 @@ PyObject *fp8_product(PyObject *const *args) {
     return wrap(y);
 }
 
-// fp8_grad_w(dy, x, order or None, groups)
+// fp8_grad_w(dy, x, order or None, groups): the weights' gradient and dy quantised by rows
 PyObject *fp8_grad_w(PyObject *const *args) {
     const char *where = "gpu_fp8_product_grad";
     View vd, vx, vo;
@@ -733,8 +733,10 @@ PyObject *fp8_grad_w(PyObject *const *args) {
     const int64_t bytes = nb200_fp8_product_grad_w_scratch(&dy, &x, (int32_t)groups);
     if (bytes < 0) check(NB200_E_BADARG, where);
     at::Tensor scratch = array(bytes, at::kByte, vd.device), z = at::Tensor(at::detail::empty_cuda({groups, dy.cols, x.cols}, at::kFloat, vd.device, std::nullopt));
-    launch({&vd, &vx, &vo}, where, [&](void *stream) { return nb200_fp8_product_grad_w(&dy, &x, (int32_t)groups, offsets, floats(z), scratch.data_ptr(), bytes, stream); });
-    return wrap(z);
+    Fp8Result rows(1, dy.rows, dy.cols, false, vd.device);
+    launch({&vd, &vx, &vo}, where,
+           [&](void *stream) { return nb200_fp8_product_grad_w(&dy, &x, (int32_t)groups, offsets, floats(z), &rows.m, scratch.data_ptr(), bytes, stream); });
+    return two(wrap(z), rows.object());
 }
 
 // ---- module --------------------------------------------------------------------------------

@@ -174,9 +174,8 @@ def gpu_fp8_product_grad(dy: torch.Tensor, x: torch.Tensor, w: FP8_gpu, order: E
     groups, n, inner = w._dims
     if dy.dim() != 2 or dy.shape[1] != n or x.dim() != 2 or x.shape[1] != inner:
         raise ValueError(f"gpu_fp8_product_grad: dy and x must have {n} and {inner} columns")
-    dx = _native.fp8_product(to_fp8_rows(dy), w.transposed(), order, dx_type)
-    dw = _native.fp8_grad_w(dy, x, order, groups)
-    return dx, dw
+    dw, rows = _native.fp8_grad_w(dy, x, order, groups)
+    return _native.fp8_product(rows, w.transposed(), order, dx_type), dw
 
 
 _native.bind_experts((ExpertOrder_gpu, FP8_gpu))
