@@ -540,10 +540,11 @@ __global__ void __launch_bounds__(NT) k_sort_few_fp8(Order o, int per_cta, int t
 
 // ---- host ------------------------------------------------------------------------------
 
-// Threads per token for rows that take `loads` of 16 bytes: up to two each.
-int team_of(int64_t loads) {
+// Threads per token for rows that take `loads` of 16 bytes: up to four each (the way back of 131072 rows of 8 KB 187 us, with two each 191, with eight
+// 186, but odd rows of 4 KB 14.6, 14.8 and 18.3), and two each while all tokens together leave most of the GPU free.
+int team_of(int64_t loads, int64_t tokens) {
     int t = 32;
-    while (t < NT && 2 * t < loads) t *= 2;
+    while (t < NT && (4 * t < loads || (2 * t < loads && tokens * t < (int64_t)sm_count() * 512))) t *= 2;
     return t;
 }
 
@@ -629,7 +630,7 @@ int nb200_expert_sort(const nb200_csr *r, const nb200_dense *x, nb200_expert_ord
     const nb200_dense none{r->rows, 0, 0, NB200_F32, nullptr};
     if (!x) x = &none, xs = const_cast<nb200_dense *>(&none);
     if (o.entries > FEW_ENTRIES && (st = make_order(o, stream))) return st;
-    const int word = word_bytes({x, xs}), tpr = team_of((x->cols * type_size(x->type) + 15) / 16 / 2);
+    const int word = word_bytes({x, xs}), tpr = team_of((x->cols * type_size(x->type) + 15) / 16, o.tokens);
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
@@ -656,7 +657,7 @@ int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert
     const Order o = order_of(order, r->col);
     const bool all_in_one = o.entries <= FEW_ENTRIES;
     if (!all_in_one && (st = make_order(o, stream))) return st;
-    const int word = word_bytes({x}), tpr = team_of(blocks_of(x->cols) * (all_in_one ? 32 : 16));
+    const int word = word_bytes({x}), tpr = team_of(blocks_of(x->cols) * 32, o.tokens);
     return with_type(x->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
@@ -683,7 +684,7 @@ int nb200_expert_unsort(const nb200_expert_order *order, const float *w, const n
     if (y->rows == 0 || y->cols == 0) return NB200_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, nullptr);
-    const int word = word_bytes({z, y}), tpr = team_of((z->cols * type_size(z->type) + 15) / 16);
+    const int word = word_bytes({z, y}), tpr = team_of((z->cols * type_size(z->type) + 15) / 16, o.tokens);
     return with_type(z->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
@@ -705,7 +706,7 @@ int nb200_expert_unsort_grad(const nb200_expert_order *order, const float *w, co
     if (order->entries == 0) return NB200_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, nullptr);
-    const int word = word_bytes({z, dy, dz}), tpr = team_of((z->cols * type_size(z->type) + 15) / 16);
+    const int word = word_bytes({z, dy, dz}), tpr = team_of((z->cols * type_size(z->type) + 15) / 16, o.tokens);
     return with_type(z->type, [&](auto e) {
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
