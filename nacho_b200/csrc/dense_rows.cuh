@@ -215,9 +215,9 @@ inline bool fp8_ok(const nb200_fp8 *m) {
            reinterpret_cast<uintptr_t>(m->values) % 16 == 0 && reinterpret_cast<uintptr_t>(m->scales) % 16 == 0;
 }
 
-// The factors of U blocks (a power of two) of 16 threads, which all have their largest magnitudes: every thread divides for one of them, a division
-// being as much as a dozen other instructions.
-template <int U>
+// The factors of U blocks (a power of two) of G neighbouring threads, which all have their largest magnitudes: every thread divides for one of them, a
+// division being as much as a dozen other instructions.
+template <int U, int G>
 __device__ __forceinline__ void share_factors(unsigned threads, const uint32_t (&m)[U], Factors (&f)[U]) {
     const int lane = lane_id();
     uint32_t mine = m[0];
@@ -226,8 +226,8 @@ __device__ __forceinline__ void share_factors(unsigned threads, const uint32_t (
     const Factors own = factors_of(mine);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        f[u].scale = __shfl_sync(threads, own.scale, (lane & 16) + u);
-        f[u].inverse = __shfl_sync(threads, own.inverse, (lane & 16) + u);
+        f[u].scale = __shfl_sync(threads, own.scale, (lane & (32 - G)) + u);
+        f[u].inverse = __shfl_sync(threads, own.inverse, (lane & (32 - G)) + u);
     }
 }
 
@@ -236,5 +236,28 @@ template <typename T>
 __device__ __forceinline__ uint2 codes8(const Eight<T> &v, float inverse) {
     return make_uint2(codes4(v.get(0), v.get(1), v.get(2), v.get(3), inverse), codes4(v.get(4), v.get(5), v.get(6), v.get(7), inverse));
 }
+
+// A thread's eighth of a block of 128 columns: 16 elements, a piece of the codes. What eight threads share costs half of what 16 would.
+template <typename T>
+struct Piece {
+    Eight<T> lo, hi;
+
+    template <int V>
+    __device__ __forceinline__ void load(const T *row, int64_t c, int64_t cols) {
+        lo.template load<V>(row, c, cols);
+        hi.template load<V>(row, c + 8, cols);
+    }
+    // The block's largest magnitude; `threads`: its eight.
+    __device__ __forceinline__ uint32_t top(unsigned threads) const {
+        Top<T> t;
+        t.add(lo), t.add(hi);
+        t.join(threads, 4), t.join(threads, 2), t.join(threads, 1);
+        return t.bits();
+    }
+    __device__ __forceinline__ uint4 codes(float inverse) const {
+        const uint2 a = codes8(lo, inverse), b = codes8(hi, inverse);
+        return make_uint4(a.x, a.y, b.x, b.y);
+    }
+};
 
 }  // namespace nb200

@@ -245,19 +245,18 @@ struct Entries {
     }
 };
 
-// The same into 8-bit rows: 16 threads have a block of 128 columns, quantise it once and write it to all of the token's slots. Bound by its
-// instructions: 65536 rows of 4096 from 16384 tokens take 69 % of the issue slots.
+// The same into 8-bit rows: eight threads have a block of 128 columns, quantise it once and write it to all of the token's slots. Bound by its
+// instructions.
 template <typename T, int V, int N>
 __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const T *x, int64_t stride, int64_t cols, uint8_t *codes, float *scales) {
-    constexpr int U = 2;
     wait_for_previous();
     trigger_dependents();
     const Team team(tpr);
-    const int sub = team.lane & 15, mine = team.lane >> 4, blocks = team.size >> 4;
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
+    const int sub = team.lane & 7, mine = team.lane >> 3, blocks = team.size >> 3;
+    const unsigned eight = 0xffu << (threadIdx.x & 24);
     const int64_t pad = padded_rows(o.entries);
     const int kb = (int)blocks_of(cols);
-    auto place_of = [&](int s) { return codes + piece_at(s, sub >> 1) + (sub & 1) * 8; };
+    auto place_of = [&](int s) { return codes + piece_at(s, sub); };
     Entries<N> at(o, nullptr, team.first, team.step);
     while (at.advance()) {
         const T *row = x + at.t * stride;
@@ -266,10 +265,9 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
 #pragma unroll
             for (int i = 0; i < N; ++i) place[i] = place_of(at.slot[i]);
         }
-        for (int b = mine; b < kb; b += blocks * U) {
-            Eight<T> v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u].template load<V>(row, (int64_t)(b + u * blocks) * BLOCK8 + sub * 8, cols);
+        for (int b = mine; b < kb; b += blocks) {
+            Piece<T> v;
+            v.template load<V>(row, (int64_t)b * BLOCK8 + sub * 16, cols);
             if (b == mine) {
                 if (team.lane == 0)
                     for (int e = at.e0; e < at.e1; ++e) {
@@ -278,33 +276,19 @@ __global__ void __launch_bounds__(NT, 4) k_sort_rows_fp8(Order o, int tpr, const
                     }
                 at.ask_next();
             }
-            uint32_t m[U];
-            Factors f[U];
+            const Factors f = factors_of(v.top(eight));
+            const uint4 q = v.codes(f.inverse);
+            const int64_t block = (int64_t)b * pad;
+            auto put = [&](uint8_t *to, int s) {
+                if (s < 0) return;
+                *reinterpret_cast<uint4 *>(to + block * BLOCK8) = q;
+                if (sub == 0) scales[block + s] = f.scale;
+            };
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                Top<T> top;
-                top.add(v[u]);
-#pragma unroll
-                for (int d = 8; d; d >>= 1) top.join(half, d);
-                m[u] = top.bits();
-            }
-            share_factors<U>(half, m, f);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (b + u * blocks >= kb) break;
-                const int64_t block = (int64_t)(b + u * blocks) * pad;
-                const uint2 q = codes8(v[u], f[u].inverse);
-                auto put = [&](uint8_t *to, int s) {
-                    if (s < 0) return;
-                    *reinterpret_cast<uint2 *>(to + block * BLOCK8) = q;
-                    if (sub == 0) scales[block + s] = f[u].scale;
-                };
-#pragma unroll
-                for (int i = 0; i < N; ++i) put(N == 4 ? place[i] : place_of(at.slot[i]), at.slot[i]);
-                for (int e = at.e0 + N; e < at.e1; ++e) {
-                    const int s = o.slot(e);
-                    put(place_of(s), s);
-                }
+            for (int i = 0; i < N; ++i) put(N == 4 ? place[i] : place_of(at.slot[i]), at.slot[i]);
+            for (int e = at.e0 + N; e < at.e1; ++e) {
+                const int s = o.slot(e);
+                put(place_of(s), s);
             }
         }
         if (mine >= kb) at.ask_next();

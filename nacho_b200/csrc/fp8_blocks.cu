@@ -22,38 +22,32 @@ struct Blocks {
 
 Blocks blocks(const nb200_fp8 *m) { return {m->rows, m->cols, m->groups, blocks_of(m->cols), padded_rows(m->rows), blocks_of(m->rows), m->values, m->scales}; }
 
-// A CTA has 16 rows by four blocks: 16 threads a row's block of 128 columns, a load of eight elements of each block each, the largest magnitude by
-// four exchanges, eight codes each. So a block's 16 rows of codes are written as one stretch, and so are their scales.
-constexpr int ROWS8 = 16, BLOCKS8 = 4;
+// A CTA has 32 rows by two blocks, eight threads a row's block of 128 columns. So a block's 32 rows of codes are written as one stretch, and so are
+// their scales. Bound by its instructions.
+constexpr int ROWS8 = 32, BLOCKS8 = 2;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(NT) k_fp8_rows(Blocks z, int chunks, const T *x, int64_t stride) {
     wait_for_previous();
     trigger_dependents();
-    const int sub = threadIdx.x & 15;
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
-    const int64_t r = (int64_t)(blockIdx.x / chunks) * ROWS8 + threadIdx.x / 16;
+    const int sub = threadIdx.x & 7;
+    const unsigned eight = 0xffu << (threadIdx.x & 24);
+    const int64_t r = (int64_t)(blockIdx.x / chunks) * ROWS8 + threadIdx.x / 8;
     const int64_t b0 = (int64_t)(blockIdx.x % chunks) * BLOCKS8;
     if (r >= z.rows) return;
-    Eight<T> v[BLOCKS8];
+    Piece<T> v[BLOCKS8];
 #pragma unroll
-    for (int u = 0; u < BLOCKS8; ++u) v[u].template load<V>(x + r * stride, (b0 + u) * BLOCK8 + sub * 8, z.cols);
+    for (int u = 0; u < BLOCKS8; ++u) v[u].template load<V>(x + r * stride, (b0 + u) * BLOCK8 + sub * 16, z.cols);
     uint32_t m[BLOCKS8];
     Factors f[BLOCKS8];
 #pragma unroll
-    for (int u = 0; u < BLOCKS8; ++u) {
-        Top<T> top;
-        top.add(v[u]);
-#pragma unroll
-        for (int d = 8; d; d >>= 1) top.join(half, d);
-        m[u] = top.bits();
-    }
-    share_factors<BLOCKS8>(half, m, f);
+    for (int u = 0; u < BLOCKS8; ++u) m[u] = v[u].top(eight);
+    share_factors<BLOCKS8, 8>(eight, m, f);
 #pragma unroll
     for (int u = 0; u < BLOCKS8; ++u) {
         const int64_t b = b0 + u;
         if (b >= z.kb) break;
-        *reinterpret_cast<uint2 *>(z.block(0, b) + piece_at(r, sub >> 1) + (sub & 1) * 8) = codes8(v[u], f[u].inverse);
+        *reinterpret_cast<uint4 *>(z.block(0, b) + piece_at(r, sub)) = v[u].codes(f[u].inverse);
         if (sub == 0) z.scales[b * z.pad + r] = f[u].scale;
     }
 }

@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(cons
             for (int d = 8; d; d >>= 1) row.join(half, d);
             top_of[i] = row.bits();
         }
-        share_factors<8>(half, top_of, f);
+        share_factors<8, 16>(half, top_of, f);
         const int64_t at = c0 / BLOCK8 * row_pad + rows.x;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
