@@ -888,14 +888,16 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     //     to be worth sharing, up to 64 (4096 x 4096: 12 against 17; 1024 x 2048: 10 either way; 2048 x 1024: 13 against 7) and beyond, while
     //     tiles leave half of the SMs idle (128 rows, 1024 x 8192: 13 against 30; 4096 x 4096: 17 either way);
     //   - pairs of CTAs from where single ones have a second tile (4096 x 4096, 512 rows: 19 against 18; 768 rows: 20 against 31) and groups fill
-    //     most of 128 rows (32 groups of 2048 x 2048 with 96 rows: 41 against 36, with 128 rows: 42 against 50).
+    //     most of 128 rows (32 groups of 2048 x 2048 with 96 rows: 41 against 36, with 128 rows: 42 against 50);
+    //   - no groups: the tiles' kernel, which finds none and clears the rows, all of them rows of no group.
     // tiles at most: a group may begin and end inside tiles
-    const int64_t groups = w->groups, mean = (y->rows + groups - 1) / groups, singles = blocks_of(y->rows) * blocks_of(y->cols);
+    const int64_t groups = w->groups, mean = groups ? (y->rows + groups - 1) / groups : 0, singles = blocks_of(y->rows) * blocks_of(y->cols);
     const bool one = groups == 1, idle = 2 * singles <= sm_count(), pair = mean >= 112 && singles > sm_count();
     const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * groups) * ((y->cols + side - 1) / side);
     if (tiles > INT32_MAX / 64 || y->rows > INT32_MAX - 1024 || y->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     return with_type(y->type, [&](auto e) {
         using T = decltype(e);
+        if (groups == 0) return launch_product<T, false>("fp8_product", false, tiles, oa, ow, offsets, 0, *y, stream);
         if (mean <= (one ? 16 : 5)) return launch_few<T, 16>(oa, ow, offsets, w->groups, *y, stream);
         if (mean <= (one ? 32 : 20)) return launch_few<T, 32>(oa, ow, offsets, w->groups, *y, stream);
         if (one && idle && mean <= 64 && oa.blocks >= 24) return launch_few<T, 64>(oa, ow, offsets, 1, *y, stream);
