@@ -40,9 +40,10 @@ struct Shape {
     static constexpr int CTAS = PAIR ? 2 : 1, BM = 128 * CTAS, BN = 128 * CTAS;  // a tile of the result
     static constexpr int A_ROWS = 128, B_ROWS = 128;                             // what a CTA brings per block
     static constexpr int STAGES = 4, SUMS = 512 / BN;                            // blocks under way; places for their sums in tensor memory
-    // Scales are written into a place STAGES + SUMS blocks after it was used before: by then their matrix instructions, and with them those of
-    // STAGES blocks earlier, are done, which had to wait until the sums of SUMS blocks earlier had been read.
-    static constexpr int SCALES = STAGES + SUMS;
+    // Scales are written into a place STAGES + SUMS + 1 blocks after it was used before: by then the matrix instructions of STAGES blocks earlier are
+    // done, which had to wait until every warp had said that it has read the sums of SUMS blocks before those. It says so once it has read all scales of
+    // the block before (of that block itself the columns' last ones may still be missing).
+    static constexpr int SCALES = STAGES + SUMS + 1;
     static constexpr int PANEL = PAIR ? 8 : 16;  // tiles that share columns follow one another: 2048 rows, then the next columns
 
     // What a CTA has in shared memory; tiles and the stores' staging begin at 1024-byte boundaries.
