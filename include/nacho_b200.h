@@ -394,7 +394,8 @@ int64_t nb200_fp8_value_count(const nb200_fp8 *m);
 int64_t nb200_fp8_scale_count(const nb200_fp8 *m);
 
 /* order of R, and (where x is not NULL) xs[slot] = x[token], zeros for slots of nobody. order->row_ptr is set to R's. The
- * other three arrays are the caller's. The form with fp8 rows quantises on the way. At most NB200_MAX_EXPERTS columns. */
+ * other three arrays are the caller's. The form with fp8 rows quantises on the way. At most NB200_MAX_EXPERTS columns, and
+ * 2^31 - 1025 tokens and entries. */
 int nb200_expert_sort(const nb200_csr *r, const nb200_dense *x, nb200_expert_order *order, nb200_dense *xs, void *stream);
 int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert_order *order, nb200_fp8 *xs, void *stream);
 /* y[t] = sum over the kept entries e of token t of w[e] * z[slot(e)]; w = NULL stands for ones (the gradient of the sort). */

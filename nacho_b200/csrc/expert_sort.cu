@@ -134,9 +134,11 @@ __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles
 
 // ---- moving rows -----------------------------------------------------------------------
 
-// `tpr` threads (a power of two from 32 to NT) have a token together; a CTA has NT / tpr tokens at a time.
+// `tpr` threads (a power of two from 32 to NT) have a token together; a CTA has NT / tpr tokens at a time. Loops over tokens and slots count without a
+// sign: the last of them may lie less than a step below 2^31.
 struct Team {
-    int size, lane, first, step;  // first token, distance to the next
+    int size, lane;
+    unsigned first, step;  // first token, distance to the next
     __device__ explicit Team(int tpr) : size(tpr), lane(threadIdx.x & (tpr - 1)), first(blockIdx.x * (NT / tpr) + threadIdx.x / tpr), step(gridDim.x * (NT / tpr)) {}
 };
 
@@ -169,7 +171,7 @@ __device__ __forceinline__ void copy_rows(const Order &o, const Team &team, int 
 
 template <typename T, int V>
 __device__ __forceinline__ void clear_rows(const Order &o, int kept, const Team &team, int64_t cols, T *xs) {
-    for (int s = kept + team.first; s < o.entries; s += team.step) {
+    for (unsigned s = kept + team.first; s < (unsigned)o.entries; s += team.step) {
         if (o.rows && team.lane == 0) o.rows[s] = -1;
         for (int64_t c = team.lane * V; c < cols; c += team.size * V) {
             Vec<T, V> zero;
@@ -185,14 +187,14 @@ __global__ void __launch_bounds__(NT) k_sort_rows(Order o, int tpr, const T *x, 
     wait_for_previous();
     trigger_dependents();
     const Team team(tpr);
-    for (int t = team.first; t < o.tokens; t += team.step) copy_rows<T, V>(o, team, t, x, stride, cols, xs);
+    for (unsigned t = team.first; t < (unsigned)o.tokens; t += team.step) copy_rows<T, V>(o, team, t, x, stride, cols, xs);
     clear_rows<T, V>(o, o.kept(), team, cols, xs);
 }
 
 __device__ __forceinline__ void clear_rows8(const Order &o, int kept, const Team &team, int64_t kb, uint8_t *codes, float *scales) {
     const int sub = team.lane & 15;
     const int64_t pad = padded_rows(o.entries);
-    for (int s = kept + team.first; s < o.entries; s += team.step) {
+    for (unsigned s = kept + team.first; s < (unsigned)o.entries; s += team.step) {
         if (team.lane == 0) o.rows[s] = -1;
         for (int64_t b = team.lane >> 4; b < kb; b += team.size >> 4) {
             *reinterpret_cast<uint2 *>(codes + b * pad * BLOCK8 + piece_at(s, sub >> 1) + (sub & 1) * 8) = make_uint2(0, 0);
@@ -208,12 +210,12 @@ template <int N>
 struct Entries {
     const Order &o;
     const float *w;
-    int t, step;
+    unsigned t, step;
     int e0, e1, next0, next1, slot[N], raw[N];
     float weight[N];
 
-    __device__ Entries(const Order &order, const float *weights, int first, int distance) : o(order), w(weights), t(first - distance), step(distance) {
-        next0 = o.entry_of(min(first, o.tokens)), next1 = o.entry_of(min(first + 1, o.tokens));
+    __device__ Entries(const Order &order, const float *weights, unsigned first, unsigned distance) : o(order), w(weights), t(first - distance), step(distance) {
+        next0 = o.entry_of(min(first, (unsigned)o.tokens)), next1 = o.entry_of(min(first + 1, (unsigned)o.tokens));
         ask();
     }
     __device__ void ask() {
@@ -227,7 +229,7 @@ struct Entries {
     // The next token, if there is one.
     __device__ bool advance() {
         t += step;
-        if (t >= o.tokens) return false;
+        if (t >= (unsigned)o.tokens) return false;
         const int64_t after = min((int64_t)t + step, (int64_t)o.tokens);
         e0 = next0, e1 = next1;
         next0 = ld_late(o.row_ptr + after), next1 = ld_late(o.row_ptr + min(after + 1, (int64_t)o.tokens));
@@ -412,8 +414,8 @@ __global__ void __launch_bounds__(NT, N == 8 ? 2 : 3) k_unsort_grad(Order o, int
     clear_rows<T, V>(tail, o.kept(), team, cols, dz);
     // entries of no row: views into larger arrays
     const int lo = o.entry_of(0), hi = o.entry_of(o.tokens);
-    for (int e = blockIdx.x * NT + threadIdx.x; e < o.entries; e += gridDim.x * NT)
-        if (e < lo || e >= hi) dw[e] = 0.f;
+    for (unsigned e = blockIdx.x * NT + threadIdx.x; e < (unsigned)o.entries; e += gridDim.x * NT)
+        if (e < (unsigned)lo || e >= (unsigned)hi) dw[e] = 0.f;
 }
 
 // ---- few entries: all in one launch ------------------------------------------------------
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(NT) k_sort_few(Order o, int per_cta, int tpr, 
     extern __shared__ int32_t counts[];
     wait_for_previous();
     trigger_dependents();
-    const int t0 = min((int)blockIdx.x * per_cta, o.tokens), t1 = min(t0 + per_cta, o.tokens);
+    const int t0 = (int)min(blockIdx.x * (unsigned)per_cta, (unsigned)o.tokens), t1 = (int)min((unsigned)t0 + per_cta, (unsigned)o.tokens);
     const int kept = place_few(o, t0, t1, counts);
     Team team(tpr);
     for (int t = t0 + (int)threadIdx.x / tpr; t < t1; t += NT / tpr) copy_rows<T, V>(o, team, t, x, stride, cols, xs);
@@ -490,7 +492,7 @@ __global__ void __launch_bounds__(NT) k_sort_few_fp8(Order o, int per_cta, int t
     extern __shared__ int32_t counts[];
     wait_for_previous();
     trigger_dependents();
-    const int t0 = min((int)blockIdx.x * per_cta, o.tokens), t1 = min(t0 + per_cta, o.tokens);
+    const int t0 = (int)min(blockIdx.x * (unsigned)per_cta, (unsigned)o.tokens), t1 = (int)min((unsigned)t0 + per_cta, (unsigned)o.tokens);
     const int kept = place_few(o, t0, t1, counts);
     const Team team(tpr);
     const int sub = team.lane & 15;
@@ -551,7 +553,8 @@ bool many_entries(const Order &o) { return (int64_t)o.entries > 4 * (int64_t)o.t
 int check_order(const nb200_expert_order *o, bool slots_given) {
     if (!o || o->tokens < 0 || o->experts < 0 || o->entries < 0 || !o->row_ptr || !o->offsets) return NB200_E_BADARG;
     if (o->entries > 0 && (!o->slots || (!slots_given && !o->rows))) return NB200_E_BADARG;
-    return o->experts > NB200_MAX_EXPERTS ? NB200_E_UNSUPPORTED : NB200_OK;
+    // the last numbers in front of 2^31 are what kernels that look a few entries or tokens ahead may count up to
+    return o->experts > NB200_MAX_EXPERTS || o->tokens > INT32_MAX - 1024 || o->entries > INT32_MAX - 1024 ? NB200_E_UNSUPPORTED : NB200_OK;
 }
 
 Order order_of(const nb200_expert_order *o, const int32_t *expert) {
@@ -572,16 +575,24 @@ struct Few {
     size_t smem;
     Few(const Order &o, int tpr) {
         const int teams = NT / tpr, most = 2 * sm_count();
-        per_cta = std::max(teams, (o.tokens + most - 1) / most);
-        grid = dim3((unsigned)std::max(1, (o.tokens + per_cta - 1) / per_cta));
+        per_cta = (int)std::max<int64_t>(teams, ((int64_t)o.tokens + most - 1) / most);
+        grid = dim3((unsigned)std::max<int64_t>(1, ((int64_t)o.tokens + per_cta - 1) / per_cta));
         smem = sizeof(int32_t) * 2 * o.experts;
     }
 };
 
+// The entries of a CTA, a multiple of the warps' 32 each, and how many CTAs there are.
+struct OrderTiles {
+    int tile = 2048, tiles;
+    explicit OrderTiles(int64_t entries) {
+        while ((entries + tile - 1) / tile > MAX_TILES) tile *= 2;
+        tiles = (int)std::max<int64_t>(1, (entries + tile - 1) / tile);
+    }
+};
+
 int make_order(const Order &o, cudaStream_t stream) {
-    int tile = 2048;  // a multiple of the warps' 32 each
-    while ((o.entries + (int64_t)tile - 1) / tile > MAX_TILES) tile *= 2;
-    const int tiles = std::max(1, (o.entries + tile - 1) / tile);
+    const OrderTiles cut(o.entries);
+    const int tile = cut.tile, tiles = cut.tiles;
     Workspace *ws = nullptr;
     int st;
     if ((st = acquire_workspace(stream, sizeof(int32_t) * (size_t)tiles * std::max(o.experts, 1), &ws, ORDER_SLOT))) return st;

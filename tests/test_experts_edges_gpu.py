@@ -25,3 +25,83 @@ def test_no_experts(dtype, tokens, k, n):
     assert z.shape == (tokens, n) and not z.any()
     dx, dw = nacho().gpu_fp8_product_grad(normal((tokens * k, n), dtype, 3), normal((tokens * k, 200), dtype, 4), w, order)
     assert dx.shape == (tokens * k, 200) and not dx.any() and dw.shape == (0, n, 200)
+
+
+MOST = (1 << 31) - 1 - 1024  # tokens and entries that an order takes
+CHUNK = 1 << 26
+
+
+def filled(n, values):
+    """n 32-bit numbers on the GPU, from a function of a chunk of their places (64-bit)."""
+    out = torch.empty(n, dtype=torch.int32, device="cuda")
+    for at in range(0, n, CHUNK):
+        out[at:at + CHUNK] = values(torch.arange(at, min(at + CHUNK, n), device="cuda"))
+    return out
+
+
+@pytest.fixture
+def room():
+    """The memory of a large test goes back to the device."""
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("entries", [(1 << 31) - (1 << 22), MOST])
+def test_as_many_entries_as_there_can_be(entries, room):
+    """Entry e goes to expert e % 6, every sixth one is dropped, so its slot is known."""
+    tokens = (1 << 20) + 77
+    row_ptr = filled(tokens + 1, lambda t: t * entries // tokens)
+    expert = filled(entries, lambda e: e % 6)
+    weight = torch.ones(entries, device="cuda")
+    weight[1::2] = 2
+    r = nacho().CSR_gpu(row_ptr, expert, weight, (tokens, 5))
+    order = nacho().gpu_expert_order(r)
+    first = [0]
+    for c in range(5):
+        first.append(first[-1] + (entries - c + 5) // 6)
+    assert order.offsets.tolist() == first
+    base = torch.tensor(first, device="cuda")
+    for at in range(0, entries, CHUNK):
+        e = torch.arange(at, min(at + CHUNK, entries), device="cuda")
+        want = torch.where(e % 6 < 5, base[e % 6] + e // 6, -1)
+        assert torch.equal(order.slots[at:at + CHUNK], want.int())
+        kept = want >= 0
+        token = torch.searchsorted(row_ptr, e[kept].int(), right=True) - 1
+        assert torch.equal(order.rows[want[kept]], token.int())
+    assert torch.all(order.rows[first[-1]:] == -1)
+    z, dy = torch.ones(entries, 1, dtype=torch.bfloat16, device="cuda"), torch.full((tokens, 1), 3.0, dtype=torch.bfloat16, device="cuda")
+    y = nacho().gpu_expert_sort_grad(order, z)
+    some = [0, 1, tokens // 2, tokens - 1]
+    want = [sum(e % 6 < 5 for e in range(t * entries // tokens, (t + 1) * entries // tokens)) for t in some]
+    assert torch.equal(y[some].flatten(), torch.tensor(want, device="cuda").to(torch.bfloat16))
+    dz, dw = nacho().gpu_expert_unsort_grad(r, order, z, dy)
+    for at in range(0, entries, CHUNK):
+        e = torch.arange(at, min(at + CHUNK, entries), device="cuda")
+        assert torch.equal(dw[at:at + CHUNK], torch.where(e % 6 < 5, 3.0, 0.0))
+        kept = e[e % 6 < 5]
+        assert torch.equal(dz[base[kept % 6] + kept // 6, 0], (3.0 * weight[kept]).to(torch.bfloat16))
+    assert not dz[first[-1]:].any()
+
+
+def test_as_many_tokens_as_there_can_be(room):
+    """A thousand entries over the rows of all numbers of tokens that 32 bits count."""
+    row_ptr = filled(MOST + 1, lambda t: t * 1000 // MOST)
+    expert = torch.arange(1000, dtype=torch.int32, device="cuda") % 7
+    r = nacho().CSR_gpu(row_ptr, expert, torch.ones(1000, device="cuda"), (MOST, 7))
+    order = nacho().gpu_expert_order(r)
+    token = torch.searchsorted(row_ptr, torch.arange(1000, dtype=torch.int32, device="cuda"), right=True) - 1
+    assert_order(order, token.cpu().numpy(), expert.cpu().numpy(), 7)
+    y = nacho().gpu_expert_sort_grad(order, torch.ones(1000, 1, dtype=torch.bfloat16, device="cuda"))
+    assert y.shape == (MOST, 1) and torch.equal(torch.nonzero(y.view(torch.int16).flatten()).flatten(), token)
+
+
+def test_extents_that_leave_no_room_to_count():
+    """The last 1024 numbers in front of 2^31 are refused before anything runs."""
+    one = torch.zeros(2, dtype=torch.int32, device="cuda")
+    import ctypes as C
+    from nacho_b200 import _capi
+    for tokens, entries in ((MOST + 1, 0), (0, MOST + 1), (1, (1 << 31) - 1)):
+        r = _capi.CsrStruct(tokens, 3, entries, one.data_ptr(), one.data_ptr(), None)
+        order = _capi.ExpertOrderStruct(0, 0, 0, None, one.data_ptr(), one.data_ptr(), one.data_ptr())
+        assert _capi.lib.nb200_expert_sort(C.byref(r), None, C.byref(order), None, None) == _capi.E_UNSUPPORTED

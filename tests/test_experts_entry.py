@@ -1,7 +1,10 @@
 """CPU suite: entry points of the operators around a router whose host side can be seen without a GPU."""
 import os
+import shutil
 import subprocess
 import sys
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -21,3 +24,26 @@ a, w, y = Fp8Struct(1, 5, 256, 0, 4096, 8192), Fp8Struct(0, 16, 256, 1, 12288, 1
 print(lib.nb200_fp8_product(C.byref(a), C.byref(w), C.c_void_p(24576), C.byref(y), None) == _capi.E_CUDA)
 print(lib.nb200_fp8_product(C.byref(a), C.byref(w), None, C.byref(y), None) == _capi.E_BADARG)
 """).split() == ["True", "True"]
+
+
+def rule(name, source="expert_sort.cu"):
+    """The definition of a host-side rule, as its source has it."""
+    text = open(os.path.join(ROOT, "nacho_b200", "csrc", source)).read()
+    text = text[text.index(f"struct {name} {{"):]
+    return text[:text.index("\n};") + 4]
+
+
+def compiled(tmp_path, definitions, body):
+    (tmp_path / "rule.cpp").write_text("#include <algorithm>\n#include <cstdint>\n#include <cstdio>\n" + definitions + "\nint main() {" + body + "}")
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "rule"), str(tmp_path / "rule.cpp")], check=True)
+    return subprocess.run([str(tmp_path / "rule")], check=True, capture_output=True, text=True).stdout
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="no host compiler")
+def test_tiles_of_an_order_hold_all_entries(tmp_path):
+    entries = [0, 1, 2561, 2048 * 256, 2048 * 256 + 1, 1 << 30, (1 << 31) - (1 << 23), (1 << 31) - (1 << 23) + 1, (1 << 31) - 1025, (1 << 31) - 1]
+    out = compiled(tmp_path, "constexpr int MAX_TILES = 256;\n" + rule("OrderTiles"),
+                   "for (long long n : {" + ", ".join(f"{n}ll" for n in entries) + '}) { OrderTiles c((int32_t)n); printf("%d %d\\n", c.tile, c.tiles); }')
+    for n, line in zip(entries, out.splitlines()):
+        tile, tiles = map(int, line.split())
+        assert tile % 256 == 0 and 1 <= tiles <= 256 and (tiles - 1) * tile < max(n, 1) <= tiles * tile, (n, tile, tiles)
