@@ -353,8 +353,9 @@ int nb200_inner_prod_coo_f32(const nb200_coo3 *a, const nb200_coo3 *b, float *z,
  * weights in 8-bit floating point, and bring them back. They have no counterpart in the reference.
  *   - Rows of R may be empty or hold any number of entries, in any order of experts (duplicates count twice).
  *     An entry whose column lies outside [0, cols) is dropped: it has no slot and takes part in nothing.
- *   - None of the calls waits for the device: all result lengths are known before. They can be captured in a
- *     CUDA graph once a call of that size has been made on the stream (scratch arrays grow on first use).
+ *   - None of the calls waits for the device: all result lengths are known before. They can be captured in a CUDA
+ *     graph once a call of their kind has been made on the stream, and use no device memory but what the caller gives
+ *     them, so graphs may be replayed on any stream, beside one another and after calls of any size.
  *   - Sums are 32-bit, in a fixed order: the same call gives the same bits. */
 
 /* Dense rows in device memory: element (r, c) lies at data[r * stride + c]. */

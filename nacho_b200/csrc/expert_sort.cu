@@ -12,7 +12,6 @@ namespace nb200 {
 namespace {
 
 constexpr int NT = 256;
-constexpr int ORDER_SLOT = 8;  // of the scratch pool
 
 // R and its order as kernels see them. `first` .. `last` is the range of entries that belong to rows of R: row offsets may point into
 // larger arrays.
@@ -37,8 +36,10 @@ struct Order {
 
 constexpr int MAX_TILES = 256, AT_ONCE = 8;  // entries per thread that are on their way together
 
-// How often each key occurs in this CTA's tile of entries: counts[tile][key].
-__global__ void __launch_bounds__(NT) k_order_count(Order o, int tile, int32_t *counts) {
+// How often each key occurs in this CTA's tile of entries: counts[tile][key]. They lie where the order's rows come to lie once all slots are known: a
+// call has no memory of its own that another stream, or a later call beside a captured graph, could have too.
+template <typename C>
+__global__ void __launch_bounds__(NT) k_order_count(Order o, int tile) {
     extern __shared__ int32_t hist[];
     wait_for_previous();
     trigger_dependents();
@@ -51,12 +52,14 @@ __global__ void __launch_bounds__(NT) k_order_count(Order o, int tile, int32_t *
         if (k < o.experts) atomicAdd(&hist[k], 1);
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < o.experts; k += NT) counts[(int64_t)blockIdx.x * o.experts + k] = hist[k];
+    C *counts = reinterpret_cast<C *>(o.rows) + (int64_t)blockIdx.x * o.experts;
+    for (int k = threadIdx.x; k < o.experts; k += NT) counts[k] = (C)hist[k];
 }
 
 // Slots of a tile's entries. Every warp has a stretch of the tile and a counter per expert, which starts at the slots in front of its stretch:
 // those of all smaller experts, of this expert's entries in the tiles before, and of the warps before.
-__global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles, const int32_t *counts) {
+template <typename C>
+__global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles) {
     extern __shared__ int32_t next[];  // [warp][expert], then the experts' totals and their entries in the tiles before
     __shared__ int tmp[33];
     int32_t *total = next + (NT / 32) * o.experts, *before = total + o.experts;
@@ -81,6 +84,7 @@ __global__ void __launch_bounds__(NT) k_order_place(Order o, int tile, int tiles
     // an expert's entries in all tiles and in the tiles before, all threads over all counts, eight of them on their way at a time
     for (int k = threadIdx.x; k < 2 * o.experts; k += NT) total[k] = 0;
     __syncthreads();
+    const C *counts = reinterpret_cast<const C *>(o.rows);
     const int64_t all = (int64_t)tiles * o.experts, mine_too = (int64_t)blockIdx.x * o.experts;
     for (int64_t i0 = threadIdx.x; i0 < all; i0 += 8 * NT) {
         int c[8];
@@ -581,31 +585,37 @@ struct Few {
     }
 };
 
-// The entries of a CTA, a multiple of the warps' 32 each, and how many CTAs there are.
+// The entries of a CTA, a multiple of the warps' 32 each, and how many CTAs there are: as few entries as leave no more than MAX_TILES CTAs and
+// tables of counts, 16 bits each while a tile's entries can be counted in those, that fit into the order's `rows` (up to 2560 experts they do with 2048).
 struct OrderTiles {
     int tile = 2048, tiles;
-    explicit OrderTiles(int64_t entries) {
-        while ((entries + tile - 1) / tile > MAX_TILES) tile *= 2;
-        tiles = (int)std::max<int64_t>(1, (entries + tile - 1) / tile);
+    OrderTiles(int64_t entries, int64_t experts) {  // entries > FEW_ENTRIES, so that one table fits
+        auto fits = [&] {
+            tiles = (int)((entries + tile - 1) / tile);
+            return tiles <= MAX_TILES && tiles * experts * (narrow() ? 2 : 4) <= entries * 4;
+        };
+        while (!fits()) tile *= 2;
     }
+    bool narrow() const { return tile < 1 << 16; }
 };
+static_assert(2 * NB200_MAX_EXPERTS <= 4 * FEW_ENTRIES, "");
 
-int make_order(const Order &o, cudaStream_t stream) {
-    const OrderTiles cut(o.entries);
-    const int tile = cut.tile, tiles = cut.tiles;
-    Workspace *ws = nullptr;
+template <typename C>
+int make_order(const Order &o, int tile, int tiles, cudaStream_t stream) {
     int st;
-    if ((st = acquire_workspace(stream, sizeof(int32_t) * (size_t)tiles * std::max(o.experts, 1), &ws, ORDER_SLOT))) return st;
-    int32_t *counts = static_cast<int32_t *>(ws->dev);
     const size_t count_smem = sizeof(int32_t) * o.experts, place_smem = sizeof(int32_t) * o.experts * (NT / 32 + 2);
-    if (place_smem > 48 * 1024 && (st = allow_shared(k_order_place, place_smem))) return st;
+    if (place_smem > 48 * 1024 && (st = allow_shared(k_order_place<C>, place_smem))) return st;
     {
         LaunchScope scope("order_count", stream);
-        NB200_CUDA(launch_overlapped(k_order_count, dim3(tiles), dim3(NT), count_smem, stream, o, tile, counts));
+        NB200_CUDA(launch_overlapped(k_order_count<C>, dim3(tiles), dim3(NT), count_smem, stream, o, tile));
     }
     LaunchScope scope("order_place", stream);
-    NB200_CUDA(launch_overlapped(k_order_place, dim3(tiles), dim3(NT), place_smem, stream, o, tile, tiles, counts));
+    NB200_CUDA(launch_overlapped(k_order_place<C>, dim3(tiles), dim3(NT), place_smem, stream, o, tile, tiles));
     return NB200_OK;
+}
+int make_order(const Order &o, cudaStream_t stream) {
+    const OrderTiles cut(o.entries, o.experts);
+    return cut.narrow() ? make_order<uint16_t>(o, cut.tile, cut.tiles, stream) : make_order<int32_t>(o, cut.tile, cut.tiles, stream);
 }
 
 }  // namespace

@@ -27,6 +27,57 @@ def test_no_experts(dtype, tokens, k, n):
     assert dx.shape == (tokens * k, 200) and not dx.any() and dw.shape == (0, n, 200)
 
 
+def test_graphs_outlive_larger_calls_and_one_another():
+    """Two graphs captured on one stream, a larger call there afterwards, and both replayed at once on two other streams: each one's order is its own."""
+    cases = [routing(3000, 64, 4, seed=1), routing(2500, 300, 7, seed=2, ragged=True, drop=0.1)]
+    tokens = [normal((len(c[0].dim_j_offsets) - 1, 96), torch.bfloat16, 3) for c in cases]
+    stream, graphs, held = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for (r, *_), x in zip(cases, tokens):
+            nacho().gpu_expert_sort(r, x)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                held.append(nacho().gpu_expert_sort(r, x))
+            graphs.append(graph)
+        nacho().gpu_expert_order(routing(200000, 300, 5, seed=3)[0])
+    torch.cuda.synchronize()
+    others = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for (order, xs), _ in zip(held, graphs):
+            for t in (order.offsets, order.rows, order.slots, xs):
+                t.zero_()
+        torch.cuda.synchronize()
+        for graph, other in zip(graphs, others):
+            with torch.cuda.stream(other):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (r, token, expert, _), x, (order, xs) in zip(cases, tokens, held):
+            assert_order(order, token, expert, int(r.shape[1]))
+            rows = order.rows.long()
+            assert torch.equal(xs, torch.where((rows >= 0)[:, None], x[rows.clamp(min=0)], torch.zeros((), dtype=x.dtype, device="cuda")))
+
+
+@pytest.mark.parametrize("experts", [1280, 2560, 2561, 4096])
+@pytest.mark.parametrize("tokens,k", [(2561, 1), (1025, 4), (8193, 1), (70001, 3)])
+def test_many_experts(experts, tokens, k):
+    """Tables of counts as large as the place where they lie."""
+    r, token, expert, _ = routing(tokens, experts, k, seed=experts, drop=0.02)
+    assert_order(nacho().gpu_expert_order(r), token, expert, experts)
+
+
+def test_tiles_whose_entries_16_bits_do_not_count():
+    """More than 2^15 entries a tile, all of them of one expert."""
+    entries = (1 << 23) + 12345
+    r = nacho().CSR_gpu(torch.arange(0, entries + 1, 5, dtype=torch.int32, device="cuda"), torch.ones(entries, dtype=torch.int32, device="cuda"),
+                        torch.ones(entries, device="cuda"), (entries // 5, 3))
+    entries = entries // 5 * 5
+    order = nacho().gpu_expert_order(r)
+    assert order.offsets.tolist() == [0, 0, entries, entries]
+    assert torch.equal(order.slots[:entries], torch.arange(entries, dtype=torch.int32, device="cuda")) and torch.all(order.slots[entries:] == -1)
+    assert torch.equal(order.rows[:entries], torch.arange(entries, dtype=torch.int32, device="cuda") // 5)
+
+
 MOST = (1 << 31) - 1 - 1024  # tokens and entries that an order takes
 CHUNK = 1 << 26
 

@@ -1,5 +1,6 @@
 """CPU suite: entry points of the operators around a router whose host side can be seen without a GPU."""
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -41,9 +42,24 @@ def compiled(tmp_path, definitions, body):
 
 @pytest.mark.skipif(not shutil.which("g++"), reason="no host compiler")
 def test_tiles_of_an_order_hold_all_entries(tmp_path):
-    entries = [0, 1, 2561, 2048 * 256, 2048 * 256 + 1, 1 << 30, (1 << 31) - (1 << 23), (1 << 31) - (1 << 23) + 1, (1 << 31) - 1025, (1 << 31) - 1]
+    """All entries have a tile, no tile is one too many, and the tiles' counts fit in where the order's rows go, for any number of experts."""
+    entries = [2561, 4096, 4097, 6145, 8193, 2048 * 256, 2048 * 256 + 1, 1 << 23, (1 << 23) + 1, (1 << 24) - 1, (1 << 24) + 1, 1 << 30, (1 << 31) - (1 << 23),
+               (1 << 31) - (1 << 23) + 1, (1 << 31) - 1025, (1 << 31) - 1]
     out = compiled(tmp_path, "constexpr int MAX_TILES = 256;\n" + rule("OrderTiles"),
-                   "for (long long n : {" + ", ".join(f"{n}ll" for n in entries) + '}) { OrderTiles c((int32_t)n); printf("%d %d\\n", c.tile, c.tiles); }')
-    for n, line in zip(entries, out.splitlines()):
-        tile, tiles = map(int, line.split())
-        assert tile % 256 == 0 and 1 <= tiles <= 256 and (tiles - 1) * tile < max(n, 1) <= tiles * tile, (n, tile, tiles)
+                   "for (long long n : {" + ", ".join(f"{n}ll" for n in entries) + """}) for (int experts : {0, 1, 64, 1280, 2559, 2560, 2561, 4095, 4096}) {
+                        OrderTiles c((int32_t)n, experts);
+                        printf("%lld %d %d %d %d\\n", n, experts, c.tile, c.tiles, (int)c.narrow());
+                    }""")
+    lines = out.splitlines()
+    assert len(lines) == 9 * len(entries)
+    for line in lines:
+        n, experts, tile, tiles, narrow = map(int, line.split())
+        assert tile % 256 == 0 and 1 <= tiles <= 256 and (tiles - 1) * tile < n <= tiles * tile, line
+        assert tiles * experts * (2 if narrow else 4) <= 4 * n and (not narrow or tile < 1 << 16), line
+        assert tile == 2048 or tiles > 64 or experts > 2560, line  # no larger than it has to be
+
+
+def test_an_order_keeps_nothing_between_calls():
+    """What a captured graph writes into has to be the graph's own: a pool that grows frees what it had, and two graphs would share it."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "nacho_b200", "csrc", "expert_sort.cu")).read())
+    assert not re.search(r"acquire_workspace|acquire_tagged|cudaMalloc", text)
