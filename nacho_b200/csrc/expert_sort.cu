@@ -604,7 +604,7 @@ template <typename C>
 int make_order(const Order &o, int tile, int tiles, cudaStream_t stream) {
     int st;
     const size_t count_smem = sizeof(int32_t) * o.experts, place_smem = sizeof(int32_t) * o.experts * (NT / 32 + 2);
-    if (place_smem > 48 * 1024 && (st = allow_shared(k_order_place<C>, place_smem))) return st;
+    if (place_smem > 32 * 1024 && (st = allow_shared(k_order_place<C>, place_smem))) return st;
     {
         LaunchScope scope("order_count", stream);
         NB200_CUDA(launch_overlapped(k_order_count<C>, dim3(tiles), dim3(NT), count_smem, stream, o, tile));

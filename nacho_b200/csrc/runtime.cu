@@ -179,9 +179,10 @@ int wait_result_word(const unsigned long long *word, cudaStream_t stream, int64_
 }
 
 namespace {
-// Per device and kernel: the shared memory allowed so far, and the CTAs per SM (0: not asked yet).
+// Per device and kernel: the dynamic shared memory allowed so far (the 48 KB that need not be asked for are a kernel's static and dynamic memory
+// together, so a kernel is allowed what it first asks for), and the CTAs per SM (0: not asked yet).
 struct KernelFacts {
-    size_t shared = 48 * 1024;
+    size_t shared = 0;
     int resident = 0;
 };
 std::mutex g_facts_mutex;

@@ -66,6 +66,13 @@ def test_many_experts(experts, tokens, k):
     assert_order(nacho().gpu_expert_order(r), token, expert, experts)
 
 
+@pytest.mark.parametrize("experts", range(1224, 1231))
+def test_experts_whose_counters_take_48_kb(experts):
+    """With a kernel's other shared memory that is more than it has without asking."""
+    r, token, expert, _ = routing(3000, experts, 1, seed=experts)
+    assert_order(nacho().gpu_expert_order(r), token, expert, experts)
+
+
 def test_tiles_whose_entries_16_bits_do_not_count():
     """More than 2^15 entries a tile, all of them of one expert."""
     entries = (1 << 23) + 12345
