@@ -658,6 +658,7 @@ int nb200_expert_sort_fp8(const nb200_csr *r, const nb200_dense *x, nb200_expert
     int st;
     if ((st = check_routing(r, order))) return st;
     if (!dense_ok(x) || !fp8_ok(xs) || x->rows != r->rows || xs->groups != 1 || xs->tiled || xs->rows != r->nnz || xs->cols != x->cols) return NB200_E_BADARG;
+    if (x->cols == 0) return nb200_expert_sort(r, nullptr, order, nullptr, stream_);  // the kernels below fill in the order beside a token's first block
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const Order o = order_of(order, r->col);
     const bool all_in_one = o.entries <= FEW_ENTRIES;

@@ -27,6 +27,23 @@ def test_no_experts(dtype, tokens, k, n):
     assert dx.shape == (tokens * k, 200) and not dx.any() and dw.shape == (0, n, 200)
 
 
+@pytest.mark.parametrize("tokens", [0, 7, 3000])
+def test_no_columns(tokens):
+    """Rows without columns still have an order, and nothing is summed over them."""
+    r, token, expert, _ = routing(tokens, 6, 3, seed=tokens, ragged=True, drop=0.1)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.zeros(tokens, 0, dtype=dtype, device="cuda")
+        order, a = nacho().gpu_expert_sort_fp8(r, x)
+        assert_order(order, token, expert, 6)
+        assert tuple(a.shape.tolist()) == (1, len(expert), 0)
+        assert_order(nacho().gpu_expert_sort(r, x)[0], token, expert, 6)
+        y = nacho().gpu_fp8_product(a, nacho().to_fp8_tiles(torch.zeros(6, 40, 0, device="cuda")), order, dtype=dtype)
+        assert y.shape == (len(expert), 40) and not y.any()
+        dx, dw = nacho().gpu_fp8_product_grad(normal((len(expert), 40), dtype, 1), torch.zeros(len(expert), 0, dtype=dtype, device="cuda"),
+                                              nacho().to_fp8_tiles(torch.zeros(6, 40, 0, device="cuda")), order)
+        assert dx.shape == (len(expert), 0) and dw.shape == (6, 40, 0)
+
+
 def test_graphs_outlive_larger_calls_and_one_another():
     """Two graphs captured on one stream, a larger call there afterwards, and both replayed at once on two other streams: each one's order is its own."""
     cases = [routing(3000, 64, 4, seed=1), routing(2500, 300, 7, seed=2, ragged=True, drop=0.1)]
