@@ -459,7 +459,7 @@ nb200_dense view_dense(PyObject *o, View &v, const char *where, const char *name
     if (three) {
         all = t.size(0) * rows;
         if (rows == 1) stride = t.size(0) > 1 ? t.stride(0) : cols;
-        else if (t.size(0) > 1 && t.stride(0) != rows * stride) refuse(PyExc_TypeError, "%s: the groups of %s must follow one another", where, name);
+        else if (t.size(0) > 1 && t.numel() > 0 && t.stride(0) != rows * stride) refuse(PyExc_TypeError, "%s: the groups of %s must follow one another", where, name);
     }
     if (groups) *groups = three ? t.size(0) : 1;
     v.device = t.device();

@@ -42,6 +42,18 @@ def test_no_columns(tokens):
         dx, dw = nacho().gpu_fp8_product_grad(normal((len(expert), 40), dtype, 1), torch.zeros(len(expert), 0, dtype=dtype, device="cuda"),
                                               nacho().to_fp8_tiles(torch.zeros(6, 40, 0, device="cuda")), order)
         assert dx.shape == (len(expert), 0) and dw.shape == (6, 40, 0)
+        dx, dw = nacho().gpu_fp8_product_grad(torch.zeros(len(expert), 0, dtype=dtype, device="cuda"), normal((len(expert), 40), dtype, 1),
+                                              nacho().to_fp8_tiles(torch.zeros(6, 0, 40, device="cuda")), order)
+        assert dx.shape == (len(expert), 40) and not dx.any() and dw.shape == (6, 0, 40)
+
+
+@pytest.mark.parametrize("shape", [(3, 0, 128), (2, 0, 1), (3, 5, 0), (0, 0, 0), (4, 0, 0)])
+def test_tiles_of_groups_without_elements(shape):
+    w = nacho().to_fp8_tiles(torch.zeros(shape, device="cuda"))
+    assert tuple(w.shape.tolist()) == shape and w.to_dense().shape == shape
+    assert tuple(w.transposed().shape.tolist()) == (shape[0], shape[2], shape[1])
+    wide = torch.zeros(shape[0], shape[1] + 3, shape[2] + 3, device="cuda")
+    assert tuple(nacho().to_fp8_tiles(wide[:, 3:, 3:]).shape.tolist()) == shape
 
 
 def test_graphs_outlive_larger_calls_and_one_another():
