@@ -611,12 +611,13 @@ __global__ void __launch_bounds__(FEW_THREADS, NB == 16 ? 3 : NB == 128 ? 1 : 2)
 
 // ---- operands of the gradient ------------------------------------------------------------
 
-// Blocks of 128 rows, counted from each group's first: where a group's blocks begin, and every block's rows {first, how many}. One CTA.
+// Blocks of 128 rows, counted from each group's first: where a group's blocks begin, and every block's rows {first, how many}. One CTA. Offsets that fall
+// stand for up to 2^35 blocks, which are counted in two parts of 12 and more bits; those from `bound` on are left out.
 __global__ void __launch_bounds__(1024) k_group_blocks(const int32_t *offsets, int groups, int rows, int bound, int32_t *first_block, int2 *block) {
-    __shared__ int tmp[33];
+    __shared__ int tmp[66];
     wait_for_previous();
     trigger_dependents();
-    int base = 0;
+    int64_t base = 0;
     for (int g0 = 0; g0 < groups; g0 += 1024) {
         const int g = g0 + threadIdx.x;
         int from = 0, to = 0;
@@ -624,16 +625,18 @@ __global__ void __launch_bounds__(1024) k_group_blocks(const int32_t *offsets, i
             from = offsets ? min(max(ld_late(offsets + g), 0), rows) : 0;
             to = offsets ? min(max(ld_late(offsets + g + 1), from), rows) : rows;
         }
-        int sum;
-        const int at = base + block_excl_sum<1024>((to - from + BLOCK8 - 1) / BLOCK8, tmp, sum);
+        const int n = (to - from + BLOCK8 - 1) / BLOCK8;
+        int high, low, all_high, all_low;
+        block_excl_sum2<1024>(n >> 12, n & 4095, tmp, high, low, all_high, all_low);
+        const int64_t at = base + ((int64_t)high << 12) + low;
         if (g < groups) {
-            first_block[g] = min(at, bound);
+            first_block[g] = (int)min(at, (int64_t)bound);
             for (int b = 0; from + b * BLOCK8 < to && at + b < bound; ++b) block[at + b] = make_int2(from + b * BLOCK8, min(BLOCK8, to - from - b * BLOCK8));
         }
-        base += sum;
+        base += ((int64_t)all_high << 12) + all_low;
     }
-    if (threadIdx.x == 0) first_block[groups] = min(base, bound);
-    for (int b = base + threadIdx.x; b < bound; b += 1024) block[b] = make_int2(0, 0);
+    if (threadIdx.x == 0) first_block[groups] = (int)min(base, (int64_t)bound);
+    for (int64_t b = base + threadIdx.x; b < bound; b += 1024) block[b] = make_int2(0, 0);
 }
 
 // x by blocks of rows: column c becomes row c of the result, a scale for it per block. A CTA per block and 128 columns: a thread has eight columns of

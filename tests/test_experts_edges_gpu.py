@@ -171,6 +171,22 @@ def test_as_many_entries_as_there_can_be(entries, room):
     assert not dz[first[-1]:].any()
 
 
+def test_offsets_that_fall_stand_for_more_blocks_than_32_bits_count(room):
+    """Every other group has all rows: the first one's gradient is whole, the next one gets what blocks are left, the others none."""
+    rows, groups = 140_000_000, 4096
+    zigzag = torch.arange(groups + 1, device="cuda", dtype=torch.int32) % 2 * rows
+    nobody = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    order = nacho().ExpertOrder_gpu(zigzag, nobody, nobody, torch.zeros(1, dtype=torch.int32, device="cuda"), (0, groups))
+    ones = torch.ones(rows, 1, dtype=torch.bfloat16, device="cuda")
+    dx, dw = nacho().gpu_fp8_product_grad(ones, ones, nacho().to_fp8_tiles(torch.ones(groups, 1, 1, device="cuda")), order)
+    assert dx.shape == (rows, 1)
+    want = torch.zeros(groups, device="cuda")
+    want[0], want[2] = rows, groups * 128  # there is room for a block per group more than the rows have
+    # every block stands for 128 within two roundings of its scales; a million of them are added in 32 bits
+    assert torch.all((dw.flatten() - want).abs() <= want * (2 ** -22 + rows / 128 * 2 ** -24))
+    assert not dw[1].any() and not dw[3:].any()
+
+
 def test_as_many_tokens_as_there_can_be(room):
     """A thousand entries over the rows of all numbers of tokens that 32 bits count."""
     row_ptr = filled(MOST + 1, lambda t: t * 1000 // MOST)
