@@ -57,6 +57,9 @@ int acquire_tagged(cudaStream_t stream, size_t words, Tagged *out);
 // says so itself where it fails or the word reports an error.)
 void spoil_tagged(cudaStream_t stream);
 
+// The slot whose pinned words nb200_release_workspaces leaves alone: calls do not wait for the kernels that write there, and neither do graphs of them.
+constexpr int REPORT_SLOT = 9;
+
 // Gives the device memory of one block back once the work queued on `stream` is done with it. Returns whether there was any.
 bool drop_workspace(cudaStream_t stream, int slot);
 

@@ -728,10 +728,9 @@ dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min
 
 // The word by which a product of this stream says that a wait gave up. The call does not wait for its kernel, so the next one on the stream
 // finds it and returns the error in its place.
-constexpr int PRODUCT_SLOT = 9;
 int report_of(cudaStream_t stream, Workspace **ws) {
     int st;
-    if ((st = acquire_workspace(stream, 0, ws, PRODUCT_SLOT))) return st;
+    if ((st = acquire_workspace(stream, 0, ws, REPORT_SLOT))) return st;
     volatile unsigned long long *word = reinterpret_cast<volatile unsigned long long *>((*ws)->host) + 32;
     const unsigned long long said = *word;
     if (!(said & RW_VALID)) return NB200_OK;

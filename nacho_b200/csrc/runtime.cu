@@ -265,15 +265,19 @@ int nb200_release_workspaces(void) {
     std::lock_guard<std::mutex> g(g_ws_mutex);
     int prev = 0;
     cudaGetDevice(&prev);
-    for (auto &kv : g_workspaces) {
-        cudaSetDevice(kv.first.first.first);
-        if (kv.second.dev) {
-            cudaDeviceSynchronize();
-            cudaFree(kv.second.dev);
+    for (auto it = g_workspaces.begin(); it != g_workspaces.end();) {
+        if (it->first.first.second == REPORT_SLOT) {
+            ++it;
+            continue;
         }
-        if (kv.second.host) cudaFreeHost(kv.second.host);
+        cudaSetDevice(it->first.first.first);
+        if (it->second.dev) {
+            cudaDeviceSynchronize();
+            cudaFree(it->second.dev);
+        }
+        if (it->second.host) cudaFreeHost(it->second.host);
+        it = g_workspaces.erase(it);
     }
-    g_workspaces.clear();
     g_ws_epoch.fetch_add(1, std::memory_order_release);
     cudaSetDevice(prev);
     return NB200_OK;

@@ -87,6 +87,30 @@ def test_graphs_outlive_larger_calls_and_one_another():
             assert torch.equal(xs, torch.where((rows >= 0)[:, None], x[rows.clamp(min=0)], torch.zeros((), dtype=x.dtype, device="cuda")))
 
 
+def test_a_report_finds_its_word_after_a_release():
+    """A product that gives up while the scratch pools are released still has a place to say so."""
+    import ctypes as C
+    from nacho_b200 import _capi
+    n = nacho()
+    a, w = n.to_fp8_rows(normal((300, 700), torch.float32, 1)), n.to_fp8_tiles(normal((200, 700), torch.float32, 2))
+    want = n.gpu_fp8_product(a, w, dtype=torch.float32)
+    y = torch.full((300, 200), 7.0, device="cuda")
+    struct = lambda m: _capi.Fp8Struct(*m._dims, int(m.tiled), m._values.data_ptr(), m._scales.data_ptr())
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()  # without scratch of its own, for which a release would wait
+    status = _capi.lib.nb200_selftest_product_timeout(C.byref(struct(a)), C.byref(struct(w)), C.byref(_capi.DenseStruct(300, 200, 200, 0, y.data_ptr())),
+                                                      C.c_void_p(stream.cuda_stream))
+    assert status == _capi.OK and _capi.lib.nb200_release_workspaces() == _capi.OK
+    torch.cuda.synchronize()
+    assert torch.all(y == 7.0)
+    with torch.cuda.stream(stream):
+        with pytest.raises(RuntimeError, match="earlier 8-bit product: matrix product pipeline gave up"):
+            n.gpu_fp8_product(a, w)
+        got = n.gpu_fp8_product(a, w, dtype=torch.float32)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("experts", [1280, 2560, 2561, 4096])
 @pytest.mark.parametrize("tokens,k", [(2561, 1), (1025, 4), (8193, 1), (70001, 3)])
 def test_many_experts(experts, tokens, k):
