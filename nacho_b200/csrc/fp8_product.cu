@@ -724,8 +724,6 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(cons
 
 // ---- host ------------------------------------------------------------------------------
 
-dim3 grid_of(int64_t ctas) { return dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, sm_count() * 64ll))); }
-
 // The word by which a product of this stream says that a wait gave up. The call does not wait for its kernel, so the next one on the stream
 // finds it and returns the error in its place.
 int report_of(cudaStream_t stream, Workspace **ws) {
