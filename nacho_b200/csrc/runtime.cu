@@ -180,10 +180,10 @@ int wait_result_word(const unsigned long long *word, cudaStream_t stream, int64_
 
 namespace {
 // Per device and kernel: the dynamic shared memory allowed so far (the 48 KB that need not be asked for are a kernel's static and dynamic memory
-// together, so a kernel is allowed what it first asks for), and the CTAs per SM (0: not asked yet).
+// together, so a kernel is allowed what it first asks for), and the CTAs per SM by their threads.
 struct KernelFacts {
     size_t shared = 0;
-    int resident = 0;
+    std::map<int, int> resident;
 };
 std::mutex g_facts_mutex;
 std::map<std::pair<int, const void *>, KernelFacts> g_facts;
@@ -204,9 +204,9 @@ int resident_ctas(const void *kernel, int threads) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
     std::lock_guard<std::mutex> g(g_facts_mutex);
-    KernelFacts &f = g_facts[{dev, kernel}];
-    if (!f.resident && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&f.resident, kernel, threads, 0) != cudaSuccess || f.resident < 1)) f.resident = 1;
-    return f.resident;
+    int &n = g_facts[{dev, kernel}].resident[threads];
+    if (!n && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1)) n = 1;
+    return n;
 }
 
 uint64_t workspace_epoch() { return g_ws_epoch.load(std::memory_order_acquire); }
