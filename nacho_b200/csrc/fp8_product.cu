@@ -762,13 +762,16 @@ int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int g
     int each = 1;
     while (slices == 1 && each < 8 && a.blocks * each <= 8 && wide * used * turns >= (int64_t)16 * each * sm_count()) each *= 2;
     if (wide * slices > INT32_MAX || turns > 65535) return NB200_E_UNSUPPORTED;
-    auto kernel = slices > 1 ? k_product_few<T, NB, true> : k_product_few<T, NB, false>;
-    const size_t smem = slices > 1 ? FewShape<NB, true>::SHARED_BYTES : FewShape<NB, false>::SHARED_BYTES;
-    if ((st = allow_shared(kernel, smem))) return st;
-    LaunchScope scope("fp8_product_few", stream);
-    NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)((wide + each - 1) / each * slices), (unsigned)groups, (unsigned)turns), dim3(FEW_THREADS), smem, stream, a, w, offsets, groups, y.rows, y.cols,
-                                          static_cast<T *>(y.data), y.stride, each, report));
-    return NB200_OK;
+    auto go = [&](auto kernel, size_t smem) -> int {
+        if ((st = allow_shared(kernel, smem))) return st;
+        LaunchScope scope("fp8_product_few", stream);
+        NB200_CUDA(launch_overlapped_clusters(slices, kernel, dim3((unsigned)((wide + each - 1) / each * slices), (unsigned)groups, (unsigned)turns), dim3(FEW_THREADS), smem, stream, a, w,
+                                              offsets, groups, y.rows, y.cols, static_cast<T *>(y.data), y.stride, each, report));
+        return NB200_OK;
+    };
+    if constexpr (NB < 64)  // of more rows, long sums of so few tiles that they are always shared
+        if (slices == 1) return go(k_product_few<T, NB, false>, FewShape<NB, false>::SHARED_BYTES);
+    return go(k_product_few<T, NB, true>, FewShape<NB, true>::SHARED_BYTES);
 }
 
 // The result as the copy engine sees it: boxes of 32 rows by 128 bytes.
@@ -887,13 +890,14 @@ int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *off
     //   - few rows: with groups while NB rows are three times the mean, so that hardly a group takes two turns (32 groups of 2048 x 2048: 28 against
     //     34 with 16 rows each, 35 against 34 with 24); one group up to 32 rows (4096 x 4096: 7 to 8 against 17), and where the sums are long enough
     //     to be worth sharing, up to 64 (4096 x 4096: 12 against 17; 1024 x 2048: 10 either way; 2048 x 1024: 13 against 7) and beyond, while
-    //     tiles leave half of the SMs idle (128 rows, 1024 x 8192: 13 against 30; 4096 x 4096: 17 either way);
+    //     tiles leave more than half of the SMs idle, so that a cluster shares them (128 rows, 1024 x 8192: 13 against 30; 4096 x 4096: 17 either
+    //     way; at half, 9472 x 8192, nothing is shared: 42 against 29);
     //   - pairs of CTAs from where single ones have a second tile (4096 x 4096, 512 rows: 19 against 18; 768 rows: 20 against 31) and groups fill
     //     most of 128 rows (32 groups of 2048 x 2048 with 96 rows: 41 against 36, with 128 rows: 42 against 50);
     //   - no groups: the tiles' kernel, which finds none and clears the rows, all of them rows of no group.
     // tiles at most: a group may begin and end inside tiles
     const int64_t groups = w->groups, mean = groups ? (y->rows + groups - 1) / groups : 0, singles = blocks_of(y->rows) * blocks_of(y->cols);
-    const bool one = groups == 1, idle = 2 * singles <= sm_count(), pair = mean >= 112 && singles > sm_count();
+    const bool one = groups == 1, idle = 2 * singles < sm_count(), pair = mean >= 112 && singles > sm_count();
     const int64_t side = pair ? 256 : 128, tiles = ((y->rows + side - 1) / side + 2 * groups) * ((y->cols + side - 1) / side);
     if (tiles > INT32_MAX / 64 || y->rows > INT32_MAX - 1024 || y->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     return with_type(y->type, [&](auto e) {
