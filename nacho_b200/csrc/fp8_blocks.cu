@@ -182,7 +182,8 @@ extern "C" {
 
 int64_t nb200_fp8_value_count(const nb200_fp8 *m) {
     if (!m || m->groups < 0 || m->rows < 0 || m->cols < 0 || (!m->tiled && m->groups != 1)) return -1;
-    return m->groups * blocks_of(m->cols) * padded_rows(m->rows) * BLOCK8;
+    const int64_t rows = (int64_t)m->groups * padded_rows(m->rows), line = blocks_of(m->cols) * BLOCK8;
+    return line > 0 && rows > INT64_MAX / line ? -1 : rows * line;
 }
 
 int64_t nb200_fp8_scale_count(const nb200_fp8 *m) {

@@ -63,3 +63,16 @@ def test_an_order_keeps_nothing_between_calls():
     """What a captured graph writes into has to be the graph's own: a pool that grows frees what it had, and two graphs would share it."""
     text = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "nacho_b200", "csrc", "expert_sort.cu")).read())
     assert not re.search(r"acquire_workspace|acquire_tagged|cudaMalloc", text)
+
+
+def test_extents_whose_codes_64_bits_do_not_count():
+    from nacho_b200._capi import Fp8Struct, lib
+    import ctypes as C
+    values, scales = (lambda *m: lib.nb200_fp8_value_count(C.byref(Fp8Struct(*m, None, None)))), (lambda *m: lib.nb200_fp8_scale_count(C.byref(Fp8Struct(*m, None, None))))
+    most = (1 << 31) - 1
+    assert values(1, 9, 129, 0) == 2 * 16 * 128 and scales(1, 9, 129, 0) == 2 * 16
+    assert values(3, 130, 129, 1) == 3 * 2 * 136 * 128 and scales(3, 130, 129, 1) == 3 * 2 * 2
+    assert values(1, most, most, 0) == (1 << 24) * (1 << 31) * 128 and scales(1, most, most, 0) == (1 << 24) * (1 << 31)
+    for m in ((2, most, most, 1), (4096, most, most, 1), (most, most, most, 1), (-1, 1, 1, 1), (2, 1, 1, 0)):
+        assert values(*m) == -1 and scales(*m) == -1
+    assert values(most, 0, most, 1) == 0 and values(most, most, 0, 1) == 0
