@@ -182,8 +182,8 @@ extern "C" {
 
 int64_t nb200_fp8_value_count(const nb200_fp8 *m) {
     if (!m || m->groups < 0 || m->rows < 0 || m->cols < 0 || (!m->tiled && m->groups != 1)) return -1;
-    const int64_t rows = (int64_t)m->groups * padded_rows(m->rows), line = blocks_of(m->cols) * BLOCK8;
-    return line > 0 && rows > INT64_MAX / line ? -1 : rows * line;
+    int64_t all;  // a division to look ahead would take longer than all else that a call checks
+    return __builtin_mul_overflow(m->groups * padded_rows(m->rows), blocks_of(m->cols) * BLOCK8, &all) ? -1 : all;
 }
 
 int64_t nb200_fp8_scale_count(const nb200_fp8 *m) {
