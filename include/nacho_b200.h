@@ -354,8 +354,9 @@ int nb200_inner_prod_coo_f32(const nb200_coo3 *a, const nb200_coo3 *b, float *z,
  *   - Rows of R may be empty or hold any number of entries, in any order of experts (duplicates count twice).
  *     An entry whose column lies outside [0, cols) is dropped: it has no slot and takes part in nothing.
  *   - None of the calls waits for the device: all result lengths are known before. They can be captured in a CUDA
- *     graph once a call of their kind has been made on the stream, and use no device memory but what the caller gives
- *     them, so graphs may be replayed on any stream, beside one another and after calls of any size.
+ *     graph once a call of their kind has been made on the stream (a product's first one there allocates 512 bytes of
+ *     pinned memory for its report), and use no device memory but what the caller gives them, so graphs may be
+ *     replayed on any stream, beside one another and after calls of any size.
  *   - Sums are 32-bit, in a fixed order: the same call gives the same bits. */
 
 /* Dense rows in device memory: element (r, c) lies at data[r * stride + c]. */
@@ -372,7 +373,7 @@ typedef struct nb200_expert_order {
     int32_t tokens, experts, entries;
     int32_t *row_ptr; /* R's own, tokens + 1 */
     int32_t *offsets; /* experts + 1: where each expert's slots begin */
-    int32_t *rows;    /* entries: the token of every slot, -1 for a slot of nobody */
+    int32_t *rows;    /* entries: the token of every slot, -1 for a slot of nobody (and counts while the order is made) */
     int32_t *slots;   /* entries: the slot of every entry of R, -1 for a dropped one */
 } nb200_expert_order;
 
@@ -416,11 +417,12 @@ int nb200_fp8_unpack(const nb200_fp8 *a, float *z, void *stream);
 int nb200_fp8_transpose(const nb200_fp8 *a, nb200_fp8 *z, void *stream);
 
 /* The products' waits for copies and matrix instructions are bounded (two seconds, where microseconds are usual). One that gave up is reported by
- * the next product on the stream, which returns NB200_E_TIMEOUT and does nothing.
+ * the next product called on the stream, which returns NB200_E_TIMEOUT and does nothing. One in a graph reports to the stream that it was captured
+ * on, wherever the graph is replayed.
  *
  * y[i] = a[i] * w[g]^T: rows a (tiled = 0), weights w (tiled = 1) with as many columns, y of a->rows x w->rows in any type. With
  * `offsets` (w->groups + 1 of them, rising, in device memory) rows offsets[g] .. offsets[g + 1] - 1 take group g and rows
- * in front of the first or behind the last are zeros; without it there is one group. Products of a block of 128 columns are summed on
+ * in front of the first or behind the last are zeros, all rows where there are no groups; without it there is one group. Products of a block of 128 columns are summed on
  * the tensor cores and the blocks, times their two scales, in 32 bits. */
 int nb200_fp8_product(const nb200_fp8 *a, const nb200_fp8 *w, const int32_t *offsets, nb200_dense *y, void *stream);
 /* The gradient for the weights: z[g] = sum over the rows i of group g of dy[i]^T x[i], z = [groups][dy->cols][x->cols] 32-bit. Both

@@ -8,7 +8,8 @@ weights in 8-bit floating point, and brought back:
     y = gpu_expert_unsort(r, order, z)
 
 Dense operands are 2-D CUDA tensors of float32, float16 or bfloat16 with contiguous rows at any distance; results are new
-contiguous tensors. No call waits for the device. Sums are 32-bit in a fixed order and rounded once.
+contiguous tensors without an autograd graph: gradients are calls of their own. No call waits for the device, and all of them can be captured in graphs, products once one
+has been called on the stream. Sums are 32-bit in a fixed order and rounded once.
 """
 from __future__ import annotations
 
@@ -125,7 +126,7 @@ def to_fp8_tiles(w, scales=None) -> FP8_gpu:
 
 
 def gpu_expert_order(r: CSR_gpu) -> ExpertOrder_gpu:
-    """The order of the experts, for rows that are moved later. At most 4096 experts."""
+    """The order of the experts, for rows that are moved later. At most 4096 experts, and 2^31 - 1025 tokens and entries."""
     return _native.expert_order(r)
 
 
@@ -156,7 +157,8 @@ def gpu_expert_unsort_grad(r: CSR_gpu, order: ExpertOrder_gpu, z: torch.Tensor, 
 
 
 def gpu_fp8_product(a: FP8_gpu, w: FP8_gpu, order: ExpertOrder_gpu | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``a @ w.T`` for rows ``a`` and tiles ``w``; with an order, the rows of expert ``c`` are multiplied with ``w[c]``, and slots of nobody get zeros."""
+    """``a @ w.T`` for rows ``a`` and tiles ``w``; with an order, the rows of expert ``c`` are multiplied with ``w[c]``, and slots of nobody get
+    zeros (all of them where there are no experts)."""
     if dtype not in _TYPES:
         raise TypeError("gpu_fp8_product: dtype must be float32, float16 or bfloat16")
     return _native.fp8_product(a, w, order, _TYPES[dtype])
