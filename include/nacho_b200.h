@@ -434,6 +434,70 @@ int nb200_fp8_product_grad_w(const nb200_dense *dy, const nb200_dense *x, int32_
 /* Bytes of scratch, 256-byte aligned device memory, that it needs: the quantised operands; -1 for impossible operands. */
 int64_t nb200_fp8_product_grad_w_scratch(const nb200_dense *dy, const nb200_dense *x, int32_t groups);
 
+/* ---- gated layers ------------------------------------------------------------------------- */
+
+/* The gated half of a feed-forward layer, dense or by expert, in 16 bits: with g = x Wg^T and u = x Wu^T, h = act(g) u. w holds `groups` matrices of
+ * 2 * hidden x x->cols, one after another (w->rows = groups * 2 * hidden): first the hidden rows of Wg, then those of Wu. All operands of a call are of one type,
+ * float16 or bfloat16; sums are 32-bit, in a fixed order, and rounded once. `offsets` as in the products above: groups + 1 of them, rising, rows of no
+ * group are zeros; without it there is one group. None of the calls waits for the device, and they can be captured as the products can.
+ * act: v s(v) with the logistic function s (silu), or v s(2 sqrt(2 / pi) (v + 0.044715 v^3)), the tanh form of gelu. */
+typedef enum nb200_activation { NB200_SILU = 0, NB200_GELU = 1 } nb200_activation;
+
+/* both: NULL, or [g u] rounded to the type (2 * hidden columns, rows one after another), which the backward pass takes. scratch: 256-byte aligned device
+ * memory of nb200_gated_product_scratch bytes (rows that the copy engine cannot read are copied there; mostly 0); -1 for impossible operands. */
+int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t groups, const int32_t *offsets, int32_t activation, nb200_dense *h,
+                        nb200_dense *both, void *scratch, int64_t scratch_bytes, void *stream);
+int64_t nb200_gated_product_scratch(const nb200_dense *x, const nb200_dense *w, int32_t groups);
+/* Gradients: with dboth = [dh u act'(g), dh act(g)] rounded to the type, dx = dboth w (zeros for rows of no group) and, for every group, its matrix of
+ * dw = dboth^T x over the group's rows (zeros where it has none), dw laid out as w without gaps between groups. */
+int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, const nb200_dense *x, const nb200_dense *w, int32_t groups,
+                             const int32_t *offsets, int32_t activation, nb200_dense *dx, nb200_dense *dw, void *scratch, int64_t scratch_bytes,
+                             void *stream);
+int64_t nb200_gated_product_grad_scratch(const nb200_dense *x, const nb200_dense *w, int32_t groups);
+
+/* ---- products in 8-bit integers ------------------------------------------------------------ */
+
+/* Rows of 8-bit integers with a 32-bit scale each. With m the largest magnitude of a row, at least 2^-110: scale = m / 127, code = x * (127 / m) rounded to
+ * the nearest whole number (ties to even), the quotients and the product rounded to 32 bits. A row that holds a NaN or an infinity stands for NaNs.
+ * values: [groups * rows][nb200_int8_pitch codes], filled up with zeros, 16-byte aligned. scales: [groups * rows]. */
+typedef struct nb200_int8 {
+    int32_t groups, rows, cols;
+    int8_t *values;
+    float *scales;
+} nb200_int8;
+
+#define NB200_MAX_INT8_COLUMNS 131071 /* a product's sums fit 32 bits, whatever the codes */
+
+int64_t nb200_int8_pitch(const nb200_int8 *m);
+/* Bytes of values for the extents in `m`, -1 if those are not possible. */
+int64_t nb200_int8_value_count(const nb200_int8 *m);
+/* Quantises. The rows of x are those of z, group after group. */
+int nb200_int8_quantise(const nb200_dense *x, nb200_int8 *z, void *stream);
+/* Takes over codes [groups * rows][cols] and scales [groups * rows] that exist. */
+int nb200_int8_pack(const int8_t *codes, const float *scales, nb200_int8 *z, void *stream);
+/* The 32-bit values that a matrix stands for, [groups * rows][cols] one after another. */
+int nb200_int8_unpack(const nb200_int8 *a, float *z, void *stream);
+/* y[i, n] = sa[i] sw[n] sum_k a[i, k] w[g][n, k]: rows a (one group) and channels w (a group per expert), y of any type; offsets as above. The sum is
+ * exact, its product with the two scales rounded to 32 bits each time. At most NB200_MAX_INT8_COLUMNS columns. */
+int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *offsets, nb200_dense *y, void *stream);
+
+/* ---- the norm of gradients ------------------------------------------------------------------ */
+
+/* One of many tensors: `count` elements of a type at `from`, and where the scaled ones go, as another type if need be. `from` and `to` may be the same
+ * place (of one type); otherwise nothing that is written may overlap anything else. */
+typedef struct nb200_span {
+    const void *from;
+    void *to;
+    int64_t count;
+    int32_t type, to_type;
+} nb200_span;
+
+/* norm = the root of the sum of all squares, one float32 in device memory; every element goes over times max_norm / (norm + 1e-6) where that is below 1,
+ * unchanged otherwise, and unchanged if the norm is no finite number. Sums in a fixed order, 64-bit beyond a few elements. `spans` is host memory; scratch:
+ * 256-byte aligned device memory of nb200_clip_scratch bytes. Does not wait for the device; can be captured. */
+int nb200_clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, void *scratch, int64_t scratch_bytes, void *stream);
+int64_t nb200_clip_scratch(const nb200_span *spans, int64_t n);
+
 /* ---- self-test -------------------------------------------------------------------------- */
 
 /* Exercises the give-up path of the bounded device-side waits without faulting or hanging the

@@ -64,6 +64,16 @@ class Fp8Struct(C.Structure):
                 ("values", C.c_void_p), ("scales", C.c_void_p)]
 
 
+class Int8Struct(C.Structure):
+    """``nb200_int8``."""
+    _fields_ = [("groups", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("values", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class SpanStruct(C.Structure):
+    """``nb200_span``."""
+    _fields_ = [("from_", C.c_void_p), ("to", C.c_void_p), ("count", C.c_int64), ("type", C.c_int32), ("to_type", C.c_int32)]
+
+
 OK, E_BADARG, E_CUDA, E_OVERFLOW, E_CAPACITY, E_TIMEOUT, E_NOMEM, E_UNSUPPORTED = range(8)
 
 # name -> (restype, argtypes); every symbol include/nacho_b200.h declares.
@@ -129,6 +139,18 @@ PROTOTYPES = {
     "nb200_fp8_transpose": (C.c_int, [_P(Fp8Struct), _P(Fp8Struct), C.c_void_p]),
     "nb200_fp8_product": (C.c_int, [_P(Fp8Struct), _P(Fp8Struct), C.c_void_p, _P(DenseStruct), C.c_void_p]),
     "nb200_fp8_product_grad_w": (C.c_int, [_P(DenseStruct)] * 2 + [C.c_int32, C.c_void_p, C.c_void_p, _P(Fp8Struct), C.c_void_p, C.c_int64, C.c_void_p]),
+    "nb200_gated_product": (C.c_int, [_P(DenseStruct)] * 2 + [C.c_int32, C.c_void_p, C.c_int32] + [_P(DenseStruct)] * 2 + [C.c_void_p, C.c_int64, C.c_void_p]),
+    "nb200_gated_product_scratch": (C.c_int64, [_P(DenseStruct)] * 2 + [C.c_int32]),
+    "nb200_gated_product_grad": (C.c_int, [_P(DenseStruct)] * 4 + [C.c_int32, C.c_void_p, C.c_int32] + [_P(DenseStruct)] * 2 + [C.c_void_p, C.c_int64, C.c_void_p]),
+    "nb200_gated_product_grad_scratch": (C.c_int64, [_P(DenseStruct)] * 2 + [C.c_int32]),
+    "nb200_int8_pitch": (C.c_int64, [_P(Int8Struct)]),
+    "nb200_int8_value_count": (C.c_int64, [_P(Int8Struct)]),
+    "nb200_int8_quantise": (C.c_int, [_P(DenseStruct), _P(Int8Struct), C.c_void_p]),
+    "nb200_int8_pack": (C.c_int, [C.c_void_p, C.c_void_p, _P(Int8Struct), C.c_void_p]),
+    "nb200_int8_unpack": (C.c_int, [_P(Int8Struct), C.c_void_p, C.c_void_p]),
+    "nb200_int8_product": (C.c_int, [_P(Int8Struct)] * 2 + [C.c_void_p, _P(DenseStruct), C.c_void_p]),
+    "nb200_clip": (C.c_int, [_P(SpanStruct), C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "nb200_clip_scratch": (C.c_int64, [_P(SpanStruct), C.c_int64]),
     "nb200_selftest_product_timeout": (C.c_int, [_P(Fp8Struct)] * 2 + [_P(DenseStruct), C.c_void_p]),
     "nb200_fp8_product_grad_w_scratch": (C.c_int64, [_P(DenseStruct)] * 2 + [C.c_int32]),
 }

@@ -109,6 +109,12 @@ int with_vector(int word, F f) {
     return f(std::integral_constant<int, 1>{});
 }
 
+// ---- 8-bit integers --------------------------------------------------------------------
+
+// A sum of integers times the scales of its row and its channel, the smaller one first: only where the result does so does a product on the way
+// run over, and it loses nothing to numbers that are too small. A scale that is no number makes the result none.
+__device__ __forceinline__ float scaled(int sum, float a, float b) { return (float)sum * (a < b ? a : b) * (a < b ? b : a); }
+
 // ---- 8-bit blocks ----------------------------------------------------------------------
 
 constexpr int BLOCK8 = 128;

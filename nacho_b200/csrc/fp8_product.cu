@@ -3,11 +3,10 @@
 // all rows by one matrix or every group of rows by its own, and the gradient for the weights of the latter,
 //     z[g][n, k] = sum_b sd[n, b] sx[k, b] sum_{i in block b} dy[i, n] x[i, k],   b over blocks of 128 rows of group g.
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "dense_rows.cuh"
-#include "tensor_core.cuh"
+#include "product_waits.cuh"
 
 namespace nb200 {
 namespace {
@@ -32,7 +31,6 @@ constexpr int STORE_WARPS = 8, THREADS = (STORE_WARPS + 4) * 32;
 // Registers a thread: 168 at launch (65536 / 384), then 216 for the two groups of four warps that hold sums and 72 for the third: 64512 as before.
 constexpr int REGS_SUMS = 216, REGS_OTHERS = 72;
 static_assert(256 * REGS_SUMS + 128 * REGS_OTHERS <= 168 * THREADS, "");
-constexpr uint64_t PATIENCE = 2000000000, SHORT_PATIENCE = 20000000;  // ns, after which a wait gives up (microseconds are usual); the self-test's
 
 // A CTA has 128 rows of the result and 128 columns, in a pair 256. Both CTAs of a pair have the same columns, each brings half of their codes.
 template <bool PAIR>
@@ -62,30 +60,11 @@ struct Shape {
     static_assert(SHARED_BYTES <= 227 * 1024, "");
 };
 
-// Which of N places is next, and in which phase of its barriers.
-template <int N>
-struct Ring {
-    int at = 0;
-    uint32_t phase = 0;
-    __device__ void next() {
-        if (++at == N) at = 0, phase ^= 1;
-    }
-};
-
 // A tile of the result: its group, first row (a multiple of 8) and column, the rows that count, and the blocks that are summed.
 struct Tile {
     int g, row, from, to, col;
     int first_block, blocks;
 };
-
-// The order of the tiles of `high` x `wide`: panels of rows, column by column.
-template <int PANEL>
-__device__ __forceinline__ void place_tile(int within, int high, int wide, int *row, int *col) {
-    const unsigned panel = (unsigned)within / (unsigned)(PANEL * wide), width = min((unsigned)PANEL, (unsigned)high - panel * PANEL);
-    const unsigned rest = (unsigned)within - panel * PANEL * wide, column = rest / width;
-    *row = (int)(panel * PANEL + rest - column * width);
-    *col = (int)column;
-}
 
 // Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order. `most`: as many as there
 // are with offsets that rise; others end there.
@@ -145,32 +124,6 @@ struct GradWalk {
         return true;
     }
 };
-
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-
-// For a whole warp; false for all of it once one of its threads, or another warp of the CTA, has given up.
-template <bool SELFTEST = false>
-__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed) {
-    uint64_t start = 0;
-    for (int i = 1;; ++i) {
-        if (__all_sync(FULL_MASK, mbar_try_wait(bar, parity))) return true;
-        if (i % 64) continue;
-        if (__any_sync(FULL_MASK, *failed)) return false;
-        if (!start) start = now_ns();
-        if (__any_sync(FULL_MASK, now_ns() - start > (SELFTEST ? SHORT_PATIENCE : PATIENCE))) break;
-    }
-    *failed = 1;
-    return false;
-}
-
-// After a give-up: what is still on its way lands first, or never will.
-__device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
-    for (const uint64_t start = now_ns(); now_ns() - start < SHORT_PATIENCE && !mbar_try_wait(bar, parity);) {}
-}
 
 // 32 rows of a warp, N columns from `col` on, from registers to memory, through two places in shared memory of 128 bytes of every row. WORD: rows
 // can be written in words of so many bytes. With 16 the copy engine stores a place while the next one is filled, for which all 32 rows have to count (`base`: the
@@ -724,18 +677,6 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 3 : 2) k_fp8_columns(cons
 
 // ---- host ------------------------------------------------------------------------------
 
-// The word by which a product of this stream says that a wait gave up. The call does not wait for its kernel, so the next one on the stream
-// finds it and returns the error in its place.
-int report_of(cudaStream_t stream, Workspace **ws) {
-    int st;
-    if ((st = acquire_workspace(stream, 0, ws, REPORT_SLOT))) return st;
-    volatile unsigned long long *word = reinterpret_cast<volatile unsigned long long *>((*ws)->host) + 32;
-    const unsigned long long said = *word;
-    if (!(said & RW_VALID)) return NB200_OK;
-    *word = 0;
-    return note_timeout(3, (int)(said & RW_VALUE_MASK), "an earlier 8-bit product");
-}
-
 // Slices of the summed axis, CTAs of a cluster, for `tiles` CTAs' worth of work: more while the SMs are not all busy (where one CTA fills an SM: while
 // they would not be more than the SMs), eight at most, of four blocks at least. 256 tiles of 8 blocks
 // take 9 us in one slice and 15 in two, 32 tiles of 32 blocks that fill an SM 11 us in four and 21 in eight.
@@ -776,27 +717,12 @@ int launch_few(const Operand &a, const Operand &w, const int32_t *offsets, int g
 
 // The result as the copy engine sees it: boxes of 32 rows by 128 bytes.
 int describe(const nb200_dense &y, CUtensorMap *map) {
-    typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static std::atomic<encode_fn> known{nullptr};
-    encode_fn encode = known.load(std::memory_order_acquire);
-    if (!encode) {
-        void *found = nullptr;
-        cudaDriverEntryPointQueryResult how = cudaDriverEntryPointSymbolNotFound;
-        NB200_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault, &how));
-        if (how != cudaDriverEntryPointSuccess || !found) return note_cuda_error(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
-        encode = reinterpret_cast<encode_fn>(found);
-        known.store(encode, std::memory_order_release);
-    }
     const CUtensorMapDataType type = y.type == NB200_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : y.type == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const cuuint64_t extents[2] = {(cuuint64_t)y.cols, (cuuint64_t)y.rows}, pitch[1] = {(cuuint64_t)(y.rows > 1 ? y.stride : y.cols) * type_size(y.type)};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / type_size(y.type)), 32}, steps[2] = {1, 1};
-    if (encode(map, type, 2, y.data, extents, pitch, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return note_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
-    return NB200_OK;
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / type_size(y.type)), 32};
+    return encode_matrix(map, type, 2, y.data, extents, pitch, box);
 }
 
 // `tiles` of the shape that `pair` selects, at most.

@@ -1,0 +1,245 @@
+// The gated half of a feed-forward layer, dense or by expert, in 16 bits with 32-bit sums:
+//     g = x Wg^T, u = x Wu^T, h = act(g) u,
+// both products, the activation and their product in one kernel, and its gradients
+//     dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x.
+#include "few_rows.cuh"
+#include "tile_product.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr int NT = 256;
+
+// [rows][cols] with rows at a distance that the copy engine takes. A thread has 16 bytes of a row.
+template <typename T, int V>
+__global__ void __launch_bounds__(NT) k_align_rows(const T *x, int64_t stride, int64_t rows, int64_t cols, T *z, int64_t pitch) {
+    wait_for_previous();
+    trigger_dependents();
+    const int64_t pieces = pitch / 8, all = rows * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
+        const int64_t r = i / pieces, c = (i - r * pieces) * 8;
+        Eight<T> v;
+        v.template load<V>(x + r * stride, c, cols);
+        *reinterpret_cast<uint4 *>(z + r * pitch + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    }
+}
+
+// dboth = [dg du] from dh and [g u], rounded to 16 bits for the tensor cores: off by half a step of the type, as much as the gradients' own rounding.
+template <typename T, int V>
+__global__ void __launch_bounds__(NT) k_gate_grad(const T *dh, int64_t dh_stride, const T *both, int64_t both_stride, int64_t rows, int64_t hidden, bool gelu, T *z, int64_t pitch) {
+    wait_for_previous();
+    trigger_dependents();
+    constexpr int N = Chunk<T, V>::N;
+    const int64_t per_row = (hidden + N - 1) / N, all = rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
+        const int64_t r = i / per_row, at = i - r * per_row, p = V;
+        const int64_t c = at * N;
+        Chunk<T, V> d, g, u, dg, du;
+        d.load(dh + r * dh_stride, c, p, hidden);
+        g.load(both + r * both_stride, c, p, hidden);
+        u.load(both + r * both_stride + hidden, c, p, hidden);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (!Chunk<T, V>::there(k, c, p, hidden)) continue;
+            const float v = g.get(k), dv = d.get(k);
+            float s, rest;  // the logistic function of p(v), and of -|p(v)|
+            const float inner = act_inner(v, gelu);
+            s = logistic(inner, &rest);
+            const float slope = rest * (1.f - rest);  // s (1 - s)
+            const float more = slope == 0.f ? 0.f : v * slope * (gelu ? __fmaf_rn(3.f * GELU3 * v, v, GELU1) : 1.f);
+            dg.set(k, dv * u.get(k) * (s + more));
+            du.set(k, dv * (v * s));
+        }
+        dg.store(z + r * pitch, c, p, hidden);
+        du.store(z + r * pitch + hidden, c, p, hidden);
+    }
+}
+
+unsigned grid_of(int64_t threads) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>((threads + NT - 1) / NT, sm_count() * 16ll)); }
+
+int64_t pitch_of(int64_t cols) { return (cols + 7) / 8 * 8; }
+
+bool act_ok(int32_t activation) { return activation == NB200_SILU || activation == NB200_GELU; }
+bool operands_ok(const nb200_dense *x, const nb200_dense *w, int32_t groups, const int32_t *offsets) {
+    return dense_ok(x) && dense_ok(w) && x->type != NB200_F32 && x->type == w->type && groups >= 0 && x->cols == w->cols && (offsets || groups == 1) &&
+           (groups == 0 ? w->rows == 0 : w->rows % groups == 0 && w->rows / groups % 2 == 0);
+}
+
+template <typename F>
+int with_half(int type, F f) {
+    return type == NB200_F16 ? f(__half{}) : f(__nv_bfloat16{});
+}
+template <typename T>
+constexpr Sum sum_of = std::is_same<T, __half>::value ? Sum::F16 : Sum::BF16;
+
+// Rows as the copy engine reads them: as they are, or copied to `to`.
+int aligned(const nb200_dense &x, int64_t groups, void *to, nb200_dense *z, cudaStream_t stream) {
+    *z = x;
+    if (tiles_readable(x, groups)) return NB200_OK;
+    z->data = to, z->stride = pitch_of(x.cols);
+    return with_half(x.type, [&](auto e) {
+        using T = decltype(e);
+        return with_vector<T>(word_bytes({&x}), [&](auto v) {
+            LaunchScope scope("align_rows", stream);
+            NB200_CUDA(launch_overlapped(k_align_rows<T, decltype(v)::value>, dim3(grid_of(x.rows * (z->stride / 8))), dim3(NT), 0, stream, static_cast<const T *>(x.data), x.stride,
+                                         x.rows, x.cols, static_cast<T *>(to), z->stride));
+            return (int)NB200_OK;
+        });
+    });
+}
+
+// Few rows, whose products take the weights' bytes: they are read as they lie.
+bool few(const nb200_dense *x, int64_t groups) { return x->rows <= 32 * groups; }
+
+struct ForwardScratch {
+    uint8_t *x = nullptr, *w = nullptr;
+    size_t bytes = 0;
+
+    ForwardScratch(void *base, const nb200_dense *xx, const nb200_dense *ww, int64_t groups) {
+        if (few(xx, groups)) return;
+        Carver c(base);
+        if (!tiles_readable(*xx, 1)) x = c.take<uint8_t>((size_t)(xx->rows * pitch_of(xx->cols)) * 2);
+        if (!tiles_readable(*ww, groups)) w = c.take<uint8_t>((size_t)(ww->rows * pitch_of(ww->cols)) * 2);
+        bytes = c.used();
+    }
+};
+
+struct GradScratch {
+    uint8_t *d, *x = nullptr, *w = nullptr;
+    size_t bytes;
+
+    GradScratch(void *base, const nb200_dense *xx, const nb200_dense *ww, int64_t groups) {
+        Carver c(base);
+        d = c.take<uint8_t>((size_t)(xx->rows * pitch_of(groups ? ww->rows / groups : 0)) * 2);
+        if (!tiles_readable(*xx, 1)) x = c.take<uint8_t>((size_t)(xx->rows * pitch_of(xx->cols)) * 2);
+        if (!tiles_readable(*ww, groups)) w = c.take<uint8_t>((size_t)(ww->rows * pitch_of(ww->cols)) * 2);
+        bytes = c.used();
+    }
+};
+
+int zeros(const nb200_dense &y, cudaStream_t stream) {
+    if (y.rows == 0 || y.cols == 0) return NB200_OK;
+    const size_t size = type_size(y.type);
+    NB200_CUDA(cudaMemset2DAsync(y.data, (size_t)(y.rows > 1 ? y.stride : y.cols) * size, 0, (size_t)y.cols * size, (size_t)y.rows, stream));
+    return NB200_OK;
+}
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" {
+
+int64_t nb200_gated_product_scratch(const nb200_dense *x, const nb200_dense *w, int32_t groups) {
+    if (!dense_ok(x) || !dense_ok(w) || groups < 0) return -1;
+    return (int64_t)ForwardScratch(nullptr, x, w, groups).bytes;
+}
+
+int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t groups, const int32_t *offsets, int32_t activation, nb200_dense *h, nb200_dense *both, void *scratch,
+                        int64_t scratch_bytes, void *stream_) {
+    if (!operands_ok(x, w, groups, offsets) || !act_ok(activation) || !dense_ok(h) || h->rows != x->rows || h->type != x->type) return NB200_E_BADARG;
+    const int64_t hidden = groups ? w->rows / groups / 2 : h->cols;
+    if (h->cols != hidden || (both && (!dense_ok(both) || both->rows != x->rows || both->cols != 2 * hidden || both->type != x->type || (both->rows > 1 && both->stride != both->cols))))
+        return NB200_E_BADARG;
+    if (groups > NB200_MAX_EXPERTS || hidden > INT32_MAX / 2 - 1024 || x->rows > INT32_MAX - 1024 || x->cols > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (x->rows == 0 || hidden == 0) return NB200_OK;
+    int st;
+    if (groups == 0 || x->cols == 0) {
+        if ((st = zeros(*h, stream)) || (both && (st = zeros(*both, stream)))) return st;
+        return NB200_OK;
+    }
+    const bool gelu = activation == NB200_GELU;
+    if (few(x, groups)) {
+        const int64_t mean = (x->rows + groups - 1) / groups;
+        const FewArgs args{x->data, w->data, x->rows > 1 ? x->stride : x->cols, w->rows > 1 ? w->stride : w->cols, offsets, groups, (int)x->rows, (int)hidden, (int)x->cols, h->data,
+                           both ? both->data : nullptr, h->rows > 1 ? h->stride : h->cols, nullptr, nullptr, gelu};
+        return with_half(x->type, [&](auto e) {
+            using T = decltype(e);
+            return with_vector<T>(word_bytes({x, w}), [&](auto v) { return launch_few_rows<sum_of<T>, true, decltype(v)::value, T>("gated_few", args, mean, stream); });
+        });
+    }
+    const ForwardScratch s(scratch, x, w, groups);
+    if (s.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0)) return NB200_E_BADARG;
+    if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
+    nb200_dense ax, aw;
+    if ((st = aligned(*x, 1, s.x, &ax, stream)) || (st = aligned(*w, groups, s.w, &aw, stream))) return st;
+    CUtensorMap wide{}, narrow{};
+    if ((st = describe_rows(&wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16)) ||
+        (st = describe_rows(&narrow, map_type(x->type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 32)))
+        return st;
+    TileArgs args{};
+    args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows, args.wide = (int)hidden, args.blocks = (int)((x->cols + 63) / 64);
+    args.tile_n = tile_n_of(x->rows, groups, (hidden + TILE_M / 2 - 1) / (TILE_M / 2));
+    args.y = h->data, args.stride = h->rows > 1 ? h->stride : h->cols, args.both = both ? both->data : nullptr, args.gelu = gelu;
+    args.words = word_bytes({h}) == 16 && (!both || word_bytes({both}) == 16);
+    return with_half(x->type, [&](auto e) {
+        using T = decltype(e);
+        return launch_tiles<sum_of<T>, Form::GATED, false, T>("gated_product", args, wide, narrow, stream);
+    });
+}
+
+int64_t nb200_gated_product_grad_scratch(const nb200_dense *x, const nb200_dense *w, int32_t groups) {
+    if (!dense_ok(x) || !dense_ok(w) || groups < 0) return -1;
+    return (int64_t)GradScratch(nullptr, x, w, groups).bytes;
+}
+
+int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, const nb200_dense *x, const nb200_dense *w, int32_t groups, const int32_t *offsets, int32_t activation,
+                             nb200_dense *dx, nb200_dense *dw, void *scratch, int64_t scratch_bytes, void *stream_) {
+    if (!operands_ok(x, w, groups, offsets) || !act_ok(activation) || !dense_ok(dh) || !dense_ok(both) || !dense_ok(dx) || !dense_ok(dw)) return NB200_E_BADARG;
+    const int type = x->type;
+    const int64_t hidden = groups ? w->rows / groups / 2 : dh->cols;
+    if (dh->type != type || both->type != type || dx->type != type || dw->type != type || dh->rows != x->rows || both->rows != x->rows || dh->cols != hidden || both->cols != 2 * hidden ||
+        dx->rows != x->rows || dx->cols != x->cols || dw->rows != w->rows || dw->cols != w->cols)
+        return NB200_E_BADARG;
+    if (groups > NB200_MAX_EXPERTS || hidden > INT32_MAX / 2 - 1024 || x->rows > INT32_MAX - 1024 || x->cols > INT32_MAX / 2 - 1024) return NB200_E_UNSUPPORTED;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    int st;
+    if (x->cols == 0) return NB200_OK;
+    if (x->rows == 0 || hidden == 0 || groups == 0) {
+        if ((st = zeros(*dx, stream)) || (st = zeros(*dw, stream))) return st;
+        return NB200_OK;
+    }
+    const GradScratch s(scratch, x, w, groups);
+    if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return NB200_E_BADARG;
+    if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
+    nb200_dense ax, aw;
+    if ((st = aligned(*x, 1, s.x, &ax, stream)) || (st = aligned(*w, groups, s.w, &aw, stream))) return st;
+    const int64_t pitch = pitch_of(2 * hidden);
+    const bool gelu = activation == NB200_GELU;
+    // du begins `hidden` elements behind dg, and so does u behind g
+    nb200_dense half = *both;
+    half.cols = hidden, half.data = static_cast<uint8_t *>(both->data) + hidden * 2;
+    nb200_dense to{x->rows, hidden, pitch, type, s.d + hidden * 2};
+    return with_half(type, [&](auto e) -> int {
+        using T = decltype(e);
+        st = with_vector<T>(word_bytes({dh, both, &half, &to}), [&](auto v) {
+            constexpr int V = decltype(v)::value;
+            LaunchScope scope("gate_grad", stream);
+            NB200_CUDA(launch_overlapped(k_gate_grad<T, V>, dim3(grid_of(x->rows * ((hidden + 7) / 8))), dim3(NT), 0, stream, static_cast<const T *>(dh->data), dh->stride,
+                                         static_cast<const T *>(both->data), both->stride, x->rows, hidden, gelu, reinterpret_cast<T *>(s.d), pitch));
+            return (int)NB200_OK;
+        });
+        if (st) return st;
+        CUtensorMap wide{}, narrow{};
+        TileArgs args{};
+        args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows;
+        // dx: the weights' columns on the wide side
+        if ((st = describe_rows(&wide, map_type(type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 64)) ||
+            (st = describe_rows(&narrow, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 32)))
+            return st;
+        args.wide = (int)x->cols, args.blocks = (int)((2 * hidden + 63) / 64), args.tile_n = tile_n_of(x->rows, groups, (x->cols + TILE_M - 1) / TILE_M);
+        args.y = dx->data, args.stride = dx->rows > 1 ? dx->stride : dx->cols, args.words = word_bytes({dx}) == 16;
+        if ((st = launch_tiles<sum_of<T>, Form::ROWS, true, T>("gated_grad_x", args, wide, narrow, stream))) return st;
+        // dw: both operands turned
+        if ((st = describe_rows(&wide, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 64)) ||
+            (st = describe_rows(&narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)))
+            return st;
+        args.wide = (int)(2 * hidden), args.across = (int)x->cols, args.tile_n = x->cols > 128 ? TILE_N : 128;
+        args.y = dw->data, args.stride = dw->rows > 1 ? dw->stride : dw->cols, args.words = word_bytes({dw}) == 16;
+        return launch_tiles<sum_of<T>, Form::WEIGHTS, true, T>("gated_grad_w", args, wide, narrow, stream);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,183 @@
+// Rows in 8-bit integers with a scale each, and products of them: y[i, n] = sa[i] sw[n] sum_k a[i, k] w[n, k], the sum in whole numbers.
+#include "few_rows.cuh"
+#include "tile_product.cuh"
+
+namespace nb200 {
+namespace {
+
+constexpr int NT = 256;
+constexpr float TOP_INT8 = 127.f;
+
+int64_t pitch_of(int64_t cols) { return (cols + 31) / 32 * 32; }
+int64_t all_rows(const nb200_int8 *m) { return (int64_t)m->groups * m->rows; }
+bool int8_ok(const nb200_int8 *m) {
+    return m && m->groups >= 0 && m->rows >= 0 && m->cols >= 0 && nb200_int8_value_count(m) >= 0 && (all_rows(m) == 0 || m->scales) &&
+           (nb200_int8_value_count(m) == 0 || m->values) && reinterpret_cast<uintptr_t>(m->values) % 16 == 0 && reinterpret_cast<uintptr_t>(m->scales) % 4 == 0;
+}
+
+__device__ __forceinline__ uint32_t int_codes4(float a, float b, float c, float d, float inverse) {
+    const int i0 = __float2int_rn(a * inverse), i1 = __float2int_rn(b * inverse), i2 = __float2int_rn(c * inverse), i3 = __float2int_rn(d * inverse);
+    return __byte_perm(__byte_perm(i0, i1, 0x0040), __byte_perm(i2, i3, 0x0040), 0x5410);
+}
+
+// THREADS threads have a row (32, or all of a CTA): they read it for its largest magnitude and again, out of registers as far as KEEP pieces of 16
+// elements a thread go, for its codes.
+template <typename T, int V, int THREADS, int KEEP>
+__global__ void __launch_bounds__(NT) k_int8_rows(const T *x, int64_t stride, int64_t rows, int64_t cols, int8_t *values, int64_t pitch, float *scales) {
+    __shared__ uint32_t top[NT / 32];
+    wait_for_previous();
+    trigger_dependents();
+    const int64_t r = (int64_t)blockIdx.x * (NT / THREADS) + threadIdx.x / THREADS;
+    const int sub = threadIdx.x % THREADS;
+    if (THREADS == 32 && r >= rows) return;
+    const T *const row = x + r * stride;
+    Piece<T> kept[KEEP];
+    Top<T> m;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        kept[i].template load<V>(row, ((int64_t)i * THREADS + sub) * 16, cols);
+        m.add(kept[i].lo), m.add(kept[i].hi);
+    }
+    for (int64_t c = ((int64_t)KEEP * THREADS + sub) * 16; c < cols; c += THREADS * 16) {
+        Piece<T> p;
+        p.template load<V>(row, c, cols);
+        m.add(p.lo), m.add(p.hi);
+    }
+    uint32_t all = __reduce_max_sync(FULL_MASK, m.bits());
+    if constexpr (THREADS != 32) {
+        if (lane_id() == 0) top[warp_id()] = all;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) all = max(all, top[i]);
+    }
+    // a row that holds a NaN or an infinity stands for NaNs: its codes are zeros and its scale is none
+    const bool finite = all < 0x7f800000u;
+    const float largest = __uint_as_float(max(all, FLOOR8)), inverse = finite ? __fdiv_rn(TOP_INT8, largest) : 0.f;
+    if (sub == 0) scales[r] = finite ? __fdiv_rn(largest, TOP_INT8) : __uint_as_float(0x7fc00000u);
+    auto put = [&](const Piece<T> &p, int64_t c) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (finite) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                w[i] = int_codes4(p.lo.get(4 * i), p.lo.get(4 * i + 1), p.lo.get(4 * i + 2), p.lo.get(4 * i + 3), inverse);
+                w[2 + i] = int_codes4(p.hi.get(4 * i), p.hi.get(4 * i + 1), p.hi.get(4 * i + 2), p.hi.get(4 * i + 3), inverse);
+            }
+        }
+        *reinterpret_cast<uint4 *>(values + r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const int64_t c = ((int64_t)i * THREADS + sub) * 16;
+        if (c < pitch) put(kept[i], c);
+    }
+    for (int64_t c = ((int64_t)KEEP * THREADS + sub) * 16; c < pitch; c += THREADS * 16) {
+        Piece<T> p;
+        p.template load<V>(row, c, cols);
+        put(p, c);
+    }
+}
+
+__global__ void __launch_bounds__(NT) k_int8_unpack(const int8_t *values, int64_t pitch, const float *scales, int64_t rows, int64_t cols, float *z) {
+    wait_for_previous();
+    trigger_dependents();
+    const int64_t all = rows * cols;
+    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
+        const int64_t r = i / cols;
+        z[i] = (float)values[r * pitch + i - r * cols] * scales[r];
+    }
+}
+
+}  // namespace
+}  // namespace nb200
+
+using namespace nb200;
+
+extern "C" {
+
+int64_t nb200_int8_pitch(const nb200_int8 *m) { return m && m->cols >= 0 ? pitch_of(m->cols) : -1; }
+
+int64_t nb200_int8_value_count(const nb200_int8 *m) {
+    if (!m || m->groups < 0 || m->rows < 0 || m->cols < 0) return -1;
+    const int64_t rows = all_rows(m), pitch = pitch_of(m->cols);
+    if (rows > 0 && pitch > INT64_MAX / rows) return -1;
+    return rows * pitch;
+}
+
+int nb200_int8_quantise(const nb200_dense *x, nb200_int8 *z, void *stream_) {
+    if (!dense_ok(x) || !int8_ok(z) || x->rows != all_rows(z) || x->cols != z->cols) return NB200_E_BADARG;
+    if (x->rows == 0) return NB200_OK;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (x->rows > INT32_MAX) return NB200_E_UNSUPPORTED;
+    return with_type(x->type, [&](auto e) {
+        using T = decltype(e);
+        return with_vector<T>(word_bytes({x}), [&](auto v) {
+            constexpr int V = decltype(v)::value;
+            auto go = [&](auto kernel, int64_t rows_each) -> int {
+                LaunchScope scope("int8_rows", stream);
+                NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)((x->rows + rows_each - 1) / rows_each)), dim3(NT), 0, stream, static_cast<const T *>(x->data), x->stride, x->rows,
+                                             x->cols, z->values, pitch_of(x->cols), z->scales));
+                return NB200_OK;
+            };
+            // A warp per row where two pieces a thread hold it and there are rows for all warps, else a CTA.
+            if (x->cols <= 1024) return go(k_int8_rows<T, V, 32, 2>, NT / 32);
+            return go(k_int8_rows<T, V, NT, sizeof(T) == 2 ? 2 : 1>, 1);
+        });
+    });
+}
+
+int nb200_int8_pack(const int8_t *codes, const float *scales, nb200_int8 *z, void *stream_) {
+    if (!int8_ok(z) || (all_rows(z) > 0 && !scales) || (nb200_int8_value_count(z) > 0 && !codes)) return NB200_E_BADARG;
+    const int64_t rows = all_rows(z), cols = z->cols, pitch = pitch_of(cols);
+    if (rows == 0) return NB200_OK;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    NB200_CUDA(cudaMemcpyAsync(z->scales, scales, (size_t)rows * sizeof(float), cudaMemcpyDeviceToDevice, stream));
+    if (cols == 0) return NB200_OK;
+    if (pitch > cols) NB200_CUDA(cudaMemset2DAsync(z->values + cols, (size_t)pitch, 0, (size_t)(pitch - cols), (size_t)rows, stream));
+    NB200_CUDA(cudaMemcpy2DAsync(z->values, (size_t)pitch, codes, (size_t)cols, (size_t)cols, (size_t)rows, cudaMemcpyDeviceToDevice, stream));
+    return NB200_OK;
+}
+
+int nb200_int8_unpack(const nb200_int8 *a, float *z, void *stream_) {
+    if (!int8_ok(a) || (all_rows(a) > 0 && a->cols > 0 && !z)) return NB200_E_BADARG;
+    const int64_t rows = all_rows(a);
+    if (rows == 0 || a->cols == 0) return NB200_OK;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    LaunchScope scope("int8_unpack", stream);
+    const int64_t ctas = std::min<int64_t>((rows * a->cols + NT - 1) / NT, sm_count() * 64ll);
+    NB200_CUDA(launch_overlapped(k_int8_unpack, dim3((unsigned)ctas), dim3(NT), 0, stream, a->values, pitch_of(a->cols), a->scales, rows, a->cols, z));
+    return NB200_OK;
+}
+
+int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *offsets, nb200_dense *y, void *stream_) {
+    if (!int8_ok(a) || !int8_ok(w) || !dense_ok(y) || a->groups != 1 || a->cols != w->cols || y->rows != a->rows || y->cols != w->rows || (!offsets && w->groups != 1)) return NB200_E_BADARG;
+    if (w->groups > NB200_MAX_EXPERTS || a->cols > NB200_MAX_INT8_COLUMNS || a->rows > INT32_MAX - 1024 || w->rows > INT32_MAX / 2 - 1024) return NB200_E_UNSUPPORTED;
+    if (y->rows == 0 || y->cols == 0) return NB200_OK;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    const int64_t stride = y->rows > 1 ? y->stride : y->cols, pitch = pitch_of(a->cols), groups = w->groups;
+    int st;
+    if (groups == 0 || a->cols == 0) {
+        // nothing is summed; a row or a channel that stands for NaNs (its scale is one) is zeros too
+        const size_t size = type_size(y->type);
+        NB200_CUDA(cudaMemset2DAsync(y->data, (size_t)stride * size, 0, (size_t)y->cols * size, (size_t)y->rows, stream));
+        return NB200_OK;
+    }
+    return with_type(y->type, [&](auto e) -> int {
+        using T = decltype(e);
+        if (y->rows <= 32 * groups) {
+            const FewArgs args{a->values, w->values, pitch, pitch, offsets, w->groups, a->rows, w->rows, (int)pitch, y->data, nullptr, stride, a->scales, w->scales, false};
+            return launch_few_rows<Sum::S8, false, 16, T>("int8_few", args, (y->rows + groups - 1) / groups, stream);
+        }
+        CUtensorMap wide{}, narrow{};
+        if ((st = describe_rows(&wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, w->values, 1, pitch, w->rows, groups, pitch, 128)) ||
+            (st = describe_rows(&narrow, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, 1, pitch, 32)))
+            return st;
+        TileArgs args{};
+        args.offsets = offsets, args.groups = w->groups, args.rows = a->rows, args.wide = w->rows, args.blocks = (int)((a->cols + 127) / 128);
+        args.tile_n = tile_n_of(a->rows, groups, (w->rows + TILE_M - 1) / TILE_M);
+        args.y = y->data, args.stride = stride, args.row_scale = a->scales, args.col_scale = w->scales, args.words = word_bytes({y}) == 16;
+        return launch_tiles<Sum::S8, Form::ROWS, false, T>("int8_product", args, wide, narrow, stream);
+    });
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@
 #include <map>
 #include <mutex>
 #include <utility>
+#include <vector>
 
 #include "nacho_b200.h"
 
@@ -26,8 +27,8 @@ namespace {
 
 // ---- what nacho_ext.py binds ---------------------------------------------------------------
 
-enum Kind { CSR = 0, COO = 1, DCSR = 2, COO3 = 3, CSF3 = 4, SCALAR = 5, KINDS = 6, ORDER = 6, FP8 = 7, ALL_KINDS = 8 };
-PyTypeObject *g_class[ALL_KINDS] = {};  // the first KINDS from nacho_ext.py, the others from experts.py
+enum Kind { CSR = 0, COO = 1, DCSR = 2, COO3 = 3, CSF3 = 4, SCALAR = 5, KINDS = 6, ORDER = 6, FP8 = 7, INT8 = 8, ALL_KINDS = 9 };
+PyTypeObject *g_class[ALL_KINDS] = {};  // the first KINDS from nacho_ext.py, the others from experts.py and layers.py
 PyObject *g_check = nullptr;  // check(status, where): raises on a non-zero status
 enum Name { N_offsets, N_indices, N_values, N_dims, N_i, N_j, N_k, N_jp, N_kp, N_rows, N_slots, N_token_offsets, N_scales, N_tiled, NAMES };
 PyObject *g_name[NAMES] = {};  // interned slot names
@@ -739,6 +740,234 @@ PyObject *fp8_grad_w(PyObject *const *args) {
     return two(wrap(z), rows.object());
 }
 
+// ---- layers ----------------------------------------------------------------------------------
+
+// A dense operand of a gated layer: 16-bit.
+nb200_dense view_half(PyObject *o, View &v, const char *where, const char *name, int64_t *groups = nullptr) {
+    const nb200_dense x = view_dense(o, v, where, name, groups);
+    if (x.type == NB200_F32) refuse(PyExc_TypeError, "%s: %s must be float16 or bfloat16", where, name);
+    return x;
+}
+
+// w: [2 hidden][width] or one per expert; hidden
+int64_t hidden_of(const View &vw, const char *where) {
+    const int64_t rows = vw.arrays[0].size(-2);
+    if (rows % 2) refuse(PyExc_ValueError, "%s: %s must hold as many rows of gates as of values", where, "w");
+    return rows / 2;
+}
+
+int64_t with_scratch(int64_t bytes, const char *where) {
+    if (bytes < 0) check(NB200_E_BADARG, where);
+    return bytes;
+}
+
+// gated_product(x, w, order or None, activation, keep): h, or (h, both)
+PyObject *gated_product(PyObject *const *args) {
+    const char *where = "gpu_gated_product";
+    View vx, vw, vo;
+    int64_t groups = 1;
+    const nb200_dense x = view_half(args[0], vx, where, "x"), w = view_half(args[1], vw, where, "w", &groups);
+    same_device(vx, vw);
+    same_type(x.type, w.type, where);
+    extent(x.cols, w.cols, where, "x", "columns");
+    const int64_t hidden = hidden_of(vw, where);
+    vo.device = vx.device;
+    const int32_t *offsets = ranges_of(args[2], vo, x.rows, groups, where);
+    same_device(vx, vo);
+    const int activation = (int)PyLong_AsLong(args[3]);
+    const bool keep = args[4] == Py_True;
+    at::Tensor h = matrix(x.rows, hidden, x.type, vx.device), both;
+    nb200_dense out = dense(h, x.type), sums{};
+    if (keep) both = matrix(x.rows, 2 * hidden, x.type, vx.device), sums = dense(both, x.type);
+    const int64_t bytes = with_scratch(nb200_gated_product_scratch(&x, &w, (int32_t)groups), where);
+    at::Tensor scratch;
+    if (bytes) scratch = array(bytes, at::kByte, vx.device);
+    launch({&vx, &vw, &vo}, where, [&](void *stream) {
+        return nb200_gated_product(&x, &w, (int32_t)groups, offsets, activation, &out, keep ? &sums : nullptr, bytes ? scratch.data_ptr() : nullptr, bytes, stream);
+    });
+    return keep ? two(wrap(h), wrap(both)) : wrap(h);
+}
+
+// gated_product_grad(dh, both, x, w, order or None, activation): (dx, dw)
+PyObject *gated_product_grad(PyObject *const *args) {
+    const char *where = "gpu_gated_product_grad";
+    View vd, vb, vx, vw, vo;
+    int64_t groups = 1;
+    const nb200_dense dh = view_half(args[0], vd, where, "dh"), both = view_half(args[1], vb, where, "both"), x = view_half(args[2], vx, where, "x");
+    const nb200_dense w = view_half(args[3], vw, where, "w", &groups);
+    for (const View *v : {&vb, &vx, &vw}) same_device(vd, *v);
+    for (const nb200_dense *o : {&both, &x, &w}) same_type(dh.type, o->type, where);
+    const int64_t hidden = hidden_of(vw, where);
+    extent(x.cols, w.cols, where, "x", "columns");
+    extent(dh.cols, hidden, where, "dh", "columns");
+    extent(both.cols, 2 * hidden, where, "both", "columns");
+    extent(dh.rows, x.rows, where, "dh", "rows");
+    extent(both.rows, x.rows, where, "both", "rows");
+    vo.device = vx.device;
+    const int32_t *offsets = ranges_of(args[4], vo, x.rows, groups, where);
+    same_device(vx, vo);
+    const int activation = (int)PyLong_AsLong(args[5]);
+    at::Tensor dx = matrix(x.rows, x.cols, x.type, vx.device), dw = at::Tensor(at::detail::empty_cuda(vw.arrays[0].sizes(), scalar_of(x.type), vx.device, std::nullopt));
+    nb200_dense out_x = dense(dx, x.type), out_w{w.rows, w.cols, w.cols, x.type, dw.data_ptr()};
+    const int64_t bytes = with_scratch(nb200_gated_product_grad_scratch(&x, &w, (int32_t)groups), where);
+    at::Tensor scratch = array(bytes, at::kByte, vx.device);
+    launch({&vd, &vb, &vx, &vw, &vo}, where, [&](void *stream) {
+        return nb200_gated_product_grad(&dh, &both, &x, &w, (int32_t)groups, offsets, activation, &out_x, &out_w, scratch.data_ptr(), bytes, stream);
+    });
+    return two(wrap(dx), wrap(dw));
+}
+
+nb200_int8 view_int8(PyObject *o, View &v) {
+    const at::Tensor &values = v.array(o, N_values), &scales = v.array(o, N_scales);
+    int32_t d[3];
+    dims_of<3>(o, d);
+    v.device = values.device();
+    return nb200_int8{d[0], d[1], d[2], static_cast<int8_t *>(values.data_ptr()), floats(scales)};
+}
+
+struct Int8Result {
+    at::Tensor values, scales;
+    nb200_int8 m{};
+
+    Int8Result(int64_t groups, int64_t rows, int64_t cols, c10::Device dev, const char *where) {
+        m = nb200_int8{(int32_t)groups, (int32_t)rows, (int32_t)cols, nullptr, nullptr};
+        const int64_t n = with_scratch(nb200_int8_value_count(&m), where), s = groups * rows;
+        values = array(n, at::kChar, dev), scales = float_array(s, dev);
+        m.values = static_cast<int8_t *>(values.data_ptr()), m.scales = floats(scales);
+        used(values, n), used(scales, s);
+    }
+    PyObject *object() {
+        Result r(INT8);
+        r.set(N_values, values), r.set(N_scales, scales);
+        const int32_t d[3] = {m.groups, m.rows, m.cols};
+        r.dims<3>(d);
+        return r.obj.release();
+    }
+};
+
+PyObject *int8_rows(PyObject *const *args) {
+    const char *where = "to_int8_rows";
+    View vx;
+    int64_t groups = 1;
+    const nb200_dense a = view_dense(args[0], vx, where, "x", &groups);
+    Int8Result z(groups, vx.arrays[0].size(-2), a.cols, vx.device, where);
+    launch({&vx}, where, [&](void *stream) { return nb200_int8_quantise(&a, &z.m, stream); });
+    return z.object();
+}
+
+// int8_pack(codes, scales): int8 codes of 2 or 3 dimensions, a scale per row; both contiguous (the caller has checked)
+PyObject *int8_pack(PyObject *const *args) {
+    const char *where = "to_int8_rows";
+    if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) refuse(PyExc_TypeError, "%s: %s must be torch tensors", where, "codes and scales");
+    View vc;
+    vc.arrays[vc.n++] = THPVariable_Unpack(args[0]);
+    vc.arrays[vc.n++] = THPVariable_Unpack(args[1]);
+    const at::Tensor &codes = vc.arrays[0], &scales = vc.arrays[1];
+    vc.device = codes.device();
+    Int8Result z(codes.dim() == 3 ? codes.size(0) : 1, codes.size(-2), codes.size(-1), vc.device, where);
+    launch({&vc}, where, [&](void *stream) { return nb200_int8_pack(static_cast<const int8_t *>(codes.data_ptr()), floats(scales), &z.m, stream); });
+    return z.object();
+}
+
+PyObject *int8_unpack(PyObject *const *args) {
+    const char *where = "to_dense";
+    need_kind(args[0], INT8, where, "INT8_gpu");
+    View va;
+    const nb200_int8 a = view_int8(args[0], va);
+    at::Tensor z = matrix((int64_t)a.groups * a.rows, a.cols, NB200_F32, va.device);
+    launch({&va}, where, [&](void *stream) { return nb200_int8_unpack(&a, floats(z), stream); });
+    return wrap(z);
+}
+
+// int8_product(a, w, order or None, type)
+PyObject *int8_product(PyObject *const *args) {
+    const char *where = "gpu_int8_product";
+    for (int k = 0; k < 2; ++k) need_kind(args[k], INT8, where, "INT8_gpu");
+    View va, vw, vo;
+    const nb200_int8 a = view_int8(args[0], va), w = view_int8(args[1], vw);
+    same_device(va, vw);
+    extent(a.groups, 1, where, "the left operand", "groups");
+    extent(a.cols, w.cols, where, "the left operand", "columns");
+    vo.device = va.device;
+    const int32_t *offsets = ranges_of(args[2], vo, a.rows, w.groups, where);
+    same_device(va, vo);
+    const int type = (int)PyLong_AsLong(args[3]);
+    at::Tensor y = matrix(a.rows, w.rows, type, va.device);
+    nb200_dense out = dense(y, type);
+    launch({&va, &vw, &vo}, where, [&](void *stream) { return nb200_int8_product(&a, &w, offsets, &out, stream); });
+    return wrap(y);
+}
+
+// Tensors in a row, as a list or a tuple.
+std::vector<at::Tensor> tensors_of(PyObject *o, const char *where, const char *name) {
+    if (!PyList_Check(o) && !PyTuple_Check(o)) refuse(PyExc_TypeError, "%s: %s must be a list or a tuple of CUDA tensors", where, name);
+    std::vector<at::Tensor> all;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+    all.reserve((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject *t = PySequence_Fast_GET_ITEM(o, i);
+        if (!THPVariable_Check(t)) refuse(PyExc_TypeError, "%s: %s must be a list or a tuple of CUDA tensors", where, name);
+        all.push_back(THPVariable_Unpack(t));
+        const at::Tensor &x = all.back();
+        if (!x.is_cuda() || x.layout() != at::kStrided || type_of(x) < 0) refuse(PyExc_TypeError, "%s: %s must hold CUDA tensors of float32, float16 or bfloat16", where, name);
+        if (!x.is_non_overlapping_and_dense()) refuse(PyExc_ValueError, "%s: the elements of each of %s must lie one after another", where, name);
+        if (x.device() != all.front().device()) refuse(PyExc_ValueError, "%s: %s live on different devices", where, name);
+    }
+    return all;
+}
+
+// clip(tensors, results or None, max_norm): the norm
+PyObject *clip(PyObject *const *args) {
+    const char *where = "gpu_clip_gradients";
+    const std::vector<at::Tensor> from = tensors_of(args[0], where, "gradients");
+    const bool in_place = args[1] == Py_None;
+    const std::vector<at::Tensor> to = in_place ? from : tensors_of(args[1], where, "out");
+    if (from.empty()) refuse(PyExc_ValueError, "%s: %s are none", where, "gradients");
+    if (from.size() != to.size()) refuse(PyExc_ValueError, "%s: %s must hold as many tensors as there are gradients", where, "out");
+    const double max_norm = PyFloat_AsDouble(args[2]);
+    const c10::Device device = from[0].device();
+    if (to[0].device() != device) refuse(PyExc_ValueError, "%s: gradients and %s live on different devices", where, "out");
+    std::vector<nb200_span> spans;
+    struct Range {
+        uintptr_t begin, end;
+        bool written;
+    };
+    std::vector<Range> ranges;
+    spans.reserve(from.size()), ranges.reserve(from.size() * (in_place ? 1 : 2));
+    for (size_t i = 0; i < from.size(); ++i) {
+        const at::Tensor &x = from[i], &z = to[i];
+        if (!in_place && (x.sizes() != z.sizes() || !(x.strides() == z.strides() || (x.is_contiguous() && z.is_contiguous()))))
+            refuse(PyExc_ValueError, "%s: a tensor of %s differs from its gradient in shape or layout", where, "out");
+        const int64_t n = x.numel();
+        if (n == 0) continue;
+        const nb200_span s{x.data_ptr(), z.data_ptr(), n, type_of(x), type_of(z)};
+        spans.push_back(s);
+        const uintptr_t a = reinterpret_cast<uintptr_t>(s.from), b = reinterpret_cast<uintptr_t>(s.to);
+        const bool same = a == b && s.type == s.to_type;
+        if (!same) ranges.push_back({a, a + (size_t)n * x.element_size(), false});
+        ranges.push_back({b, b + (size_t)n * z.element_size(), true});
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
+    uintptr_t read = 0, written = 0;
+    for (const Range &r : ranges) {
+        if (r.begin < written || (r.written && r.begin < read)) refuse(PyExc_ValueError, "%s: %s overlap one another in memory", where, in_place ? "gradients" : "gradients and out");
+        (r.written ? written : read) = std::max(r.written ? written : read, r.end);
+    }
+    at::Tensor norm = at::Tensor(at::detail::empty_cuda(c10::IntArrayRef(), at::kFloat, device, std::nullopt));
+    const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);
+    at::Tensor scratch = array(bytes, at::kByte, device);
+    View v;
+    v.device = device;
+    launch({&v}, where, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });
+    const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(device.index());
+    for (const at::Tensor &x : from) c10::cuda::CUDACachingAllocator::recordStream(x.storage().data_ptr(), current);
+    for (const at::Tensor &z : to) {
+        if (!in_place) c10::cuda::CUDACachingAllocator::recordStream(z.storage().data_ptr(), current);
+        z.unsafeGetTensorImpl()->bump_version();
+    }
+    return wrap(norm);
+}
+
 // ---- module --------------------------------------------------------------------------------
 
 template <PyObject *(*OP)(PyObject *const *), int ARGS>
@@ -783,6 +1012,15 @@ PyObject *bind_experts(PyObject *, PyObject *args) {
     Py_RETURN_NONE;
 }
 
+// bind_layers(INT8_gpu)
+PyObject *bind_layers(PyObject *, PyObject *args) {
+    PyObject *c;
+    if (!PyArg_ParseTuple(args, "O!", &PyType_Type, &c)) return nullptr;
+    Py_INCREF(c);
+    g_class[INT8] = reinterpret_cast<PyTypeObject *>(c);
+    Py_RETURN_NONE;
+}
+
 // turn_of(device, stream handle): identity of the lock by which calls there take turns (for tests)
 PyObject *turn_of(PyObject *, PyObject *args) {
     int device;
@@ -807,6 +1045,9 @@ PyMethodDef g_methods[] = {
     op<expert_sort_grad, 2>("expert_sort_grad"), op<expert_unsort, 3>("expert_unsort"), op<expert_unsort_grad, 4>("expert_unsort_grad"),
     op<fp8_rows, 1>("fp8_rows"), op<fp8_tiles, 1>("fp8_tiles"), op<fp8_pack, 3>("fp8_pack"), op<fp8_unpack, 1>("fp8_unpack"),
     op<fp8_transpose, 1>("fp8_transpose"), op<fp8_product, 4>("fp8_product"), op<fp8_grad_w, 4>("fp8_grad_w"),
+    {"bind_layers", bind_layers, METH_VARARGS, nullptr},
+    op<gated_product, 5>("gated_product"), op<gated_product_grad, 6>("gated_product_grad"), op<int8_rows, 1>("int8_rows"), op<int8_pack, 2>("int8_pack"),
+    op<int8_unpack, 1>("int8_unpack"), op<int8_product, 4>("int8_product"), op<clip, 3>("clip"),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -11,6 +11,7 @@
 
 #include "common.cuh"
 #include "dense_rows.cuh"
+#include "product_waits.cuh"
 
 namespace nb200 {
 
@@ -207,6 +208,36 @@ int resident_ctas(const void *kernel, int threads) {
     int &n = g_facts[{dev, kernel}].resident[threads];
     if (!n && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1)) n = 1;
     return n;
+}
+
+int report_of(cudaStream_t stream, Workspace **ws) {
+    int st;
+    if ((st = acquire_workspace(stream, 0, ws, REPORT_SLOT))) return st;
+    volatile unsigned long long *word = reinterpret_cast<volatile unsigned long long *>((*ws)->host) + 32;
+    const unsigned long long said = *word;
+    if (!(said & RW_VALID)) return NB200_OK;
+    *word = 0;
+    return note_timeout(3, (int)(said & INT32_MAX), said & REPORT_OTHER ? "an earlier gated or integer product" : "an earlier 8-bit product");
+}
+
+int encode_matrix(CUtensorMap *map, CUtensorMapDataType type, int rank, void *data, const cuuint64_t *extents, const cuuint64_t *pitches, const cuuint32_t *box) {
+    typedef CUresult (*encode_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::atomic<encode_fn> known{nullptr};
+    encode_fn encode = known.load(std::memory_order_acquire);
+    if (!encode) {
+        void *found = nullptr;
+        cudaDriverEntryPointQueryResult how = cudaDriverEntryPointSymbolNotFound;
+        NB200_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault, &how));
+        if (how != cudaDriverEntryPointSuccess || !found) return note_cuda_error(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
+        encode = reinterpret_cast<encode_fn>(found);
+        known.store(encode, std::memory_order_release);
+    }
+    const cuuint32_t steps[3] = {1, 1, 1};
+    if (encode(map, type, (cuuint32_t)rank, data, extents, pitches, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return note_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+    return NB200_OK;
 }
 
 uint64_t workspace_epoch() { return g_ws_epoch.load(std::memory_order_acquire); }

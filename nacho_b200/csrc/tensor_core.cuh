@@ -1,5 +1,5 @@
-// Thin wrappers over the sm_100a tensor-core PTX that the 8-bit products use: tensor memory, descriptors of shared-memory tiles,
-// matrix instructions on e4m3 operands with 32-bit sums, and the barriers they complete on.
+// Thin wrappers over the sm_100a tensor-core PTX that the products use: tensor memory, descriptors of shared-memory tiles,
+// matrix instructions with 32-bit sums (on e4m3, 16-bit and 8-bit integer operands), and the barriers they complete on.
 #pragma once
 
 #include <cuda.h>
@@ -64,6 +64,16 @@ __device__ __forceinline__ void tmem_wait_loads(uint32_t (&v)[32]) {
                  : "memory");
 }
 
+// 32 columns of 16 of this warp's lanes (the address is that of the first, the warp's own or 16 further) as matrix fragments of 8 x 8: thread i gets
+// of lanes i / 4 and i / 4 + 8 the columns 8 j + 2 (i % 4) and the next one as v[4 j] .. v[4 j + 1] and v[4 j + 2] .. v[4 j + 3].
+__device__ __forceinline__ void tmem_load_fragments(uint32_t address, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                   "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(address)
+                 : "memory");
+}
+
 // Orders tensor-memory accesses with the barrier operations of other threads.
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -108,6 +118,40 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uin
             : "memory");
 }
 
+// What 16-bit and integer products multiply.
+enum class Sum { F16, BF16, S8 };
+
+// The same where the tile's rows run across the summed axis: blocks of 64 elements of 16 bits, each 64 rows of 128 bytes, 8192 bytes apart. A step of
+// 16 along the summed axis is 16 rows and adds 128.
+__device__ __forceinline__ uint64_t turned_descriptor(uint32_t smem_address) {
+    return (uint64_t)((smem_address >> 4) & 0x3fff) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+template <Sum SUM>
+__host__ __device__ constexpr uint32_t sum_descriptor(bool a_turned, bool b_turned, int m) {
+    return (SUM == Sum::S8 ? 2u << 4 | 1u << 7 | 1u << 10 : SUM == Sum::BF16 ? 1u << 4 | 1u << 7 | 1u << 10 : 1u << 4) | (a_turned ? 1u << 15 : 0u) | (b_turned ? 1u << 16 : 0u) |
+           (uint32_t)(m >> 4) << 24;
+}
+
+// d (+)= a b^T over 32 bytes of the operands' rows (16 rows of turned ones), by a pair of CTAs; its leader's thread issues it. `shape`: the
+// descriptor above with n >> 3 at bit 17.
+template <Sum SUM>
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    if constexpr (SUM == Sum::S8)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+            : "memory");
+}
+
 // The barrier (at this place in both CTAs of a pair) gets an arrival when all matrix instructions that this thread has issued so far are done.
 template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
@@ -116,7 +160,22 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// ---- stores of tiles -------------------------------------------------------------------
+// ---- loads and stores of tiles -------------------------------------------------------------------
+
+// A tile of rows of 128 bytes from the place (x, y) of matrix z, where nothing is below zero; what lies beyond the matrix comes as zeros.
+__device__ __forceinline__ void load_tile(void *smem, const CUtensorMap *matrix, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem)), "l"(matrix), "r"(x), "r"(y),
+                 "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// Four matrices of 8 x 8 words of 16 bits from the warp's registers (thread i has two neighbours of row i / 4) to shared memory, row r of matrix m to
+// the 16 bytes at the address that thread 8 m + r gives; TURNED: their columns.
+template <bool TURNED>
+__device__ __forceinline__ void store_matrices(void *row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    if constexpr (TURNED) asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    else asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 
 // A tile of rows of 128 bytes from shared memory, laid out as above, to the place (x, y) of a matrix; what lies beyond the matrix is left out. The
 // thread that starts such stores also closes them into groups and waits until all but its last N groups have been read (or written).
@@ -165,6 +224,15 @@ __device__ __forceinline__ void mbar_arrive_leader(uint64_t *bar) {
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// The same for ordinary stores to shared memory that matrix instructions of the leader read (behind fence_async_shared), and its other side.
+__device__ __forceinline__ void mbar_arrive_leader_release(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .b32 remote;\n\t"
+        "mapa.shared::cluster.u32 remote, %0, 0;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 // All threads of all CTAs of the cluster meet.
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");

@@ -1,0 +1,460 @@
+// Products on the tensor cores whose sums stay in tensor memory until a tile is done: 16-bit floats and 8-bit integers. Tokens, which groups share
+// unevenly, lie on the narrow side of the matrix instructions (N, any multiple of 64), weights on the wide one (M = 256), so that a group's
+// last tile does hardly more work than its rows need.
+//   GATED:   h[t, j] = act(sum_k x[t, k] w[g][j, k]) * sum_k x[t, k] w[g][hidden + j, k], and both sums where they are kept
+//   ROWS:    y[t, j] = sum_k x[t, k] w[g][j, k], the second operand by rows or turned
+//   WEIGHTS: z[g][m, n] = sum over the tokens t of group g of d[t, m] x[t, n]
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "activation.cuh"
+#include "dense_rows.cuh"
+#include "product_waits.cuh"
+
+namespace nb200 {
+
+enum class Form { GATED, ROWS, WEIGHTS };
+
+constexpr int TILE_STORE_WARPS = 8, TILE_THREADS = (TILE_STORE_WARPS + 2) * 32;
+constexpr int TILE_M = 256, TILE_N = 256, TILE_STEP = 64, TILE_PANEL = 8;  // of a pair of CTAs; tokens come in steps of 64; row tiles that follow one another
+
+struct TileArgs {
+    const int32_t *offsets;  // groups + 1, or none: one group of all rows
+    int groups, rows;
+    int wide;    // the result's extent on the side of M: hidden, columns of y, rows of z
+    int across;  // WEIGHTS: columns of z
+    int blocks;  // of 128 bytes along the summed axis (not WEIGHTS)
+    int tile_n;  // TILE_N at most
+    int most;    // tiles, at most
+    void *y;
+    int64_t stride;
+    void *both;  // GATED: [rows][2 hidden] or none
+    const float *row_scale, *col_scale;  // S8: of the rows, of every group's columns
+    bool gelu;
+    bool words;  // results in words of 16 bytes
+    unsigned long long *report;
+};
+
+// What a CTA of a pair has in shared memory; tiles begin at 1024-byte boundaries.
+struct TileShared {
+    static constexpr int STAGES = 6, SUMS = 2;  // blocks under way; places for a tile's sums in tensor memory
+    uint8_t a[STAGES][128 * 128];               // 128 rows of the wide side (turned: two blocks of 64 by 64 of the summed axis)
+    uint8_t b[STAGES][128 * 128];               // half of the tile's narrow side
+    uint8_t out[TILE_STORE_WARPS][32 * 96];     // GATED: 32 x 32 bytes of h, 32 x 64 of both sums; else 32 x 64
+    uint64_t full[STAGES], empty[STAGES];       // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
+    uint64_t sum_full[SUMS], sum_empty[SUMS];   // a tile's sums lie in tensor memory; they have been read
+    uint64_t drained;
+    uint32_t tmem;
+    int failed;
+};
+constexpr size_t TILE_SHARED_BYTES = sizeof(TileShared) + 1024;
+static_assert(TILE_SHARED_BYTES <= 227 * 1024, "");
+
+// A tile of the result: its group, where its rows begin and how many there are (for WEIGHTS: its columns), its first column (row), and the blocks that are summed.
+struct Place {
+    int g, from, count, col, blocks;
+    int first, last;  // WEIGHTS: the group's tokens
+};
+
+// Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order. `most`: as many as there
+// are with offsets that rise; others end there.
+template <Form FORM>
+struct TileWalk {
+    const TileArgs &p;
+    int per_tile;  // columns of the result in a tile
+    int chunk = -32, base = 0, incl = 0, from = 0, to = 0;
+
+    __device__ explicit TileWalk(const TileArgs &args) : p(args), per_tile(FORM == Form::GATED ? TILE_M / 2 : TILE_M) {}
+
+    __device__ void range(int g, int &lo, int &hi) const {
+        lo = p.offsets ? min(max(ld_late(p.offsets + g), 0), p.rows) : 0;
+        hi = p.offsets ? min(max(ld_late(p.offsets + g + 1), lo), p.rows) : p.rows;
+    }
+    __device__ bool find(int tile, Place &t) {
+        if (tile >= p.most) return false;
+        const int wide = (p.wide + per_tile - 1) / per_tile;
+        int row, col;
+        if constexpr (FORM == Form::WEIGHTS) {
+            const int narrow = (p.across + p.tile_n - 1) / p.tile_n;
+            t.g = (int)((unsigned)tile / (unsigned)(narrow * wide));
+            if (t.g >= p.groups) return false;
+            range(t.g, t.first, t.last);
+            place_tile<TILE_PANEL>(tile - t.g * narrow * wide, narrow, wide, &row, &col);
+            t.from = row * p.tile_n;
+            t.count = min(p.tile_n, p.across - t.from);
+            t.blocks = (t.last - t.first + 63) / 64;
+        } else {
+            int total;
+            while (total = __shfl_sync(FULL_MASK, incl, 31), tile >= base + total) {
+                base += total;
+                chunk += 32;
+                if (chunk >= p.groups) return false;
+                const int g = chunk + lane_id();
+                from = to = 0;
+                if (g < p.groups) range(g, from, to);
+                incl = warp_incl_sum((int)min((int64_t)((to - from + p.tile_n - 1) / p.tile_n) * wide, (int64_t)p.most));
+            }
+            const int src = __ffs(__ballot_sync(FULL_MASK, base + incl > tile)) - 1;
+            const int begin = __shfl_sync(FULL_MASK, from, src), end = __shfl_sync(FULL_MASK, to, src), high = (end - begin + p.tile_n - 1) / p.tile_n;
+            t.g = chunk + src;
+            place_tile<TILE_PANEL>(tile - base - (__shfl_sync(FULL_MASK, incl, src) - high * wide), high, wide, &row, &col);
+            t.from = begin + row * p.tile_n;
+            t.count = min(p.tile_n, end - t.from);
+            t.blocks = p.blocks;
+        }
+        t.col = col * per_tile;
+        return true;
+    }
+};
+
+// ---- the kernel ------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+
+// Rows from the warp's place in shared memory to memory: `to(r, p)` is where the 16-byte piece p of row r goes, `count(r, p)` how many of its eight elements.
+template <int PIECES, typename T, typename To, typename Count>
+__device__ __forceinline__ void flush(const uint8_t *place, bool words, To to, Count count) {
+    const int lane = lane_id();
+    constexpr int ROW = PIECES * 16, TURN = 128 / ROW, EACH = 32 / PIECES;
+    auto at = [&](int r, int p) { return place + r * ROW + ((p ^ (r / TURN & (PIECES - 1))) << 4); };
+    if (words) {
+#pragma unroll
+        for (int i = 0; i < 32; i += EACH) {
+            const int r = i + lane / PIECES, p = lane & (PIECES - 1);
+            if (count(r, p) >= 8) *reinterpret_cast<uint4 *>(to(r, p)) = *reinterpret_cast<const uint4 *>(at(r, p));
+        }
+    } else {
+        constexpr int AT_ONCE = 32 / (PIECES * 8);  // rows
+#pragma unroll 4
+        for (int i = 0; i < 32; i += AT_ONCE) {
+            const int r = i + lane / (PIECES * 8), e = lane & (PIECES * 8 - 1), p = e / 8;
+            if (e % 8 < count(r, p)) to(r, p)[e % 8] = reinterpret_cast<const T *>(at(r, p))[e % 8];
+        }
+    }
+}
+
+// The warp's 32 lanes of M by 32 columns of N, from fragments lo (lanes 0 .. 15) and hi to its place, by columns (rows of 32 elements of M) or by lanes.
+template <bool BY_COLUMNS, typename T>
+__device__ __forceinline__ void put_square(uint8_t *place, const float (&lo)[16], const float (&hi)[16]) {
+    const int q = lane_id() >> 3, r = lane_id() & 7;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = BY_COLUMNS ? 8 * j + r : 8 * q + r, piece = BY_COLUMNS ? q : j;
+        store_matrices<BY_COLUMNS>(place + row * 64 + ((piece ^ (row / 2 & 3)) << 4), pack2<T>(lo[4 * j], lo[4 * j + 1]), pack2<T>(lo[4 * j + 2], lo[4 * j + 3]),
+                                   pack2<T>(hi[4 * j], hi[4 * j + 1]), pack2<T>(hi[4 * j + 2], hi[4 * j + 3]));
+    }
+}
+
+// Pairs of CTAs, one per SM, take tiles of 256 x 256 at most in turn. One warp brings blocks of 128 bytes of both operands into shared memory (the copy
+// engine's tiled form, which turns them as the tensor cores take them and fills up with zeros what lies beyond a matrix), one issues the matrix instructions, and
+// eight read the sums of a whole tile while those of the next one are made: tensor memory holds two.
+//
+// GATED: 16 rows of gates and 16 of values alternate in the wide operand's tile, so that a gate and its value lie 16 lanes apart in tensor memory and fragments
+// of both land in the same thread.
+// WEIGHTS: the last block of a group's tokens runs into the next group's, whose rows are cleared in shared memory before they are multiplied.
+template <Sum SUM, Form FORM, bool A_TURNED, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, const __grid_constant__ CUtensorMap wide_map, const __grid_constant__ CUtensorMap narrow_map) {
+    constexpr int STAGES = TileShared::STAGES, SUMS = TileShared::SUMS;
+    constexpr bool B_TURNED = FORM == Form::WEIGHTS, GATED = FORM == Form::GATED;
+    constexpr int PER_BLOCK = SUM == Sum::S8 ? 128 : 64;
+    extern __shared__ uint8_t raw[];
+    TileShared &sh = *reinterpret_cast<TileShared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int warp = warp_id(), lane = lane_id(), rank = (int)cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[s], rank == 0 ? 2 : 1), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < SUMS; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], TILE_STORE_WARPS * 2);
+        mbar_init(&sh.drained, 1);
+        mbar_fence_init();
+        sh.failed = 0;
+    }
+    if (warp == TILE_STORE_WARPS) tmem_alloc<true>(&sh.tmem, 512);
+    tmem_fence_before();
+    __syncthreads();
+    cluster_sync();  // nobody arrives at a barrier that is not there yet
+    tmem_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    volatile int *failed = &sh.failed;
+    trigger_dependents();
+    wait_for_previous();
+
+    const int first = blockIdx.x / 2, step = gridDim.x / 2;
+    TileWalk<FORM> walk(args);
+    Place t{};
+    // Columns of N that the tile's matrix instructions have, and those that this CTA brings.
+    auto narrow = [&] { return (t.count + TILE_STEP - 1) / TILE_STEP * TILE_STEP; };
+    // The tail of a group's last block: rows of the summed axis, in this CTA's halves of both operands.
+    auto clear_tail = [&](int stage, int n, int rows) {
+        uint8_t *const a = sh.a[stage], *const b = sh.b[stage];
+        const int chunks = 2 + (n / 2 + 63) / 64;
+        for (int i = lane; i < chunks * (64 - rows) * 8; i += 32) {
+            const int chunk = i / ((64 - rows) * 8), at = i - chunk * (64 - rows) * 8;
+            uint8_t *const tile = chunk < 2 ? a + chunk * 8192 : b + (chunk - 2) * 8192;
+            *reinterpret_cast<uint4 *>(tile + rows * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_shared();
+        __syncwarp();
+    };
+    if (warp < TILE_STORE_WARPS) {
+        const int lanes = warp & 3, half = warp >> 2;
+        Ring<SUMS> sums;
+        uint8_t *const place = sh.out[warp], *const place_both = sh.out[warp] + 32 * 32;
+        T *const y = static_cast<T *>(args.y);
+        bool fine = true;
+        for (int tile = first; fine && walk.find(tile, t); tile += step) {
+            const int n = narrow();
+            // the first column (row of z) of this warp's lanes
+            const int col = t.col + (GATED ? rank * 64 + lanes * 16 : rank * 128 + lanes * 32);
+            if (t.blocks) {
+                if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
+                tmem_fence_after();
+            }
+            float col_scale[4];
+            if constexpr (SUM == Sum::S8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = std::is_same<T, float>::value ? col + lane : col + lane / 4 + 8 * i;
+                    col_scale[i] = c < args.wide ? ld_late(args.col_scale + (int64_t)t.g * args.wide + c) : 0.f;
+                }
+            }
+            for (int c = half * (n / 2); c < (half + 1) * (n / 2); c += 32) {
+                const uint32_t at = tmem + ((uint32_t)(lanes * 32) << 16) + sums.at * TILE_N + c;
+                const bool last = c + 32 >= (half + 1) * (n / 2);
+                auto read_all = [&] {  // this warp has read the tile's sums
+                    if (!last || !t.blocks) return;
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
+                };
+                const int left = t.count - c;  // rows of the result from here on (columns of z)
+                float row_scale = 0.f;
+                if constexpr (SUM == Sum::S8) row_scale = lane < left ? ld_late(args.row_scale + t.from + c + lane) : 0.f;
+                if constexpr (std::is_same<T, float>::value) {
+                    uint32_t v[32] = {};
+                    if (t.blocks) tmem_load(at, v), tmem_wait_loads(v);
+                    read_all();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float f = SUM == Sum::S8 ? scaled((int)v[j], __shfl_sync(FULL_MASK, row_scale, j), col_scale[0]) : __uint_as_float(v[j]);
+                        if (j < left && col + lane < args.wide) y[(int64_t)(t.from + c + j) * args.stride + col + lane] = f;
+                    }
+                } else {
+                    uint32_t v[2][16] = {};
+                    if (t.blocks) {
+                        tmem_load_fragments(at, v[0]);
+                        tmem_load_fragments(at + (16u << 16), v[1]);
+                        tmem_wait_loads(v[0]);
+                        tmem_wait_loads(v[1]);
+                    }
+                    read_all();
+                    float lo[16], hi[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if constexpr (SUM == Sum::S8) {
+                            const float s = __shfl_sync(FULL_MASK, row_scale, i / 4 * 8 + (lane & 3) * 2 + (i & 1));
+                            lo[i] = scaled((int)v[0][i], s, col_scale[(i & 2) / 2]);
+                            hi[i] = scaled((int)v[1][i], s, col_scale[2 + (i & 2) / 2]);
+                        } else {
+                            lo[i] = __uint_as_float(v[0][i]), hi[i] = __uint_as_float(v[1][i]);
+                        }
+                    }
+                    if (left <= 0) continue;
+                    __syncwarp();  // the place has been read
+                    if constexpr (GATED) {
+                        const int wide = args.wide, stride = 2 * wide;
+                        if (args.both) put_square<true, T>(place_both, lo, hi);
+                        float h[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) h[i] = lo[i] * logistic(act_inner(lo[i], args.gelu)) * hi[i];
+                        const int q = lane >> 3, r = lane & 7;
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2) {  // rows of 16 elements: two pieces
+                            const int row = 8 * (j + q / 2) + r;
+                            store_matrices<true>(place + row * 32 + (((q & 1) ^ (row / 4 & 1)) << 4), pack2<T>(h[4 * j], h[4 * j + 1]), pack2<T>(h[4 * j + 2], h[4 * j + 3]),
+                                                 pack2<T>(h[4 * j + 4], h[4 * j + 5]), pack2<T>(h[4 * j + 6], h[4 * j + 7]));
+                        }
+                        __syncwarp();
+                        flush<2, T>(place, args.words, [&](int row, int p) { return y + (int64_t)(t.from + c + row) * args.stride + col + p * 8; },
+                                    [&](int row, int p) { return row < left ? wide - col - p * 8 : 0; });
+                        if (args.both)
+                            flush<4, T>(place_both, args.words, [&](int row, int p) { return static_cast<T *>(args.both) + (int64_t)(t.from + c + row) * stride + (p >= 2 ? wide : 0) + col + (p & 1) * 8; },
+                                        [&](int row, int p) { return row < left ? wide - col - (p & 1) * 8 : 0; });
+                    } else if constexpr (FORM == Form::ROWS) {
+                        put_square<true, T>(place, lo, hi);
+                        __syncwarp();
+                        flush<4, T>(place, args.words, [&](int row, int p) { return y + (int64_t)(t.from + c + row) * args.stride + col + p * 8; },
+                                    [&](int row, int p) { return row < left ? args.wide - col - p * 8 : 0; });
+                    } else {
+                        put_square<false, T>(place, lo, hi);
+                        __syncwarp();
+                        flush<4, T>(place, args.words, [&](int row, int p) { return y + ((int64_t)t.g * args.wide + col + row) * args.stride + t.from + c + p * 8; },
+                                    [&](int row, int p) { return col + row < args.wide ? left - p * 8 : 0; });
+                    }
+                }
+            }
+            if (t.blocks) sums.next();
+        }
+        // rows of no group
+        if (FORM != Form::WEIGHTS && args.offsets) {
+            const int64_t rows = args.rows, lo = min(max((int64_t)ld_late(args.offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(args.offsets + args.groups), lo), rows);
+            for (int64_t r = blockIdx.x * TILE_STORE_WARPS + warp; r < rows; r += (int64_t)gridDim.x * TILE_STORE_WARPS) {
+                if (r >= lo && r < hi) continue;
+                for (int64_t c = lane; c < args.wide; c += 32) y[r * args.stride + c] = from_float<T>(0.f);
+                if (GATED && args.both)
+                    for (int64_t c = lane; c < 2 * (int64_t)args.wide; c += 32) static_cast<T *>(args.both)[r * 2 * args.wide + c] = from_float<T>(0.f);
+            }
+        }
+    } else {
+        Ring<STAGES> stage;
+        bool fine = true;
+        if (warp == TILE_STORE_WARPS + 1) {  // copies
+            for (int tile = first; fine && walk.find(tile, t); tile += step) {
+                const int n = narrow(), mine = n / 2;
+                const uint32_t bytes = 128 * 128 + (B_TURNED ? (mine + 63) / 64 * 8192 : mine * 128);
+                const int at = t.from + rank * mine;
+                for (int b = 0; b < t.blocks; ++b, stage.next()) {
+                    if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
+                    if (elected()) {
+                        uint64_t *const bar = &sh.full[stage.at];
+                        mbar_arrive_expect_tx(bar, bytes);
+                        const int k = FORM == Form::WEIGHTS ? t.first + b * 64 : b * PER_BLOCK;
+                        uint8_t *const to_a = sh.a[stage.at], *const to_b = sh.b[stage.at];
+                        if constexpr (GATED) {
+                            const int col = t.col + rank * 64;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                load_tile(to_a + i * 4096, &wide_map, k, col + 16 * i, t.g, bar);
+                                load_tile(to_a + i * 4096 + 2048, &wide_map, k, args.wide + col + 16 * i, t.g, bar);
+                            }
+                        } else if constexpr (A_TURNED) {
+                            const int col = t.col + rank * 128, g = FORM == Form::WEIGHTS ? 0 : t.g;
+                            load_tile(to_a, &wide_map, col, k, g, bar);
+                            load_tile(to_a + 8192, &wide_map, col + 64, k, g, bar);
+                        } else {
+                            load_tile(to_a, &wide_map, k, t.col + rank * 128, t.g, bar);
+                        }
+                        if constexpr (B_TURNED) {
+                            for (int i = 0; i < mine; i += 64) load_tile(to_b + i * 128, &narrow_map, at + i, k, 0, bar);
+                        } else {
+                            for (int i = 0; i < mine; i += 32) load_tile(to_b + i * 128, &narrow_map, k, at + i, 0, bar);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!fine)  // nothing may land in shared memory that is no longer this CTA's
+                for (int s = 0; s < STAGES; ++s) drain(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1);
+        } else if (rank == 0) {  // matrix instructions
+            const uint64_t tile_a = A_TURNED ? turned_descriptor(smem_u32(sh.a[0])) : tile_descriptor(smem_u32(sh.a[0]));
+            const uint64_t tile_b = B_TURNED ? turned_descriptor(smem_u32(sh.b[0])) : tile_descriptor(smem_u32(sh.b[0]));
+            Ring<SUMS> sums;
+            for (int tile = first; fine && walk.find(tile, t); tile += step) {
+                const int n = narrow();
+                const uint32_t shape = sum_descriptor<SUM>(A_TURNED, B_TURNED, TILE_M) | (uint32_t)(n >> 3) << 17;
+                if (t.blocks && !(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                for (int b = 0; b < t.blocks; ++b, stage.next()) {
+                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (FORM == Form::WEIGHTS && t.last - t.first - b * 64 < 64) {
+                        clear_tail(stage.at, n, t.last - t.first - b * 64);
+                        fence_cluster();
+                    }
+                    tmem_fence_after();
+                    if (elected()) {
+                        const uint64_t da = tile_a + (uint64_t)(stage.at * (128 * 128 >> 4)), db = tile_b + (uint64_t)(stage.at * (128 * 128 >> 4));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma_pair<SUM>(tmem + sums.at * TILE_N, da + (A_TURNED ? 128 : 2) * k, db + (B_TURNED ? 128 : 2) * k, shape, b > 0 || k > 0);
+                        mma_commit<true>(&sh.empty[stage.at]);
+                        if (b + 1 == t.blocks) mma_commit<true>(&sh.sum_full[sums.at]);
+                    }
+                    __syncwarp();
+                }
+                if (t.blocks) sums.next();
+            }
+            if (!fine) {
+                if (elected()) mma_commit<true>(&sh.drained);
+                __syncwarp();
+                drain(&sh.drained, 0);
+            }
+        } else {  // tells the leader of the copies that have landed here
+            for (int tile = first; fine && walk.find(tile, t); tile += step) {
+                const int n = narrow();
+                for (int b = 0; b < t.blocks; ++b, stage.next()) {
+                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    const bool tail = FORM == Form::WEIGHTS && t.last - t.first - b * 64 < 64;
+                    if (tail) clear_tail(stage.at, n, t.last - t.first - b * 64);
+                    if (elected()) {
+                        if (tail) mbar_arrive_leader_release(&sh.full[stage.at]);
+                        else mbar_arrive_leader(&sh.full[stage.at]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    cluster_sync();  // no arrival is on its way to a CTA that is gone
+    if (warp == TILE_STORE_WARPS) {
+        tmem_fence_after();
+        tmem_free<true>(tmem, 512);
+        if (lane == 0 && *failed) publish_result_word(args.report, 1, REPORT_OTHER | blockIdx.x);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+// Whether the copy engine can read the rows: 16-byte boundaries, rows that do not overlap, less than 2^40 bytes from row to row and group to group.
+inline bool tiles_readable(const nb200_dense &x, int64_t groups) {
+    const int64_t size = (int64_t)type_size(x.type), per_group = groups ? x.rows / groups : 0;
+    return reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && (x.rows <= 1 || (x.stride * size % 16 == 0 && x.stride >= x.cols && x.stride < (int64_t(1) << 40) / size)) &&
+           (groups <= 1 || per_group * x.stride < (int64_t(1) << 40) / size);
+}
+
+// `groups` matrices of rows, one after another, in boxes of `box_rows` rows of 128 bytes.
+inline int describe_rows(CUtensorMap *map, CUtensorMapDataType type, void *data, int64_t size, int64_t cols, int64_t rows, int64_t groups, int64_t stride, int box_rows) {
+    const cuuint64_t extents[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t pitch = (cuuint64_t)(rows * groups > 1 ? stride : (cols * size + 15) / 16 * 16 / size) * size;
+    const cuuint64_t pitches[2] = {pitch, groups > 1 ? pitch * (cuuint64_t)rows : pitch};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
+    return encode_matrix(map, type, 3, data, extents, pitches, box);
+}
+inline CUtensorMapDataType map_type(int type) { return type == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+
+// The narrow side of the tiles: 256 while that leaves work for most SMs, else less, for which a tile costs more to bring than to multiply.
+inline int tile_n_of(int64_t rows, int64_t groups, int64_t wide_tiles) {
+    int n = TILE_N;
+    while (n > TILE_STEP && ((rows + n - 1) / n + (groups > 1 ? groups / 2 : 0)) * wide_tiles * 4 < sm_count()) n /= 2;
+    return n;
+}
+
+template <Sum SUM, Form FORM, bool A_TURNED, typename T>
+int launch_tiles(const char *name, TileArgs args, const CUtensorMap &wide_map, const CUtensorMap &narrow_map, cudaStream_t stream) {
+    Workspace *ws = nullptr;
+    int st;
+    if ((st = report_of(stream, &ws))) return st;
+    args.report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
+    const int64_t per_tile = FORM == Form::GATED ? TILE_M / 2 : TILE_M, wide = (args.wide + per_tile - 1) / per_tile;
+    const int64_t tiles = FORM == Form::WEIGHTS ? (int64_t)args.groups * ((args.across + args.tile_n - 1) / args.tile_n) * wide
+                                                : (args.rows / args.tile_n + (int64_t)args.groups) * wide;
+    if (tiles > INT32_MAX / 64 || args.rows > INT32_MAX - 1024 || args.wide > INT32_MAX / 2 - 1024 || args.across > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
+    args.most = (int)tiles;
+    auto kernel = k_tiles<SUM, FORM, A_TURNED, T>;
+    if ((st = allow_shared(kernel, TILE_SHARED_BYTES))) return st;
+    const int64_t ctas = std::max<int64_t>(2, std::min<int64_t>(tiles * 2, sm_count() / 2 * 2));
+    LaunchScope scope(name, stream);
+    NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(TILE_THREADS), TILE_SHARED_BYTES, stream, args, wide_map, narrow_map));
+    return NB200_OK;
+}
+
+}  // namespace nb200
