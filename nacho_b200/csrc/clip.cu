@@ -13,7 +13,7 @@ namespace {
 
 constexpr int NT = 256, TURNS = 4;              // threads; 16-byte chunks that a thread has on its way
 constexpr int CHUNK_BYTES = NT * TURNS * 16;    // what a CTA takes at a time, of the elements' own type
-constexpr int MAX_CTAS = 4 * 148 * 2;           // partial sums of a launch
+constexpr int MAX_CTAS = 4 * 148;               // that are at work at once, and partial sums of a launch
 
 // A launch's tensors lie in its parameters: a captured graph has them with it.
 template <int N>
@@ -28,7 +28,7 @@ struct Spans {
 
 __host__ __device__ constexpr int64_t chunk_elements(int type) { return CHUNK_BYTES / (type == NB200_F32 ? 4 : 2); }
 
-// The tensor that a chunk belongs to; `at`: one that lies in front of it or is it.
+// The tensor that a chunk belongs to.
 template <int N>
 __device__ __forceinline__ int span_of(const Spans<N> &s, int chunk) {
     int lo = 0, hi = s.n;
@@ -40,47 +40,106 @@ __device__ __forceinline__ int span_of(const Spans<N> &s, int chunk) {
     return lo;
 }
 
-// Squares of N elements: in 32 bits, unless those run over or lose what there is.
+// What a thread has of a CTA's chunk: TURNS pieces of V elements, a CTA's width apart, of the `count` elements from `from` on. The words are kept whole: as
+// elements of 16 bits they would take a register each, and spill.
 template <typename T, int V>
-__device__ __forceinline__ double squares(const Chunk<T, V> (&x)[TURNS], int64_t c, int64_t step, int64_t pitch, int64_t count) {
-    constexpr int N = Chunk<T, V>::N;
-    float sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < TURNS; ++u)
-        if (c + u * step < count) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (Chunk<T, V>::there(i, c + u * step, pitch, count)) sum = __fmaf_rn(x[u].get(i), x[u].get(i), sum);
-        }
-    if (sum > 0x1p-90f && sum < 0x1p126f) return sum;
-    double exact = 0.0;
-#pragma unroll
-    for (int u = 0; u < TURNS; ++u)
-        if (c + u * step < count) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (Chunk<T, V>::there(i, c + u * step, pitch, count)) exact += (double)x[u].get(i) * (double)x[u].get(i);
-        }
-    return exact;
-}
+struct Mine {
+    static constexpr int STEP = NT * V, WORDS = V * (int)sizeof(T) < 4 ? 1 : V * (int)sizeof(T) / 4;
+    uint32_t w[TURNS][WORDS];
 
-// A CTA's chunk as its threads have it: TURNS words (or several, of V elements, a CTA's width apart) each.
-template <typename T, int V, typename F>
-__device__ __forceinline__ void with_chunk(const T *from, int64_t begin, int64_t count, F f) {
-    constexpr int64_t pitch = (int64_t)NT * V, step = (int64_t)NT * Chunk<T, V>::N;
-    const int64_t c = begin + (int64_t)threadIdx.x * V;
-    Chunk<T, V> x[TURNS];
+    __device__ __forceinline__ void load(const T *from, int at, int count) {
 #pragma unroll
-    for (int u = 0; u < TURNS; ++u)
-        if (c + u * step < count) x[u].load(from, c + u * step, pitch, count);
-    f(x, c, step, pitch);
-}
+        for (int u = 0; u < TURNS; ++u) {
+            Vec<uint32_t, WORDS> in{};
+            if (at + u * STEP < count) {
+                if constexpr (V * sizeof(T) == 2) in.v[0] = *reinterpret_cast<const uint16_t *>(from + at + u * STEP);
+                else in = *reinterpret_cast<const Vec<uint32_t, WORDS> *>(from + at + u * STEP);
+            }
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[u][i] = in.v[i];
+        }
+    }
+    __device__ __forceinline__ float get(int u, int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[u][i]);
+        else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[u][i / 2] >> 16 : w[u][i / 2])));
+        else return __uint_as_float(i & 1 ? w[u][i / 2] & 0xffff0000u : w[u][i / 2] << 16);
+    }
+    // The sum of the squares: in 32 bits, unless those run over or lose what there is.
+    __device__ __forceinline__ double squares() const {
+        float part[TURNS] = {};
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) part[u] = __fmaf_rn(get(u, i), get(u, i), part[u]);
+        const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+        if (sum > 0x1p-90f && sum < 0x1p126f) return sum;
+        double exact = 0.0;
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) exact += (double)get(u, i) * (double)get(u, i);
+        return exact;
+    }
+    // Elements go over times the factor (1 changes none of them).
+    template <typename Z>
+    __device__ __forceinline__ void store(Z *to, int at, int count, float factor) const {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            if (at + u * STEP >= count) break;
+            Z *const z = to + at + u * STEP;
+            if constexpr (V == 1) {
+                z[0] = from_float<Z>(get(u, 0) * factor);
+            } else if constexpr (sizeof(Z) == 4) {
+#pragma unroll
+                for (int i = 0; i < V; i += 4)
+                    *reinterpret_cast<float4 *>(z + i) = make_float4(get(u, i) * factor, get(u, i + 1) * factor, get(u, i + 2) * factor, get(u, i + 3) * factor);
+            } else {
+                Vec<uint32_t, V / 2> out;
+#pragma unroll
+                for (int i = 0; i < V; i += 2) out.v[i / 2] = pack2<Z>(get(u, i) * factor, get(u, i + 1) * factor);
+                *reinterpret_cast<Vec<uint32_t, V / 2> *>(z) = out;
+            }
+        }
+    }
+};
+static_assert(TURNS == 4, "");
 
 template <typename F>
-__device__ __forceinline__ void with_span(int type, bool words, F f) {
-    if (type == NB200_F32) words ? f(float{}, std::integral_constant<int, 4>{}) : f(float{}, std::integral_constant<int, 1>{});
-    else if (type == NB200_F16) words ? f(__half{}, std::integral_constant<int, 8>{}) : f(__half{}, std::integral_constant<int, 1>{});
-    else words ? f(__nv_bfloat16{}, std::integral_constant<int, 8>{}) : f(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+__device__ __forceinline__ void with_type_of(int type, F f) {
+    if (type == NB200_F32) f(float{});
+    else if (type == NB200_F16) f(__half{});
+    else f(__nv_bfloat16{});
+}
+
+// A chunk of a tensor, by words of V elements and behind the last whole one of the tensor by single elements: f(Mine, where in the chunk, up to where).
+template <typename T, int V, typename F>
+__device__ __forceinline__ void with_chunk(const T *from, int count, F f) {
+    const int whole = count / V * V;
+#pragma unroll 1
+    for (int at = threadIdx.x * V; at < whole; at += TURNS * Mine<T, V>::STEP) {
+        Mine<T, V> mine;
+        mine.load(from, at, whole);
+        f(mine, at, whole);
+    }
+    if (V > 1 && (int)threadIdx.x < count - whole) {
+        Mine<T, 1> mine;
+        mine.load(from, whole + threadIdx.x, whole + threadIdx.x + 1);
+        f(mine, whole + (int)threadIdx.x, whole + (int)threadIdx.x + 1);
+    }
+}
+template <typename T>
+__device__ __forceinline__ double sum_chunk(const T *from, int count, bool words) {
+    double sum = 0.0;
+    auto add = [&](const auto &mine, int, int) { sum += mine.squares(); };
+    if (words) with_chunk<T, 16 / sizeof(T)>(from, count, add);
+    else with_chunk<T, 1>(from, count, add);
+    return sum;
+}
+template <typename T, typename Z>
+__device__ __forceinline__ void scale_chunk(const T *from, Z *to, int count, bool words, float factor) {
+    auto put = [&](const auto &mine, int at, int stop) { mine.store(to, at, stop, factor); };
+    if (words) with_chunk<T, 16 / sizeof(T)>(from, count, put);
+    else with_chunk<T, 1>(from, count, put);
 }
 
 __device__ __forceinline__ double cta_sum(double v, double *tmp) {
@@ -94,6 +153,8 @@ __device__ __forceinline__ double cta_sum(double v, double *tmp) {
     return v;
 }
 
+// Neighbouring CTAs have neighbouring chunks, and all of them move through the tensors together: with ranges of their own, reads and writes of 1184
+// places at once, scaling 500 M elements took 493 us.
 template <int N>
 __global__ void __launch_bounds__(NT, 4) k_squares(const __grid_constant__ Spans<N> s, double *partial) {
     __shared__ double tmp[NT / 32];
@@ -101,13 +162,14 @@ __global__ void __launch_bounds__(NT, 4) k_squares(const __grid_constant__ Spans
     wait_for_previous();
     double sum = 0.0;
     const int chunks = s.first[s.n];
+    int k = span_of(s, blockIdx.x);
     for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-        const int k = span_of(s, chunk);
-        with_span(s.type[k], s.words[k], [&](auto e, auto v) {
+        while (s.first[k + 1] <= chunk) ++k;
+        with_type_of(s.type[k], [&](auto e) {
             using T = decltype(e);
-            const int64_t count = s.count[k];
-            with_chunk<T, decltype(v)::value>(static_cast<const T *>(s.from[k]), (chunk - s.first[k]) * chunk_elements(s.type[k]), count,
-                                              [&](auto &x, int64_t c, int64_t step, int64_t pitch) { sum += squares(x, c, step, pitch, count); });
+            constexpr int64_t EACH = CHUNK_BYTES / sizeof(T);
+            const int64_t at = (chunk - s.first[k]) * EACH;
+            sum += sum_chunk(static_cast<const T *>(s.from[k]) + at, (int)min(EACH, s.count[k] - at), s.words[k]);
         });
     }
     sum = cta_sum(sum, tmp);
@@ -124,37 +186,19 @@ __global__ void __launch_bounds__(NT, 4) k_scale(const __grid_constant__ Spans<N
     sum = cta_sum(sum, tmp);
     const float root = (float)sqrt(sum), wanted = __fdiv_rn(max_norm, root + 1e-6f);
     const float factor = root < __uint_as_float(0x7f800000u) && wanted < 1.f ? wanted : 1.f;
-    if (blockIdx.x == 0 && threadIdx.x == 0 && norm) *norm = root;
-    const int chunks = s.first[s.n];
-    for (int chunk = chunks - 1 - blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
-        const int k = span_of(s, chunk);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = root;
+    int chunk = s.first[s.n] - 1 - (int)blockIdx.x;
+    if (chunk < 0) return;
+    for (int k = span_of(s, chunk); chunk >= 0; chunk -= gridDim.x) {
+        while (s.first[k] > chunk) --k;
         if (factor == 1.f && s.from[k] == s.to[k]) continue;
-        with_span(s.type[k], s.words[k], [&](auto e, auto v) {
+        with_type_of(s.type[k], [&](auto e) {
             using T = decltype(e);
-            constexpr int V = decltype(v)::value;
-            const int64_t count = s.count[k];
-            with_chunk<T, V>(static_cast<const T *>(s.from[k]), (chunk - s.first[k]) * chunk_elements(s.type[k]), count, [&](auto &x, int64_t c, int64_t step, int64_t pitch) {
-                auto each = [&](auto put) {
-#pragma unroll
-                    for (int u = 0; u < TURNS; ++u)
-                        if (c + u * step < count) {
-#pragma unroll
-                            for (int i = 0; i < Chunk<T, V>::N; ++i)
-                                if (Chunk<T, V>::there(i, c + u * step, pitch, count)) put(u, i, factor == 1.f ? x[u].get(i) : x[u].get(i) * factor);
-                        }
-                };
-                if (s.to_type[k] == s.type[k]) {
-                    if (factor != 1.f) each([&](int u, int i, float f) { x[u].set(i, f); });
-#pragma unroll
-                    for (int u = 0; u < TURNS; ++u)
-                        if (c + u * step < count) x[u].store(static_cast<T *>(s.to[k]), c + u * step, pitch, count);
-                } else {
-                    auto at = [&](int u, int i) { return c + u * step + i / V * pitch + i % V; };
-                    if (s.to_type[k] == NB200_F32) each([&](int u, int i, float f) { static_cast<float *>(s.to[k])[at(u, i)] = f; });
-                    else if (s.to_type[k] == NB200_F16) each([&](int u, int i, float f) { static_cast<__half *>(s.to[k])[at(u, i)] = __float2half_rn(f); });
-                    else each([&](int u, int i, float f) { static_cast<__nv_bfloat16 *>(s.to[k])[at(u, i)] = __float2bfloat16_rn(f); });
-                }
-            });
+            constexpr int64_t EACH = CHUNK_BYTES / sizeof(T);
+            const int64_t at = (chunk - s.first[k]) * EACH;
+            const T *const from = static_cast<const T *>(s.from[k]) + at;
+            const int count = (int)min(EACH, s.count[k] - at);
+            with_type_of(s.to_type[k], [&](auto z) { scale_chunk(from, static_cast<decltype(z) *>(s.to[k]) + at, count, s.words[k], factor); });
         });
     }
 }
@@ -179,9 +223,7 @@ int clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, double
         for (int i = 0; i < s.n; ++i) {
             const nb200_span &x = spans[l * N + i];
             s.from[i] = x.from, s.to[i] = x.to, s.count[i] = x.count, s.type[i] = (uint8_t)x.type, s.to_type[i] = (uint8_t)x.to_type;
-            // words of 16 bytes; the last one need not be whole if the next element is where another word would begin
-            const bool even = x.count * type_size(x.type) % 16 == 0 && reinterpret_cast<uintptr_t>(x.from) % 16 == 0;
-            s.words[i] = even && (x.type != x.to_type || reinterpret_cast<uintptr_t>(x.to) % 16 == 0);
+            s.words[i] = reinterpret_cast<uintptr_t>(x.from) % 16 == 0 && reinterpret_cast<uintptr_t>(x.to) % 16 == 0;
             s.first[i] = (int32_t)chunks;
             chunks += (x.count + chunk_elements(x.type) - 1) / chunk_elements(x.type);
             if (chunks > INT32_MAX) return (int)NB200_E_UNSUPPORTED;

@@ -111,17 +111,6 @@ struct TileWalk {
 
 // ---- the kernel ------------------------------------------------------------------------
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (std::is_same<T, __half>::value) {
-        const __half2 v = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-}
-
 // Rows from the warp's place in shared memory to memory: `to(r, p)` is where the 16-byte piece p of row r goes, `count(r, p)` how many of its eight elements.
 template <int PIECES, typename T, typename To, typename Count>
 __device__ __forceinline__ void flush(const uint8_t *place, bool words, To to, Count count) {
