@@ -151,7 +151,8 @@ __device__ __forceinline__ void put_square(uint8_t *place, const float (&lo)[16]
 //
 // GATED: 16 rows of gates and 16 of values alternate in the wide operand's tile, so that a gate and its value lie 16 lanes apart in tensor memory and fragments
 // of both land in the same thread.
-// WEIGHTS: the last block of a group's tokens runs into the next group's, whose rows are cleared in shared memory before they are multiplied.
+// WEIGHTS: the last block of a group's tokens runs into the next group's. Steps of 16 tokens that are not the group's are left out, and in the last step the rows
+// behind its last token are cleared in shared memory.
 template <Sum SUM, Form FORM, bool A_TURNED, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, const __grid_constant__ CUtensorMap wide_map, const __grid_constant__ CUtensorMap narrow_map) {
     constexpr int STAGES = TileShared::STAGES, SUMS = TileShared::SUMS;
@@ -182,14 +183,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
     Place t{};
     // Columns of N that the tile's matrix instructions have, and those that this CTA brings.
     auto narrow = [&] { return (t.count + TILE_STEP - 1) / TILE_STEP * TILE_STEP; };
-    // The tail of a group's last block: rows of the summed axis, in this CTA's halves of both operands.
+    // The last block of a group's tokens has `rows` of them: what follows up to the next 16 is cleared in this CTA's halves of both operands.
     auto clear_tail = [&](int stage, int n, int rows) {
-        uint8_t *const a = sh.a[stage], *const b = sh.b[stage];
-        const int chunks = 2 + (n / 2 + 63) / 64;
-        for (int i = lane; i < chunks * (64 - rows) * 8; i += 32) {
-            const int chunk = i / ((64 - rows) * 8), at = i - chunk * (64 - rows) * 8;
-            uint8_t *const tile = chunk < 2 ? a + chunk * 8192 : b + (chunk - 2) * 8192;
-            *reinterpret_cast<uint4 *>(tile + rows * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+        const int stop = (rows + 15) / 16 * 16, chunks = (n / 2 + 63) / 64;
+        for (int r = rows + lane / 8; r < stop; r += 4) {
+            const int at = r * 128 + (lane & 7) * 16;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4 *>(sh.a[stage] + i * 8192 + at) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < chunks; ++i) *reinterpret_cast<uint4 *>(sh.b[stage] + i * 8192 + at) = make_uint4(0, 0, 0, 0);
         }
         fence_async_shared();
         __syncwarp();
@@ -353,8 +354,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                 if (t.blocks && !(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
                 for (int b = 0; b < t.blocks; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
-                    if (FORM == Form::WEIGHTS && t.last - t.first - b * 64 < 64) {
-                        clear_tail(stage.at, n, t.last - t.first - b * 64);
+                    const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
+                    if (rows < 64 && rows % 16) {
+                        clear_tail(stage.at, n, rows);
                         fence_cluster();
                     }
                     tmem_fence_after();
@@ -362,7 +364,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                         const uint64_t da = tile_a + (uint64_t)(stage.at * (128 * 128 >> 4)), db = tile_b + (uint64_t)(stage.at * (128 * 128 >> 4));
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_pair<SUM>(tmem + sums.at * TILE_N, da + (A_TURNED ? 128 : 2) * k, db + (B_TURNED ? 128 : 2) * k, shape, b > 0 || k > 0);
+                            if (FORM != Form::WEIGHTS || k * 16 < rows)
+                                mma_pair<SUM>(tmem + sums.at * TILE_N, da + (A_TURNED ? 128 : 2) * k, db + (B_TURNED ? 128 : 2) * k, shape, b > 0 || k > 0);
                         mma_commit<true>(&sh.empty[stage.at]);
                         if (b + 1 == t.blocks) mma_commit<true>(&sh.sum_full[sums.at]);
                     }
@@ -380,8 +383,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                 const int n = narrow();
                 for (int b = 0; b < t.blocks; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
-                    const bool tail = FORM == Form::WEIGHTS && t.last - t.first - b * 64 < 64;
-                    if (tail) clear_tail(stage.at, n, t.last - t.first - b * 64);
+                    const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
+                    const bool tail = rows < 64 && rows % 16;
+                    if (tail) clear_tail(stage.at, n, rows);
                     if (elected()) {
                         if (tail) mbar_arrive_leader_release(&sh.full[stage.at]);
                         else mbar_arrive_leader(&sh.full[stage.at]);
