@@ -165,18 +165,24 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
     if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
     nb200_dense ax, aw;
     if ((st = aligned(*x, 1, s.x, &ax, stream)) || (st = aligned(*w, groups, s.w, &aw, stream))) return st;
-    CUtensorMap wide{}, narrow{};
-    if ((st = describe_rows(&wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16)) ||
-        (st = describe_rows(&narrow, map_type(x->type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 32)))
-        return st;
+    TileMaps maps{};
     TileArgs args{};
+    if ((st = describe_rows(&maps.wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16)) ||
+        (st = describe_rows(&maps.narrow, map_type(x->type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 32)) || (st = describe_result(&maps.y, &args.words, map_type(x->type), *h, 1)))
+        return st;
+    if (both) {
+        args.words = args.words && word_bytes({both}) == 16;
+        // gates and values as two matrices, so that a tile of one ends where the other begins
+        const cuuint64_t extents[3] = {(cuuint64_t)hidden, 2, (cuuint64_t)x->rows}, pitches[2] = {(cuuint64_t)hidden * 2, (cuuint64_t)hidden * 4};
+        const cuuint32_t box[3] = {64, 1, 32};
+        if (args.words && (st = encode_matrix(&maps.both, map_type(x->type), 3, both->data, extents, pitches, box))) return st;
+    }
     args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows, args.wide = (int)hidden, args.blocks = (int)((x->cols + 63) / 64);
     args.tile_n = tile_n_of(x->rows, groups, (hidden + TILE_M / 2 - 1) / (TILE_M / 2));
     args.y = h->data, args.stride = h->rows > 1 ? h->stride : h->cols, args.both = both ? both->data : nullptr, args.gelu = gelu;
-    args.words = word_bytes({h}) == 16 && (!both || word_bytes({both}) == 16);
     return with_half(x->type, [&](auto e) {
         using T = decltype(e);
-        return launch_tiles<sum_of<T>, Form::GATED, false, T>("gated_product", args, wide, narrow, stream);
+        return launch_tiles<sum_of<T>, Form::GATED, false, T>("gated_product", args, maps, stream);
     });
 }
 
@@ -222,23 +228,24 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
             return (int)NB200_OK;
         });
         if (st) return st;
-        CUtensorMap wide{}, narrow{};
+        TileMaps maps{};
         TileArgs args{};
         args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows;
         // dx: the weights' columns on the wide side
-        if ((st = describe_rows(&wide, map_type(type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 64)) ||
-            (st = describe_rows(&narrow, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 32)))
+        if ((st = describe_rows(&maps.wide, map_type(type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 64)) ||
+            (st = describe_rows(&maps.narrow, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 32)) || (st = describe_result(&maps.y, &args.words, map_type(type), *dx, 1)))
             return st;
         args.wide = (int)x->cols, args.blocks = (int)((2 * hidden + 63) / 64), args.tile_n = tile_n_of(x->rows, groups, (x->cols + TILE_M - 1) / TILE_M);
-        args.y = dx->data, args.stride = dx->rows > 1 ? dx->stride : dx->cols, args.words = word_bytes({dx}) == 16;
-        if ((st = launch_tiles<sum_of<T>, Form::ROWS, true, T>("gated_grad_x", args, wide, narrow, stream))) return st;
+        args.y = dx->data, args.stride = dx->rows > 1 ? dx->stride : dx->cols;
+        if ((st = launch_tiles<sum_of<T>, Form::ROWS, true, T>("gated_grad_x", args, maps, stream))) return st;
         // dw: both operands turned
-        if ((st = describe_rows(&wide, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 64)) ||
-            (st = describe_rows(&narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)))
+        if ((st = describe_rows(&maps.wide, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 64)) ||
+            (st = describe_rows(&maps.narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)) ||
+            (st = describe_result(&maps.y, &args.words, map_type(type), *dw, groups)))
             return st;
         args.wide = (int)(2 * hidden), args.across = (int)x->cols, args.tile_n = x->cols > 128 ? TILE_N : 128;
-        args.y = dw->data, args.stride = dw->rows > 1 ? dw->stride : dw->cols, args.words = word_bytes({dw}) == 16;
-        return launch_tiles<sum_of<T>, Form::WEIGHTS, true, T>("gated_grad_w", args, wide, narrow, stream);
+        args.y = dw->data, args.stride = dw->rows > 1 ? dw->stride : dw->cols;
+        return launch_tiles<sum_of<T>, Form::WEIGHTS, true, T>("gated_grad_w", args, maps, stream);
     });
 }
 

@@ -168,15 +168,16 @@ int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *
             const FewArgs args{a->values, w->values, pitch, pitch, offsets, w->groups, a->rows, w->rows, (int)pitch, y->data, nullptr, stride, a->scales, w->scales, false};
             return launch_few_rows<Sum::S8, false, 16, T>("int8_few", args, (y->rows + groups - 1) / groups, stream);
         }
-        CUtensorMap wide{}, narrow{};
-        if ((st = describe_rows(&wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, w->values, 1, pitch, w->rows, groups, pitch, 128)) ||
-            (st = describe_rows(&narrow, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, 1, pitch, 32)))
-            return st;
+        TileMaps maps{};
         TileArgs args{};
+        if ((st = describe_rows(&maps.wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, w->values, 1, pitch, w->rows, groups, pitch, 128)) ||
+            (st = describe_rows(&maps.narrow, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, 1, pitch, 32)) ||
+            (st = describe_result(&maps.y, &args.words, map_type(y->type), *y, 1)))
+            return st;
         args.offsets = offsets, args.groups = w->groups, args.rows = a->rows, args.wide = w->rows, args.blocks = (int)((a->cols + 127) / 128);
         args.tile_n = tile_n_of(a->rows, groups, (w->rows + TILE_M - 1) / TILE_M);
-        args.y = y->data, args.stride = stride, args.row_scale = a->scales, args.col_scale = w->scales, args.words = word_bytes({y}) == 16;
-        return launch_tiles<Sum::S8, Form::ROWS, false, T>("int8_product", args, wide, narrow, stream);
+        args.y = y->data, args.stride = stride, args.row_scale = a->scales, args.col_scale = w->scales;
+        return launch_tiles<Sum::S8, Form::ROWS, false, T>("int8_product", args, maps, stream);
     });
 }
 

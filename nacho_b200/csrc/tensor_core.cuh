@@ -182,6 +182,9 @@ __device__ __forceinline__ void store_matrices(void *row, uint32_t a, uint32_t b
 __device__ __forceinline__ void store_tile(const CUtensorMap *matrix, const void *smem, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(matrix), "r"(smem_u32(smem)), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void store_tile3(const CUtensorMap *matrix, const void *smem, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(matrix), "r"(smem_u32(smem)), "r"(x), "r"(y), "r"(z) : "memory");
+}
 __device__ __forceinline__ void close_stores() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void stores_read_but() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }

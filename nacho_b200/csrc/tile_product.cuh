@@ -1,5 +1,5 @@
 // Products on the tensor cores whose sums stay in tensor memory until a tile is done: 16-bit floats and 8-bit integers. Tokens, which groups share
-// unevenly, lie on the narrow side of the matrix instructions (N, any multiple of 64), weights on the wide one (M = 256), so that a group's
+// unevenly, lie on the narrow side of the matrix instructions (N, any multiple of 32), weights on the wide one (M = 256), so that a group's
 // last tile does hardly more work than its rows need.
 //   GATED:   h[t, j] = act(sum_k x[t, k] w[g][j, k]) * sum_k x[t, k] w[g][hidden + j, k], and both sums where they are kept
 //   ROWS:    y[t, j] = sum_k x[t, k] w[g][j, k], the second operand by rows or turned
@@ -18,7 +18,7 @@ namespace nb200 {
 enum class Form { GATED, ROWS, WEIGHTS };
 
 constexpr int TILE_STORE_WARPS = 8, TILE_THREADS = (TILE_STORE_WARPS + 2) * 32;
-constexpr int TILE_M = 256, TILE_N = 256, TILE_STEP = 64, TILE_PANEL = 8;  // of a pair of CTAs; tokens come in steps of 64; row tiles that follow one another
+constexpr int TILE_M = 256, TILE_N = 256, TILE_STEP = 32, TILE_PANEL = 8;  // of a pair of CTAs; the narrow side comes in steps; row tiles that follow one another
 
 struct TileArgs {
     const int32_t *offsets;  // groups + 1, or none: one group of all rows
@@ -33,16 +33,21 @@ struct TileArgs {
     void *both;  // GATED: [rows][2 hidden] or none
     const float *row_scale, *col_scale;  // S8: of the rows, of every group's columns
     bool gelu;
-    bool words;  // results in words of 16 bytes
+    bool words;  // results in words of 16 bytes, whole tiles by the copy engine
     unsigned long long *report;
+};
+
+// The operands and the results as the copy engine sees them: boxes of rows of 128 bytes. Results: y [rows][columns], both [rows][2][hidden], z [group][rows][columns].
+struct TileMaps {
+    CUtensorMap wide, narrow, y, both;
 };
 
 // What a CTA of a pair has in shared memory; tiles begin at 1024-byte boundaries.
 struct TileShared {
-    static constexpr int STAGES = 6, SUMS = 2;  // blocks under way; places for a tile's sums in tensor memory
+    static constexpr int STAGES = 5, SUMS = 2;  // blocks under way; places for a tile's sums in tensor memory
     uint8_t a[STAGES][128 * 128];               // 128 rows of the wide side (turned: two blocks of 64 by 64 of the summed axis)
     uint8_t b[STAGES][128 * 128];               // half of the tile's narrow side
-    uint8_t out[TILE_STORE_WARPS][32 * 96];     // GATED: 32 x 32 bytes of h, 32 x 64 of both sums; else 32 x 64
+    uint8_t out[2][24 * 1024];                  // tiles of 32 rows by 128 bytes on their way out, of four warps each
     uint64_t full[STAGES], empty[STAGES];       // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
     uint64_t sum_full[SUMS], sum_empty[SUMS];   // a tile's sums lie in tensor memory; they have been read
     uint64_t drained;
@@ -109,39 +114,71 @@ struct TileWalk {
     }
 };
 
+// The tiles of a pair of CTAs: one of every round of as many as there are pairs, another place in each, since groups' last tiles, which cost less, may come
+// at a distance that divides the round (experts of 1000 rows: every fourth tile, and half of 74 pairs got all of them).
+struct Turns {
+    int base = 0, place, pairs, turn;
+    __device__ Turns(int pair, int all) : place(pair), pairs(all), turn(31 % all) {}
+    __device__ int tile() const { return base + place; }
+    __device__ void next() {
+        base += pairs;
+        place += turn;
+        if (place >= pairs) place -= pairs;
+    }
+};
+
 // ---- the kernel ------------------------------------------------------------------------
 
-// Rows from the warp's place in shared memory to memory: `to(r, p)` is where the 16-byte piece p of row r goes, `count(r, p)` how many of its eight elements.
-template <int PIECES, typename T, typename To, typename Count>
-__device__ __forceinline__ void flush(const uint8_t *place, bool words, To to, Count count) {
-    const int lane = lane_id();
-    constexpr int ROW = PIECES * 16, TURN = 128 / ROW, EACH = 32 / PIECES;
-    auto at = [&](int r, int p) { return place + r * ROW + ((p ^ (r / TURN & (PIECES - 1))) << 4); };
-    if (words) {
-#pragma unroll
-        for (int i = 0; i < 32; i += EACH) {
-            const int r = i + lane / PIECES, p = lane & (PIECES - 1);
-            if (count(r, p) >= 8) *reinterpret_cast<uint4 *>(to(r, p)) = *reinterpret_cast<const uint4 *>(at(r, p));
-        }
-    } else {
-        constexpr int AT_ONCE = 32 / (PIECES * 8);  // rows
-#pragma unroll 4
-        for (int i = 0; i < 32; i += AT_ONCE) {
-            const int r = i + lane / (PIECES * 8), e = lane & (PIECES * 8 - 1), p = e / 8;
-            if (e % 8 < count(r, p)) to(r, p)[e % 8] = reinterpret_cast<const T *>(at(r, p))[e % 8];
-        }
-    }
+// The four warps that share half of a tile's columns meet.
+__device__ __forceinline__ void half_sync(int half) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(half + 1) : "memory"); }
+// And learn whether all of them are fine.
+__device__ __forceinline__ bool half_all(int half, bool fine) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)fine), "r"(half + 1)
+        : "memory");
+    return all != 0;
 }
 
-// The warp's 32 lanes of M by 32 columns of N, from fragments lo (lanes 0 .. 15) and hi to its place, by columns (rows of 32 elements of M) or by lanes.
-template <bool BY_COLUMNS, typename T>
-__device__ __forceinline__ void put_square(uint8_t *place, const float (&lo)[16], const float (&hi)[16]) {
+// Fragments of 16 lanes of M by 32 columns of N into tiles of 128-byte rows laid out as the copy engine takes them. By columns: row n of the tile, 16 elements
+// from the 16-byte piece `piece` on.
+template <typename T>
+__device__ __forceinline__ void put_columns(uint8_t *tile, int piece, const float (&v)[16]) {
     const int q = lane_id() >> 3, r = lane_id() & 7;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int row = BY_COLUMNS ? 8 * j + r : 8 * q + r, piece = BY_COLUMNS ? q : j;
-        store_matrices<BY_COLUMNS>(place + row * 64 + ((piece ^ (row / 2 & 3)) << 4), pack2<T>(lo[4 * j], lo[4 * j + 1]), pack2<T>(lo[4 * j + 2], lo[4 * j + 3]),
-                                   pack2<T>(hi[4 * j], hi[4 * j + 1]), pack2<T>(hi[4 * j + 2], hi[4 * j + 3]));
+    for (int j = 0; j < 4; j += 2) {
+        const int row = 8 * (j + q / 2) + r;
+        store_matrices<true>(tile + piece_at(row, piece + (q & 1)), pack2<T>(v[4 * j], v[4 * j + 1]), pack2<T>(v[4 * j + 2], v[4 * j + 3]), pack2<T>(v[4 * j + 4], v[4 * j + 5]),
+                             pack2<T>(v[4 * j + 6], v[4 * j + 7]));
+    }
+}
+// By lanes: rows `row` .. row + 15, 32 elements from `piece` on.
+template <typename T>
+__device__ __forceinline__ void put_lanes(uint8_t *tile, int row, int piece, const float (&v)[16]) {
+    const int q = lane_id() >> 3, r = lane_id() & 7;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2)
+        store_matrices<false>(tile + piece_at(row + 8 * (q & 1) + r, piece + j + q / 2), pack2<T>(v[4 * j], v[4 * j + 1]), pack2<T>(v[4 * j + 2], v[4 * j + 3]),
+                              pack2<T>(v[4 * j + 4], v[4 * j + 5]), pack2<T>(v[4 * j + 6], v[4 * j + 7]));
+}
+// Rows first, first + step, .. below `rows` of such a tile to memory, `cols` elements of each. WORDS: in words of 16 bytes.
+template <typename T>
+__device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, int64_t stride, int first, int step, int rows, int cols) {
+    const int lane = lane_id();
+    if (words) {
+        const int p = lane & 7;
+        for (int r = first + lane / 8 * step; r < rows; r += 4 * step)
+            if (p * 8 < cols) *reinterpret_cast<uint4 *>(to + r * stride + p * 8) = *reinterpret_cast<const uint4 *>(tile + piece_at(r, p));
+    } else {
+        for (int r = first; r < rows; r += step)
+#pragma unroll
+            for (int e = lane; e < 64; e += 32)
+                if (e < cols) to[r * stride + e] = reinterpret_cast<const T *>(tile + piece_at(r, e / 8))[e % 8];
     }
 }
 
@@ -154,7 +191,7 @@ __device__ __forceinline__ void put_square(uint8_t *place, const float (&lo)[16]
 // WEIGHTS: the last block of a group's tokens runs into the next group's. Steps of 16 tokens that are not the group's are left out, and in the last step the rows
 // behind its last token are cleared in shared memory.
 template <Sum SUM, Form FORM, bool A_TURNED, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, const __grid_constant__ CUtensorMap wide_map, const __grid_constant__ CUtensorMap narrow_map) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, const __grid_constant__ TileMaps maps) {
     constexpr int STAGES = TileShared::STAGES, SUMS = TileShared::SUMS;
     constexpr bool B_TURNED = FORM == Form::WEIGHTS, GATED = FORM == Form::GATED;
     constexpr int PER_BLOCK = SUM == Sum::S8 ? 128 : 64;
@@ -178,7 +215,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
     trigger_dependents();
     wait_for_previous();
 
-    const int first = blockIdx.x / 2, step = gridDim.x / 2;
+    Turns at(blockIdx.x / 2, gridDim.x / 2);
     TileWalk<FORM> walk(args);
     Place t{};
     // Columns of N that the tile's matrix instructions have, and those that this CTA brings.
@@ -198,102 +235,172 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
     if (warp < TILE_STORE_WARPS) {
         const int lanes = warp & 3, half = warp >> 2;
         Ring<SUMS> sums;
-        uint8_t *const place = sh.out[warp], *const place_both = sh.out[warp] + 32 * 32;
         T *const y = static_cast<T *>(args.y);
+        uint8_t *const out = sh.out[half];
+        int turn = 0;
         bool fine = true;
-        for (int tile = first; fine && walk.find(tile, t); tile += step) {
+        for (; walk.find(at.tile(), t); at.next()) {
             const int n = narrow();
-            // the first column (row of z) of this warp's lanes
-            const int col = t.col + (GATED ? rank * 64 + lanes * 16 : rank * 128 + lanes * 32);
             if (t.blocks) {
-                if (!(fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed))) break;
+                fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed);
                 tmem_fence_after();
             }
-            float col_scale[4];
-            if constexpr (SUM == Sum::S8) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = std::is_same<T, float>::value ? col + lane : col + lane / 4 + 8 * i;
-                    col_scale[i] = c < args.wide ? ld_late(args.col_scale + (int64_t)t.g * args.wide + c) : 0.f;
+            if (!half_all(half, fine)) break;  // nobody waits for a warp that has given up
+            const uint32_t base = tmem + ((uint32_t)(lanes * 32) << 16) + sums.at * TILE_N;
+            // 32 columns of this warp's lanes; behind the last ones the tile's place is free again
+            auto read = [&](int c, bool last, float (&lo)[16], float (&hi)[16], const float (&col_scale)[4], float row_scale) {
+                uint32_t v[2][16] = {};
+                if (t.blocks) {
+                    tmem_load_fragments(base + c, v[0]);
+                    tmem_load_fragments(base + c + (16u << 16), v[1]);
+                    tmem_wait_loads(v[0]);
+                    tmem_wait_loads(v[1]);
+                    if (last) {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
+                    }
                 }
-            }
-            for (int c = half * (n / 2); c < (half + 1) * (n / 2); c += 32) {
-                const uint32_t at = tmem + ((uint32_t)(lanes * 32) << 16) + sums.at * TILE_N + c;
-                const bool last = c + 32 >= (half + 1) * (n / 2);
-                auto read_all = [&] {  // this warp has read the tile's sums
-                    if (!last || !t.blocks) return;
-                    tmem_fence_before();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if constexpr (SUM == Sum::S8) {
+                        const float s = __shfl_sync(FULL_MASK, row_scale, i / 4 * 8 + (lane & 3) * 2 + (i & 1));
+                        lo[i] = scaled((int)v[0][i], s, col_scale[(i & 2) / 2]);
+                        hi[i] = scaled((int)v[1][i], s, col_scale[2 + (i & 2) / 2]);
+                    } else {
+                        lo[i] = __uint_as_float(v[0][i]), hi[i] = __uint_as_float(v[1][i]);
+                    }
+                }
+            };
+            float lo[16], hi[16], col_scale[4] = {};
+            if constexpr (FORM == Form::WEIGHTS) {
+                // A warp has 32 rows of z and 64 of every 128 columns.
+                const int row = t.col + rank * 128 + lanes * 32;
+                uint8_t *const place = out + lanes * 6144;
+                bool read_some = false;
+                for (int c = half * 64; c < n; c += 128) {
+                    const bool last = c + 128 >= n;
+                    read_some = true;
+                    if (args.words && elected()) stores_read_but<0>();
                     __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (c + 32 * i < n) read(c + 32 * i, last && (i == 1 || c + 32 >= n), lo, hi, col_scale, 0.f);
+                        put_lanes<T>(place, 0, 4 * i, lo);
+                        put_lanes<T>(place, 16, 4 * i, hi);
+                    }
+                    if (args.words) {
+                        fence_async_shared();
+                        __syncwarp();
+                        if (row < args.wide && elected()) store_tile3(&maps.y, place, t.from + c, row, t.g), close_stores();
+                    } else {
+                        __syncwarp();
+                        flush(place, false, y + ((int64_t)t.g * args.wide + row) * args.stride + t.from + c, args.stride, 0, 1, min(32, args.wide - row), t.count - c);
+                        __syncwarp();
+                    }
+                }
+                if (!read_some && t.blocks) {  // a narrow tile is the other half's
+                    tmem_fence_before();
                     if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
-                };
-                const int left = t.count - c;  // rows of the result from here on (columns of z)
-                float row_scale = 0.f;
-                if constexpr (SUM == Sum::S8) row_scale = lane < left ? ld_late(args.row_scale + t.from + c + lane) : 0.f;
-                if constexpr (std::is_same<T, float>::value) {
-                    uint32_t v[32] = {};
-                    if (t.blocks) tmem_load(at, v), tmem_wait_loads(v);
-                    read_all();
+                }
+            } else if constexpr (std::is_same<T, float>::value) {
+                const int col = t.col + rank * 128 + lanes * 32 + lane;
+                if (SUM == Sum::S8 && col < args.wide) col_scale[0] = ld_late(args.col_scale + (int64_t)t.g * args.wide + col);
+                bool read_some = false;
+                for (int c = half * 32; c < n; c += 64) {
+                    read_some = true;
+                    const int left = t.count - c;
+                    const float row_scale = SUM == Sum::S8 && lane < left ? ld_late(args.row_scale + t.from + c + lane) : 0.f;
+                    uint32_t v[32];
+                    tmem_load(base + c, v);
+                    tmem_wait_loads(v);
+                    if (c + 64 >= n) {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
                         const float f = SUM == Sum::S8 ? scaled((int)v[j], __shfl_sync(FULL_MASK, row_scale, j), col_scale[0]) : __uint_as_float(v[j]);
-                        if (j < left && col + lane < args.wide) y[(int64_t)(t.from + c + j) * args.stride + col + lane] = f;
+                        if (j < left && col < args.wide) y[(int64_t)(t.from + c + j) * args.stride + col] = f;
                     }
-                } else {
-                    uint32_t v[2][16] = {};
-                    if (t.blocks) {
-                        tmem_load_fragments(at, v[0]);
-                        tmem_load_fragments(at + (16u << 16), v[1]);
-                        tmem_wait_loads(v[0]);
-                        tmem_wait_loads(v[1]);
-                    }
-                    read_all();
-                    float lo[16], hi[16];
+                }
+                if (!read_some) {
+                    tmem_fence_before();
+                    if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
+                }
+            } else {
+                // The four warps of a half have 32 of every 64 rows of the result, by tiles of 64 columns: of h, gates and values, or two of y.
+                constexpr int TILES = GATED ? 3 : 2;
+                const int col = t.col + (GATED ? rank * 64 : rank * 128);
+                if constexpr (SUM == Sum::S8) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if constexpr (SUM == Sum::S8) {
-                            const float s = __shfl_sync(FULL_MASK, row_scale, i / 4 * 8 + (lane & 3) * 2 + (i & 1));
-                            lo[i] = scaled((int)v[0][i], s, col_scale[(i & 2) / 2]);
-                            hi[i] = scaled((int)v[1][i], s, col_scale[2 + (i & 2) / 2]);
-                        } else {
-                            lo[i] = __uint_as_float(v[0][i]), hi[i] = __uint_as_float(v[1][i]);
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = col + lanes * 32 + lane / 4 + 8 * i;
+                        if (c < args.wide) col_scale[i] = ld_late(args.col_scale + (int64_t)t.g * args.wide + c);
                     }
-                    if (left <= 0) continue;
-                    __syncwarp();  // the place has been read
+                }
+                bool read_some = false;
+                for (int c = half * 32; c < n; c += 64, turn ^= 1) {
+                    read_some = true;
+                    const int left = t.count - c, row = t.from + c;
+                    // behind the group's last row there is no other's row, or these 32 are all the group's
+                    const bool whole = args.words && (left >= 32 || t.from + t.count == args.rows);
+                    uint8_t *const place = out + turn * TILES * 4096;
+                    float row_scale = 0.f;
+                    if constexpr (SUM == Sum::S8) row_scale = lane < left ? ld_late(args.row_scale + row + lane) : 0.f;
+                    read(c, c + 64 >= n, lo, hi, col_scale, row_scale);
+                    if (lanes == 0 && elected()) stores_read_but<1>();
+                    half_sync(half);  // this place has been read
                     if constexpr (GATED) {
-                        const int wide = args.wide, stride = 2 * wide;
-                        if (args.both) put_square<true, T>(place_both, lo, hi);
+                        if (args.both) {
+                            put_columns<T>(place + 4096, lanes * 2, lo);
+                            put_columns<T>(place + 2 * 4096, lanes * 2, hi);
+                        }
                         float h[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) h[i] = lo[i] * logistic(act_inner(lo[i], args.gelu)) * hi[i];
-                        const int q = lane >> 3, r = lane & 7;
-#pragma unroll
-                        for (int j = 0; j < 4; j += 2) {  // rows of 16 elements: two pieces
-                            const int row = 8 * (j + q / 2) + r;
-                            store_matrices<true>(place + row * 32 + (((q & 1) ^ (row / 4 & 1)) << 4), pack2<T>(h[4 * j], h[4 * j + 1]), pack2<T>(h[4 * j + 2], h[4 * j + 3]),
-                                                 pack2<T>(h[4 * j + 4], h[4 * j + 5]), pack2<T>(h[4 * j + 6], h[4 * j + 7]));
-                        }
-                        __syncwarp();
-                        flush<2, T>(place, args.words, [&](int row, int p) { return y + (int64_t)(t.from + c + row) * args.stride + col + p * 8; },
-                                    [&](int row, int p) { return row < left ? wide - col - p * 8 : 0; });
-                        if (args.both)
-                            flush<4, T>(place_both, args.words, [&](int row, int p) { return static_cast<T *>(args.both) + (int64_t)(t.from + c + row) * stride + (p >= 2 ? wide : 0) + col + (p & 1) * 8; },
-                                        [&](int row, int p) { return row < left ? wide - col - (p & 1) * 8 : 0; });
-                    } else if constexpr (FORM == Form::ROWS) {
-                        put_square<true, T>(place, lo, hi);
-                        __syncwarp();
-                        flush<4, T>(place, args.words, [&](int row, int p) { return y + (int64_t)(t.from + c + row) * args.stride + col + p * 8; },
-                                    [&](int row, int p) { return row < left ? args.wide - col - p * 8 : 0; });
+                        put_columns<T>(place, lanes * 2, h);
                     } else {
-                        put_square<false, T>(place, lo, hi);
-                        __syncwarp();
-                        flush<4, T>(place, args.words, [&](int row, int p) { return y + ((int64_t)t.g * args.wide + col + row) * args.stride + t.from + c + p * 8; },
-                                    [&](int row, int p) { return col + row < args.wide ? left - p * 8 : 0; });
+                        put_columns<T>(place + (lanes >> 1) * 4096, (lanes & 1) * 4, lo);
+                        put_columns<T>(place + (lanes >> 1) * 4096, (lanes & 1) * 4 + 2, hi);
                     }
+                    if (whole) fence_async_shared();
+                    half_sync(half);
+                    if (whole) {
+                        if (lanes == 0 && col < args.wide && elected()) {
+                            if constexpr (GATED) {
+                                store_tile3(&maps.y, place, col, row, 0);
+                                if (args.both) store_tile3(&maps.both, place + 4096, col, 0, row), store_tile3(&maps.both, place + 2 * 4096, col, 1, row);
+                            } else {
+                                store_tile3(&maps.y, place, col, row, 0);
+                                if (col + 64 < args.wide) store_tile3(&maps.y, place + 4096, col + 64, row, 0);
+                            }
+                        }
+                    } else {
+                        const int rows = min(32, left), wide = args.wide;
+                        flush(place, args.words, y + (int64_t)row * args.stride + col, args.stride, lanes, 4, rows, wide - col);
+                        if constexpr (GATED) {
+                            if (args.both) {
+                                T *const both = static_cast<T *>(args.both) + (int64_t)row * 2 * wide + col;
+                                flush(place + 4096, args.words, both, 2 * (int64_t)wide, lanes, 4, rows, wide - col);
+                                flush(place + 2 * 4096, args.words, both + wide, 2 * (int64_t)wide, lanes, 4, rows, wide - col);
+                            }
+                        } else {
+                            flush(place + 4096, args.words, y + (int64_t)row * args.stride + col + 64, args.stride, lanes, 4, rows, wide - col - 64);
+                        }
+                    }
+                    if (lanes == 0 && elected()) close_stores();  // an empty group where the warps have written themselves
+                }
+                if (!read_some && t.blocks) {  // 32 rows are the other half's
+                    tmem_fence_before();
+                    if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
                 }
             }
             if (t.blocks) sums.next();
         }
+        if (args.words && elected()) stores_done();
+        __syncwarp();
         // rows of no group
         if (FORM != Form::WEIGHTS && args.offsets) {
             const int64_t rows = args.rows, lo = min(max((int64_t)ld_late(args.offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(args.offsets + args.groups), lo), rows);
@@ -308,10 +415,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
         Ring<STAGES> stage;
         bool fine = true;
         if (warp == TILE_STORE_WARPS + 1) {  // copies
-            for (int tile = first; fine && walk.find(tile, t); tile += step) {
+            for (; fine && walk.find(at.tile(), t); at.next()) {
                 const int n = narrow(), mine = n / 2;
-                const uint32_t bytes = 128 * 128 + (B_TURNED ? (mine + 63) / 64 * 8192 : mine * 128);
-                const int at = t.from + rank * mine;
+                const uint32_t bytes = 128 * 128 + (B_TURNED ? (mine + 63) / 64 * 8192 : (mine + 31) / 32 * 4096);
+                const int begin = t.from + rank * mine;
                 for (int b = 0; b < t.blocks; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
                     if (elected()) {
@@ -323,20 +430,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                             const int col = t.col + rank * 64;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                load_tile(to_a + i * 4096, &wide_map, k, col + 16 * i, t.g, bar);
-                                load_tile(to_a + i * 4096 + 2048, &wide_map, k, args.wide + col + 16 * i, t.g, bar);
+                                load_tile(to_a + i * 4096, &maps.wide, k, col + 16 * i, t.g, bar);
+                                load_tile(to_a + i * 4096 + 2048, &maps.wide, k, args.wide + col + 16 * i, t.g, bar);
                             }
                         } else if constexpr (A_TURNED) {
                             const int col = t.col + rank * 128, g = FORM == Form::WEIGHTS ? 0 : t.g;
-                            load_tile(to_a, &wide_map, col, k, g, bar);
-                            load_tile(to_a + 8192, &wide_map, col + 64, k, g, bar);
+                            load_tile(to_a, &maps.wide, col, k, g, bar);
+                            load_tile(to_a + 8192, &maps.wide, col + 64, k, g, bar);
                         } else {
-                            load_tile(to_a, &wide_map, k, t.col + rank * 128, t.g, bar);
+                            load_tile(to_a, &maps.wide, k, t.col + rank * 128, t.g, bar);
                         }
                         if constexpr (B_TURNED) {
-                            for (int i = 0; i < mine; i += 64) load_tile(to_b + i * 128, &narrow_map, at + i, k, 0, bar);
+                            for (int i = 0; i < mine; i += 64) load_tile(to_b + i * 128, &maps.narrow, begin + i, k, 0, bar);
                         } else {
-                            for (int i = 0; i < mine; i += 32) load_tile(to_b + i * 128, &narrow_map, k, at + i, 0, bar);
+                            for (int i = 0; i < mine; i += 32) load_tile(to_b + i * 128, &maps.narrow, k, begin + i, 0, bar);
                         }
                     }
                     __syncwarp();
@@ -348,7 +455,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
             const uint64_t tile_a = A_TURNED ? turned_descriptor(smem_u32(sh.a[0])) : tile_descriptor(smem_u32(sh.a[0]));
             const uint64_t tile_b = B_TURNED ? turned_descriptor(smem_u32(sh.b[0])) : tile_descriptor(smem_u32(sh.b[0]));
             Ring<SUMS> sums;
-            for (int tile = first; fine && walk.find(tile, t); tile += step) {
+            for (; fine && walk.find(at.tile(), t); at.next()) {
                 const int n = narrow();
                 const uint32_t shape = sum_descriptor<SUM>(A_TURNED, B_TURNED, TILE_M) | (uint32_t)(n >> 3) << 17;
                 if (t.blocks && !(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
@@ -379,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                 drain(&sh.drained, 0);
             }
         } else {  // tells the leader of the copies that have landed here
-            for (int tile = first; fine && walk.find(tile, t); tile += step) {
+            for (; fine && walk.find(at.tile(), t); at.next()) {
                 const int n = narrow();
                 for (int b = 0; b < t.blocks; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
@@ -422,17 +529,23 @@ inline int describe_rows(CUtensorMap *map, CUtensorMapDataType type, void *data,
     const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
     return encode_matrix(map, type, 3, data, extents, pitches, box);
 }
+// A result of `groups` matrices, if whole tiles of it can leave through the copy engine.
+inline int describe_result(CUtensorMap *map, bool *words, CUtensorMapDataType type, const nb200_dense &y, int64_t groups) {
+    const int64_t stride = y.rows > 1 ? y.stride : y.cols, limit = (int64_t(1) << 40) / 2, rows = y.rows / groups;
+    *words = y.type != NB200_F32 && word_bytes({&y}) == 16 && stride < limit && (groups == 1 || rows * stride < limit);
+    return *words ? describe_rows(map, type, y.data, 2, y.cols, rows, groups, stride, 32) : (int)NB200_OK;
+}
 inline CUtensorMapDataType map_type(int type) { return type == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
 // The narrow side of the tiles: 256 while that leaves work for most SMs, else less, for which a tile costs more to bring than to multiply.
 inline int tile_n_of(int64_t rows, int64_t groups, int64_t wide_tiles) {
     int n = TILE_N;
-    while (n > TILE_STEP && ((rows + n - 1) / n + (groups > 1 ? groups / 2 : 0)) * wide_tiles * 4 < sm_count()) n /= 2;
+    while (n > 64 && ((rows + n - 1) / n + (groups > 1 ? groups / 2 : 0)) * wide_tiles * 4 < sm_count()) n /= 2;
     return n;
 }
 
 template <Sum SUM, Form FORM, bool A_TURNED, typename T>
-int launch_tiles(const char *name, TileArgs args, const CUtensorMap &wide_map, const CUtensorMap &narrow_map, cudaStream_t stream) {
+int launch_tiles(const char *name, TileArgs args, const TileMaps &maps, cudaStream_t stream) {
     Workspace *ws = nullptr;
     int st;
     if ((st = report_of(stream, &ws))) return st;
@@ -446,7 +559,7 @@ int launch_tiles(const char *name, TileArgs args, const CUtensorMap &wide_map, c
     if ((st = allow_shared(kernel, TILE_SHARED_BYTES))) return st;
     const int64_t ctas = std::max<int64_t>(2, std::min<int64_t>(tiles * 2, sm_count() / 2 * 2));
     LaunchScope scope(name, stream);
-    NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(TILE_THREADS), TILE_SHARED_BYTES, stream, args, wide_map, narrow_map));
+    NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(TILE_THREADS), TILE_SHARED_BYTES, stream, args, maps));
     return NB200_OK;
 }
 
