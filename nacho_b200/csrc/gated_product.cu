@@ -10,17 +10,25 @@ namespace {
 
 constexpr int NT = 256;
 
-// [rows][cols] with rows at a distance that the copy engine takes. A thread has 16 bytes of a row.
+// Rows at a distance that the copy engine takes, of up to two matrices: `first` CTAs have the first one's. A thread has 16 bytes of a row.
+struct Align {
+    const void *x;
+    int64_t stride, rows, cols;
+    void *z;
+    int64_t pitch;
+};
 template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_align_rows(const T *x, int64_t stride, int64_t rows, int64_t cols, T *z, int64_t pitch) {
+__global__ void __launch_bounds__(NT) k_align_rows(const Align a, const Align b, int first) {
     wait_for_previous();
     trigger_dependents();
-    const int64_t pieces = pitch / 8, all = rows * pieces;
-    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
+    const bool second = (int)blockIdx.x >= first;
+    const Align &m = second ? b : a;
+    const int64_t pieces = m.pitch / 8, all = m.rows * pieces, step = (int64_t)(second ? gridDim.x - first : first) * NT;
+    for (int64_t i = (int64_t)(blockIdx.x - (second ? first : 0)) * NT + threadIdx.x; i < all; i += step) {
         const int64_t r = i / pieces, c = (i - r * pieces) * 8;
         Eight<T> v;
-        v.template load<V>(x + r * stride, c, cols);
-        *reinterpret_cast<uint4 *>(z + r * pitch + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+        v.template load<V>(static_cast<const T *>(m.x) + r * m.stride, c, m.cols);
+        *reinterpret_cast<uint4 *>(static_cast<T *>(m.z) + r * m.pitch + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
     }
 }
 
@@ -29,11 +37,12 @@ template <typename T, int V>
 __global__ void __launch_bounds__(NT) k_gate_grad(const T *dh, int64_t dh_stride, const T *both, int64_t both_stride, int64_t rows, int64_t hidden, bool gelu, T *z, int64_t pitch) {
     wait_for_previous();
     trigger_dependents();
-    constexpr int N = Chunk<T, V>::N;
-    const int64_t per_row = (hidden + N - 1) / N, all = rows * per_row;
-    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < all; i += (int64_t)gridDim.x * NT) {
-        const int64_t r = i / per_row, at = i - r * per_row, p = V;
-        const int64_t c = at * N;
+    // a warp has 32 chunks of a row at a time, whose words its threads take in turn
+    constexpr int N = Chunk<T, V>::N, p = 32 * V;
+    const int64_t per_row = (hidden + 32 * N - 1) / (32 * N), all = rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * (NT / 32) + warp_id(); i < all; i += (int64_t)gridDim.x * (NT / 32)) {
+        const int64_t r = i / per_row, c = (i - r * per_row) * (32 * N) + lane_id() * V;
+        if (c >= hidden) continue;
         Chunk<T, V> d, g, u, dg, du;
         d.load(dh + r * dh_stride, c, p, hidden);
         g.load(both + r * both_stride, c, p, hidden);
@@ -72,17 +81,27 @@ int with_half(int type, F f) {
 template <typename T>
 constexpr Sum sum_of = std::is_same<T, __half>::value ? Sum::F16 : Sum::BF16;
 
-// Rows as the copy engine reads them: as they are, or copied to `to`.
-int aligned(const nb200_dense &x, int64_t groups, void *to, nb200_dense *z, cudaStream_t stream) {
-    *z = x;
-    if (tiles_readable(x, groups)) return NB200_OK;
-    z->data = to, z->stride = pitch_of(x.cols);
+// Rows and weights as the copy engine reads them: as they are, or copied to where there is room.
+int aligned(const nb200_dense &x, void *to_x, const nb200_dense &w, void *to_w, nb200_dense *ax, nb200_dense *aw, cudaStream_t stream) {
+    *ax = x, *aw = w;
+    Align copies[2] = {};
+    int n = 0, word = 16;
+    int64_t ctas[2] = {0, 0};
+    auto add = [&](const nb200_dense &from, void *to, nb200_dense *z) {
+        if (!to) return;
+        z->data = to, z->stride = pitch_of(from.cols);
+        copies[n] = Align{from.data, from.stride, from.rows, from.cols, to, z->stride};
+        ctas[n++] = grid_of(from.rows * (z->stride / 8));
+        word = std::min(word, word_bytes({&from}));
+    };
+    add(x, to_x, ax);
+    add(w, to_w, aw);
+    if (n == 0) return NB200_OK;
     return with_half(x.type, [&](auto e) {
         using T = decltype(e);
-        return with_vector<T>(word_bytes({&x}), [&](auto v) {
+        return with_vector<T>(word, [&](auto v) {
             LaunchScope scope("align_rows", stream);
-            NB200_CUDA(launch_overlapped(k_align_rows<T, decltype(v)::value>, dim3(grid_of(x.rows * (z->stride / 8))), dim3(NT), 0, stream, static_cast<const T *>(x.data), x.stride,
-                                         x.rows, x.cols, static_cast<T *>(to), z->stride));
+            NB200_CUDA(launch_overlapped(k_align_rows<T, decltype(v)::value>, dim3((unsigned)(ctas[0] + ctas[1])), dim3(NT), 0, stream, copies[0], copies[1], (int)ctas[0]));
             return (int)NB200_OK;
         });
     });
@@ -164,7 +183,7 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
     if (s.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0)) return NB200_E_BADARG;
     if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
     nb200_dense ax, aw;
-    if ((st = aligned(*x, 1, s.x, &ax, stream)) || (st = aligned(*w, groups, s.w, &aw, stream))) return st;
+    if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, stream))) return st;
     TileMaps maps{};
     TileArgs args{};
     if ((st = describe_rows(&maps.wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16)) ||
@@ -211,7 +230,7 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
     if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return NB200_E_BADARG;
     if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
     nb200_dense ax, aw;
-    if ((st = aligned(*x, 1, s.x, &ax, stream)) || (st = aligned(*w, groups, s.w, &aw, stream))) return st;
+    if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, stream))) return st;
     const int64_t pitch = pitch_of(2 * hidden);
     const bool gelu = activation == NB200_GELU;
     // du begins `hidden` elements behind dg, and so does u behind g
@@ -223,7 +242,7 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
         st = with_vector<T>(word_bytes({dh, both, &half, &to}), [&](auto v) {
             constexpr int V = decltype(v)::value;
             LaunchScope scope("gate_grad", stream);
-            NB200_CUDA(launch_overlapped(k_gate_grad<T, V>, dim3(grid_of(x->rows * ((hidden + 7) / 8))), dim3(NT), 0, stream, static_cast<const T *>(dh->data), dh->stride,
+            NB200_CUDA(launch_overlapped(k_gate_grad<T, V>, dim3(grid_of(x->rows * ((hidden + 255) / 256) * 32)), dim3(NT), 0, stream, static_cast<const T *>(dh->data), dh->stride,
                                          static_cast<const T *>(both->data), both->stride, x->rows, hidden, gelu, reinterpret_cast<T *>(s.d), pitch));
             return (int)NB200_OK;
         });
@@ -243,7 +262,7 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
             (st = describe_rows(&maps.narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)) ||
             (st = describe_result(&maps.y, &args.words, map_type(type), *dw, groups)))
             return st;
-        args.wide = (int)(2 * hidden), args.across = (int)x->cols, args.tile_n = x->cols > 128 ? TILE_N : 128;
+        args.wide = (int)(2 * hidden), args.across = (int)x->cols, args.tile_n = tile_n_of(x->cols, 1, groups * ((2 * hidden + TILE_M - 1) / TILE_M));
         args.y = dw->data, args.stride = dw->rows > 1 ? dw->stride : dw->cols;
         return launch_tiles<sum_of<T>, Form::WEIGHTS, true, T>("gated_grad_w", args, maps, stream);
     });

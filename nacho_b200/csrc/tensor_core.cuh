@@ -162,6 +162,7 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
 
 // ---- loads and stores of tiles -------------------------------------------------------------------
 
+__device__ __forceinline__ void ask_for_map(const CUtensorMap *matrix) { asm volatile("prefetch.tensormap [%0];" ::"l"(matrix) : "memory"); }
 // A tile of rows of 128 bytes from the place (x, y) of matrix z, where nothing is below zero; what lies beyond the matrix comes as zeros.
 __device__ __forceinline__ void load_tile(void *smem, const CUtensorMap *matrix, int x, int y, int z, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem)), "l"(matrix), "r"(x), "r"(y),

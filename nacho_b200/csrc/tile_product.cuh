@@ -166,7 +166,8 @@ __device__ __forceinline__ void put_lanes(uint8_t *tile, int row, int piece, con
         store_matrices<false>(tile + piece_at(row + 8 * (q & 1) + r, piece + j + q / 2), pack2<T>(v[4 * j], v[4 * j + 1]), pack2<T>(v[4 * j + 2], v[4 * j + 3]),
                               pack2<T>(v[4 * j + 4], v[4 * j + 5]), pack2<T>(v[4 * j + 6], v[4 * j + 7]));
 }
-// Rows first, first + step, .. below `rows` of such a tile to memory, `cols` elements of each. WORDS: in words of 16 bytes.
+// Rows first, first + step, .. below `rows` of such a tile to memory, `cols` elements of each: in words of 16 bytes, or of 4, which begin at a row's first or second
+// element, whichever lies on a boundary (element by element 1003 rows of 1501 took 6 us more).
 template <typename T>
 __device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, int64_t stride, int first, int step, int rows, int cols) {
     const int lane = lane_id();
@@ -174,11 +175,18 @@ __device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, in
         const int p = lane & 7;
         for (int r = first + lane / 8 * step; r < rows; r += 4 * step)
             if (p * 8 < cols) *reinterpret_cast<uint4 *>(to + r * stride + p * 8) = *reinterpret_cast<const uint4 *>(tile + piece_at(r, p));
-    } else {
-        for (int r = first; r < rows; r += step)
-#pragma unroll
-            for (int e = lane; e < 64; e += 32)
-                if (e < cols) to[r * stride + e] = reinterpret_cast<const T *>(tile + piece_at(r, e / 8))[e % 8];
+        return;
+    }
+    const int end = min(cols, 64);
+    auto element = [&](int r, int e) { return (uint32_t)*reinterpret_cast<const uint16_t *>(tile + piece_at(r, e / 8) + e % 8 * 2); };
+#pragma unroll 4
+    for (int r = first; r < rows; r += step) {
+        T *const row = to + r * stride;
+        const int odd = (int)(reinterpret_cast<uintptr_t>(row) / 2 & 1), e = 2 * lane + odd;
+        const uint32_t lo = element(r, e & 63), hi = element(r, (e + 1) & 63);  // behind the last one the row's first, where that is left over
+        if (e + 1 < end) *reinterpret_cast<uint32_t *>(row + e) = lo | hi << 16;
+        else if (e < end) *reinterpret_cast<uint16_t *>(row + e) = (uint16_t)lo;
+        if (odd && lane == 31 && end > 0) *reinterpret_cast<uint16_t *>(row) = (uint16_t)hi;
     }
 }
 
@@ -212,6 +220,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
     tmem_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     volatile int *failed = &sh.failed;
+    if (threadIdx.x == 0) ask_for_map(&maps.wide), ask_for_map(&maps.narrow);
     trigger_dependents();
     wait_for_previous();
 
@@ -537,11 +546,17 @@ inline int describe_result(CUtensorMap *map, bool *words, CUtensorMapDataType ty
 }
 inline CUtensorMapDataType map_type(int type) { return type == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
-// The narrow side of the tiles: 256 while that leaves work for most SMs, else less, for which a tile costs more to bring than to multiply.
+// The narrow side of the tiles, a multiple of 64: what the busiest pair of CTAs then has to bring, 256 rows of the wide side and so many of the narrow one per
+// tile, is least. `rows` of all groups together, `wide_tiles` beside one another.
 inline int tile_n_of(int64_t rows, int64_t groups, int64_t wide_tiles) {
-    int n = TILE_N;
-    while (n > 64 && ((rows + n - 1) / n + (groups > 1 ? groups / 2 : 0)) * wide_tiles * 4 < sm_count()) n /= 2;
-    return n;
+    const int64_t mean = (rows + groups - 1) / groups, pairs = std::max(1, sm_count() / 2);
+    int best = TILE_N;
+    int64_t least = INT64_MAX;
+    for (int n = TILE_N; n >= 64; n -= 64) {
+        const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, cost = (tiles + pairs - 1) / pairs * (TILE_M + std::min<int64_t>(n, mean));
+        if (cost < least) least = cost, best = n;
+    }
+    return best;
 }
 
 template <Sum SUM, Form FORM, bool A_TURNED, typename T>
