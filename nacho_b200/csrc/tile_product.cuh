@@ -166,27 +166,42 @@ __device__ __forceinline__ void put_lanes(uint8_t *tile, int row, int piece, con
         store_matrices<false>(tile + piece_at(row + 8 * (q & 1) + r, piece + j + q / 2), pack2<T>(v[4 * j], v[4 * j + 1]), pack2<T>(v[4 * j + 2], v[4 * j + 3]),
                               pack2<T>(v[4 * j + 4], v[4 * j + 5]), pack2<T>(v[4 * j + 6], v[4 * j + 7]));
 }
-// Rows first, first + step, .. below `rows` of such a tile to memory, `cols` elements of each: in words of 16 bytes, or of 4, which begin at a row's first or second
-// element, whichever lies on a boundary (element by element 1003 rows of 1501 took 6 us more).
-template <typename T>
-__device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, int64_t stride, int first, int step, int rows, int cols) {
+// Stores that depend on a condition, without a branch: a warp whose threads part and meet again at each of them takes 200 cycles a row.
+__device__ __forceinline__ void store_if(bool yes, void *p, uint32_t v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.u32 [%0], %1;\n\t}" ::"l"(p), "r"(v), "r"((uint32_t)yes) : "memory");
+}
+__device__ __forceinline__ void store_if(bool yes, void *p, uint16_t v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.u16 [%0], %1;\n\t}" ::"l"(p), "h"(v), "r"((uint32_t)yes) : "memory");
+}
+// Rows first, first + step, .. below `rows` (32 at most) of such a tile to memory, `cols` elements of each: in words of 16 bytes, or of 4, which begin at a row's
+// first or second element, whichever lies on a boundary.
+template <int STEP, typename T>
+__device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, int64_t stride, int first, int rows, int cols) {
     const int lane = lane_id();
     if (words) {
         const int p = lane & 7;
-        for (int r = first + lane / 8 * step; r < rows; r += 4 * step)
+        for (int r = first + lane / 8 * STEP; r < rows; r += 4 * STEP)
             if (p * 8 < cols) *reinterpret_cast<uint4 *>(to + r * stride + p * 8) = *reinterpret_cast<const uint4 *>(tile + piece_at(r, p));
         return;
     }
     const int end = min(cols, 64);
-    auto element = [&](int r, int e) { return (uint32_t)*reinterpret_cast<const uint16_t *>(tile + piece_at(r, e / 8) + e % 8 * 2); };
-#pragma unroll 4
-    for (int r = first; r < rows; r += step) {
-        T *const row = to + r * stride;
-        const int odd = (int)(reinterpret_cast<uintptr_t>(row) / 2 & 1), e = 2 * lane + odd;
-        const uint32_t lo = element(r, e & 63), hi = element(r, (e + 1) & 63);  // behind the last one the row's first, where that is left over
-        if (e + 1 < end) *reinterpret_cast<uint32_t *>(row + e) = lo | hi << 16;
-        else if (e < end) *reinterpret_cast<uint16_t *>(row + e) = (uint16_t)lo;
-        if (odd && lane == 31 && end > 0) *reinterpret_cast<uint16_t *>(row) = (uint16_t)hi;
+    if (end <= 0) return;
+    T *row = to + first * stride;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8 * STEP) {
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint32_t *>(tile + piece_at(first + i + k * STEP, lane / 4) + (lane & 3) * 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k, row += STEP * stride) {
+            const uint32_t next = __shfl_down_sync(FULL_MASK, w[k], 1);
+            const bool there = first + i + k * STEP < rows, odd = reinterpret_cast<uintptr_t>(row) & 2;
+            const int e = 2 * lane + odd;
+            const uint32_t out = odd ? __funnelshift_r(w[k], next, 16) : w[k];
+            store_if(there && e + 1 < end, row + e, out);
+            store_if(there && e + 1 == end, row + e, (uint16_t)out);
+            store_if(there && odd && lane == 0, row, (uint16_t)w[k]);
+        }
     }
 }
 
@@ -304,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                         if (row < args.wide && elected()) store_tile3(&maps.y, place, t.from + c, row, t.g), close_stores();
                     } else {
                         __syncwarp();
-                        flush(place, false, y + ((int64_t)t.g * args.wide + row) * args.stride + t.from + c, args.stride, 0, 1, min(32, args.wide - row), t.count - c);
+                        flush<1>(place, false, y + ((int64_t)t.g * args.wide + row) * args.stride + t.from + c, args.stride, 0, min(32, args.wide - row), t.count - c);
                         __syncwarp();
                     }
                 }
@@ -388,15 +403,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                         }
                     } else {
                         const int rows = min(32, left), wide = args.wide;
-                        flush(place, args.words, y + (int64_t)row * args.stride + col, args.stride, lanes, 4, rows, wide - col);
+                        flush<4>(place, args.words, y + (int64_t)row * args.stride + col, args.stride, lanes, rows, wide - col);
                         if constexpr (GATED) {
                             if (args.both) {
                                 T *const both = static_cast<T *>(args.both) + (int64_t)row * 2 * wide + col;
-                                flush(place + 4096, args.words, both, 2 * (int64_t)wide, lanes, 4, rows, wide - col);
-                                flush(place + 2 * 4096, args.words, both + wide, 2 * (int64_t)wide, lanes, 4, rows, wide - col);
+                                flush<4>(place + 4096, args.words, both, 2 * (int64_t)wide, lanes, rows, wide - col);
+                                flush<4>(place + 2 * 4096, args.words, both + wide, 2 * (int64_t)wide, lanes, rows, wide - col);
                             }
                         } else {
-                            flush(place + 4096, args.words, y + (int64_t)row * args.stride + col + 64, args.stride, lanes, 4, rows, wide - col - 64);
+                            flush<4>(place + 4096, args.words, y + (int64_t)row * args.stride + col + 64, args.stride, lanes, rows, wide - col - 64);
                         }
                     }
                     if (lanes == 0 && elected()) close_stores();  // an empty group where the warps have written themselves
