@@ -100,6 +100,8 @@ inline int sm_count() {
 // many CTAs of so many threads an SM holds.
 int allow_shared_memory(const void *kernel, size_t bytes);
 int resident_ctas(const void *kernel, int threads);
+// And how many clusters of `ctas` such CTAs, with so much dynamic shared memory, the device holds: SMs come in groups that no cluster reaches beyond.
+int resident_clusters(const void *kernel, int ctas, int threads, size_t bytes);
 template <typename... P>
 int allow_shared(void (*kernel)(P...), size_t bytes) { return allow_shared_memory(reinterpret_cast<const void *>(kernel), bytes); }
 

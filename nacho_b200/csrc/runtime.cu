@@ -184,7 +184,7 @@ namespace {
 // together, so a kernel is allowed what it first asks for), and the CTAs per SM by their threads.
 struct KernelFacts {
     size_t shared = 0;
-    std::map<int, int> resident;
+    std::map<int, int> resident, clusters;
 };
 std::mutex g_facts_mutex;
 std::map<std::pair<int, const void *>, KernelFacts> g_facts;
@@ -199,6 +199,26 @@ int allow_shared_memory(const void *kernel, size_t bytes) {
     NB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     f.shared = bytes;
     return NB200_OK;
+}
+
+int resident_clusters(const void *kernel, int ctas, int threads, size_t bytes) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::lock_guard<std::mutex> g(g_facts_mutex);
+    auto [it, fresh] = g_facts[{dev, kernel}].clusters.try_emplace(ctas, 0);
+    if (!fresh) return it->second;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = bytes;
+    cudaLaunchAttribute size{};
+    size.id = cudaLaunchAttributeClusterDimension;
+    size.val.clusterDim.x = ctas, size.val.clusterDim.y = size.val.clusterDim.z = 1;
+    cfg.attrs = &size, cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    return it->second = n;
 }
 
 int resident_ctas(const void *kernel, int threads) {

@@ -160,6 +160,11 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// The same for pairs in clusters of several: `ctas` has a bit for each CTA of the pair.
+__device__ __forceinline__ void mma_commit_pair(uint64_t *bar, uint32_t ctas) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)ctas) : "memory");
+}
+
 // ---- loads and stores of tiles -------------------------------------------------------------------
 
 __device__ __forceinline__ void ask_for_map(const CUtensorMap *matrix) { asm volatile("prefetch.tensormap [%0];" ::"l"(matrix) : "memory"); }
@@ -228,13 +233,24 @@ __device__ __forceinline__ void mbar_arrive_leader(uint64_t *bar) {
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// The same for ordinary stores to shared memory that matrix instructions of the leader read (behind fence_async_shared), and its other side.
-__device__ __forceinline__ void mbar_arrive_leader_release(uint64_t *bar) {
-    asm volatile(
-        "{\n\t.reg .b32 remote;\n\t"
-        "mapa.shared::cluster.u32 remote, %0, 0;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n\t}" ::"r"(smem_u32(bar))
-        : "memory");
+// The same at the cluster's CTA `rank`. RELEASE: for ordinary stores to shared memory that matrix instructions of that CTA read (behind
+// fence_async_shared; its other side is fence_cluster).
+template <bool RELEASE>
+__device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, int rank) {
+    if constexpr (RELEASE)
+        asm volatile(
+            "{\n\t.reg .b32 remote;\n\t"
+            "mapa.shared::cluster.u32 remote, %0, %1;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n\t}" ::"r"(smem_u32(bar)),
+            "r"(rank)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .b32 remote;\n\t"
+            "mapa.shared::cluster.u32 remote, %0, %1;\n\t"
+            "mbarrier.arrive.shared::cluster.b64 _, [remote];\n\t}" ::"r"(smem_u32(bar)),
+            "r"(rank)
+            : "memory");
 }
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 // All threads of all CTAs of the cluster meet.

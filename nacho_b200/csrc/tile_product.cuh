@@ -27,6 +27,7 @@ struct TileArgs {
     int across;  // WEIGHTS: columns of z
     int blocks;  // of 128 bytes along the summed axis (not WEIGHTS)
     int tile_n;  // TILE_N at most
+    int b_bytes, stages;  // of the narrow operand in a stage; stages
     int most;    // tiles, at most
     void *y;
     int64_t stride;
@@ -44,12 +45,13 @@ struct TileMaps {
 
 // What a CTA of a pair has in shared memory; tiles begin at 1024-byte boundaries.
 struct TileShared {
-    static constexpr int STAGES = 5, SUMS = 2;  // blocks under way; places for a tile's sums in tensor memory
-    uint8_t a[STAGES][128 * 128];               // 128 rows of the wide side (turned: two blocks of 64 by 64 of the summed axis)
-    uint8_t b[STAGES][128 * 128];               // half of the tile's narrow side
-    uint8_t out[2][24 * 1024];                  // tiles of 32 rows by 128 bytes on their way out, of four warps each
-    uint64_t full[STAGES], empty[STAGES];       // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
-    uint64_t sum_full[SUMS], sum_empty[SUMS];   // a tile's sums lie in tensor memory; they have been read
+    static constexpr int STAGES = 8, SUMS = 2;  // blocks under way, at most; places for a tile's sums in tensor memory
+    static constexpr int A_BYTES = 128 * 128;   // of a block: 128 rows of the wide side (turned: two blocks of 64 by 64 of the summed axis)
+    static constexpr int STAGE_BYTES = 160 * 1024;
+    uint8_t stage[STAGE_BYTES];            // of both operands' blocks, the wide one's first; `b_bytes` of the narrow one (half of the tile's narrow side)
+    uint8_t out[2][24 * 1024];             // tiles of 32 rows by 128 bytes on their way out, of four warps each
+    uint64_t full[STAGES], empty[STAGES];  // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
+    uint64_t sum_full[SUMS], sum_empty[SUMS];  // a tile's sums lie in tensor memory; they have been read
     uint64_t drained;
     uint32_t tmem;
     int failed;
@@ -205,7 +207,145 @@ __device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, in
     }
 }
 
-// Pairs of CTAs, one per SM, take tiles of 256 x 256 at most in turn. One warp brings blocks of 128 bytes of both operands into shared memory (the copy
+// What becomes of a tile's sums: 32 columns of the warp's 32 lanes at a time, as fragments (first of the upper, then of the lower 16 lanes; where results are
+// 32-bit, all of a thread's lane). Four warps, the ones that share half of the columns, store together.
+template <Sum SUM, Form FORM, typename T>
+struct Finish {
+    static constexpr bool GATED = FORM == Form::GATED, WIDE = std::is_same<T, float>::value;
+    const TileArgs &args;
+    const TileMaps &maps;
+    uint8_t *const out;
+    const int rank, lanes, half;
+    int turn = 0;
+    float col_scale[4] = {};
+
+    __device__ T *y() const { return static_cast<T *>(args.y); }
+
+    __device__ __forceinline__ void begin(const Place &t) {
+        if constexpr (SUM == Sum::S8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = t.col + rank * 128 + lanes * 32 + (WIDE ? lane_id() : lane_id() / 4 + 8 * i);
+                if (c < args.wide) col_scale[i] = ld_late(args.col_scale + (int64_t)t.g * args.wide + c);
+            }
+        }
+    }
+    __device__ __forceinline__ void value(const uint32_t (&v)[32], int first, float row_scale, float (&f)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (SUM == Sum::S8) f[i] = scaled((int)v[first + i], __shfl_sync(FULL_MASK, row_scale, i / 4 * 8 + (lane_id() & 3) * 2 + (i & 1)), col_scale[first / 8 + (i & 2) / 2]);
+            else f[i] = __uint_as_float(v[first + i]);
+        }
+    }
+
+    // GATED, ROWS: rows t.from + c .. of the result
+    __device__ __forceinline__ void rows(const Place &t, int c, const uint32_t (&v)[32]) {
+        const int lane = lane_id(), left = t.count - c, row = t.from + c;
+        float row_scale = 0.f;
+        if constexpr (SUM == Sum::S8) row_scale = lane < left ? ld_late(args.row_scale + row + lane) : 0.f;
+        if constexpr (WIDE) {
+            const int col = t.col + rank * 128 + lanes * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float f = SUM == Sum::S8 ? scaled((int)v[j], __shfl_sync(FULL_MASK, row_scale, j), col_scale[0]) : __uint_as_float(v[j]);
+                if (j < left && col < args.wide) y()[(int64_t)(row + j) * args.stride + col] = f;
+            }
+        } else {
+            constexpr int TILES = GATED ? 3 : 2;  // of 64 columns: of h, gates and values, or two of y
+            const int col = t.col + (GATED ? rank * 64 : rank * 128), wide = args.wide;
+            // behind the group's last row there is no other's row, or these 32 are all the group's
+            const bool whole = args.words && (left >= 32 || t.from + t.count == args.rows);
+            uint8_t *const place = out + turn * TILES * 4096;
+            turn ^= 1;
+            float lo[16], hi[16];
+            value(v, 0, row_scale, lo);
+            value(v, 16, row_scale, hi);
+            if (lanes == 0 && elected()) stores_read_but<1>();
+            half_sync(half);  // this place has been read
+            if constexpr (GATED) {
+                if (args.both) {
+                    put_columns<T>(place + 4096, lanes * 2, lo);
+                    put_columns<T>(place + 2 * 4096, lanes * 2, hi);
+                }
+                float h[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) h[i] = lo[i] * logistic(act_inner(lo[i], args.gelu)) * hi[i];
+                put_columns<T>(place, lanes * 2, h);
+            } else {
+                put_columns<T>(place + (lanes >> 1) * 4096, (lanes & 1) * 4, lo);
+                put_columns<T>(place + (lanes >> 1) * 4096, (lanes & 1) * 4 + 2, hi);
+            }
+            if (whole) fence_async_shared();
+            half_sync(half);
+            if (whole) {
+                if (lanes == 0 && col < wide && elected()) {
+                    store_tile3(&maps.y, place, col, row, 0);
+                    if constexpr (GATED) {
+                        if (args.both) store_tile3(&maps.both, place + 4096, col, 0, row), store_tile3(&maps.both, place + 2 * 4096, col, 1, row);
+                    } else {
+                        if (col + 64 < wide) store_tile3(&maps.y, place + 4096, col + 64, row, 0);
+                    }
+                }
+            } else {
+                const int count = min(32, left);
+                T *const to = y() + (int64_t)row * args.stride + col;
+                flush<4>(place, args.words, to, args.stride, lanes, count, wide - col);
+                if constexpr (GATED) {
+                    if (args.both) {
+                        T *const both = static_cast<T *>(args.both) + (int64_t)row * 2 * wide + col;
+                        flush<4>(place + 4096, args.words, both, 2 * (int64_t)wide, lanes, count, wide - col);
+                        flush<4>(place + 2 * 4096, args.words, both + wide, 2 * (int64_t)wide, lanes, count, wide - col);
+                    }
+                } else {
+                    flush<4>(place + 4096, args.words, to + 64, args.stride, lanes, count, wide - col - 64);
+                }
+            }
+            if (lanes == 0 && elected()) close_stores();  // an empty group where the warps have written themselves
+        }
+    }
+
+    // WEIGHTS: columns t.from + c .. of 32 rows, 64 of them in two parts
+    __device__ __forceinline__ void columns(const Place &t, int c, const uint32_t (&v)[2][32]) {
+        const int row = t.col + rank * 128 + lanes * 32;
+        uint8_t *const place = out + lanes * 6144;
+        if (args.words && elected()) stores_read_but<0>();
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float lo[16], hi[16];
+            value(v[i], 0, 0.f, lo);
+            value(v[i], 16, 0.f, hi);
+            put_lanes<T>(place, 0, 4 * i, lo);
+            put_lanes<T>(place, 16, 4 * i, hi);
+        }
+        if (args.words) {
+            fence_async_shared();
+            __syncwarp();
+            if (row < args.wide && elected()) store_tile3(&maps.y, place, t.from + c, row, t.g), close_stores();
+        } else {
+            __syncwarp();
+            flush<1>(place, false, y() + ((int64_t)t.g * args.wide + row) * args.stride + t.from + c, args.stride, 0, min(32, args.wide - row), t.count - c);
+            __syncwarp();
+        }
+    }
+
+    __device__ __forceinline__ void end() {
+        if (args.words && elected()) stores_done();
+        __syncwarp();
+    }
+};
+
+// Which of `all` places is next, and in which phase of its barriers.
+struct Stages {
+    int all, at = 0;
+    uint32_t phase = 0;
+    __device__ explicit Stages(int n) : all(n) {}
+    __device__ void next() {
+        if (++at == all) at = 0, phase ^= 1;
+    }
+};
+
+// Pairs of CTAs, one CTA per SM, take tiles of 256 x 256 at most in turn. One warp brings blocks of 128 bytes of both operands into shared memory (the copy
 // engine's tiled form, which turns them as the tensor cores take them and fills up with zeros what lies beyond a matrix), one issues the matrix instructions, and
 // eight read the sums of a whole tile while those of the next one are made: tensor memory holds two.
 //
@@ -213,20 +353,23 @@ __device__ __forceinline__ void flush(const uint8_t *tile, bool words, T *to, in
 // of both land in the same thread.
 // WEIGHTS: the last block of a group's tokens runs into the next group's. Steps of 16 tokens that are not the group's are left out, and in the last step the rows
 // behind its last token are cleared in shared memory.
-template <Sum SUM, Form FORM, bool A_TURNED, typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, const __grid_constant__ TileMaps maps) {
-    constexpr int STAGES = TileShared::STAGES, SUMS = TileShared::SUMS;
-    constexpr bool B_TURNED = FORM == Form::WEIGHTS, GATED = FORM == Form::GATED;
-    constexpr int PER_BLOCK = SUM == Sum::S8 ? 128 : 64;
+// SPLIT: where there are tiles for a part of the SMs only, the pairs of a cluster have a part of a tile's blocks each and add up their sums, in order, through
+// one another's shared memory.
+template <Sum SUM, Form FORM, bool A_TURNED, bool SPLIT, typename T>
+__global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, const __grid_constant__ TileMaps maps) {
+    constexpr int SUMS = TileShared::SUMS;
+    constexpr bool B_TURNED = FORM == Form::WEIGHTS, GATED = FORM == Form::GATED, WIDE = std::is_same<T, float>::value;
+    constexpr int PER_BLOCK = SUM == Sum::S8 ? 128 : 64, UNIT = FORM == Form::WEIGHTS ? 64 : 32;  // elements of a block; columns that are finished at once
     extern __shared__ uint8_t raw[];
     TileShared &sh = *reinterpret_cast<TileShared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    const int warp = warp_id(), lane = lane_id(), rank = (int)cluster_rank();
+    const int warp = warp_id(), lane = lane_id(), cta = (int)cluster_rank(), rank = cta & 1, leader = cta & ~1, part = cta >> 1, parts = SPLIT ? (int)cluster_size() / 2 : 1;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(&sh.full[s], rank == 0 ? 2 : 1), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < args.stages; ++s) mbar_init(&sh.full[s], rank == 0 ? 2 : 1), mbar_init(&sh.empty[s], 1);
         for (int s = 0; s < SUMS; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], TILE_STORE_WARPS * 2);
         mbar_init(&sh.drained, 1);
         mbar_fence_init();
         sh.failed = 0;
+        ask_for_map(&maps.wide), ask_for_map(&maps.narrow);
     }
     if (warp == TILE_STORE_WARPS) tmem_alloc<true>(&sh.tmem, 512);
     tmem_fence_before();
@@ -235,198 +378,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
     tmem_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     volatile int *failed = &sh.failed;
-    if (threadIdx.x == 0) ask_for_map(&maps.wide), ask_for_map(&maps.narrow);
     trigger_dependents();
     wait_for_previous();
 
-    Turns at(blockIdx.x / 2, gridDim.x / 2);
+    Turns turns((int)blockIdx.x / (2 * parts), (int)gridDim.x / (2 * parts));
     TileWalk<FORM> walk(args);
     Place t{};
-    // Columns of N that the tile's matrix instructions have, and those that this CTA brings.
+    const int stage_bytes = TileShared::A_BYTES + args.b_bytes;
+    auto stage_a = [&](int s) { return sh.stage + s * stage_bytes; };
+    auto stage_b = [&](int s) { return sh.stage + s * stage_bytes + TileShared::A_BYTES; };
+    // Columns of N that the tile's matrix instructions have, half of which each CTA of the pair brings; the pair's part of the blocks.
     auto narrow = [&] { return (t.count + TILE_STEP - 1) / TILE_STEP * TILE_STEP; };
+    auto first_block = [&] { return SPLIT ? (int)((int64_t)t.blocks * part / parts) : 0; };
+    auto end_block = [&] { return SPLIT ? (int)((int64_t)t.blocks * (part + 1) / parts) : t.blocks; };
     // The last block of a group's tokens has `rows` of them: what follows up to the next 16 is cleared in this CTA's halves of both operands.
     auto clear_tail = [&](int stage, int n, int rows) {
         const int stop = (rows + 15) / 16 * 16, chunks = (n / 2 + 63) / 64;
         for (int r = rows + lane / 8; r < stop; r += 4) {
             const int at = r * 128 + (lane & 7) * 16;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4 *>(sh.a[stage] + i * 8192 + at) = make_uint4(0, 0, 0, 0);
-            for (int i = 0; i < chunks; ++i) *reinterpret_cast<uint4 *>(sh.b[stage] + i * 8192 + at) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4 *>(stage_a(stage) + i * 8192 + at) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < chunks; ++i) *reinterpret_cast<uint4 *>(stage_b(stage) + i * 8192 + at) = make_uint4(0, 0, 0, 0);
         }
         fence_async_shared();
         __syncwarp();
     };
+    const int lanes = warp & 3, half = warp >> 2;
+    Finish<SUM, FORM, T> finish{args, maps, sh.out[half & 1], rank, lanes, half};
+    bool fine = true;
     if (warp < TILE_STORE_WARPS) {
-        const int lanes = warp & 3, half = warp >> 2;
         Ring<SUMS> sums;
-        T *const y = static_cast<T *>(args.y);
-        uint8_t *const out = sh.out[half];
-        int turn = 0;
-        bool fine = true;
-        for (; walk.find(at.tile(), t); at.next()) {
+        for (; walk.find(turns.tile(), t); turns.next()) {
             const int n = narrow();
-            if (t.blocks) {
+            const bool any = end_block() > first_block();
+            if (any) {
                 fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed);
                 tmem_fence_after();
             }
-            if (!half_all(half, fine)) break;  // nobody waits for a warp that has given up
+            if (!half_all(half, fine)) {  // nobody waits for a warp that has given up
+                fine = false;
+                break;
+            }
             const uint32_t base = tmem + ((uint32_t)(lanes * 32) << 16) + sums.at * TILE_N;
-            // 32 columns of this warp's lanes; behind the last ones the tile's place is free again
-            auto read = [&](int c, bool last, float (&lo)[16], float (&hi)[16], const float (&col_scale)[4], float row_scale) {
-                uint32_t v[2][16] = {};
-                if (t.blocks) {
-                    tmem_load_fragments(base + c, v[0]);
-                    tmem_load_fragments(base + c + (16u << 16), v[1]);
-                    tmem_wait_loads(v[0]);
-                    tmem_wait_loads(v[1]);
-                    if (last) {
-                        tmem_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
-                    }
-                }
+            auto load = [&](int c, uint32_t (&v)[32]) {
+                if (!any || c >= n) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if constexpr (SUM == Sum::S8) {
-                        const float s = __shfl_sync(FULL_MASK, row_scale, i / 4 * 8 + (lane & 3) * 2 + (i & 1));
-                        lo[i] = scaled((int)v[0][i], s, col_scale[(i & 2) / 2]);
-                        hi[i] = scaled((int)v[1][i], s, col_scale[2 + (i & 2) / 2]);
-                    } else {
-                        lo[i] = __uint_as_float(v[0][i]), hi[i] = __uint_as_float(v[1][i]);
-                    }
-                }
-            };
-            float lo[16], hi[16], col_scale[4] = {};
-            if constexpr (FORM == Form::WEIGHTS) {
-                // A warp has 32 rows of z and 64 of every 128 columns.
-                const int row = t.col + rank * 128 + lanes * 32;
-                uint8_t *const place = out + lanes * 6144;
-                bool read_some = false;
-                for (int c = half * 64; c < n; c += 128) {
-                    const bool last = c + 128 >= n;
-                    read_some = true;
-                    if (args.words && elected()) stores_read_but<0>();
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (c + 32 * i < n) read(c + 32 * i, last && (i == 1 || c + 32 >= n), lo, hi, col_scale, 0.f);
-                        put_lanes<T>(place, 0, 4 * i, lo);
-                        put_lanes<T>(place, 16, 4 * i, hi);
-                    }
-                    if (args.words) {
-                        fence_async_shared();
-                        __syncwarp();
-                        if (row < args.wide && elected()) store_tile3(&maps.y, place, t.from + c, row, t.g), close_stores();
-                    } else {
-                        __syncwarp();
-                        flush<1>(place, false, y + ((int64_t)t.g * args.wide + row) * args.stride + t.from + c, args.stride, 0, min(32, args.wide - row), t.count - c);
-                        __syncwarp();
-                    }
-                }
-                if (!read_some && t.blocks) {  // a narrow tile is the other half's
-                    tmem_fence_before();
-                    if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
-                }
-            } else if constexpr (std::is_same<T, float>::value) {
-                const int col = t.col + rank * 128 + lanes * 32 + lane;
-                if (SUM == Sum::S8 && col < args.wide) col_scale[0] = ld_late(args.col_scale + (int64_t)t.g * args.wide + col);
-                bool read_some = false;
-                for (int c = half * 32; c < n; c += 64) {
-                    read_some = true;
-                    const int left = t.count - c;
-                    const float row_scale = SUM == Sum::S8 && lane < left ? ld_late(args.row_scale + t.from + c + lane) : 0.f;
-                    uint32_t v[32];
+                    for (int i = 0; i < 32; ++i) v[i] = 0;
+                } else if constexpr (WIDE) {
                     tmem_load(base + c, v);
                     tmem_wait_loads(v);
-                    if (c + 64 >= n) {
-                        tmem_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
-                    }
+                } else {
+                    uint32_t lo[16], hi[16];
+                    tmem_load_fragments(base + c, lo);
+                    tmem_load_fragments(base + c + (16u << 16), hi);
+                    tmem_wait_loads(lo);
+                    tmem_wait_loads(hi);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float f = SUM == Sum::S8 ? scaled((int)v[j], __shfl_sync(FULL_MASK, row_scale, j), col_scale[0]) : __uint_as_float(v[j]);
-                        if (j < left && col < args.wide) y[(int64_t)(t.from + c + j) * args.stride + col] = f;
-                    }
+                    for (int i = 0; i < 16; ++i) v[i] = lo[i], v[16 + i] = hi[i];
                 }
-                if (!read_some) {
-                    tmem_fence_before();
-                    if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
-                }
-            } else {
-                // The four warps of a half have 32 of every 64 rows of the result, by tiles of 64 columns: of h, gates and values, or two of y.
-                constexpr int TILES = GATED ? 3 : 2;
-                const int col = t.col + (GATED ? rank * 64 : rank * 128);
-                if constexpr (SUM == Sum::S8) {
+            };
+            auto all_read = [&] {  // the tile's place is free again, as far as this warp goes
+                if (!any) return;
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at<false>(&sh.sum_empty[sums.at], leader);
+            };
+            if (!SPLIT) finish.begin(t);
+            for (int c = half * UNIT; c < n; c += 2 * UNIT) {
+                uint32_t v[UNIT / 32][32];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = col + lanes * 32 + lane / 4 + 8 * i;
-                        if (c < args.wide) col_scale[i] = ld_late(args.col_scale + (int64_t)t.g * args.wide + c);
-                    }
-                }
-                bool read_some = false;
-                for (int c = half * 32; c < n; c += 64, turn ^= 1) {
-                    read_some = true;
-                    const int left = t.count - c, row = t.from + c;
-                    // behind the group's last row there is no other's row, or these 32 are all the group's
-                    const bool whole = args.words && (left >= 32 || t.from + t.count == args.rows);
-                    uint8_t *const place = out + turn * TILES * 4096;
-                    float row_scale = 0.f;
-                    if constexpr (SUM == Sum::S8) row_scale = lane < left ? ld_late(args.row_scale + row + lane) : 0.f;
-                    read(c, c + 64 >= n, lo, hi, col_scale, row_scale);
-                    if (lanes == 0 && elected()) stores_read_but<1>();
-                    half_sync(half);  // this place has been read
-                    if constexpr (GATED) {
-                        if (args.both) {
-                            put_columns<T>(place + 4096, lanes * 2, lo);
-                            put_columns<T>(place + 2 * 4096, lanes * 2, hi);
-                        }
-                        float h[16];
+                for (int i = 0; i < UNIT / 32; ++i) load(c + 32 * i, v[i]);
+                if constexpr (SPLIT) {
+                    // behind the last matrix instruction the stages are free
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) h[i] = lo[i] * logistic(act_inner(lo[i], args.gelu)) * hi[i];
-                        put_columns<T>(place, lanes * 2, h);
-                    } else {
-                        put_columns<T>(place + (lanes >> 1) * 4096, (lanes & 1) * 4, lo);
-                        put_columns<T>(place + (lanes >> 1) * 4096, (lanes & 1) * 4 + 2, hi);
-                    }
-                    if (whole) fence_async_shared();
-                    half_sync(half);
-                    if (whole) {
-                        if (lanes == 0 && col < args.wide && elected()) {
-                            if constexpr (GATED) {
-                                store_tile3(&maps.y, place, col, row, 0);
-                                if (args.both) store_tile3(&maps.both, place + 4096, col, 0, row), store_tile3(&maps.both, place + 2 * 4096, col, 1, row);
-                            } else {
-                                store_tile3(&maps.y, place, col, row, 0);
-                                if (col + 64 < args.wide) store_tile3(&maps.y, place + 4096, col + 64, row, 0);
-                            }
-                        }
-                    } else {
-                        const int rows = min(32, left), wide = args.wide;
-                        flush<4>(place, args.words, y + (int64_t)row * args.stride + col, args.stride, lanes, rows, wide - col);
-                        if constexpr (GATED) {
-                            if (args.both) {
-                                T *const both = static_cast<T *>(args.both) + (int64_t)row * 2 * wide + col;
-                                flush<4>(place + 4096, args.words, both, 2 * (int64_t)wide, lanes, rows, wide - col);
-                                flush<4>(place + 2 * 4096, args.words, both + wide, 2 * (int64_t)wide, lanes, rows, wide - col);
-                            }
-                        } else {
-                            flush<4>(place + 4096, args.words, y + (int64_t)row * args.stride + col + 64, args.stride, lanes, rows, wide - col - 64);
-                        }
-                    }
-                    if (lanes == 0 && elected()) close_stores();  // an empty group where the warps have written themselves
-                }
-                if (!read_some && t.blocks) {  // 32 rows are the other half's
-                    tmem_fence_before();
-                    if (lane == 0) mbar_arrive_leader(&sh.sum_empty[sums.at]);
+                    for (int i = 0; i < UNIT / 32; ++i)
+                        if (c + 32 * i < n)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) reinterpret_cast<uint32_t *>(sh.stage)[((c / 32 + i) * 4 + lanes) * 1024 + k * 32 + lane] = v[i][k];
+                } else {
+                    if (c + 2 * UNIT >= n) all_read();
+                    if constexpr (FORM == Form::WEIGHTS) finish.columns(t, c, v);
+                    else finish.rows(t, c, v[0]);
                 }
             }
-            if (t.blocks) sums.next();
+            if (SPLIT) break;  // one tile per cluster
+            if (half * UNIT >= n) all_read();  // a narrow tile is the other half's
+            if (any) sums.next();
         }
-        if (args.words && elected()) stores_done();
-        __syncwarp();
+        if (!SPLIT) finish.end();
         // rows of no group
         if (FORM != Form::WEIGHTS && args.offsets) {
+            T *const y = static_cast<T *>(args.y);
             const int64_t rows = args.rows, lo = min(max((int64_t)ld_late(args.offsets), (int64_t)0), rows), hi = min(max((int64_t)ld_late(args.offsets + args.groups), lo), rows);
             for (int64_t r = blockIdx.x * TILE_STORE_WARPS + warp; r < rows; r += (int64_t)gridDim.x * TILE_STORE_WARPS) {
                 if (r >= lo && r < hi) continue;
@@ -436,20 +478,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
             }
         }
     } else {
-        Ring<STAGES> stage;
-        bool fine = true;
+        Stages stage(args.stages);
         if (warp == TILE_STORE_WARPS + 1) {  // copies
-            for (; fine && walk.find(at.tile(), t); at.next()) {
+            for (; fine && walk.find(turns.tile(), t); turns.next()) {
                 const int n = narrow(), mine = n / 2;
-                const uint32_t bytes = 128 * 128 + (B_TURNED ? (mine + 63) / 64 * 8192 : (mine + 31) / 32 * 4096);
-                const int begin = t.from + rank * mine;
-                for (int b = 0; b < t.blocks; ++b, stage.next()) {
+                const uint32_t bytes = TileShared::A_BYTES + (B_TURNED ? (mine + 63) / 64 * 8192 : (mine + 31) / 32 * 4096);
+                const int begin = t.from + rank * mine, end = end_block();
+                for (int b = first_block(); b < end; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
                     if (elected()) {
                         uint64_t *const bar = &sh.full[stage.at];
                         mbar_arrive_expect_tx(bar, bytes);
                         const int k = FORM == Form::WEIGHTS ? t.first + b * 64 : b * PER_BLOCK;
-                        uint8_t *const to_a = sh.a[stage.at], *const to_b = sh.b[stage.at];
+                        uint8_t *const to_a = stage_a(stage.at), *const to_b = stage_b(stage.at);
                         if constexpr (GATED) {
                             const int col = t.col + rank * 64;
 #pragma unroll
@@ -474,16 +515,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                 }
             }
             if (!fine)  // nothing may land in shared memory that is no longer this CTA's
-                for (int s = 0; s < STAGES; ++s) drain(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1);
+                for (int s = 0; s < args.stages; ++s) drain(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1);
         } else if (rank == 0) {  // matrix instructions
-            const uint64_t tile_a = A_TURNED ? turned_descriptor(smem_u32(sh.a[0])) : tile_descriptor(smem_u32(sh.a[0]));
-            const uint64_t tile_b = B_TURNED ? turned_descriptor(smem_u32(sh.b[0])) : tile_descriptor(smem_u32(sh.b[0]));
+            const uint64_t tile_a = A_TURNED ? turned_descriptor(smem_u32(stage_a(0))) : tile_descriptor(smem_u32(stage_a(0)));
+            const uint64_t tile_b = B_TURNED ? turned_descriptor(smem_u32(stage_b(0))) : tile_descriptor(smem_u32(stage_b(0)));
+            const uint32_t both = 3u << leader;
             Ring<SUMS> sums;
-            for (; fine && walk.find(at.tile(), t); at.next()) {
-                const int n = narrow();
+            for (; fine && walk.find(turns.tile(), t); turns.next()) {
+                const int n = narrow(), begin = first_block(), end = end_block();
                 const uint32_t shape = sum_descriptor<SUM>(A_TURNED, B_TURNED, TILE_M) | (uint32_t)(n >> 3) << 17;
-                if (t.blocks && !(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
-                for (int b = 0; b < t.blocks; ++b, stage.next()) {
+                if (begin == end) continue;
+                if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                for (int b = begin; b < end; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
                     if (rows < 64 && rows % 16) {
@@ -492,38 +535,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1) k_t
                     }
                     tmem_fence_after();
                     if (elected()) {
-                        const uint64_t da = tile_a + (uint64_t)(stage.at * (128 * 128 >> 4)), db = tile_b + (uint64_t)(stage.at * (128 * 128 >> 4));
+                        const uint64_t da = tile_a + (uint64_t)(stage.at * (stage_bytes >> 4)), db = tile_b + (uint64_t)(stage.at * (stage_bytes >> 4));
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (FORM != Form::WEIGHTS || k * 16 < rows)
-                                mma_pair<SUM>(tmem + sums.at * TILE_N, da + (A_TURNED ? 128 : 2) * k, db + (B_TURNED ? 128 : 2) * k, shape, b > 0 || k > 0);
-                        mma_commit<true>(&sh.empty[stage.at]);
-                        if (b + 1 == t.blocks) mma_commit<true>(&sh.sum_full[sums.at]);
+                                mma_pair<SUM>(tmem + sums.at * TILE_N, da + (A_TURNED ? 128 : 2) * k, db + (B_TURNED ? 128 : 2) * k, shape, b > begin || k > 0);
+                        mma_commit_pair(&sh.empty[stage.at], both);
+                        if (b + 1 == end) mma_commit_pair(&sh.sum_full[sums.at], both);
                     }
                     __syncwarp();
                 }
-                if (t.blocks) sums.next();
+                sums.next();
             }
             if (!fine) {
-                if (elected()) mma_commit<true>(&sh.drained);
+                if (elected()) mma_commit_pair(&sh.drained, both);
                 __syncwarp();
                 drain(&sh.drained, 0);
             }
         } else {  // tells the leader of the copies that have landed here
-            for (; fine && walk.find(at.tile(), t); at.next()) {
-                const int n = narrow();
-                for (int b = 0; b < t.blocks; ++b, stage.next()) {
+            for (; fine && walk.find(turns.tile(), t); turns.next()) {
+                const int n = narrow(), end = end_block();
+                for (int b = first_block(); b < end; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
                     const bool tail = rows < 64 && rows % 16;
                     if (tail) clear_tail(stage.at, n, rows);
                     if (elected()) {
-                        if (tail) mbar_arrive_leader_release(&sh.full[stage.at]);
-                        else mbar_arrive_leader(&sh.full[stage.at]);
+                        if (tail) mbar_arrive_at<true>(&sh.full[stage.at], leader);
+                        else mbar_arrive_at<false>(&sh.full[stage.at], leader);
                     }
                     __syncwarp();
                 }
             }
+        }
+    }
+    if constexpr (SPLIT) {
+        cluster_sync();
+        if (warp < TILE_STORE_WARPS && half_all(half, fine && t.count > 0)) {
+            const int n = narrow();
+            finish.begin(t);
+            for (int c = (half + 2 * part) * UNIT; c < n; c += 2 * parts * UNIT) {
+                uint32_t v[UNIT / 32][32];
+#pragma unroll
+                for (int i = 0; i < UNIT / 32; ++i) {
+                    const uint32_t *const mine = reinterpret_cast<const uint32_t *>(sh.stage) + ((c / 32 + i) * 4 + lanes) * 1024 + lane;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[i][k] = 0;
+                    for (int p = 0; p < parts && c + 32 * i < n; ++p) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(load_remote(reinterpret_cast<const float *>(mine + k * 32), 2 * p + rank));
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[i][k] = SUM == Sum::S8 ? v[i][k] + w[k] : __float_as_uint(__uint_as_float(v[i][k]) + __uint_as_float(w[k]));
+                    }
+                }
+                if constexpr (FORM == Form::WEIGHTS) finish.columns(t, c, v);
+                else finish.rows(t, c, v[0]);
+            }
+            finish.end();
         }
     }
     tmem_fence_before();
@@ -585,12 +654,27 @@ int launch_tiles(const char *name, TileArgs args, const TileMaps &maps, cudaStre
                                                 : (args.rows / args.tile_n + (int64_t)args.groups) * wide;
     if (tiles > INT32_MAX / 64 || args.rows > INT32_MAX - 1024 || args.wide > INT32_MAX / 2 - 1024 || args.across > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     args.most = (int)tiles;
-    auto kernel = k_tiles<SUM, FORM, A_TURNED, T>;
-    if ((st = allow_shared(kernel, TILE_SHARED_BYTES))) return st;
-    const int64_t ctas = std::max<int64_t>(2, std::min<int64_t>(tiles * 2, sm_count() / 2 * 2));
-    LaunchScope scope(name, stream);
-    NB200_CUDA(launch_overlapped(kernel, dim3((unsigned)ctas), dim3(TILE_THREADS), TILE_SHARED_BYTES, stream, args, maps));
-    return NB200_OK;
+    args.b_bytes = FORM == Form::WEIGHTS ? (args.tile_n / 2 + 63) / 64 * 8192 : args.tile_n / 2 * 128;
+    args.stages = std::min(TileShared::STAGES, TileShared::STAGE_BYTES / (TileShared::A_BYTES + args.b_bytes));
+    // Pairs of CTAs that share a tile's blocks: as many as find room for all tiles at once, of at least eight blocks each. (A second round costs more than it
+    // gives: 16 tiles of 32 blocks take 19 us in four parts, of which the device holds fewer than 16, and 10 in two.)
+    const int64_t blocks = FORM == Form::WEIGHTS ? args.rows / args.groups / 64 : args.blocks;
+    auto split = k_tiles<SUM, FORM, A_TURNED, true, T>;
+    int parts = 4;
+    if (tiles * 4 <= sm_count() && blocks >= 16) {
+        if ((st = allow_shared(split, TILE_SHARED_BYTES))) return st;
+        while (parts > 1 && (blocks < 8 * parts || tiles > resident_clusters(reinterpret_cast<const void *>(split), 2 * parts, TILE_THREADS, TILE_SHARED_BYTES))) parts /= 2;
+    } else {
+        parts = 1;
+    }
+    const int64_t ctas = parts > 1 ? tiles * 2 * parts : std::max<int64_t>(2, std::min<int64_t>(tiles * 2, sm_count() / 2 * 2));
+    auto go = [&](auto kernel) -> int {
+        if ((st = allow_shared(kernel, TILE_SHARED_BYTES))) return st;
+        LaunchScope scope(name, stream);
+        NB200_CUDA(launch_overlapped_clusters(2 * parts, kernel, dim3((unsigned)ctas), dim3(TILE_THREADS), TILE_SHARED_BYTES, stream, args, maps));
+        return NB200_OK;
+    };
+    return parts > 1 ? go(split) : go(k_tiles<SUM, FORM, A_TURNED, false, T>);
 }
 
 }  // namespace nb200
