@@ -92,12 +92,13 @@ struct Mine {
             } else if constexpr (sizeof(Z) == 4) {
 #pragma unroll
                 for (int i = 0; i < V; i += 4)
-                    *reinterpret_cast<float4 *>(z + i) = make_float4(get(u, i) * factor, get(u, i + 1) * factor, get(u, i + 2) * factor, get(u, i + 3) * factor);
+                    __stcs(reinterpret_cast<float4 *>(z + i), make_float4(get(u, i) * factor, get(u, i + 1) * factor, get(u, i + 2) * factor, get(u, i + 3) * factor));
             } else {
                 Vec<uint32_t, V / 2> out;
 #pragma unroll
                 for (int i = 0; i < V; i += 2) out.v[i / 2] = pack2<Z>(get(u, i) * factor, get(u, i + 1) * factor);
-                *reinterpret_cast<Vec<uint32_t, V / 2> *>(z) = out;
+                if constexpr (V == 8) __stcs(reinterpret_cast<uint4 *>(z), make_uint4(out.v[0], out.v[1], out.v[2], out.v[3]));
+                else __stcs(reinterpret_cast<uint2 *>(z), make_uint2(out.v[0], out.v[1]));
             }
         }
     }

@@ -1,4 +1,4 @@
-// Products of few rows with large weights, whose bytes are all that such a product takes: 16 rows of weights (and for gated ones 16 more) per CTA, the summed
+// Products of few rows with large weights, whose bytes are all that such a product takes: up to 16 rows of weights (and for gated ones as many more) per CTA, the summed
 // axis shared by its eight warps. Weights go from memory into the registers of the matrix instructions (16 x 8, the legacy form: nothing here is
 // bound by their rate), without a stop in shared memory: with 16 bytes a thread, four threads have 64 bytes of a row, and which of a step's columns are called
 // first is the same for both operands.
@@ -18,6 +18,7 @@ struct FewArgs {
     const int32_t *offsets;
     int groups, rows;
     int wide;   // hidden, or columns of y
+    int each;   // columns of the result per CTA, at most 16
     int inner;  // elements of a row (padding counted where it holds zeros)
     void *y, *both;
     int64_t stride;
@@ -54,14 +55,14 @@ __device__ __forceinline__ uint4 load16(const E *row, int64_t c, int64_t inner) 
     }
 }
 
-// A CTA per group and 16 columns of the result; NB rows of the group in a turn over the weights.
+// A CTA per group and `each` columns of the result; NB rows of the group in a turn over the weights.
 template <Sum SUM, bool GATED, int NB, int V, typename T>
 __global__ void __launch_bounds__(FEW_NT, 2) k_few(const FewArgs args) {
     using E = std::conditional_t<SUM == Sum::S8, int8_t, std::conditional_t<SUM == Sum::F16, __half, __nv_bfloat16>>;
-    constexpr int R = GATED ? 2 : 1, Q = NB / 8, U = NB == 32 ? 2 : 4;
+    constexpr int R = GATED ? 2 : 1, Q = NB / 8, U = NB == 32 ? 2 : R == 1 && NB == 8 ? 8 : 4;
     constexpr int PER = 64 / (int)sizeof(E), PIECE = PER / 4;  // elements of a row in a step, and a thread's
     __shared__ uint32_t part[FEW_WARPS][R][NB][17];
-    const int warp = warp_id(), lane = lane_id(), g = blockIdx.y, col = blockIdx.x * 16;
+    const int warp = warp_id(), lane = lane_id(), g = blockIdx.y, col = blockIdx.x * args.each;
     trigger_dependents();
     wait_for_previous();
     const int lo = args.offsets ? min(max(ld_late(args.offsets + g), 0), args.rows) : 0;
@@ -74,11 +75,11 @@ __global__ void __launch_bounds__(FEW_NT, 2) k_few(const FewArgs args) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int c = col + lane / 4 + 8 * i;
-            there[r][i] = c < args.wide;
+            there[r][i] = c < args.wide && lane / 4 + 8 * i < args.each;
             w[r][i] = static_cast<const E *>(args.w) + (((int64_t)g * R + r) * args.wide + (there[r][i] ? c : 0)) * args.w_stride;
         }
     T *const y = static_cast<T *>(args.y);
-    for (int row0 = lo + (int)blockIdx.z * NB; row0 < hi; row0 += (int)gridDim.z * NB) {
+    for (int row0 = lo; row0 < hi; row0 += NB) {
         const int count = min(NB, hi - row0);
         uint32_t acc[R][Q][4] = {};
         for (int64_t c0 = (int64_t)warp * PER; c0 < args.inner; c0 += (int64_t)FEW_WARPS * PER * U) {
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) k_few(const FewArgs args) {
         __syncthreads();
         for (int i = threadIdx.x; i < count * 16; i += FEW_NT) {
             const int n = i / 16, c = i % 16;
-            if (col + c >= args.wide) continue;
+            if (c >= args.each || col + c >= args.wide) continue;
             const int64_t row = row0 + n;
             if constexpr (SUM == Sum::S8) {
                 int sum = 0;
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(FEW_NT, 2) k_few(const FewArgs args) {
     }
     if (args.offsets) {  // rows of no group
         const int64_t rows = args.rows, begin = min(max((int64_t)ld_late(args.offsets), (int64_t)0), rows), end = min(max((int64_t)ld_late(args.offsets + args.groups), begin), rows);
-        const int64_t cta = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, ctas = (int64_t)gridDim.x * gridDim.y * gridDim.z;
+        const int64_t cta = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, ctas = (int64_t)gridDim.x * gridDim.y;
         auto clear = [&](int64_t from, int64_t to) {
             for (int64_t r = from + cta; r < to; r += ctas) {
                 for (int64_t c = threadIdx.x; c < args.wide; c += FEW_NT) y[r * args.stride + c] = from_float<T>(0.f);
@@ -157,17 +158,36 @@ __global__ void __launch_bounds__(FEW_NT, 2) k_few(const FewArgs args) {
     }
 }
 
+// Whether so few rows go this way, by the rows of a group and the bytes of all weights, of elements of `size` bytes (us on a B200, out of device memory, this way and by tiles of the tensor
+// cores; 16-bit gated products, hidden x width):
+//   - with groups while eight rows are one turn over the weights for nearly all of them (64 experts of 1024 x 2048 with 4 rows 87 and 91, with 6 rows 122
+//     and 92); integers, of which a CTA has half the bytes, never (64 experts of 2048 x 2048 with 3 rows 79 and 47);
+//   - one group of up to 8 rows always (8192 x 8192 45 and 52); more rows, whose own bytes all CTAs read, while the weights are small (16 rows of 4096 x 4096 16 and
+//     18, of 8192 x 8192 60 and 52; 32 rows of 1500 x 1100 9 and 13, of 4096 x 4096 20 and 18).
+inline bool few_rows(int64_t rows, int64_t groups, int64_t bytes, int size) {
+    if (groups != 1) return size > 1 && rows <= 4 * groups;
+    return rows <= (bytes <= 24ll << 20 ? 32 : bytes <= 96ll << 20 ? 16 : 8);
+}
+
 template <Sum SUM, bool GATED, int V, typename T>
-int launch_few_rows(const char *name, const FewArgs &args, int64_t mean, cudaStream_t stream) {
+int launch_few_rows(const char *name, const FewArgs &args, cudaStream_t stream) {
     auto go = [&](auto rows) -> int {
         constexpr int NB = decltype(rows)::value;
-        const int64_t wide = ((int64_t)args.wide + 15) / 16, turns = args.groups == 1 ? std::min<int64_t>((args.rows + NB - 1) / NB, 65535) : 1;
+        // Two CTAs per SM are at work at once. Where there are few rounds of them, a CTA takes fewer than 16 columns so that all rounds are full: 4096 columns
+        // are 256 CTAs of 16, of which 108 SMs get two and 40 one, or 293 of 14.
+        const int64_t room = 2 * sm_count(), ctas = ((int64_t)args.wide + 15) / 16 * args.groups, rounds = (ctas + room - 1) / room;
+        FewArgs a = args;
+        a.each = 16;
+        if (rounds <= 4) {
+            const int64_t per = std::max<int64_t>(1, rounds * room / args.groups);
+            a.each = (int)std::min<int64_t>(16, (args.wide + per - 1) / per);
+        }
         LaunchScope scope(name, stream);
-        NB200_CUDA(launch_overlapped(k_few<SUM, GATED, NB, V, T>, dim3((unsigned)wide, (unsigned)args.groups, (unsigned)turns), dim3(FEW_NT), 0, stream, args));
+        NB200_CUDA(launch_overlapped(k_few<SUM, GATED, NB, V, T>, dim3((unsigned)((args.wide + a.each - 1) / a.each), (unsigned)args.groups), dim3(FEW_NT), 0, stream, a));
         return NB200_OK;
     };
-    if (mean <= 4) return go(std::integral_constant<int, 8>{});
-    if (mean <= 12) return go(std::integral_constant<int, 16>{});
+    if (args.groups != 1 || args.rows <= 8) return go(std::integral_constant<int, 8>{});
+    if (args.rows <= 16) return go(std::integral_constant<int, 16>{});
     return go(std::integral_constant<int, 32>{});
 }
 

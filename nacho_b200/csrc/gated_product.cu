@@ -107,15 +107,14 @@ int aligned(const nb200_dense &x, void *to_x, const nb200_dense &w, void *to_w, 
     });
 }
 
-// Few rows, whose products take the weights' bytes: they are read as they lie.
-bool few(const nb200_dense *x, int64_t groups) { return x->rows <= 32 * groups; }
+bool few(const nb200_dense *x, const nb200_dense *w, int64_t groups) { return few_rows(x->rows, groups, w->rows * w->cols * 2, 2); }
 
 struct ForwardScratch {
     uint8_t *x = nullptr, *w = nullptr;
     size_t bytes = 0;
 
     ForwardScratch(void *base, const nb200_dense *xx, const nb200_dense *ww, int64_t groups) {
-        if (few(xx, groups)) return;
+        if (few(xx, ww, groups)) return;
         Carver c(base);
         if (!tiles_readable(*xx, 1)) x = c.take<uint8_t>((size_t)(xx->rows * pitch_of(xx->cols)) * 2);
         if (!tiles_readable(*ww, groups)) w = c.take<uint8_t>((size_t)(ww->rows * pitch_of(ww->cols)) * 2);
@@ -170,13 +169,12 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
         return NB200_OK;
     }
     const bool gelu = activation == NB200_GELU;
-    if (few(x, groups)) {
-        const int64_t mean = (x->rows + groups - 1) / groups;
-        const FewArgs args{x->data, w->data, x->rows > 1 ? x->stride : x->cols, w->rows > 1 ? w->stride : w->cols, offsets, groups, (int)x->rows, (int)hidden, (int)x->cols, h->data,
+    if (few(x, w, groups)) {
+        const FewArgs args{x->data, w->data, x->rows > 1 ? x->stride : x->cols, w->rows > 1 ? w->stride : w->cols, offsets, groups, (int)x->rows, (int)hidden, 16, (int)x->cols, h->data,
                            both ? both->data : nullptr, h->rows > 1 ? h->stride : h->cols, nullptr, nullptr, gelu};
         return with_half(x->type, [&](auto e) {
             using T = decltype(e);
-            return with_vector<T>(word_bytes({x, w}), [&](auto v) { return launch_few_rows<sum_of<T>, true, decltype(v)::value, T>("gated_few", args, mean, stream); });
+            return with_vector<T>(word_bytes({x, w}), [&](auto v) { return launch_few_rows<sum_of<T>, true, decltype(v)::value, T>("gated_few", args, stream); });
         });
     }
     const ForwardScratch s(scratch, x, w, groups);

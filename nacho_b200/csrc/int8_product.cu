@@ -164,9 +164,9 @@ int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *
     }
     return with_type(y->type, [&](auto e) -> int {
         using T = decltype(e);
-        if (y->rows <= 32 * groups) {
-            const FewArgs args{a->values, w->values, pitch, pitch, offsets, w->groups, a->rows, w->rows, (int)pitch, y->data, nullptr, stride, a->scales, w->scales, false};
-            return launch_few_rows<Sum::S8, false, 16, T>("int8_few", args, (y->rows + groups - 1) / groups, stream);
+        if (few_rows(y->rows, groups, all_rows(w) * pitch, 1)) {
+            const FewArgs args{a->values, w->values, pitch, pitch, offsets, w->groups, a->rows, w->rows, 16, (int)pitch, y->data, nullptr, stride, a->scales, w->scales, false};
+            return launch_few_rows<Sum::S8, false, 16, T>("int8_few", args, stream);
         }
         TileMaps maps{};
         TileArgs args{};
