@@ -234,7 +234,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // The same at the cluster's CTA `rank`. RELEASE: for ordinary stores to shared memory that matrix instructions of that CTA read (behind
-// fence_async_shared; its other side is fence_cluster).
+// fence_async_shared; its other side is mbar_acquire_cluster).
 template <bool RELEASE>
 __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, int rank) {
     if constexpr (RELEASE)
@@ -252,7 +252,17 @@ __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, int rank) {
             "r"(rank)
             : "memory");
 }
-__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+// A phase of this CTA's barrier that is over, for what arrivals with RELEASE stand for.
+__device__ __forceinline__ void mbar_acquire_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+}
 // All threads of all CTAs of the cluster meet.
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");

@@ -17,7 +17,8 @@ namespace nb200 {
 
 enum class Form { GATED, ROWS, WEIGHTS };
 
-constexpr int TILE_STORE_WARPS = 8, TILE_THREADS = (TILE_STORE_WARPS + 2) * 32;
+constexpr int TILE_STORE_WARPS = 8, TILE_THREADS = (TILE_STORE_WARPS + 4) * 32;
+enum { TILE_MMA_WARP = TILE_STORE_WARPS, TILE_COPY_WARP, TILE_PLACE_WARP, TILE_TAIL_WARP };
 constexpr int TILE_M = 256, TILE_N = 256, TILE_STEP = 32, TILE_PANEL = 8;  // of a pair of CTAs; the narrow side comes in steps; row tiles that follow one another
 
 struct TileArgs {
@@ -43,27 +44,30 @@ struct TileMaps {
     CUtensorMap wide, narrow, y, both;
 };
 
+// A tile of the result: its group (-1: there are no more), where its rows begin and how many there are (for WEIGHTS: its columns), its first column (row), and the blocks that are summed.
+struct Place {
+    int g, from, count, col, blocks;
+    int first, last;  // WEIGHTS: the group's tokens
+};
+
 // What a CTA of a pair has in shared memory; tiles begin at 1024-byte boundaries.
 struct TileShared {
-    static constexpr int STAGES = 8, SUMS = 2;  // blocks under way, at most; places for a tile's sums in tensor memory
+    static constexpr int STAGES = 8, SUMS = 2, PLACES = 4;  // blocks under way, at most; places for a tile's sums in tensor memory; tiles known ahead
     static constexpr int A_BYTES = 128 * 128;   // of a block: 128 rows of the wide side (turned: two blocks of 64 by 64 of the summed axis)
     static constexpr int STAGE_BYTES = 160 * 1024;
     uint8_t stage[STAGE_BYTES];            // of both operands' blocks, the wide one's first; `b_bytes` of the narrow one (half of the tile's narrow side)
     uint8_t out[2][24 * 1024];             // tiles of 32 rows by 128 bytes on their way out, of four warps each
-    uint64_t full[STAGES], empty[STAGES];  // a stage's copies have landed (in the leader's: in both CTAs); its matrix instructions are done
+    uint64_t landed[STAGES];               // a stage's copies of this CTA have (the leader's report to `full` itself where nothing is to be cleared first)
+    uint64_t full[STAGES], empty[STAGES];  // the leader's: both CTAs' have; a stage's matrix instructions are done
     uint64_t sum_full[SUMS], sum_empty[SUMS];  // a tile's sums lie in tensor memory; they have been read
+    uint64_t place_full[PLACES], place_empty[PLACES];  // a tile's place is known; all warps know it
     uint64_t drained;
+    Place place[PLACES];
     uint32_t tmem;
     int failed;
 };
 constexpr size_t TILE_SHARED_BYTES = sizeof(TileShared) + 1024;
 static_assert(TILE_SHARED_BYTES <= 227 * 1024, "");
-
-// A tile of the result: its group, where its rows begin and how many there are (for WEIGHTS: its columns), its first column (row), and the blocks that are summed.
-struct Place {
-    int g, from, count, col, blocks;
-    int first, last;  // WEIGHTS: the group's tokens
-};
 
 // Where a tile lies, found by a whole warp: groups 32 at a time, whose tiles it counts. Tiles are asked for in rising order. `most`: as many as there
 // are with offsets that rise; others end there.
@@ -345,7 +349,8 @@ struct Stages {
     }
 };
 
-// Pairs of CTAs, one CTA per SM, take tiles of 256 x 256 at most in turn. One warp brings blocks of 128 bytes of both operands into shared memory (the copy
+// Pairs of CTAs, one CTA per SM, take tiles of 256 x 256 at most in turn. One warp finds out where they lie, some ahead of the others (half a dozen divisions and
+// the group's offsets: found by every warp for itself at the tile's beginning, the matrix instructions of short sums waited for it), one brings blocks of 128 bytes of both operands into shared memory (the copy
 // engine's tiled form, which turns them as the tensor cores take them and fills up with zeros what lies beyond a matrix), one issues the matrix instructions, and
 // eight read the sums of a whole tile while those of the next one are made: tensor memory holds two.
 //
@@ -364,14 +369,15 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     TileShared &sh = *reinterpret_cast<TileShared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = warp_id(), lane = lane_id(), cta = (int)cluster_rank(), rank = cta & 1, leader = cta & ~1, part = cta >> 1, parts = SPLIT ? (int)cluster_size() / 2 : 1;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < args.stages; ++s) mbar_init(&sh.full[s], rank == 0 ? 2 : 1), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < args.stages; ++s) mbar_init(&sh.landed[s], 1), mbar_init(&sh.full[s], 2), mbar_init(&sh.empty[s], 1);
         for (int s = 0; s < SUMS; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], TILE_STORE_WARPS * 2);
+        for (int s = 0; s < TileShared::PLACES; ++s) mbar_init(&sh.place_full[s], 1), mbar_init(&sh.place_empty[s], TILE_STORE_WARPS + 2 + (FORM == Form::WEIGHTS && rank == 0));
         mbar_init(&sh.drained, 1);
         mbar_fence_init();
         sh.failed = 0;
         ask_for_map(&maps.wide), ask_for_map(&maps.narrow);
     }
-    if (warp == TILE_STORE_WARPS) tmem_alloc<true>(&sh.tmem, 512);
+    if (warp == TILE_MMA_WARP) tmem_alloc<true>(&sh.tmem, 512);
     tmem_fence_before();
     __syncthreads();
     cluster_sync();  // nobody arrives at a barrier that is not there yet
@@ -381,9 +387,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     trigger_dependents();
     wait_for_previous();
 
-    Turns turns((int)blockIdx.x / (2 * parts), (int)gridDim.x / (2 * parts));
-    TileWalk<FORM> walk(args);
     Place t{};
+    Ring<TileShared::PLACES> places;
+    // The next tile, for a whole warp; false once a wait has given up.
+    auto next_place = [&] {
+        if (!wait_for(&sh.place_full[places.at], places.phase, failed)) return false;
+        t = sh.place[places.at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.place_empty[places.at]);
+        places.next();
+        return true;
+    };
     const int stage_bytes = TileShared::A_BYTES + args.b_bytes;
     auto stage_a = [&](int s) { return sh.stage + s * stage_bytes; };
     auto stage_b = [&](int s) { return sh.stage + s * stage_bytes + TileShared::A_BYTES; };
@@ -408,17 +422,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     bool fine = true;
     if (warp < TILE_STORE_WARPS) {
         Ring<SUMS> sums;
-        for (; walk.find(turns.tile(), t); turns.next()) {
+        for (;;) {
+            fine = next_place();
             const int n = narrow();
-            const bool any = end_block() > first_block();
+            const bool any = fine && t.g >= 0 && end_block() > first_block();
             if (any) {
                 fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed);
                 tmem_fence_after();
             }
-            if (!half_all(half, fine)) {  // nobody waits for a warp that has given up
-                fine = false;
-                break;
-            }
+            fine = half_all(half, fine);  // nobody waits for a warp that has given up
+            if (!fine || t.g < 0) break;
             const uint32_t base = tmem + ((uint32_t)(lanes * 32) << 16) + sums.at * TILE_N;
             auto load = [&](int c, uint32_t (&v)[32]) {
                 if (!any || c >= n) {
@@ -479,15 +492,29 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
         }
     } else {
         Stages stage(args.stages);
-        if (warp == TILE_STORE_WARPS + 1) {  // copies
-            for (; fine && walk.find(turns.tile(), t); turns.next()) {
+        uint64_t *const landed = FORM == Form::WEIGHTS || rank ? sh.landed : sh.full;
+        if (warp == TILE_PLACE_WARP) {
+            Turns turns((int)blockIdx.x / (2 * parts), (int)gridDim.x / (2 * parts));
+            TileWalk<FORM> walk(args);
+            for (bool more = true; more; turns.next(), places.next()) {
+                if (!wait_for(&sh.place_empty[places.at], places.phase ^ 1, failed)) break;
+                more = walk.find(turns.tile(), t);
+                if (!more) t.g = -1;
+                if (lane == 0) {
+                    sh.place[places.at] = t;
+                    mbar_arrive(&sh.place_full[places.at]);
+                }
+                __syncwarp();
+            }
+        } else if (warp == TILE_COPY_WARP) {
+            while ((fine = next_place()) && t.g >= 0) {
                 const int n = narrow(), mine = n / 2;
                 const uint32_t bytes = TileShared::A_BYTES + (B_TURNED ? (mine + 63) / 64 * 8192 : (mine + 31) / 32 * 4096);
                 const int begin = t.from + rank * mine, end = end_block();
                 for (int b = first_block(); b < end; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
                     if (elected()) {
-                        uint64_t *const bar = &sh.full[stage.at];
+                        uint64_t *const bar = &landed[stage.at];
                         mbar_arrive_expect_tx(bar, bytes);
                         const int k = FORM == Form::WEIGHTS ? t.first + b * 64 : b * PER_BLOCK;
                         uint8_t *const to_a = stage_a(stage.at), *const to_b = stage_b(stage.at);
@@ -513,15 +540,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                     }
                     __syncwarp();
                 }
+                if (!fine) break;
             }
             if (!fine)  // nothing may land in shared memory that is no longer this CTA's
-                for (int s = 0; s < args.stages; ++s) drain(&sh.full[s], s < stage.at ? stage.phase : stage.phase ^ 1);
-        } else if (rank == 0) {  // matrix instructions
+                for (int s = 0; s < args.stages; ++s) drain(&landed[s], s < stage.at ? stage.phase : stage.phase ^ 1);
+        } else if (warp == TILE_MMA_WARP && rank == 0) {
             const uint64_t tile_a = A_TURNED ? turned_descriptor(smem_u32(stage_a(0))) : tile_descriptor(smem_u32(stage_a(0)));
             const uint64_t tile_b = B_TURNED ? turned_descriptor(smem_u32(stage_b(0))) : tile_descriptor(smem_u32(stage_b(0)));
             const uint32_t both = 3u << leader;
             Ring<SUMS> sums;
-            for (; fine && walk.find(turns.tile(), t); turns.next()) {
+            while ((fine = next_place()) && t.g >= 0) {
                 const int n = narrow(), begin = first_block(), end = end_block();
                 const uint32_t shape = sum_descriptor<SUM>(A_TURNED, B_TURNED, TILE_M) | (uint32_t)(n >> 3) << 17;
                 if (begin == end) continue;
@@ -529,10 +557,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 for (int b = begin; b < end; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
                     const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
-                    if (rows < 64 && rows % 16) {
-                        clear_tail(stage.at, n, rows);
-                        fence_cluster();
-                    }
+                    if (rows < 64 && rows % 16) mbar_acquire_cluster(&sh.full[stage.at], stage.phase);  // the other CTA's warp has written there too
                     tmem_fence_after();
                     if (elected()) {
                         const uint64_t da = tile_a + (uint64_t)(stage.at * (stage_bytes >> 4)), db = tile_b + (uint64_t)(stage.at * (stage_bytes >> 4));
@@ -545,6 +570,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                     }
                     __syncwarp();
                 }
+                if (!fine) break;
                 sums.next();
             }
             if (!fine) {
@@ -552,11 +578,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 __syncwarp();
                 drain(&sh.drained, 0);
             }
-        } else {  // tells the leader of the copies that have landed here
-            for (; fine && walk.find(turns.tile(), t); turns.next()) {
+        } else if (warp == TILE_MMA_WARP || (FORM == Form::WEIGHTS && rank == 0)) {  // tells the leader's matrix instructions what has landed here
+            while ((fine = next_place()) && t.g >= 0) {
                 const int n = narrow(), end = end_block();
                 for (int b = first_block(); b < end; ++b, stage.next()) {
-                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (!(fine = wait_for(&sh.landed[stage.at], stage.phase, failed))) break;
                     const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
                     const bool tail = rows < 64 && rows % 16;
                     if (tail) clear_tail(stage.at, n, rows);
@@ -566,12 +592,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                     }
                     __syncwarp();
                 }
+                if (!fine) break;
             }
         }
     }
     if constexpr (SPLIT) {
         cluster_sync();
-        if (warp < TILE_STORE_WARPS && half_all(half, fine && t.count > 0)) {
+        if (warp < TILE_STORE_WARPS && half_all(half, fine && t.g >= 0)) {
             const int n = narrow();
             finish.begin(t);
             for (int c = (half + 2 * part) * UNIT; c < n; c += 2 * parts * UNIT) {
@@ -598,7 +625,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     tmem_fence_before();
     __syncthreads();
     cluster_sync();  // no arrival is on its way to a CTA that is gone
-    if (warp == TILE_STORE_WARPS) {
+    if (warp == TILE_MMA_WARP) {
         tmem_fence_after();
         tmem_free<true>(tmem, 512);
         if (lane == 0 && *failed) publish_result_word(args.report, 1, REPORT_OTHER | blockIdx.x);
