@@ -529,6 +529,9 @@ int nb200_selftest_levels_timeout(const nb200_csf3 *a, const nb200_csf3 *b, nb20
  * place, and the one after that works. y is 32-bit. */
 int nb200_selftest_product_timeout(const nb200_fp8 *a, const nb200_fp8 *w, nb200_dense *y, void *stream);
 
+/* The same for the kernel of gated products, their gradients and integer products of more than a few rows. */
+int nb200_selftest_tiles_timeout(const nb200_int8 *a, const nb200_int8 *w, nb200_dense *y, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

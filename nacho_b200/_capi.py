@@ -149,6 +149,7 @@ PROTOTYPES = {
     "nb200_int8_pack": (C.c_int, [C.c_void_p, C.c_void_p, _P(Int8Struct), C.c_void_p]),
     "nb200_int8_unpack": (C.c_int, [_P(Int8Struct), C.c_void_p, C.c_void_p]),
     "nb200_int8_product": (C.c_int, [_P(Int8Struct)] * 2 + [C.c_void_p, _P(DenseStruct), C.c_void_p]),
+    "nb200_selftest_tiles_timeout": (C.c_int, [_P(Int8Struct)] * 2 + [_P(DenseStruct), C.c_void_p]),
     "nb200_clip": (C.c_int, [_P(SpanStruct), C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "nb200_clip_scratch": (C.c_int64, [_P(SpanStruct), C.c_int64]),
     "nb200_selftest_product_timeout": (C.c_int, [_P(Fp8Struct)] * 2 + [_P(DenseStruct), C.c_void_p]),

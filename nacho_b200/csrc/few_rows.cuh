@@ -171,6 +171,8 @@ inline bool few_rows(int64_t rows, int64_t groups, int64_t bytes, int size) {
 
 template <Sum SUM, bool GATED, int V, typename T>
 int launch_few_rows(const char *name, const FewArgs &args, cudaStream_t stream) {
+    Workspace *ws = nullptr;
+    if (const int st = report_of(stream, &ws)) return st;  // an earlier product's: nothing here waits for anything
     auto go = [&](auto rows) -> int {
         constexpr int NB = decltype(rows)::value;
         // Two CTAs per SM are at work at once. Where there are few rounds of them, a CTA takes fewer than 16 columns so that all rounds are full: 4096 columns

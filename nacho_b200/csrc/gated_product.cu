@@ -18,8 +18,9 @@ struct Align {
     int64_t pitch;
 };
 template <typename T, int V>
-__global__ void __launch_bounds__(NT) k_align_rows(const Align a, const Align b, int first) {
-    wait_for_previous();
+__global__ void __launch_bounds__(NT) k_align_rows(const Align a, const Align b, int first, bool beside) {
+    // beside the kernel in front, which has waited for what is read here
+    if (!beside) wait_for_previous();
     trigger_dependents();
     const bool second = (int)blockIdx.x >= first;
     const Align &m = second ? b : a;
@@ -30,6 +31,7 @@ __global__ void __launch_bounds__(NT) k_align_rows(const Align a, const Align b,
         v.template load<V>(static_cast<const T *>(m.x) + r * m.stride, c, m.cols);
         *reinterpret_cast<uint4 *>(static_cast<T *>(m.z) + r * m.pitch + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
     }
+    if (beside) finish_after_previous();
 }
 
 // dboth = [dg du] from dh and [g u], rounded to 16 bits for the tensor cores: off by half a step of the type, as much as the gradients' own rounding.
@@ -82,7 +84,7 @@ template <typename T>
 constexpr Sum sum_of = std::is_same<T, __half>::value ? Sum::F16 : Sum::BF16;
 
 // Rows and weights as the copy engine reads them: as they are, or copied to where there is room.
-int aligned(const nb200_dense &x, void *to_x, const nb200_dense &w, void *to_w, nb200_dense *ax, nb200_dense *aw, cudaStream_t stream) {
+int aligned(const nb200_dense &x, void *to_x, const nb200_dense &w, void *to_w, nb200_dense *ax, nb200_dense *aw, bool beside, cudaStream_t stream) {
     *ax = x, *aw = w;
     Align copies[2] = {};
     int n = 0, word = 16;
@@ -101,7 +103,7 @@ int aligned(const nb200_dense &x, void *to_x, const nb200_dense &w, void *to_w, 
         using T = decltype(e);
         return with_vector<T>(word, [&](auto v) {
             LaunchScope scope("align_rows", stream);
-            NB200_CUDA(launch_overlapped(k_align_rows<T, decltype(v)::value>, dim3((unsigned)(ctas[0] + ctas[1])), dim3(NT), 0, stream, copies[0], copies[1], (int)ctas[0]));
+            NB200_CUDA(launch_overlapped(k_align_rows<T, decltype(v)::value>, dim3((unsigned)(ctas[0] + ctas[1])), dim3(NT), 0, stream, copies[0], copies[1], (int)ctas[0], beside));
             return (int)NB200_OK;
         });
     });
@@ -181,7 +183,7 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
     if (s.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0)) return NB200_E_BADARG;
     if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
     nb200_dense ax, aw;
-    if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, stream))) return st;
+    if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, false, stream))) return st;
     TileMaps maps{};
     TileArgs args{};
     if ((st = describe_rows(&maps.wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16)) ||
@@ -227,8 +229,6 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
     const GradScratch s(scratch, x, w, groups);
     if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0) return NB200_E_BADARG;
     if (scratch_bytes < (int64_t)s.bytes) return NB200_E_CAPACITY;
-    nb200_dense ax, aw;
-    if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, stream))) return st;
     const int64_t pitch = pitch_of(2 * hidden);
     const bool gelu = activation == NB200_GELU;
     // du begins `hidden` elements behind dg, and so does u behind g
@@ -245,6 +245,9 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
             return (int)NB200_OK;
         });
         if (st) return st;
+        // Copies for the copy engine are made beside that kernel, and the weights' gradient beside the other one: neither has anything from the kernel in front.
+        nb200_dense ax, aw;
+        if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, true, stream))) return st;
         TileMaps maps{};
         TileArgs args{};
         args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows;
@@ -256,6 +259,7 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
         args.y = dx->data, args.stride = dx->rows > 1 ? dx->stride : dx->cols;
         if ((st = launch_tiles<sum_of<T>, Form::ROWS, true, T>("gated_grad_x", args, maps, stream))) return st;
         // dw: both operands turned
+        args.beside = true;
         if ((st = describe_rows(&maps.wide, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 64)) ||
             (st = describe_rows(&maps.narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)) ||
             (st = describe_result(&maps.y, &args.words, map_type(type), *dw, groups)))

@@ -149,7 +149,7 @@ int nb200_int8_unpack(const nb200_int8 *a, float *z, void *stream_) {
     return NB200_OK;
 }
 
-int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *offsets, nb200_dense *y, void *stream_) {
+static int int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *offsets, nb200_dense *y, bool starve, void *stream_) {
     if (!int8_ok(a) || !int8_ok(w) || !dense_ok(y) || a->groups != 1 || a->cols != w->cols || y->rows != a->rows || y->cols != w->rows || (!offsets && w->groups != 1)) return NB200_E_BADARG;
     if (w->groups > NB200_MAX_EXPERTS || a->cols > NB200_MAX_INT8_COLUMNS || a->rows > INT32_MAX - 1024 || w->rows > INT32_MAX / 2 - 1024) return NB200_E_UNSUPPORTED;
     if (y->rows == 0 || y->cols == 0) return NB200_OK;
@@ -164,7 +164,7 @@ int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *
     }
     return with_type(y->type, [&](auto e) -> int {
         using T = decltype(e);
-        if (few_rows(y->rows, groups, all_rows(w) * pitch, 1)) {
+        if (!starve && few_rows(y->rows, groups, all_rows(w) * pitch, 1)) {
             const FewArgs args{a->values, w->values, pitch, pitch, offsets, w->groups, a->rows, w->rows, 16, (int)pitch, y->data, nullptr, stride, a->scales, w->scales, false};
             return launch_few_rows<Sum::S8, false, 16, T>("int8_few", args, stream);
         }
@@ -176,9 +176,14 @@ int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *
             return st;
         args.offsets = offsets, args.groups = w->groups, args.rows = a->rows, args.wide = w->rows, args.blocks = (int)((a->cols + 127) / 128);
         args.tile_n = tile_n_of(a->rows, groups, (w->rows + TILE_M - 1) / TILE_M);
+        args.starve = starve;
         args.y = y->data, args.stride = stride, args.row_scale = a->scales, args.col_scale = w->scales;
         return launch_tiles<Sum::S8, Form::ROWS, false, T>("int8_product", args, maps, stream);
     });
 }
+
+int nb200_int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t *offsets, nb200_dense *y, void *stream) { return int8_product(a, w, offsets, y, false, stream); }
+
+int nb200_selftest_tiles_timeout(const nb200_int8 *a, const nb200_int8 *w, nb200_dense *y, void *stream) { return int8_product(a, w, nullptr, y, true, stream); }
 
 }  // extern "C"

@@ -34,19 +34,22 @@ __device__ __forceinline__ uint64_t now_ns() {
     return t;
 }
 
-// For a whole warp; false for all of it once one of its threads, or another warp of the CTA, has given up.
-template <bool SELFTEST = false>
-__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed) {
+// For a whole warp; false for all of it once one of its threads, or another warp of the CTA, has given up after `patience` ns.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed, uint64_t patience) {
     uint64_t start = 0;
     for (int i = 1;; ++i) {
         if (__all_sync(FULL_MASK, mbar_try_wait(bar, parity))) return true;
         if (i % 64) continue;
         if (__any_sync(FULL_MASK, *failed)) return false;
         if (!start) start = now_ns();
-        if (__any_sync(FULL_MASK, now_ns() - start > (SELFTEST ? SHORT_PATIENCE : PATIENCE))) break;
+        if (__any_sync(FULL_MASK, now_ns() - start > patience)) break;
     }
     *failed = 1;
     return false;
+}
+template <bool SELFTEST = false>
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, volatile int *failed) {
+    return wait_for(bar, parity, failed, SELFTEST ? SHORT_PATIENCE : PATIENCE);
 }
 
 // After a give-up: what is still on its way lands first, or never will.

@@ -168,10 +168,17 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t *bar, uint32_t ctas) {
 // ---- loads and stores of tiles -------------------------------------------------------------------
 
 __device__ __forceinline__ void ask_for_map(const CUtensorMap *matrix) { asm volatile("prefetch.tensormap [%0];" ::"l"(matrix) : "memory"); }
-// A tile of rows of 128 bytes from the place (x, y) of matrix z, where nothing is below zero; what lies beyond the matrix comes as zeros.
-__device__ __forceinline__ void load_tile(void *smem, const CUtensorMap *matrix, int x, int y, int z, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem)), "l"(matrix), "r"(x), "r"(y),
-                 "r"(z), "r"(smem_u32(bar))
+// The place of this CTA's barrier in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t remote_barrier(const uint64_t *bar, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(bar)), "r"(rank));
+    return at;
+}
+// A tile of rows of 128 bytes from the place (x, y) of matrix z, where nothing is below zero; what lies beyond the matrix comes as zeros. It lands in this CTA; the
+// barrier that counts its bytes is one of the pair's, in either CTA.
+__device__ __forceinline__ void load_tile(void *smem, const CUtensorMap *matrix, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem)), "l"(matrix),
+                 "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
 

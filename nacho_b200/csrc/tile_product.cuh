@@ -36,7 +36,10 @@ struct TileArgs {
     const float *row_scale, *col_scale;  // S8: of the rows, of every group's columns
     bool gelu;
     bool words;  // results in words of 16 bytes, whole tiles by the copy engine
+    bool beside;  // nothing here depends on the kernel in front, which has itself waited for all that was before it: no wait but at the end
     unsigned long long *report;
+    uint64_t patience;
+    bool starve;  // a self-test: the first block's copies are left out
 };
 
 // The operands and the results as the copy engine sees them: boxes of rows of 128 bytes. Results: y [rows][columns], both [rows][2][hidden], z [group][rows][columns].
@@ -57,8 +60,8 @@ struct TileShared {
     static constexpr int STAGE_BYTES = 160 * 1024;
     uint8_t stage[STAGE_BYTES];            // of both operands' blocks, the wide one's first; `b_bytes` of the narrow one (half of the tile's narrow side)
     uint8_t out[2][24 * 1024];             // tiles of 32 rows by 128 bytes on their way out, of four warps each
-    uint64_t landed[STAGES];               // a stage's copies of this CTA have (the leader's report to `full` itself where nothing is to be cleared first)
-    uint64_t full[STAGES], empty[STAGES];  // the leader's: both CTAs' have; a stage's matrix instructions are done
+    uint64_t full[STAGES], empty[STAGES];  // the leader's: a stage's copies of both CTAs have landed; its matrix instructions are done
+    uint64_t landed[STAGES];               // this CTA's copies have, of a block whose tail is to be cleared
     uint64_t sum_full[SUMS], sum_empty[SUMS];  // a tile's sums lie in tensor memory; they have been read
     uint64_t place_full[PLACES], place_empty[PLACES];  // a tile's place is known; all warps know it
     uint64_t drained;
@@ -369,9 +372,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     TileShared &sh = *reinterpret_cast<TileShared *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = warp_id(), lane = lane_id(), cta = (int)cluster_rank(), rank = cta & 1, leader = cta & ~1, part = cta >> 1, parts = SPLIT ? (int)cluster_size() / 2 : 1;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < args.stages; ++s) mbar_init(&sh.landed[s], 1), mbar_init(&sh.full[s], 2), mbar_init(&sh.empty[s], 1);
+        for (int s = 0; s < args.stages; ++s) mbar_init(&sh.landed[s], 1), mbar_init(&sh.full[s], FORM == Form::WEIGHTS ? 2 : 1), mbar_init(&sh.empty[s], 1);
         for (int s = 0; s < SUMS; ++s) mbar_init(&sh.sum_full[s], 1), mbar_init(&sh.sum_empty[s], TILE_STORE_WARPS * 2);
-        for (int s = 0; s < TileShared::PLACES; ++s) mbar_init(&sh.place_full[s], 1), mbar_init(&sh.place_empty[s], TILE_STORE_WARPS + 2 + (FORM == Form::WEIGHTS && rank == 0));
+        for (int s = 0; s < TileShared::PLACES; ++s) mbar_init(&sh.place_full[s], 1), mbar_init(&sh.place_empty[s], TILE_STORE_WARPS + 1 + (rank == 0) + (FORM == Form::WEIGHTS));
         mbar_init(&sh.drained, 1);
         mbar_fence_init();
         sh.failed = 0;
@@ -384,14 +387,15 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     tmem_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     volatile int *failed = &sh.failed;
+    // In this order: what starts beside this kernel then finds everything complete that was in front of it.
+    if (!args.beside) wait_for_previous();
     trigger_dependents();
-    wait_for_previous();
 
     Place t{};
     Ring<TileShared::PLACES> places;
     // The next tile, for a whole warp; false once a wait has given up.
     auto next_place = [&] {
-        if (!wait_for(&sh.place_full[places.at], places.phase, failed)) return false;
+        if (!wait_for(&sh.place_full[places.at], places.phase, failed, args.patience)) return false;
         t = sh.place[places.at];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.place_empty[places.at]);
@@ -405,6 +409,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
     auto narrow = [&] { return (t.count + TILE_STEP - 1) / TILE_STEP * TILE_STEP; };
     auto first_block = [&] { return SPLIT ? (int)((int64_t)t.blocks * part / parts) : 0; };
     auto end_block = [&] { return SPLIT ? (int)((int64_t)t.blocks * (part + 1) / parts) : t.blocks; };
+    // Tokens of block b if it is a group's last one and its last step of 16 is not whole, else 0.
+    auto tail_rows = [&](int b) {
+        const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
+        return rows < 64 && rows % 16 ? rows : 0;
+    };
     // The last block of a group's tokens has `rows` of them: what follows up to the next 16 is cleared in this CTA's halves of both operands.
     auto clear_tail = [&](int stage, int n, int rows) {
         const int stop = (rows + 15) / 16 * 16, chunks = (n / 2 + 63) / 64;
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
             const int n = narrow();
             const bool any = fine && t.g >= 0 && end_block() > first_block();
             if (any) {
-                fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed);
+                fine = wait_for(&sh.sum_full[sums.at], sums.phase, failed, args.patience);
                 tmem_fence_after();
             }
             fine = half_all(half, fine);  // nobody waits for a warp that has given up
@@ -492,12 +501,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
         }
     } else {
         Stages stage(args.stages);
-        uint64_t *const landed = FORM == Form::WEIGHTS || rank ? sh.landed : sh.full;
         if (warp == TILE_PLACE_WARP) {
             Turns turns((int)blockIdx.x / (2 * parts), (int)gridDim.x / (2 * parts));
             TileWalk<FORM> walk(args);
             for (bool more = true; more; turns.next(), places.next()) {
-                if (!wait_for(&sh.place_empty[places.at], places.phase ^ 1, failed)) break;
+                if (!wait_for(&sh.place_empty[places.at], places.phase ^ 1, failed, args.patience)) break;
                 more = walk.find(turns.tile(), t);
                 if (!more) t.g = -1;
                 if (lane == 0) {
@@ -512,10 +520,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 const uint32_t bytes = TileShared::A_BYTES + (B_TURNED ? (mine + 63) / 64 * 8192 : (mine + 31) / 32 * 4096);
                 const int begin = t.from + rank * mine, end = end_block();
                 for (int b = first_block(); b < end; ++b, stage.next()) {
-                    if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed))) break;
-                    if (elected()) {
-                        uint64_t *const bar = &landed[stage.at];
-                        mbar_arrive_expect_tx(bar, bytes);
+                    if (!(fine = wait_for(&sh.empty[stage.at], stage.phase ^ 1, failed, args.patience))) break;
+                    if (elected() && !(args.starve && b == 0)) {
+                        // Both CTAs' copies report to the leader, which expects them; those of a block whose tail is to be cleared to their own CTA.
+                        const bool tail = tail_rows(b) > 0;
+                        const uint32_t bar = tail ? smem_u32(&sh.landed[stage.at]) : remote_barrier(&sh.full[stage.at], leader);
+                        if (tail) mbar_arrive_expect_tx(&sh.landed[stage.at], bytes);
+                        else if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage.at], 2 * bytes);
+                        if (FORM == Form::WEIGHTS && !tail && rank == 0) mbar_arrive(&sh.full[stage.at]);  // of two, for the two warps that clear tails
                         const int k = FORM == Form::WEIGHTS ? t.first + b * 64 : b * PER_BLOCK;
                         uint8_t *const to_a = stage_a(stage.at), *const to_b = stage_b(stage.at);
                         if constexpr (GATED) {
@@ -542,8 +554,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 }
                 if (!fine) break;
             }
-            if (!fine)  // nothing may land in shared memory that is no longer this CTA's
-                for (int s = 0; s < args.stages; ++s) drain(&landed[s], s < stage.at ? stage.phase : stage.phase ^ 1);
+            if (!fine)  // nothing may land in shared memory that is no longer this CTA's: what was to come until then has, or never will
+                for (const uint64_t start = now_ns(); now_ns() - start < SHORT_PATIENCE;) {}
         } else if (warp == TILE_MMA_WARP && rank == 0) {
             const uint64_t tile_a = A_TURNED ? turned_descriptor(smem_u32(stage_a(0))) : tile_descriptor(smem_u32(stage_a(0)));
             const uint64_t tile_b = B_TURNED ? turned_descriptor(smem_u32(stage_b(0))) : tile_descriptor(smem_u32(stage_b(0)));
@@ -553,11 +565,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 const int n = narrow(), begin = first_block(), end = end_block();
                 const uint32_t shape = sum_descriptor<SUM>(A_TURNED, B_TURNED, TILE_M) | (uint32_t)(n >> 3) << 17;
                 if (begin == end) continue;
-                if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed))) break;
+                if (!(fine = wait_for(&sh.sum_empty[sums.at], sums.phase ^ 1, failed, args.patience))) break;
                 for (int b = begin; b < end; ++b, stage.next()) {
-                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed))) break;
+                    if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed, args.patience))) break;
                     const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
-                    if (rows < 64 && rows % 16) mbar_acquire_cluster(&sh.full[stage.at], stage.phase);  // the other CTA's warp has written there too
+                    if (tail_rows(b)) mbar_acquire_cluster(&sh.full[stage.at], stage.phase);  // the other CTA's warp has written there too
                     tmem_fence_after();
                     if (elected()) {
                         const uint64_t da = tile_a + (uint64_t)(stage.at * (stage_bytes >> 4)), db = tile_b + (uint64_t)(stage.at * (stage_bytes >> 4));
@@ -578,18 +590,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 __syncwarp();
                 drain(&sh.drained, 0);
             }
-        } else if (warp == TILE_MMA_WARP || (FORM == Form::WEIGHTS && rank == 0)) {  // tells the leader's matrix instructions what has landed here
+        } else if (FORM == Form::WEIGHTS && warp == TILE_TAIL_WARP) {
+            uint32_t phases = 0;  // of the stages' `landed`
             while ((fine = next_place()) && t.g >= 0) {
-                const int n = narrow(), end = end_block();
-                for (int b = first_block(); b < end; ++b, stage.next()) {
-                    if (!(fine = wait_for(&sh.landed[stage.at], stage.phase, failed))) break;
-                    const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
-                    const bool tail = rows < 64 && rows % 16;
-                    if (tail) clear_tail(stage.at, n, rows);
-                    if (elected()) {
-                        if (tail) mbar_arrive_at<true>(&sh.full[stage.at], leader);
-                        else mbar_arrive_at<false>(&sh.full[stage.at], leader);
-                    }
+                const int n = narrow(), begin = first_block(), end = end_block();
+                for (int b = begin; b < end; ++b, stage.next()) {
+                    const int rows = tail_rows(b);
+                    if (!rows) continue;
+                    if (!(fine = wait_for(&sh.landed[stage.at], phases >> stage.at & 1, failed, args.patience))) break;
+                    phases ^= 1u << stage.at;
+                    clear_tail(stage.at, n, rows);
+                    if (elected()) mbar_arrive_at<true>(&sh.full[stage.at], leader);
                     __syncwarp();
                 }
                 if (!fine) break;
@@ -630,6 +641,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
         tmem_free<true>(tmem, 512);
         if (lane == 0 && *failed) publish_result_word(args.report, 1, REPORT_OTHER | blockIdx.x);
     }
+    if (args.beside) finish_after_previous();
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -681,6 +693,7 @@ int launch_tiles(const char *name, TileArgs args, const TileMaps &maps, cudaStre
                                                 : (args.rows / args.tile_n + (int64_t)args.groups) * wide;
     if (tiles > INT32_MAX / 64 || args.rows > INT32_MAX - 1024 || args.wide > INT32_MAX / 2 - 1024 || args.across > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     args.most = (int)tiles;
+    args.patience = args.starve ? SHORT_PATIENCE : PATIENCE;
     args.b_bytes = FORM == Form::WEIGHTS ? (args.tile_n / 2 + 63) / 64 * 8192 : args.tile_n / 2 * 128;
     args.stages = std::min(TileShared::STAGES, TileShared::STAGE_BYTES / (TileShared::A_BYTES + args.b_bytes));
     // Pairs of CTAs that share a tile's blocks: as many as find room for all tiles at once, of at least eight blocks each. (A second round costs more than it

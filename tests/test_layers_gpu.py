@@ -398,3 +398,244 @@ def test_clip_without_a_norm(bad):
     nacho().gpu_clip_gradients(tensors, 0.1, out)
     for t, k, z in zip(tensors, kept, out):
         assert torch.equal(t.nan_to_num(7.0), k.nan_to_num(7.0)) and torch.equal(z.nan_to_num(7.0), k.nan_to_num(7.0))
+
+
+# ---- all of them ------------------------------------------------------------------------------------
+
+
+def some_operands(rows=300, hidden=96, width=200, dtype=torch.bfloat16, seed=0):
+    return (normal((rows, width), dtype, seed), normal((2 * hidden, width), dtype, seed + 1, width ** -0.5), normal((rows, hidden), dtype, seed + 2),
+            normal((rows, 2 * hidden), dtype, seed + 3))
+
+
+def all_calls(x, w, dh, both, order=None):
+    """Every operator once, on the current stream; new tensors."""
+    n = nacho()
+    h, kept = n.gpu_gated_product(x, w, order, keep=True)
+    dx, dw = n.gpu_gated_product_grad(dh, both, x, w, order, activation="gelu")
+    few = n.gpu_gated_product(x[:5], w) if order is None else h
+    y = n.gpu_int8_product(n.to_int8_rows(x), n.to_int8_rows(w), order, dtype=torch.float32)
+    y1 = n.gpu_int8_product(n.to_int8_rows(x[:3]), n.to_int8_rows(w), dtype=torch.float16) if order is None else y
+    out = [torch.empty_like(dx), torch.empty(dw.shape, device="cuda")]
+    norm = n.gpu_clip_gradients([dx, dw], 0.5, out)
+    return [h, kept, dx, dw, few, y, y1, norm, *out]
+
+
+def equal(a, b):
+    return all(torch.equal(p.nan_to_num(3.0), q.nan_to_num(3.0)) for p, q in zip(a, b))
+
+
+def test_the_same_call_gives_the_same_bits():
+    operands = some_operands()
+    want = all_calls(*operands)
+    for _ in range(5):
+        assert equal(all_calls(*operands), want)
+
+
+def test_streams_of_their_own():
+    """Operands made on one stream, calls on two others at once, memory given back in between."""
+    operands = some_operands(rows=700)
+    want = all_calls(*operands)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for turn in range(6):
+        s = streams[turn % 2]
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            copies = [t.clone() for t in operands]
+            got.append(all_calls(*copies))
+            del copies
+    torch.cuda.synchronize()
+    assert all(equal(g, want) for g in got)
+
+
+def test_captured_calls():
+    """Two graphs, replayed beside one another and after other calls, on operands that have changed since."""
+    operands, others = some_operands(seed=0), some_operands(seed=10)
+    order, _ = order_of([100, 0, 150, 33], tail=17)
+    grouped = [normal((300, 200), torch.float16, 20), normal((4, 192, 200), torch.float16, 21, 0.1), normal((300, 96), torch.float16, 22), normal((300, 192), torch.float16, 23)]
+    held = [t.clone() for t in operands]
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        all_calls(*held)
+        all_calls(*grouped, order)
+    torch.cuda.synchronize()
+    graphs, results = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    with torch.cuda.graph(graphs[0], stream=stream):
+        results.append(all_calls(*held))
+    with torch.cuda.graph(graphs[1], stream=stream):
+        results.append(all_calls(*grouped, order))
+    want_grouped = all_calls(*grouped, order)
+    for given in (others, operands):
+        for h, t in zip(held, given):
+            h.copy_(t)
+        want = all_calls(*given)
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        assert equal(results[0], want) and equal(results[1], want_grouped)
+
+
+def test_a_layer_forwards_backwards_clipped_and_served():
+    """Tokens to their experts, the gated layer and its way down, back, gradients clipped, a step; then the layer served in integers. Against the same in 64 bits."""
+    n, dtype = nacho(), torch.bfloat16
+    tokens, experts, k, width, hidden = 200, 6, 2, 96, 80
+    g = torch.Generator(device="cuda").manual_seed(5)
+    expert = torch.topk(torch.rand(tokens, experts, generator=g, device="cuda"), k, dim=1).indices.flatten().int()
+    expert[::17] = -1
+    weight = torch.rand(tokens * k, generator=g, device="cuda")
+    r = n.CSR_gpu(torch.arange(0, tokens * k + 1, k, dtype=torch.int32, device="cuda"), expert, weight, (tokens, experts))
+    x, w, target = normal((tokens, width), dtype, 1), normal((experts, 2 * hidden, width), dtype, 2, width ** -0.5), normal((tokens, hidden), torch.float32, 3)
+    order, xs = n.gpu_expert_sort(r, x)
+    h, both = n.gpu_gated_product(xs, w, order, keep=True)
+    y = n.gpu_expert_unsort(r, order, h)
+    dz, dgate = n.gpu_expert_unsort_grad(r, order, h, (y.float() - target).to(dtype))
+    dxs, dw = n.gpu_gated_product_grad(dz, both, xs, w, order)
+    dx = n.gpu_expert_sort_grad(order, dxs)
+    master = torch.empty(w.shape, device="cuda")
+    norm = n.gpu_clip_gradients([dw], 0.25, [master])
+    # in 64 bits, entry by entry
+    want_y, keep = torch.zeros(tokens, hidden, dtype=torch.float64, device="cuda"), expert >= 0
+    token, e = torch.arange(tokens * k, device="cuda")[keep] // k, expert[keep].long()
+    p = torch.einsum("ij,ikj->ik", x[token].double(), w[e].double())
+    a, slope = act64(p[:, :hidden], "silu")
+    want_h = a * p[:, hidden:]
+    want_y.index_add_(0, token, want_h * weight[keep].double()[:, None])
+    dy = want_y - target.double()
+    dh = dy[token] * weight[keep].double()[:, None]
+    dp = torch.cat([dh * p[:, hidden:] * slope, dh * a], dim=1)
+    want_dw = torch.zeros(w.shape, dtype=torch.float64, device="cuda").index_add_(0, e, torch.einsum("ik,ij->ikj", dp, x[token].double()))
+    want_dx = torch.zeros(tokens, width, dtype=torch.float64, device="cuda").index_add_(0, token, torch.einsum("ik,ikj->ij", dp, w[e].double()))
+    want_gate = torch.zeros(tokens * k, dtype=torch.float64, device="cuda")
+    want_gate[keep] = (dy[token] * want_h).sum(1)
+    # the chain rounds to 2^-8 at each of six steps; sums of some 100 terms: within 6 * 2^-8 of the largest in the root of the squares' mean
+    for got, want in ((y, want_y), (dx, want_dx), (dw, want_dw), (dgate, want_gate)):
+        assert float((got.double() - want).square().mean().sqrt()) <= 6 * 2.0 ** -8 * float(want.square().mean().sqrt())
+    assert abs(float(norm) - float(dw.double().norm())) <= 1e-5 * float(norm)
+    assert torch.allclose(master, dw.float() * min(1.0, 0.25 / (float(norm) + 1e-6)), rtol=1e-5, atol=1e-12)
+    served = n.gpu_int8_product(n.to_int8_rows(xs), n.to_int8_rows(w), order, dtype=torch.float32)
+    q, s = codes64(xs)
+    qw, sw = codes64(w)
+    for c in range(experts):
+        lo, hi = order.offsets[c:c + 2].tolist()
+        want = (q[lo:hi] @ qw[c].t()) * s[lo:hi, None].double() * sw[c].double()
+        assert float((served[lo:hi].double() - want).abs().max() if hi > lo else 0) <= 4 * 2.0 ** -24 * float(want.abs().max() if hi > lo else 0)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_extents_of_zero(dtype):
+    n = nacho()
+    z = lambda *s: torch.zeros(*s, dtype=dtype, device="cuda")
+    ones = lambda *s: torch.ones(*s, dtype=dtype, device="cuda")
+    order, _ = order_of([], tail=4)
+    for rows, hidden, width in ((0, 8, 8), (4, 0, 8), (4, 8, 0), (0, 0, 0), (40, 8, 0), (40, 0, 8)):
+        h, both = n.gpu_gated_product(ones(rows, width), ones(2 * hidden, width), keep=True)
+        assert h.shape == (rows, hidden) and both.shape == (rows, 2 * hidden) and not bool(h.any()) and not bool(both.any())
+        dx, dw = n.gpu_gated_product_grad(ones(rows, hidden), ones(rows, 2 * hidden), ones(rows, width), ones(2 * hidden, width))
+        assert dx.shape == (rows, width) and dw.shape == (2 * hidden, width)
+        if rows == 0 or hidden == 0:
+            assert not bool(dx.any()) and not bool(dw.any())
+        y = n.gpu_int8_product(n.to_int8_rows(ones(rows, width)), n.to_int8_rows(ones(hidden, width)), dtype=dtype)
+        assert y.shape == (rows, hidden) and (width or not bool(y.any()))
+    # no experts: rows of nobody
+    h, both = n.gpu_gated_product(ones(4, 8), z(0, 12, 8), order, keep=True)
+    assert h.shape == (4, 6) and not bool(h.any()) and not bool(both.any())
+    dx, dw = n.gpu_gated_product_grad(ones(4, 6), ones(4, 12), ones(4, 8), z(0, 12, 8), order)
+    assert dx.shape == (4, 8) and not bool(dx.any()) and dw.shape == (0, 12, 8)
+    assert not bool(n.gpu_int8_product(n.to_int8_rows(ones(4, 8)), n.to_int8_rows(z(0, 5, 8)), order).any())
+
+
+def test_offsets_that_fall_end_too():
+    """Offsets that rise and fall again and again stand for more tiles than there are rows: the calls end, and no row is written outside its matrix."""
+    n, dtype = nacho(), torch.bfloat16
+    rows, groups = 3000, 300
+    zigzag = torch.arange(groups + 1, device="cuda", dtype=torch.int32) % 2 * rows
+    nobody = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    order = n.ExpertOrder_gpu(zigzag, nobody, nobody, torch.tensor([0, rows], dtype=torch.int32, device="cuda"), (1, groups))
+    x, w = normal((rows, 64), dtype, 1), normal((groups, 64, 64), dtype, 2)
+    n.gpu_gated_product(x, w, order, keep=True)
+    n.gpu_gated_product_grad(normal((rows, 32), dtype, 3), normal((rows, 64), dtype, 4), x, w, order)
+    n.gpu_int8_product(n.to_int8_rows(x), n.to_int8_rows(w), order)
+    torch.cuda.synchronize()
+    check_gated(x, w[0], None, [0, rows], "silu", dtype)
+
+
+def test_rows_farther_than_32_bits_reach():
+    """Rows two million elements apart, in storage of five gigabytes."""
+    n, dtype, stride = nacho(), torch.bfloat16, 1 << 21
+    store = torch.empty(1200 * stride, dtype=dtype, device="cuda")
+    far = lambda t, at: store.view(-1, stride)[:, at:at + t.shape[1]].copy_(t)
+    x, w, dh, both = some_operands(rows=1200, hidden=72, width=136)
+    fx, fd, fb = far(x, 0), far(dh, 1024), far(both, 2048)
+    assert equal(n.gpu_gated_product(fx, w, keep=True), n.gpu_gated_product(x, w, keep=True))
+    assert equal(n.gpu_gated_product_grad(fd, fb, fx, w), n.gpu_gated_product_grad(dh, both, x, w))
+    assert equal(n.gpu_gated_product_grad(fd, fb, far(x, 4097), w), n.gpu_gated_product_grad(dh, both, x, w))
+    fw = far(normal((1200, 136), dtype, 9, 0.1), 8192)
+    assert equal([n.gpu_gated_product(x[:3], fw)], [n.gpu_gated_product(x[:3], fw.contiguous())])
+    assert equal([n.gpu_gated_product(x, fw)], [n.gpu_gated_product(x, fw.contiguous())])
+    a, b = n.to_int8_rows(fx), n.to_int8_rows(x)
+    assert torch.equal(a.scales, b.scales) and torch.equal(a.to_dense(), b.to_dense())
+
+
+def test_a_wait_that_gives_up_is_reported():
+    import ctypes as C
+    from nacho_b200 import _capi
+    n = nacho()
+    x = normal((300, 700), torch.float32, 1)
+    a, w = n.to_int8_rows(x), n.to_int8_rows(normal((200, 700), torch.float32, 2))
+    want = n.gpu_int8_product(a, w, dtype=torch.float32)
+    y = torch.full((300, 200), 7.0, device="cuda")
+    struct = lambda m: _capi.Int8Struct(*m._dims, m._values.data_ptr(), m._scales.data_ptr())
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for call in (lambda: n.gpu_int8_product(a, w), lambda: n.gpu_gated_product(x[:2].half(), x[:8].half()), lambda: n.gpu_gated_product(x.half(), x[:8].half())):
+        status = _capi.lib.nb200_selftest_tiles_timeout(C.byref(struct(a)), C.byref(struct(w)), C.byref(_capi.DenseStruct(300, 200, 200, 0, y.data_ptr())), stream)
+        assert status == _capi.OK
+        torch.cuda.synchronize()
+        assert torch.all(y == 7.0)
+        with pytest.raises(RuntimeError, match="earlier gated or integer product: matrix product pipeline gave up"):
+            call()
+        assert torch.equal(n.gpu_int8_product(a, w, dtype=torch.float32), want)
+
+
+def test_refusals():
+    n = nacho()
+    x, w, dh, both = some_operands()
+    order, _ = order_of([100, 200])
+    three = torch.stack([w, w])
+    grad = lambda *a, **k: n.gpu_gated_product_grad(*a, **k)
+    for error, call in [
+            (TypeError, lambda: n.gpu_gated_product(x.float(), w.float())), (TypeError, lambda: n.gpu_gated_product(x, w.half())), (TypeError, lambda: n.gpu_gated_product(x.cpu(), w)),
+            (TypeError, lambda: n.gpu_gated_product(x, w.t().contiguous().t())), (TypeError, lambda: n.gpu_gated_product(None, w)), (ValueError, lambda: n.gpu_gated_product(x, w[:-1])),
+            (ValueError, lambda: n.gpu_gated_product(x[:, :-1], w)), (ValueError, lambda: n.gpu_gated_product(x, w, activation="relu")), (ValueError, lambda: n.gpu_gated_product(x, three)),
+            (ValueError, lambda: n.gpu_gated_product(x, w, order)), (ValueError, lambda: n.gpu_gated_product(x[:-1], three, order)), (TypeError, lambda: n.gpu_gated_product(x, three, "order")),
+            (TypeError, lambda: n.gpu_gated_product(x, torch.stack([w] * 4)[::2], order)), (TypeError, lambda: n.gpu_gated_product(x[0], w)),
+            (ValueError, lambda: grad(dh[:-1], both, x, w)), (ValueError, lambda: grad(dh, both[:, :-2], x, w)), (ValueError, lambda: grad(dh[:, 1:], both, x, w)),
+            (TypeError, lambda: grad(dh.half(), both, x, w)), (TypeError, lambda: grad(dh, both.float(), x, w)), (ValueError, lambda: grad(dh, both, x, w, activation="")),
+            (TypeError, lambda: n.INT8_gpu(1)), (TypeError, lambda: n.to_int8_rows(x.cpu())), (TypeError, lambda: n.to_int8_rows(x.int())), (TypeError, lambda: n.to_int8_rows(x, x)),
+            (TypeError, lambda: n.to_int8_rows(x.char().t(), torch.ones(200, device="cuda"))), (ValueError, lambda: n.to_int8_rows(x.char(), torch.ones(299, device="cuda"))),
+            (ValueError, lambda: n.to_int8_rows(x.char(), torch.ones(300, device="cuda").half())), (ValueError, lambda: n.to_int8_rows(x.char(), torch.ones(300))),
+            (ValueError, lambda: n.gpu_int8_product(n.to_int8_rows(x), n.to_int8_rows(w[:, 1:]))), (ValueError, lambda: n.gpu_int8_product(n.to_int8_rows(x), n.to_int8_rows(three))),
+            (ValueError, lambda: n.gpu_int8_product(n.to_int8_rows(three), n.to_int8_rows(w))), (TypeError, lambda: n.gpu_int8_product(x, n.to_int8_rows(w))),
+            (TypeError, lambda: n.gpu_int8_product(n.to_int8_rows(x), n.to_int8_rows(w), dtype=torch.float64)),
+            (TypeError, lambda: n.gpu_clip_gradients(x, 1.0)), (ValueError, lambda: n.gpu_clip_gradients([], 1.0)), (ValueError, lambda: n.gpu_clip_gradients([x], -1.0)),
+            (ValueError, lambda: n.gpu_clip_gradients([x], float("nan"))), (TypeError, lambda: n.gpu_clip_gradients([x.cpu()], 1.0)), (TypeError, lambda: n.gpu_clip_gradients([x.double()], 1.0)),
+            (TypeError, lambda: n.gpu_clip_gradients([x, 1.0], 1.0)), (ValueError, lambda: n.gpu_clip_gradients([x[:, ::2]], 1.0)), (ValueError, lambda: n.gpu_clip_gradients([x, x], 1.0)),
+            (ValueError, lambda: n.gpu_clip_gradients([x[:100], x[99:]], 1.0)), (ValueError, lambda: n.gpu_clip_gradients([x], 1.0, [])), (ValueError, lambda: n.gpu_clip_gradients([x], 1.0, [w])),
+            (ValueError, lambda: n.gpu_clip_gradients([x, w], 1.0, [torch.empty_like(x)] * 2)), (ValueError, lambda: n.gpu_clip_gradients([x[:100], x[100:200]], 1.0, [x[100:200], x[200:]])),
+            (ValueError, lambda: n.gpu_clip_gradients([x[:100]], 1.0, [x.view(torch.float16)[:100]])), (ValueError, lambda: n.gpu_clip_gradients([x[:200]], 1.0, [x[:200].t().contiguous().t()])),
+            (TypeError, lambda: n.gpu_clip_gradients([x.to_sparse()], 1.0))]:
+        kept = x.clone()
+        with pytest.raises(error):
+            call()
+        assert torch.equal(x, kept)
+
+
+def test_clipping_counts_as_a_change_in_place():
+    t = torch.ones(10, device="cuda")
+    version = t._version
+    nacho().gpu_clip_gradients([t], 0.1)
+    assert t._version > version
