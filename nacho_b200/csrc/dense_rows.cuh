@@ -123,6 +123,48 @@ int with_vector(int word, F f) {
     return f(std::integral_constant<int, 1>{});
 }
 
+// Four neighbouring elements of a row that lies on no boundary, from element c (a multiple of four) on, zeros from `cols` on. 16-bit rows are read in words of two
+// elements, which begin at the row's first or second one, whichever lies on a boundary; in the latter case the first element is the last one of the thread in
+// front (of a whole warp, whose threads have consecutive fours). Loading and taking apart are two steps, so that all loads of a thread are on their way first.
+template <typename T>
+struct Four {
+    uint32_t w[sizeof(T)], first = 0;
+
+    __device__ __forceinline__ void load(const T *row, uint32_t c, uint32_t cols) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = 0;
+                if (c + i < cols) w[i] = __float_as_uint(row[c + i]);
+            }
+        } else {
+            const uint16_t *const from = reinterpret_cast<const uint16_t *>(row);
+            const uint32_t odd = reinterpret_cast<uintptr_t>(row) / 2 & 1;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t at = c + 2 * i + odd;
+                w[i] = 0;
+                if (at + 1 < cols) w[i] = *reinterpret_cast<const uint32_t *>(from + at);
+                if (at + 1 == cols) w[i] = from[at];
+            }
+            if (odd && lane_id() == 0 && c < cols) first = from[c];
+        }
+    }
+    __device__ __forceinline__ void get(const T *row, float (&v)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+        } else {
+            const bool odd = reinterpret_cast<uintptr_t>(row) / 2 & 1;
+            uint32_t before = __shfl_up_sync(FULL_MASK, w[1], 1) >> 16;
+            if (lane_id() == 0) before = first;
+            const uint32_t lo = odd ? before | w[0] << 16 : w[0], hi = odd ? w[0] >> 16 | w[1] << 16 : w[1];
+            auto value = [](uint32_t bits) { return to_float(*reinterpret_cast<const T *>(&bits)); };
+            v[0] = value(lo & 0xffff), v[1] = value(lo >> 16), v[2] = value(hi & 0xffff), v[3] = value(hi >> 16);
+        }
+    }
+};
+
 // ---- 8-bit integers --------------------------------------------------------------------
 
 // A sum of integers times the scales of its row and its channel, the smaller one first: only where the result does so does a product on the way

@@ -10,7 +10,7 @@ namespace {
 
 constexpr int NT = 256;
 
-// Rows at a distance that the copy engine takes, of up to two matrices: `first` CTAs have the first one's. A thread has 16 bytes of a row.
+// Rows at a distance that the copy engine takes, of up to two matrices: `first` CTAs have the first one's. A thread has 16 bytes of a row where rows lie on boundaries of four.
 struct Align {
     const void *x;
     int64_t stride, rows, cols;
@@ -24,12 +24,40 @@ __global__ void __launch_bounds__(NT) k_align_rows(const Align a, const Align b,
     trigger_dependents();
     const bool second = (int)blockIdx.x >= first;
     const Align &m = second ? b : a;
-    const int64_t pieces = m.pitch / 8, all = m.rows * pieces, step = (int64_t)(second ? gridDim.x - first : first) * NT;
-    for (int64_t i = (int64_t)(blockIdx.x - (second ? first : 0)) * NT + threadIdx.x; i < all; i += step) {
-        const int64_t r = i / pieces, c = (i - r * pieces) * 8;
-        Eight<T> v;
-        v.template load<V>(static_cast<const T *>(m.x) + r * m.stride, c, m.cols);
-        *reinterpret_cast<uint4 *>(static_cast<T *>(m.z) + r * m.pitch + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    const int64_t cta = blockIdx.x - (second ? first : 0), ctas = second ? gridDim.x - first : first;
+    if constexpr (V == 1) {
+        // rows on no boundary: a warp has 128 elements of a row at a time, TURNS of them on their way
+        constexpr int TURNS = 4;
+        const int64_t per_row = (m.pitch + 127) / 128, all = m.rows * per_row, step = ctas * (NT / 32);
+        for (int64_t i = cta * (NT / 32) + warp_id(); i < all; i += TURNS * step) {
+            Four<T> raw[TURNS];
+            auto place = [&](int u, int64_t *r) {
+                const int64_t at = i + u * step < all ? i + u * step : i;
+                *r = at / per_row;
+                return (uint32_t)(at - *r * per_row) * 128 + lane_id() * 4;
+            };
+            int64_t r;
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u) {
+                const uint32_t c = place(u, &r);
+                raw[u].load(static_cast<const T *>(m.x) + r * m.stride, c, (uint32_t)m.cols);
+            }
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u) {
+                const uint32_t c = place(u, &r);
+                float v[4];
+                raw[u].get(static_cast<const T *>(m.x) + r * m.stride, v);
+                if (i + u * step < all && c < m.pitch) *reinterpret_cast<uint2 *>(static_cast<T *>(m.z) + r * m.pitch + c) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+            }
+        }
+    } else {
+        const int64_t pieces = m.pitch / 8, all = m.rows * pieces, step = ctas * NT;
+        for (int64_t i = cta * NT + threadIdx.x; i < all; i += step) {
+            const int64_t r = i / pieces, c = (i - r * pieces) * 8;
+            Eight<T> v;
+            v.template load<V>(static_cast<const T *>(m.x) + r * m.stride, c, m.cols);
+            *reinterpret_cast<uint4 *>(static_cast<T *>(m.z) + r * m.pitch + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+        }
     }
     if (beside) finish_after_previous();
 }

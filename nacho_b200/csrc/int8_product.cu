@@ -20,16 +20,43 @@ __device__ __forceinline__ uint32_t int_codes4(float a, float b, float c, float 
     return __byte_perm(__byte_perm(i0, i1, 0x0040), __byte_perm(i2, i3, 0x0040), 0x5410);
 }
 
-// THREADS threads have a row (32, or all of a CTA): they read it for its largest magnitude and again, out of registers as far as KEEP pieces of 16
-// elements a thread go, for its codes.
+// The largest magnitude of what THREADS neighbouring threads have (8, 32, or all of a CTA), for all of them.
+template <int THREADS>
+__device__ __forceinline__ uint32_t row_top(uint32_t mine) {
+    if constexpr (THREADS == 8) {
+        const unsigned eight = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+        for (int d = 4; d; d >>= 1) mine = max(mine, __shfl_xor_sync(eight, mine, d));
+        return mine;
+    }
+    mine = __reduce_max_sync(FULL_MASK, mine);
+    if constexpr (THREADS == 32) return mine;
+    __shared__ uint32_t top[NT / 32];
+    if (lane_id() == 0) top[warp_id()] = mine;
+    __syncthreads();
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) mine = max(mine, top[i]);
+    return mine;
+}
+
+// The factor of a row's codes, and its scale. A row that holds a NaN or an infinity stands for NaNs: its codes are zeros and its scale is none.
+__device__ __forceinline__ float row_factor(uint32_t top, float *scale) {
+    const bool finite = top < 0x7f800000u;
+    const float largest = __uint_as_float(max(top, FLOOR8));
+    *scale = finite ? __fdiv_rn(largest, TOP_INT8) : __uint_as_float(0x7fc00000u);
+    return finite ? __fdiv_rn(TOP_INT8, largest) : 0.f;
+}
+
+// THREADS threads have a row: they read it for its largest magnitude and again, out of registers as far as KEEP pieces of 16 elements a thread go, for its
+// codes. (32768 rows of 2048 by CTAs 64 us, by warps 37.)
 template <typename T, int V, int THREADS, int KEEP>
 __global__ void __launch_bounds__(NT) k_int8_rows(const T *x, int64_t stride, int64_t rows, int64_t cols, int8_t *values, int64_t pitch, float *scales) {
-    __shared__ uint32_t top[NT / 32];
     wait_for_previous();
     trigger_dependents();
     const int64_t r = (int64_t)blockIdx.x * (NT / THREADS) + threadIdx.x / THREADS;
     const int sub = threadIdx.x % THREADS;
-    if (THREADS == 32 && r >= rows) return;
+    if (r >= rows) return;  // whole rows' threads
     const T *const row = x + r * stride;
     Piece<T> kept[KEEP];
     Top<T> m;
@@ -38,30 +65,22 @@ __global__ void __launch_bounds__(NT) k_int8_rows(const T *x, int64_t stride, in
         kept[i].template load<V>(row, ((int64_t)i * THREADS + sub) * 16, cols);
         m.add(kept[i].lo), m.add(kept[i].hi);
     }
-    for (int64_t c = ((int64_t)KEEP * THREADS + sub) * 16; c < cols; c += THREADS * 16) {
-        Piece<T> p;
-        p.template load<V>(row, c, cols);
-        m.add(p.lo), m.add(p.hi);
-    }
-    uint32_t all = __reduce_max_sync(FULL_MASK, m.bits());
-    if constexpr (THREADS != 32) {
-        if (lane_id() == 0) top[warp_id()] = all;
-        __syncthreads();
-        all = 0;
-#pragma unroll
-        for (int i = 0; i < NT / 32; ++i) all = max(all, top[i]);
-    }
-    // a row that holds a NaN or an infinity stands for NaNs: its codes are zeros and its scale is none
-    const bool finite = all < 0x7f800000u;
-    const float largest = __uint_as_float(max(all, FLOOR8)), inverse = finite ? __fdiv_rn(TOP_INT8, largest) : 0.f;
-    if (sub == 0) scales[r] = finite ? __fdiv_rn(largest, TOP_INT8) : __uint_as_float(0x7fc00000u);
+    if constexpr (THREADS == NT)
+        for (int64_t c = ((int64_t)KEEP * THREADS + sub) * 16; c < cols; c += THREADS * 16) {
+            Piece<T> p;
+            p.template load<V>(row, c, cols);
+            m.add(p.lo), m.add(p.hi);
+        }
+    float scale;
+    const float factor = row_factor(row_top<THREADS>(m.bits()), &scale);
+    if (sub == 0) scales[r] = scale;
     auto put = [&](const Piece<T> &p, int64_t c) {
         uint32_t w[4] = {0, 0, 0, 0};
-        if (finite) {
+        if (factor != 0.f) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                w[i] = int_codes4(p.lo.get(4 * i), p.lo.get(4 * i + 1), p.lo.get(4 * i + 2), p.lo.get(4 * i + 3), inverse);
-                w[2 + i] = int_codes4(p.hi.get(4 * i), p.hi.get(4 * i + 1), p.hi.get(4 * i + 2), p.hi.get(4 * i + 3), inverse);
+                w[i] = int_codes4(p.lo.get(4 * i), p.lo.get(4 * i + 1), p.lo.get(4 * i + 2), p.lo.get(4 * i + 3), factor);
+                w[2 + i] = int_codes4(p.hi.get(4 * i), p.hi.get(4 * i + 1), p.hi.get(4 * i + 2), p.hi.get(4 * i + 3), factor);
             }
         }
         *reinterpret_cast<uint4 *>(values + r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -71,10 +90,64 @@ __global__ void __launch_bounds__(NT) k_int8_rows(const T *x, int64_t stride, in
         const int64_t c = ((int64_t)i * THREADS + sub) * 16;
         if (c < pitch) put(kept[i], c);
     }
-    for (int64_t c = ((int64_t)KEEP * THREADS + sub) * 16; c < pitch; c += THREADS * 16) {
-        Piece<T> p;
-        p.template load<V>(row, c, cols);
-        put(p, c);
+    if constexpr (THREADS == NT)
+        for (int64_t c = ((int64_t)KEEP * THREADS + sub) * 16; c < pitch; c += THREADS * 16) {
+            Piece<T> p;
+            p.template load<V>(row, c, cols);
+            put(p, c);
+        }
+}
+
+// The same for rows that lie on no boundary: a thread has four elements at a time and KEEP fours in registers. (With 16 elements in a row a thread, read one by one, 8192 rows of 8191
+// took 73 us; with single elements that neighbouring threads share out, 97.)
+template <typename T, int THREADS, int KEEP>
+__global__ void __launch_bounds__(NT) k_int8_rows_odd(const T *x, int64_t stride, int64_t rows, int64_t cols_, int8_t *values, int64_t pitch_, float *scales) {
+    wait_for_previous();
+    trigger_dependents();
+    const int64_t r = (int64_t)blockIdx.x * (NT / THREADS) + threadIdx.x / THREADS;
+    const uint32_t sub = threadIdx.x % THREADS, cols = (uint32_t)cols_, pitch = (uint32_t)pitch_;
+    if (r >= rows) return;
+    const T *const row = x + r * stride;
+    int8_t *const codes = values + r * pitch_;
+    float kept[KEEP][4];
+    uint32_t m = 0;
+    auto add = [&](const float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    };
+    {
+        Four<T> raw[KEEP];
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) raw[u].load(row, (sub + u * THREADS) * 4, cols);
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) {
+            raw[u].get(row, kept[u]);
+            add(kept[u]);
+        }
+    }
+    auto later = [&](uint32_t c, float (&v)[4]) {
+        Four<T> raw;
+        raw.load(row, c, cols);
+        raw.get(row, v);
+    };
+    const uint32_t rest = KEEP * THREADS * 4, turns = pitch > rest ? (pitch - rest + THREADS * 4 - 1) / (THREADS * 4) : 0;  // for whole warps
+    for (uint32_t i = 0; i < turns; ++i) {
+        float v[4];
+        later(rest + (i * THREADS + sub) * 4, v);
+        add(v);
+    }
+    float scale;
+    const float factor = row_factor(row_top<THREADS>(m), &scale);
+    if (sub == 0) scales[r] = scale;
+    auto put = [&](uint32_t c, const float (&v)[4]) {
+        if (c < pitch) *reinterpret_cast<uint32_t *>(codes + c) = factor != 0.f ? int_codes4(v[0], v[1], v[2], v[3], factor) : 0;
+    };
+#pragma unroll
+    for (int u = 0; u < KEEP; ++u) put((sub + u * THREADS) * 4, kept[u]);
+    for (uint32_t i = 0; i < turns; ++i) {
+        float v[4];
+        later(rest + (i * THREADS + sub) * 4, v);
+        put(rest + (i * THREADS + sub) * 4, v);
     }
 }
 
@@ -119,9 +192,16 @@ int nb200_int8_quantise(const nb200_dense *x, nb200_int8 *z, void *stream_) {
                                              x->cols, z->values, pitch_of(x->cols), z->scales));
                 return NB200_OK;
             };
-            // A warp per row where two pieces a thread hold it and there are rows for all warps, else a CTA.
-            if (x->cols <= 1024) return go(k_int8_rows<T, V, 32, 2>, NT / 32);
-            return go(k_int8_rows<T, V, NT, sizeof(T) == 2 ? 2 : 1>, 1);
+            // As few threads per row as hold it in registers.
+            if constexpr (V == 1) {
+                if (x->cols <= 1024) return go(k_int8_rows_odd<T, 32, 8>, NT / 32);
+                return go(k_int8_rows_odd<T, NT, 8>, 1);
+            } else {
+                if (x->cols <= 256) return go(k_int8_rows<T, V, 8, 2>, NT / 8);
+                if (x->cols <= 1024) return go(k_int8_rows<T, V, 32, 2>, NT / 32);
+                if (x->cols <= 2048) return go(k_int8_rows<T, V, 32, 4>, NT / 32);
+                return go(k_int8_rows<T, V, NT, sizeof(T) == 2 ? 2 : 1>, 1);
+            }
         });
     });
 }

@@ -921,37 +921,40 @@ PyObject *clip(PyObject *const *args) {
     const char *where = "gpu_clip_gradients";
     const std::vector<at::Tensor> from = tensors_of(args[0], where, "gradients");
     const bool in_place = args[1] == Py_None;
-    const std::vector<at::Tensor> to = in_place ? from : tensors_of(args[1], where, "out");
+    const std::vector<at::Tensor> others = in_place ? std::vector<at::Tensor>() : tensors_of(args[1], where, "out"), &to = in_place ? from : others;
     if (from.empty()) refuse(PyExc_ValueError, "%s: %s are none", where, "gradients");
-    if (from.size() != to.size()) refuse(PyExc_ValueError, "%s: %s must hold as many tensors as there are gradients", where, "out");
+    if (from.size() != to.size() || to.empty()) refuse(PyExc_ValueError, "%s: %s must hold as many tensors as there are gradients", where, "out");
     const double max_norm = PyFloat_AsDouble(args[2]);
     const c10::Device device = from[0].device();
     if (to[0].device() != device) refuse(PyExc_ValueError, "%s: gradients and %s live on different devices", where, "out");
     std::vector<nb200_span> spans;
-    struct Range {
-        uintptr_t begin, end;
-        bool written;
-    };
-    std::vector<Range> ranges;
-    spans.reserve(from.size()), ranges.reserve(from.size() * (in_place ? 1 : 2));
+    typedef std::pair<uintptr_t, uintptr_t> Range;
+    std::vector<Range> read, written;  // what is both is written
+    spans.reserve(from.size()), written.reserve(from.size());
+    if (!in_place) read.reserve(from.size());
     for (size_t i = 0; i < from.size(); ++i) {
         const at::Tensor &x = from[i], &z = to[i];
         if (!in_place && (x.sizes() != z.sizes() || !(x.strides() == z.strides() || (x.is_contiguous() && z.is_contiguous()))))
             refuse(PyExc_ValueError, "%s: a tensor of %s differs from its gradient in shape or layout", where, "out");
         const int64_t n = x.numel();
         if (n == 0) continue;
-        const nb200_span s{x.data_ptr(), z.data_ptr(), n, type_of(x), type_of(z)};
+        const int type = type_of(x), to_type = in_place ? type : type_of(z);
+        const nb200_span s{x.data_ptr(), in_place ? x.data_ptr() : z.data_ptr(), n, type, to_type};
         spans.push_back(s);
         const uintptr_t a = reinterpret_cast<uintptr_t>(s.from), b = reinterpret_cast<uintptr_t>(s.to);
-        const bool same = a == b && s.type == s.to_type;
-        if (!same) ranges.push_back({a, a + (size_t)n * x.element_size(), false});
-        ranges.push_back({b, b + (size_t)n * z.element_size(), true});
+        if (a != b || type != to_type) read.emplace_back(a, a + (size_t)n * (type == NB200_F32 ? 4 : 2));
+        written.emplace_back(b, b + (size_t)n * (to_type == NB200_F32 ? 4 : 2));
     }
-    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
-    uintptr_t read = 0, written = 0;
-    for (const Range &r : ranges) {
-        if (r.begin < written || (r.written && r.begin < read)) refuse(PyExc_ValueError, "%s: %s overlap one another in memory", where, in_place ? "gradients" : "gradients and out");
-        (r.written ? written : read) = std::max(r.written ? written : read, r.end);
+    for (std::vector<Range> *r : {&read, &written})
+        if (!std::is_sorted(r->begin(), r->end())) std::sort(r->begin(), r->end());
+    const char *what = in_place ? "gradients" : "gradients and out";
+    uintptr_t end = 0;
+    size_t next = 0;
+    for (const Range &w : written) {
+        if (w.first < end) refuse(PyExc_ValueError, "%s: %s overlap one another in memory", where, what);
+        end = w.second;
+        while (next < read.size() && read[next].second <= w.first) ++next;
+        if (next < read.size() && read[next].first < w.second) refuse(PyExc_ValueError, "%s: %s overlap one another in memory", where, what);
     }
     at::Tensor norm = at::Tensor(at::detail::empty_cuda(c10::IntArrayRef(), at::kFloat, device, std::nullopt));
     const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);
@@ -960,9 +963,15 @@ PyObject *clip(PyObject *const *args) {
     v.device = device;
     launch({&v}, where, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });
     const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(device.index());
-    for (const at::Tensor &x : from) c10::cuda::CUDACachingAllocator::recordStream(x.storage().data_ptr(), current);
+    const void *last = nullptr;  // parts of one long buffer follow one another
+    auto record = [&](const at::Tensor &t) {
+        const c10::DataPtr &p = t.storage().data_ptr();
+        if (p.get() != last) c10::cuda::CUDACachingAllocator::recordStream(p, current);
+        last = p.get();
+    };
+    for (const at::Tensor &x : from) record(x);
     for (const at::Tensor &z : to) {
-        if (!in_place) c10::cuda::CUDACachingAllocator::recordStream(z.storage().data_ptr(), current);
+        if (!in_place) record(z);
         z.unsafeGetTensorImpl()->bump_version();
     }
     return wrap(norm);
