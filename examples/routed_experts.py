@@ -1,9 +1,10 @@
 """A layer of routed experts, forwards and backwards, with the operators of ``nacho_b200.nacho``: a router gives every token its best experts, an
 expert is a gated pair of 8-bit products, and the results come back weighted by the router.
 
-    python -m examples.routed_experts [--tokens 1024] [--experts 16] [--best 2] [--width 512] [--hidden 1024]
+    python -m examples.routed_experts [--tokens 1024] [--experts 16] [--best 2] [--width 512] [--hidden 1024] [--halves] [--clip 0.5]
 
-prints the loss of a few steps of gradient descent on a fixed random target; it falls."""
+prints the loss of a few steps of gradient descent on a fixed random target; it falls. With --halves the gated product is one call in 16 bits, forwards and
+backwards, and only the way down is multiplied in 8; with --clip the gradients of the weights are scaled to that norm at most."""
 import argparse
 
 import torch
@@ -45,7 +46,23 @@ def backward(r, x, up, down, kept, dy):
     return nacho.gpu_expert_sort_grad(order, dxs), dgate, dup, ddown
 
 
-def descend(tokens=1024, experts=16, best=2, width=512, hidden=1024, steps=5, rate=0.5):
+def forward_halves(r, x, up, down):
+    """The same with up in 16 bits."""
+    order, xs = nacho.gpu_expert_sort(r, x)
+    hidden, both = nacho.gpu_gated_product(xs, up, order, keep=True)
+    z = nacho.gpu_fp8_product(nacho.to_fp8_rows(hidden), down, order)
+    return nacho.gpu_expert_unsort(r, order, z), (order, xs, both, hidden, z)
+
+
+def backward_halves(r, up, down, kept, dy):
+    order, xs, both, hidden, z = kept
+    dz, dgate = nacho.gpu_expert_unsort_grad(r, order, z, dy)
+    dhidden, ddown = nacho.gpu_fp8_product_grad(dz, hidden, down, order)
+    dxs, dup = nacho.gpu_gated_product_grad(dhidden, both, xs, up, order)
+    return nacho.gpu_expert_sort_grad(order, dxs), dgate, dup, ddown
+
+
+def descend(tokens=1024, experts=16, best=2, width=512, hidden=1024, steps=5, rate=0.5, halves=False, clip=None):
     g = torch.Generator(device="cuda").manual_seed(0)
     draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda")
     x, target = draw(tokens, width).bfloat16(), draw(tokens, width)
@@ -54,11 +71,14 @@ def descend(tokens=1024, experts=16, best=2, width=512, hidden=1024, steps=5, ra
     for _ in range(steps):
         scores = x.float() @ router
         r, weight, expert = route(scores, best, capacity=2 * tokens * best // experts + 1)
-        up8, down8 = nacho.to_fp8_tiles(up), nacho.to_fp8_tiles(down)
-        y, kept = forward(r, x, up8, down8)
+        up8, down8 = up.bfloat16() if halves else nacho.to_fp8_tiles(up), nacho.to_fp8_tiles(down)
+        y, kept = forward_halves(r, x, up8, down8) if halves else forward(r, x, up8, down8)
         off = y.float() - target
         losses.append(float((off * off).mean()))
-        dx, dgate, dup, ddown = backward(r, x, up8, down8, kept, (off * (2 / width)).bfloat16())
+        dy = (off * (2 / width)).bfloat16()
+        dx, dgate, dup, ddown = backward_halves(r, up8, down8, kept, dy) if halves else backward(r, x, up8, down8, kept, dy)
+        if clip is not None:
+            nacho.gpu_clip_gradients([dup, ddown], clip)
         # the softmax over a token's best scores, then the router's matrix
         dgate = dgate.view(tokens, best)
         dtop = weight * (dgate - (dgate * weight).sum(1, keepdim=True))
@@ -73,5 +93,7 @@ if __name__ == "__main__":
     parser = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     for name, value in (("tokens", 1024), ("experts", 16), ("best", 2), ("width", 512), ("hidden", 1024), ("steps", 5)):
         parser.add_argument(f"--{name}", type=int, default=value)
+    parser.add_argument("--halves", action="store_true")
+    parser.add_argument("--clip", type=float)
     for loss in descend(**vars(parser.parse_args()))[0]:
         print(f"loss {loss:.5f}")

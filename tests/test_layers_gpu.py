@@ -634,6 +634,22 @@ def test_refusals():
         assert torch.equal(x, kept)
 
 
+def test_the_example_runs_with_the_layer_in_16_bits():
+    from examples import routed_experts as example
+    losses, dx = example.descend(tokens=130, experts=5, best=2, width=72, hidden=56, steps=2, halves=True, clip=0.5)
+    assert len(losses) == 2 and all(math.isfinite(v) for v in losses) and dx.shape == (130, 72) and bool(torch.isfinite(dx).all())
+    r, x = None, normal((40, 72), torch.bfloat16, 1)
+    up, down = normal((1, 112, 72), torch.bfloat16, 2, 0.1), nacho().to_fp8_tiles(normal((1, 64, 56), torch.float32, 3, 0.1))
+    r = nacho().CSR_gpu(torch.arange(41, dtype=torch.int32, device="cuda"), torch.zeros(40, dtype=torch.int32, device="cuda"), torch.ones(40, device="cuda"), (40, 1))
+    y, kept = example.forward_halves(r, x, up, down)
+    dx, dgate, dup, ddown = example.backward_halves(r, up, down, kept, normal((40, 64), torch.bfloat16, 4))
+    # its gated half against the operator's own gradient, whose result it is
+    order, xs, both, hidden, z = kept
+    dz, _ = nacho().gpu_expert_unsort_grad(r, order, z, normal((40, 64), torch.bfloat16, 4))
+    want = nacho().gpu_gated_product_grad(nacho().gpu_fp8_product_grad(dz, hidden, down, order)[0], both, xs, up, order)
+    assert torch.equal(dup, want[1]) and torch.equal(dx, want[0])
+
+
 def test_clipping_counts_as_a_change_in_place():
     t = torch.ones(10, device="cuda")
     version = t._version
