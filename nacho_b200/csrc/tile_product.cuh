@@ -28,6 +28,8 @@ struct TileArgs {
     int across;  // WEIGHTS: columns of z
     int blocks;  // of 128 bytes along the summed axis (not WEIGHTS)
     int tile_n;  // TILE_N at most
+    int pairs;   // of CTAs that the launch may take
+    int parts;   // pairs that share a tile's blocks
     int b_bytes, stages;  // of the narrow operand in a stage; stages
     int most;    // tiles, at most
     void *y;
@@ -669,17 +671,44 @@ inline int describe_result(CUtensorMap *map, bool *words, CUtensorMapDataType ty
 }
 inline CUtensorMapDataType map_type(int type) { return type == NB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
-// The narrow side of the tiles, a multiple of 64: what the busiest pair of CTAs then has to bring, 256 rows of the wide side and so many of the narrow one per
-// tile, is least. `rows` of all groups together, `wide_tiles` beside one another.
-inline int tile_n_of(int64_t rows, int64_t groups, int64_t wide_tiles) {
-    const int64_t mean = (rows + groups - 1) / groups, pairs = std::max(1, sm_count() / 2);
-    int best = TILE_N;
-    int64_t least = INT64_MAX;
-    for (int n = TILE_N; n >= 64; n -= 64) {
-        const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, cost = (tiles + pairs - 1) / pairs * (TILE_M + std::min<int64_t>(n, mean));
-        if (cost < least) least = cost, best = n;
+inline int64_t all_pairs() { return std::max(1, sm_count() / 2); }
+
+// A product as tiles: `rows` on the narrow side of all groups together, `wide_tiles` beside one another on the wide one, `blocks` summed for each.
+struct TileWork {
+    int64_t rows, groups, wide_tiles, blocks;
+
+    // How it goes on so many pairs of CTAs: the narrow side of its tiles, a multiple of 64, the pairs that share a tile's blocks, and what the busiest pair then has to
+    // bring, in rows of blocks: 256 of the wide side and n of the narrow one for every tile and block (1330 of them take a microsecond); adding up parts takes as long
+    // as 50 for each of the n columns.
+    struct Way {
+        int n, parts;
+        int64_t cost;
+    };
+    // Parts: as many pairs as find room for all tiles at once, of at least eight blocks each (`clusters`: of four and eight CTAs that the device holds. A second round
+    // costs more than parts give: 16 tiles of 32 blocks take 19 us in four parts, of which the device holds fewer than 16, and 10 in two).
+    Way best(int64_t pairs, const int (&clusters)[2]) const {
+        const int64_t mean = (rows + groups - 1) / groups;
+        Way way{0, 1, INT64_MAX};
+        for (int n = TILE_N; n >= 64; n -= 64) {
+            const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, each = TILE_M + std::min<int64_t>(n, mean);
+            for (int k = 0; k < 3; ++k) {
+                const int parts = 1 << k;
+                if (parts > 1 && (tiles * parts > pairs || tiles > clusters[k - 1] || blocks < 8 * parts)) break;
+                const int64_t cost = (tiles + pairs - 1) / pairs * each * ((blocks + parts - 1) / parts) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
+                if (cost < way.cost) way = Way{n, parts, cost};
+            }
+        }
+        return way;
     }
-    return best;
+};
+
+// Clusters of four and of eight CTAs that the device holds (all these kernels have the same threads and shared memory).
+template <Sum SUM, Form FORM, bool A_TURNED, typename T>
+int tile_clusters(int (&clusters)[2]) {
+    auto split = k_tiles<SUM, FORM, A_TURNED, true, T>;
+    if (const int st = allow_shared(split, TILE_SHARED_BYTES)) return st;
+    for (int k = 0; k < 2; ++k) clusters[k] = resident_clusters(reinterpret_cast<const void *>(split), 4 << k, TILE_THREADS, TILE_SHARED_BYTES);
+    return NB200_OK;
 }
 
 template <Sum SUM, Form FORM, bool A_TURNED, typename T>
@@ -696,18 +725,9 @@ int launch_tiles(const char *name, TileArgs args, const TileMaps &maps, cudaStre
     args.patience = args.starve ? SHORT_PATIENCE : PATIENCE;
     args.b_bytes = FORM == Form::WEIGHTS ? (args.tile_n / 2 + 63) / 64 * 8192 : args.tile_n / 2 * 128;
     args.stages = std::min(TileShared::STAGES, TileShared::STAGE_BYTES / (TileShared::A_BYTES + args.b_bytes));
-    // Pairs of CTAs that share a tile's blocks: as many as find room for all tiles at once, of at least eight blocks each. (A second round costs more than it
-    // gives: 16 tiles of 32 blocks take 19 us in four parts, of which the device holds fewer than 16, and 10 in two.)
-    const int64_t blocks = FORM == Form::WEIGHTS ? args.rows / args.groups / 64 : args.blocks;
     auto split = k_tiles<SUM, FORM, A_TURNED, true, T>;
-    int parts = 4;
-    if (tiles * 4 <= sm_count() && blocks >= 16) {
-        if ((st = allow_shared(split, TILE_SHARED_BYTES))) return st;
-        while (parts > 1 && (blocks < 8 * parts || tiles > resident_clusters(reinterpret_cast<const void *>(split), 2 * parts, TILE_THREADS, TILE_SHARED_BYTES))) parts /= 2;
-    } else {
-        parts = 1;
-    }
-    const int64_t ctas = parts > 1 ? tiles * 2 * parts : std::max<int64_t>(2, std::min<int64_t>(tiles * 2, sm_count() / 2 * 2));
+    const int parts = tiles * args.parts <= args.pairs ? args.parts : 1;  // groups may begin and end inside tiles: there may be more than the way counts
+    const int64_t ctas = parts > 1 ? tiles * 2 * parts : 2 * std::max<int64_t>(1, std::min<int64_t>(tiles, args.pairs));
     auto go = [&](auto kernel) -> int {
         if ((st = allow_shared(kernel, TILE_SHARED_BYTES))) return st;
         LaunchScope scope(name, stream);
