@@ -176,7 +176,7 @@ struct GradPlan {
         const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64}, work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64};
         x = work_x.best(all, clusters), w = work_w.best(all, clusters);
         pairs_x = pairs_w = (int)all;
-        int64_t least = (x.cost + w.cost) * 7 / 8;  // worth the smaller launches
+        double least = (x.cost + w.cost) * 7 / 8;  // worth the smaller launches
         for (int64_t k = 1; k < 16; ++k) {
             const int64_t part = all * k / 16;
             if (part < 1 || part >= all) continue;

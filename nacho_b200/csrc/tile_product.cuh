@@ -682,20 +682,20 @@ struct TileWork {
     // as 50 for each of the n columns.
     struct Way {
         int n, parts;
-        int64_t cost;
+        double cost;
     };
     // Parts: as many pairs as find room for all tiles at once, of at least eight blocks each (`clusters`: of four and eight CTAs that the device holds. A second round
     // costs more than parts give: 16 tiles of 32 blocks take 19 us in four parts, of which the device holds fewer than 16, and 10 in two).
     Way best(int64_t pairs, const int (&clusters)[2]) const {
         const int64_t mean = (rows + groups - 1) / groups;
-        Way way{0, 1, INT64_MAX};
+        Way way{0, 1, 0};
         for (int n = TILE_N; n >= 64; n -= 64) {
             const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, each = TILE_M + std::min<int64_t>(n, mean);
             for (int k = 0; k < 3; ++k) {
                 const int parts = 1 << k;
                 if (parts > 1 && (tiles * parts > pairs || tiles > clusters[k - 1] || blocks < 8 * parts)) break;
-                const int64_t cost = (tiles + pairs - 1) / pairs * each * ((blocks + parts - 1) / parts) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
-                if (cost < way.cost) way = Way{n, parts, cost};
+                const double cost = (double)((tiles + pairs - 1) / pairs) * (double)each * (double)((blocks + parts - 1) / parts) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
+                if (way.n == 0 || cost < way.cost) way = Way{n, parts, cost};
             }
         }
         return way;

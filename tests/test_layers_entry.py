@@ -1,6 +1,7 @@
 """CPU suite: entry points of gated layers, integer products and clipped gradients whose host side can be seen without a GPU: what they refuse, and rules of theirs."""
 import os
 import re
+import shutil
 import subprocess
 import sys
 
@@ -119,3 +120,34 @@ def test_shares_of_a_launch_that_starts_beside_another():
     grad = gated[gated.index("int nb200_gated_product_grad(const"):]
     order = [grad.index(w) for w in ('LaunchScope scope("gate_grad"', "aligned(*x, s.x, *w, s.w, &ax, &aw, true", '"gated_grad_x"', "args.beside = true", '"gated_grad_w"')]
     assert order == sorted(order)
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="no host compiler")
+def test_the_way_of_a_product(tmp_path):
+    """The choice of tiles by itself: narrow sides that the kernels take, parts only where all of them find room at once and have blocks enough, and never a dearer way than
+    the plain one."""
+    text = open(os.path.join(ROOT, "nacho_b200", "csrc", "tile_product.cuh")).read()
+    rule = text[text.index("struct TileWork {"):]
+    rule = rule[:rule.index("\n};") + 4]
+    (tmp_path / "rule.cpp").write_text("""
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+constexpr int TILE_M = 256, TILE_N = 256;
+""" + rule + """
+int main() {
+    const int clusters[2] = {33, 14};
+    long long seen[3] = {};
+    for (long long rows : {1ll, 33ll, 64ll, 65ll, 500ll, 1003ll, 8192ll, 2147482623ll}) for (long long groups : {1ll, 3ll, 64ll, 4096ll}) for (long long wide : {1ll, 6ll, 32ll, 4000000ll})
+        for (long long blocks : {1ll, 15ll, 16ll, 40ll, 128ll, 33554432ll}) for (long long pairs : {1ll, 9ll, 74ll}) {
+            const TileWork work{rows, groups, wide, blocks};
+            const TileWork::Way way = work.best(pairs, clusters);
+            const long long mean = (rows + groups - 1) / groups, tiles = groups * ((mean + way.n - 1) / way.n) * wide;
+            const bool fits = way.parts == 1 || (tiles * way.parts <= pairs && tiles <= clusters[way.parts / 4] && blocks >= 8 * way.parts);
+            if (way.n < 64 || way.n > 256 || way.n % 64 || !(way.parts == 1 || way.parts == 2 || way.parts == 4) || !fits || way.cost <= 0) printf("bad %lld %lld %lld %lld %lld\\n", rows, groups, wide, blocks, pairs);
+            ++seen[way.parts / 2];
+        }
+    printf("%d\\n", seen[0] > 0 && seen[1] > 0 && seen[2] > 0);
+}""")
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "rule"), str(tmp_path / "rule.cpp")], check=True)
+    assert subprocess.run([str(tmp_path / "rule")], check=True, capture_output=True, text=True).stdout.split() == ["1"]

@@ -106,6 +106,31 @@ def test_gated(rows, hidden, width, dtype, act):
     check_gated(x, w, None, [0, rows], act, dtype, keep=False)
 
 
+# sums so long, of so few tiles, that pairs of CTAs share them by two or by four: along the width, along the hidden units, along the rows
+LONG = [(64, 130, 2100), (200, 64, 1100), (40, 1100, 64), (300, 600, 200), (2500, 40, 72), (1100, 64, 136), (2055, 33, 65)]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows,hidden,width", LONG)
+def test_gated_long_sums(rows, hidden, width, dtype):
+    x, w = normal((rows, width), dtype, 1), normal((2 * hidden, width), dtype, 2, width ** -0.5)
+    check_gated(x, w, None, [0, rows], "gelu", dtype)
+    check_grad(normal((rows, hidden), dtype, 5), normal((rows, 2 * hidden), dtype, 6, 2.0), x, w, None, [0, rows], "gelu", dtype)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("counts,hidden,width", [([40, 0, 33], 96, 2100), ([70, 1, 5], 1100, 40), ([2100, 0, 1500, 33], 40, 72)])
+def test_gated_long_sums_by_expert(counts, hidden, width, dtype):
+    order, bounds = order_of(counts, 2, 5)
+    rows = 7 + sum(counts)
+    x, w = normal((rows, width), dtype, 3), normal((len(counts), 2 * hidden, width), dtype, 4, width ** -0.5)
+    dh, both = normal((rows, hidden), dtype, 5), normal((rows, 2 * hidden), dtype, 6, 2.0)
+    for t in (x, dh, both):
+        t[:2], t[bounds[-1]:] = float("nan"), float("nan")
+    check_gated(x, w, order, bounds, "silu", dtype)
+    check_grad(dh, both, x, w, order, bounds, "silu", dtype)
+
+
 COUNTS = [([0, 3, 0, 1, 9, 0], 0, 0), ([17, 0, 33, 2], 0, 5), ([100, 0, 1, 257, 64, 63], 0, 3), ([0, 0], 0, 40), ([300], 3, 0), ([40, 500, 0], 2, 7), ([1] * 70, 0, 0), ([65] * 40, 1, 1)]
 
 
@@ -289,7 +314,7 @@ def check_int8(a, w, order, bounds, dtype, codes_a, scales_a, codes_w, scales_w)
 
 @pytest.mark.parametrize("dtype", [torch.float32, *HALVES])
 @pytest.mark.parametrize("rows,n,inner", [(1, 1, 1), (1, 17, 4096), (7, 100, 33), (8, 16, 64), (13, 129, 300), (32, 40, 1000), (33, 40, 1000), (33, 8, 7), (64, 256, 128), (100, 300, 129),
-                                          (257, 513, 640), (700, 1500, 1100)])
+                                          (257, 513, 640), (700, 1500, 1100), (50, 300, 4100), (130, 200, 2100)])
 def test_int8_product(rows, n, inner, dtype):
     x, w = normal((rows, inner), torch.float32, 1), normal((n, inner), torch.float32, 2, 0.05)
     (qa, sa), (qw, sw) = codes64(x), codes64(w)
