@@ -204,16 +204,29 @@ __global__ void __launch_bounds__(NT, 8) k_scale(const __grid_constant__ Spans<N
     }
 }
 
-constexpr int FEW = 32, MANY = 512;
+constexpr int FEW = 32, SOME = 128, MANY = 512;  // tensors of a launch: what its parameters hold is copied with it
+
+// With a pointer to the tensors: passed by value they are copied three times on the way, 14 KB of them in a microsecond each.
+int launch_spans(const char *name, const void *kernel, int ctas, void **args, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3(NT), cfg.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early, cfg.numAttrs = 1;
+    LaunchScope scope(name, stream);
+    NB200_CUDA(cudaLaunchKernelExC(&cfg, kernel, args));
+    return NB200_OK;
+}
 
 bool span_ok(const nb200_span &s) {
     if (s.count < 0 || s.type < NB200_F32 || s.type > NB200_BF16 || s.to_type < NB200_F32 || s.to_type > NB200_BF16) return false;
     if (s.count == 0) return true;
-    return s.from && s.to && reinterpret_cast<uintptr_t>(s.from) % type_size(s.type) == 0 && reinterpret_cast<uintptr_t>(s.to) % type_size(s.to_type) == 0 &&
+    return s.from && s.to && (reinterpret_cast<uintptr_t>(s.from) & (type_size(s.type) - 1)) == 0 && (reinterpret_cast<uintptr_t>(s.to) & (type_size(s.to_type) - 1)) == 0 &&
            (s.from != s.to || s.type == s.to_type);
 }
 
-int64_t launches_of(int64_t n) { return n <= FEW ? 1 : (n + MANY - 1) / MANY; }
+int64_t launches_of(int64_t n) { return n <= SOME ? 1 : (n + MANY - 1) / MANY; }
 
 template <int N>
 int clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, double *partial, cudaStream_t stream) {
@@ -226,7 +239,7 @@ int clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, double
             s.from[i] = x.from, s.to[i] = x.to, s.count[i] = x.count, s.type[i] = (uint8_t)x.type, s.to_type[i] = (uint8_t)x.to_type;
             s.words[i] = reinterpret_cast<uintptr_t>(x.from) % 16 == 0 && reinterpret_cast<uintptr_t>(x.to) % 16 == 0;
             s.first[i] = (int32_t)chunks;
-            chunks += (x.count + chunk_elements(x.type) - 1) / chunk_elements(x.type);
+            chunks += x.type == NB200_F32 ? (x.count + chunk_elements(NB200_F32) - 1) / chunk_elements(NB200_F32) : (x.count + chunk_elements(NB200_F16) - 1) / chunk_elements(NB200_F16);
             if (chunks > INT32_MAX) return (int)NB200_E_UNSUPPORTED;
         }
         for (int i = s.n; i <= N; ++i) s.first[i] = (int32_t)chunks;
@@ -237,14 +250,16 @@ int clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, double
     for (int64_t l = 0; l < launches; ++l) {
         if ((st = fill(l, s))) return st;
         const int ctas = std::max(1, std::min(s.first[N], SUM_CTAS));
-        LaunchScope scope("clip_squares", stream);
-        NB200_CUDA(launch_overlapped(k_squares<N>, dim3((unsigned)ctas), dim3(NT), 0, stream, s, partial + partials));
+        double *const at = partial + partials;
+        void *args[] = {&s, const_cast<double **>(&at)};
+        if ((st = launch_spans("clip_squares", reinterpret_cast<const void *>(k_squares<N>), ctas, args, stream))) return st;
         partials += ctas;
     }
     for (int64_t l = launches - 1; l >= 0; --l) {
         if (launches > 1) fill(l, s);
-        LaunchScope scope("clip_scale", stream);
-        NB200_CUDA(launch_overlapped(k_scale<N>, dim3((unsigned)std::max(1, std::min(s.first[N], SCALE_CTAS))), dim3(NT), 0, stream, s, partial, partials, max_norm, norm));
+        const double *const sums = partial;
+        void *args[] = {&s, const_cast<const double **>(&sums), &partials, &max_norm, &norm};
+        if ((st = launch_spans("clip_scale", reinterpret_cast<const void *>(k_scale<N>), std::max(1, std::min(s.first[N], SCALE_CTAS)), args, stream))) return st;
     }
     return NB200_OK;
 }
@@ -269,7 +284,8 @@ int nb200_clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, 
     if (scratch_bytes < bytes) return NB200_E_CAPACITY;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     double *partial = static_cast<double *>(scratch);
-    return n <= FEW ? clip<FEW>(spans, n, max_norm, norm, partial, stream) : clip<MANY>(spans, n, max_norm, norm, partial, stream);
+    if (n <= FEW) return clip<FEW>(spans, n, max_norm, norm, partial, stream);
+    return n <= SOME ? clip<SOME>(spans, n, max_norm, norm, partial, stream) : clip<MANY>(spans, n, max_norm, norm, partial, stream);
 }
 
 }  // extern "C"
