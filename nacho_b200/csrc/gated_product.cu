@@ -237,9 +237,24 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
     if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, false, stream))) return st;
     TileMaps maps{};
     TileArgs args{};
-    if ((st = describe_rows(&maps.wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16)) ||
-        (st = describe_rows(&maps.narrow, map_type(x->type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 32)) || (st = describe_result(&maps.y, &args.words, map_type(x->type), *h, 1)))
-        return st;
+    int clusters[2];
+    if ((st = with_half(x->type, [&](auto e) { return tile_clusters<sum_of<decltype(e)>, Form::GATED, false, decltype(e)>(clusters); }))) return st;
+    args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows, args.wide = (int)hidden, args.blocks = (int)((x->cols + 63) / 64);
+    args.pairs = (int)all_pairs();
+    const TileWork::Way way = TileWork{x->rows, groups, (hidden + TILE_M / 2 - 1) / (TILE_M / 2), args.blocks}.best(args.pairs, clusters);
+    args.tile_n = way.n, args.parts = way.parts;
+    // Sixteen rows of gates and sixteen of values in turn: as one box where the hidden units are sixteens, else by boxes of 16 rows (4096 x 8192 x 4096 368 us that way
+    // where the clocks hold, 337 by one box).
+    args.in_turn = hidden % 16 == 0;
+    if (args.in_turn) {
+        const cuuint64_t pitch = (cuuint64_t)(w->rows > 1 ? aw.stride : pitch_of(w->cols)) * 2;
+        const cuuint64_t extents[5] = {(cuuint64_t)w->cols, 16, 2, (cuuint64_t)hidden / 16, (cuuint64_t)groups}, pitches[4] = {pitch, pitch * hidden, pitch * 16, pitch * 2 * hidden};
+        const cuuint32_t box[5] = {64, 16, 2, 4, 1};
+        st = encode_matrix(&maps.wide, map_type(w->type), 5, aw.data, extents, pitches, box);
+    } else {
+        st = describe_rows(&maps.wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16);
+    }
+    if (st || (st = describe_narrow(&maps, map_type(x->type), ax.data, 2, x->cols, x->rows, ax.stride, way.n)) || (st = describe_result(&maps.y, &args.words, map_type(x->type), *h, 1))) return st;
     if (both) {
         args.words = args.words && word_bytes({both}) == 16;
         // gates and values as two matrices, so that a tile of one ends where the other begins
@@ -247,15 +262,9 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
         const cuuint32_t box[3] = {64, 1, 32};
         if (args.words && (st = encode_matrix(&maps.both, map_type(x->type), 3, both->data, extents, pitches, box))) return st;
     }
-    args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows, args.wide = (int)hidden, args.blocks = (int)((x->cols + 63) / 64);
     args.y = h->data, args.stride = h->rows > 1 ? h->stride : h->cols, args.both = both ? both->data : nullptr, args.gelu = gelu;
     return with_half(x->type, [&](auto e) {
         using T = decltype(e);
-        int clusters[2];
-        if ((st = tile_clusters<sum_of<T>, Form::GATED, false, T>(clusters))) return st;
-        args.pairs = (int)all_pairs();
-        const TileWork::Way way = TileWork{x->rows, groups, (hidden + TILE_M / 2 - 1) / (TILE_M / 2), args.blocks}.best(args.pairs, clusters);
-        args.tile_n = way.n, args.parts = way.parts;
         return launch_tiles<sum_of<T>, Form::GATED, false, T>("gated_product", args, maps, stream);
     });
 }
@@ -311,7 +320,7 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
         args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows;
         // dx: the weights' columns on the wide side
         if ((st = describe_rows(&maps.wide, map_type(type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 64)) ||
-            (st = describe_rows(&maps.narrow, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 32)) || (st = describe_result(&maps.y, &args.words, map_type(type), *dx, 1)))
+            (st = describe_narrow(&maps, map_type(type), s.d, 2, 2 * hidden, x->rows, pitch, plan.x.n)) || (st = describe_result(&maps.y, &args.words, map_type(type), *dx, 1)))
             return st;
         args.wide = (int)x->cols, args.blocks = (int)((2 * hidden + 63) / 64), args.tile_n = plan.x.n, args.parts = plan.x.parts, args.pairs = plan.pairs_x;
         args.y = dx->data, args.stride = dx->rows > 1 ? dx->stride : dx->cols;

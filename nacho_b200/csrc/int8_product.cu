@@ -250,16 +250,15 @@ static int int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t 
         }
         TileMaps maps{};
         TileArgs args{};
-        if ((st = describe_rows(&maps.wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, w->values, 1, pitch, w->rows, groups, pitch, 128)) ||
-            (st = describe_rows(&maps.narrow, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, 1, pitch, 32)) ||
-            (st = describe_result(&maps.y, &args.words, map_type(y->type), *y, 1)))
-            return st;
-        args.offsets = offsets, args.groups = w->groups, args.rows = a->rows, args.wide = w->rows, args.blocks = (int)((a->cols + 127) / 128);
         int clusters[2];
         if ((st = tile_clusters<Sum::S8, Form::ROWS, false, T>(clusters))) return st;
+        args.offsets = offsets, args.groups = w->groups, args.rows = a->rows, args.wide = w->rows, args.blocks = (int)((a->cols + 127) / 128);
         args.pairs = (int)all_pairs();
         const TileWork::Way way = TileWork{a->rows, groups, (w->rows + TILE_M - 1) / TILE_M, args.blocks}.best(args.pairs, clusters);
         args.tile_n = way.n, args.parts = way.parts;
+        if ((st = describe_rows(&maps.wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, w->values, 1, pitch, w->rows, groups, pitch, 128)) ||
+            (st = describe_narrow(&maps, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, pitch, way.n)) || (st = describe_result(&maps.y, &args.words, map_type(y->type), *y, 1)))
+            return st;
         args.starve = starve;
         args.y = y->data, args.stride = stride, args.row_scale = a->scales, args.col_scale = w->scales;
         return launch_tiles<Sum::S8, Form::ROWS, false, T>("int8_product", args, maps, stream);

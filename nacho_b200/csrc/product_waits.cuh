@@ -64,7 +64,7 @@ __device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity) {
 constexpr unsigned long long REPORT_OTHER = 1ull << 32;
 int report_of(cudaStream_t stream, Workspace **ws);
 
-// A matrix (or several of them, `rank` 3) as the copy engine sees it, in boxes of rows of 128 bytes, turned as the tensor cores take them; what lies
+// A matrix (or several of them, `rank` 3 to 5) as the copy engine sees it, in boxes of rows of 128 bytes, turned as the tensor cores take them; what lies
 // beyond it is read as zeros.
 int encode_matrix(CUtensorMap *map, CUtensorMapDataType type, int rank, void *data, const cuuint64_t *extents, const cuuint64_t *pitches, const cuuint32_t *box);
 

@@ -253,7 +253,7 @@ int encode_matrix(CUtensorMap *map, CUtensorMapDataType type, int rank, void *da
         encode = reinterpret_cast<encode_fn>(found);
         known.store(encode, std::memory_order_release);
     }
-    const cuuint32_t steps[3] = {1, 1, 1};
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     if (encode(map, type, (cuuint32_t)rank, data, extents, pitches, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return note_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");

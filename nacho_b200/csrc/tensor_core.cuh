@@ -182,6 +182,13 @@ __device__ __forceinline__ void load_tile(void *smem, const CUtensorMap *matrix,
                  : "memory");
 }
 
+// The same of a matrix of five extents, of which the second and third begin at zero.
+__device__ __forceinline__ void load_tile5(void *smem, const CUtensorMap *matrix, int x, int z, int group, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %4, %5}], [%6];" ::"r"(smem_u32(smem)),
+                 "l"(matrix), "r"(x), "r"(0), "r"(z), "r"(group), "r"(bar)
+                 : "memory");
+}
+
 // Four matrices of 8 x 8 words of 16 bits from the warp's registers (thread i has two neighbours of row i / 4) to shared memory, row r of matrix m to
 // the 16 bytes at the address that thread 8 m + r gives; TURNED: their columns.
 template <bool TURNED>

@@ -38,6 +38,7 @@ struct TileArgs {
     const float *row_scale, *col_scale;  // S8: of the rows, of every group's columns
     bool gelu;
     bool words;  // results in words of 16 bytes, whole tiles by the copy engine
+    bool in_turn;  // GATED: 64 rows of gates and 64 of values come by one copy
     bool beside;  // nothing here depends on the kernel in front, which has itself waited for all that was before it: no wait but at the end
     unsigned long long *report;
     uint64_t patience;
@@ -46,7 +47,7 @@ struct TileArgs {
 
 // The operands and the results as the copy engine sees them: boxes of rows of 128 bytes. Results: y [rows][columns], both [rows][2][hidden], z [group][rows][columns].
 struct TileMaps {
-    CUtensorMap wide, narrow, y, both;
+    CUtensorMap wide, narrow, narrow_whole, y, both;  // narrow_whole: boxes of half a tile's narrow side
 };
 
 // A tile of the result: its group (-1: there are no more), where its rows begin and how many there are (for WEIGHTS: its columns), its first column (row), and the blocks that are summed.
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
         mbar_init(&sh.drained, 1);
         mbar_fence_init();
         sh.failed = 0;
-        ask_for_map(&maps.wide), ask_for_map(&maps.narrow);
+        ask_for_map(&maps.wide), ask_for_map(B_TURNED ? &maps.narrow : &maps.narrow_whole);
     }
     if (warp == TILE_MMA_WARP) tmem_alloc<true>(&sh.tmem, 512);
     tmem_fence_before();
@@ -534,10 +535,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                         uint8_t *const to_a = stage_a(stage.at), *const to_b = stage_b(stage.at);
                         if constexpr (GATED) {
                             const int col = t.col + rank * 64;
+                            if (args.in_turn) {
+                                load_tile5(to_a, &maps.wide, k, col / 16, t.g, bar);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                load_tile(to_a + i * 4096, &maps.wide, k, col + 16 * i, t.g, bar);
-                                load_tile(to_a + i * 4096 + 2048, &maps.wide, k, args.wide + col + 16 * i, t.g, bar);
+                                for (int i = 0; i < 4; ++i) {
+                                    load_tile(to_a + i * 4096, &maps.wide, k, col + 16 * i, t.g, bar);
+                                    load_tile(to_a + i * 4096 + 2048, &maps.wide, k, args.wide + col + 16 * i, t.g, bar);
+                                }
                             }
                         } else if constexpr (A_TURNED) {
                             const int col = t.col + rank * 128, g = FORM == Form::WEIGHTS ? 0 : t.g;
@@ -548,6 +553,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                         }
                         if constexpr (B_TURNED) {
                             for (int i = 0; i < mine; i += 64) load_tile(to_b + i * 128, &maps.narrow, begin + i, k, 0, bar);
+                        } else if (n == args.tile_n) {
+                            load_tile(to_b, &maps.narrow_whole, k, begin, 0, bar);
                         } else {
                             for (int i = 0; i < mine; i += 32) load_tile(to_b + i * 128, &maps.narrow, k, begin + i, 0, bar);
                         }
@@ -662,6 +669,11 @@ inline int describe_rows(CUtensorMap *map, CUtensorMapDataType type, void *data,
     const cuuint64_t pitches[2] = {pitch, groups > 1 ? pitch * (cuuint64_t)rows : pitch};
     const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
     return encode_matrix(map, type, 3, data, extents, pitches, box);
+}
+// The narrow operand by rows, in boxes for parts of a tile and for half of a whole one.
+inline int describe_narrow(TileMaps *maps, CUtensorMapDataType type, void *data, int64_t size, int64_t cols, int64_t rows, int64_t stride, int tile_n) {
+    const int st = describe_rows(&maps->narrow, type, data, size, cols, rows, 1, stride, 32);
+    return st ? st : describe_rows(&maps->narrow_whole, type, data, size, cols, rows, 1, stride, tile_n / 2);
 }
 // A result of `groups` matrices, if whole tiles of it can leave through the copy engine.
 inline int describe_result(CUtensorMap *map, bool *words, CUtensorMapDataType type, const nb200_dense &y, int64_t groups) {
