@@ -243,10 +243,9 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
     args.pairs = (int)all_pairs();
     const TileWork::Way way = TileWork{x->rows, groups, (hidden + TILE_M / 2 - 1) / (TILE_M / 2), args.blocks}.best(args.pairs, clusters);
     args.tile_n = way.n, args.parts = way.parts;
-    // Sixteen rows of gates and sixteen of values in turn: as one box where the hidden units are sixteens, else by boxes of 16 rows (4096 x 8192 x 4096 368 us that way
-    // where the clocks hold, 337 by one box).
-    args.in_turn = hidden % 16 == 0;
-    if (args.in_turn) {
+    // Sixteen rows of gates and sixteen of values in turn: as one box where the hidden units are sixteens, else by boxes of 16 rows.
+    args.whole_wide = hidden % 16 == 0;
+    if (args.whole_wide) {
         const cuuint64_t pitch = (cuuint64_t)(w->rows > 1 ? aw.stride : pitch_of(w->cols)) * 2;
         const cuuint64_t extents[5] = {(cuuint64_t)w->cols, 16, 2, (cuuint64_t)hidden / 16, (cuuint64_t)groups}, pitches[4] = {pitch, pitch * hidden, pitch * 16, pitch * 2 * hidden};
         const cuuint32_t box[5] = {64, 16, 2, 4, 1};
@@ -254,7 +253,7 @@ int nb200_gated_product(const nb200_dense *x, const nb200_dense *w, int32_t grou
     } else {
         st = describe_rows(&maps.wide, map_type(w->type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 16);
     }
-    if (st || (st = describe_narrow(&maps, map_type(x->type), ax.data, 2, x->cols, x->rows, ax.stride, way.n)) || (st = describe_result(&maps.y, &args.words, map_type(x->type), *h, 1))) return st;
+    if (st || (st = describe_narrow(&maps, &args, map_type(x->type), ax.data, 2, x->cols, x->rows, ax.stride)) || (st = describe_result(&maps.y, &args.words, map_type(x->type), *h, 1))) return st;
     if (both) {
         args.words = args.words && word_bytes({both}) == 16;
         // gates and values as two matrices, so that a tile of one ends where the other begins
@@ -319,20 +318,23 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
         TileArgs args{};
         args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows;
         // dx: the weights' columns on the wide side
-        if ((st = describe_rows(&maps.wide, map_type(type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 64)) ||
-            (st = describe_narrow(&maps, map_type(type), s.d, 2, 2 * hidden, x->rows, pitch, plan.x.n)) || (st = describe_result(&maps.y, &args.words, map_type(type), *dx, 1)))
-            return st;
         args.wide = (int)x->cols, args.blocks = (int)((2 * hidden + 63) / 64), args.tile_n = plan.x.n, args.parts = plan.x.parts, args.pairs = plan.pairs_x;
         args.y = dx->data, args.stride = dx->rows > 1 ? dx->stride : dx->cols;
+        if ((st = describe_turned(&maps.wide, &args.whole_wide, map_type(type), aw.data, w->cols, 2 * hidden, groups, aw.stride, 2)) ||
+            (!args.whole_wide && (st = describe_rows(&maps.wide, map_type(type), aw.data, 2, w->cols, 2 * hidden, groups, aw.stride, 64))) ||
+            (st = describe_narrow(&maps, &args, map_type(type), s.d, 2, 2 * hidden, x->rows, pitch)) || (st = describe_result(&maps.y, &args.words, map_type(type), *dx, 1)))
+            return st;
         if ((st = launch_tiles<sum_of<T>, Form::ROWS, true, T>("gated_grad_x", args, maps, stream))) return st;
         // dw: both operands turned
         args.beside = true;
-        if ((st = describe_rows(&maps.wide, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 64)) ||
-            (st = describe_rows(&maps.narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)) ||
-            (st = describe_result(&maps.y, &args.words, map_type(type), *dw, groups)))
-            return st;
         args.wide = (int)(2 * hidden), args.across = (int)x->cols, args.tile_n = plan.w.n, args.parts = plan.w.parts, args.pairs = plan.pairs_w;
         args.y = dw->data, args.stride = dw->rows > 1 ? dw->stride : dw->cols;
+        if ((st = describe_turned(&maps.wide, &args.whole_wide, map_type(type), s.d, 2 * hidden, x->rows, 1, pitch, 2)) ||
+            (!args.whole_wide && (st = describe_rows(&maps.wide, map_type(type), s.d, 2, 2 * hidden, x->rows, 1, pitch, 64))) ||
+            (st = describe_rows(&maps.narrow, map_type(type), ax.data, 2, x->cols, x->rows, 1, ax.stride, 64)) ||
+            (st = describe_turned(&maps.narrow_whole, &args.whole_narrow, map_type(type), ax.data, x->cols, x->rows, 1, ax.stride, args.tile_n % 128 == 0 ? args.tile_n / 128 : 0)) ||
+            (st = describe_result(&maps.y, &args.words, map_type(type), *dw, groups)))
+            return st;
         return launch_tiles<sum_of<T>, Form::WEIGHTS, true, T>("gated_grad_w", args, maps, stream);
     });
 }

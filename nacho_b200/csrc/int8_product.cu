@@ -257,7 +257,7 @@ static int int8_product(const nb200_int8 *a, const nb200_int8 *w, const int32_t 
         const TileWork::Way way = TileWork{a->rows, groups, (w->rows + TILE_M - 1) / TILE_M, args.blocks}.best(args.pairs, clusters);
         args.tile_n = way.n, args.parts = way.parts;
         if ((st = describe_rows(&maps.wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, w->values, 1, pitch, w->rows, groups, pitch, 128)) ||
-            (st = describe_narrow(&maps, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, pitch, way.n)) || (st = describe_result(&maps.y, &args.words, map_type(y->type), *y, 1)))
+            (st = describe_narrow(&maps, &args, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->values, 1, pitch, a->rows, pitch)) || (st = describe_result(&maps.y, &args.words, map_type(y->type), *y, 1)))
             return st;
         args.starve = starve;
         args.y = y->data, args.stride = stride, args.row_scale = a->scales, args.col_scale = w->scales;

@@ -182,6 +182,12 @@ __device__ __forceinline__ void load_tile(void *smem, const CUtensorMap *matrix,
                  : "memory");
 }
 
+// The same of a matrix of four extents, from its first column on.
+__device__ __forceinline__ void load_tile4(void *smem, const CUtensorMap *matrix, int y, int z, int group, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(smem)), "l"(matrix),
+                 "r"(0), "r"(y), "r"(z), "r"(group), "r"(bar)
+                 : "memory");
+}
 // The same of a matrix of five extents, of which the second and third begin at zero.
 __device__ __forceinline__ void load_tile5(void *smem, const CUtensorMap *matrix, int x, int z, int group, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %3, %4, %5}], [%6];" ::"r"(smem_u32(smem)),

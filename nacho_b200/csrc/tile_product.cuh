@@ -38,7 +38,8 @@ struct TileArgs {
     const float *row_scale, *col_scale;  // S8: of the rows, of every group's columns
     bool gelu;
     bool words;  // results in words of 16 bytes, whole tiles by the copy engine
-    bool in_turn;  // GATED: 64 rows of gates and 64 of values come by one copy
+    bool whole_wide;    // a block of the wide operand comes by one copy: 64 rows of gates and 64 of values, or 128 columns of a turned one
+    bool whole_narrow;  // a whole tile's of the narrow one
     bool beside;  // nothing here depends on the kernel in front, which has itself waited for all that was before it: no wait but at the end
     unsigned long long *report;
     uint64_t patience;
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                         uint8_t *const to_a = stage_a(stage.at), *const to_b = stage_b(stage.at);
                         if constexpr (GATED) {
                             const int col = t.col + rank * 64;
-                            if (args.in_turn) {
+                            if (args.whole_wide) {
                                 load_tile5(to_a, &maps.wide, k, col / 16, t.g, bar);
                             } else {
 #pragma unroll
@@ -546,14 +547,20 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                             }
                         } else if constexpr (A_TURNED) {
                             const int col = t.col + rank * 128, g = FORM == Form::WEIGHTS ? 0 : t.g;
-                            load_tile(to_a, &maps.wide, col, k, g, bar);
-                            load_tile(to_a + 8192, &maps.wide, col + 64, k, g, bar);
+                            if (args.whole_wide) {
+                                load_tile4(to_a, &maps.wide, k, col / 64, g, bar);
+                            } else {
+                                load_tile(to_a, &maps.wide, col, k, g, bar);
+                                load_tile(to_a + 8192, &maps.wide, col + 64, k, g, bar);
+                            }
                         } else {
                             load_tile(to_a, &maps.wide, k, t.col + rank * 128, t.g, bar);
                         }
                         if constexpr (B_TURNED) {
-                            for (int i = 0; i < mine; i += 64) load_tile(to_b + i * 128, &maps.narrow, begin + i, k, 0, bar);
-                        } else if (n == args.tile_n) {
+                            if (args.whole_narrow && n == args.tile_n) load_tile4(to_b, &maps.narrow_whole, k, begin / 64, 0, bar);
+                            else
+                                for (int i = 0; i < mine; i += 64) load_tile(to_b + i * 128, &maps.narrow, begin + i, k, 0, bar);
+                        } else if (args.whole_narrow && n == args.tile_n) {
                             load_tile(to_b, &maps.narrow_whole, k, begin, 0, bar);
                         } else {
                             for (int i = 0; i < mine; i += 32) load_tile(to_b + i * 128, &maps.narrow, k, begin + i, 0, bar);
@@ -670,10 +677,24 @@ inline int describe_rows(CUtensorMap *map, CUtensorMapDataType type, void *data,
     const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
     return encode_matrix(map, type, 3, data, extents, pitches, box);
 }
+// The engine takes a copy for every block of an operand, not so much its bytes: with boxes of 16 and 32 rows, 12 copies for a block, 4096 x 8192 x 4096 gated took 368 us
+// (where the clocks hold), with the largest ones 337.
+
 // The narrow operand by rows, in boxes for parts of a tile and for half of a whole one.
-inline int describe_narrow(TileMaps *maps, CUtensorMapDataType type, void *data, int64_t size, int64_t cols, int64_t rows, int64_t stride, int tile_n) {
+inline int describe_narrow(TileMaps *maps, TileArgs *args, CUtensorMapDataType type, void *data, int64_t size, int64_t cols, int64_t rows, int64_t stride) {
+    args->whole_narrow = true;
     const int st = describe_rows(&maps->narrow, type, data, size, cols, rows, 1, stride, 32);
-    return st ? st : describe_rows(&maps->narrow_whole, type, data, size, cols, rows, 1, stride, tile_n / 2);
+    return st ? st : describe_rows(&maps->narrow_whole, type, data, size, cols, rows, 1, stride, args->tile_n / 2);
+}
+// A turned operand of 16-bit elements in blocks of 64 columns by 64 rows, `blocks` of them in a box, if its columns are sixty-fours (a row's last block would reach into
+// the next row, the last row's beyond the matrix).
+inline int describe_turned(CUtensorMap *map, bool *whole, CUtensorMapDataType type, void *data, int64_t cols, int64_t rows, int64_t groups, int64_t stride, int blocks) {
+    *whole = cols % 64 == 0 && blocks > 0;
+    if (!*whole) return NB200_OK;
+    const cuuint64_t pitch = (cuuint64_t)(rows * groups > 1 ? stride : cols) * 2;
+    const cuuint64_t extents[4] = {64, (cuuint64_t)rows, (cuuint64_t)cols / 64, (cuuint64_t)groups}, pitches[3] = {pitch, 128, groups > 1 ? pitch * (cuuint64_t)rows : pitch};
+    const cuuint32_t box[4] = {64, 64, (cuuint32_t)blocks, 1};
+    return encode_matrix(map, type, 4, data, extents, pitches, box);
 }
 // A result of `groups` matrices, if whole tiles of it can leave through the copy engine.
 inline int describe_result(CUtensorMap *map, bool *words, CUtensorMapDataType type, const nb200_dense &y, int64_t groups) {
