@@ -315,7 +315,8 @@ struct Finish {
         }
     }
 
-    // WEIGHTS: columns t.from + c .. of 32 rows, 64 of them in two parts
+    // WEIGHTS: columns t.from + c .. of 32 rows, 64 of them in two parts. (Written by the threads, a row each, without a stop in shared memory, both gradients of 16
+    // experts took 535 us where this takes 520.)
     __device__ __forceinline__ void columns(const Place &t, int c, const uint32_t (&v)[2][32]) {
         const int row = t.col + rank * 128 + lanes * 32;
         uint8_t *const place = out + lanes * 6144;
