@@ -825,16 +825,25 @@ nb200_int8 view_int8(PyObject *o, View &v) {
     return nb200_int8{d[0], d[1], d[2], static_cast<int8_t *>(values.data_ptr()), floats(scales)};
 }
 
+// `n` elements of another type `offset` bytes into an array's memory, which both then hold: half of what a second allocation costs a call.
+at::Tensor part_of(const at::Tensor &t, int64_t offset, c10::IntArrayRef sizes, at::ScalarType type) {
+    const caffe2::TypeMeta meta = caffe2::TypeMeta::fromScalarType(type);
+    at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), meta);
+    part.unsafeGetTensorImpl()->set_storage_offset(offset / (int64_t)meta.itemsize());
+    part.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return part;
+}
+
 struct Int8Result {
     at::Tensor values, scales;
     nb200_int8 m{};
 
     Int8Result(int64_t groups, int64_t rows, int64_t cols, c10::Device dev, const char *where) {
         m = nb200_int8{(int32_t)groups, (int32_t)rows, (int32_t)cols, nullptr, nullptr};
-        const int64_t n = with_scratch(nb200_int8_value_count(&m), where), s = groups * rows;
-        values = array(n, at::kChar, dev), scales = float_array(s, dev);
+        const int64_t n = with_scratch(nb200_int8_value_count(&m), where), s = groups * rows;  // n: whole rows of 32 bytes
+        values = array(n + s * (int64_t)sizeof(float), at::kChar, dev), scales = part_of(values, n, s, at::kFloat);
         m.values = static_cast<int8_t *>(values.data_ptr()), m.scales = floats(scales);
-        used(values, n), used(scales, s);
+        used(values, n);
     }
     PyObject *object() {
         Result r(INT8);
@@ -956,9 +965,8 @@ PyObject *clip(PyObject *const *args) {
         while (next < read.size() && read[next].second <= w.first) ++next;
         if (next < read.size() && read[next].first < w.second) refuse(PyExc_ValueError, "%s: %s overlap one another in memory", where, what);
     }
-    at::Tensor norm = at::Tensor(at::detail::empty_cuda(c10::IntArrayRef(), at::kFloat, device, std::nullopt));
-    const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);
-    at::Tensor scratch = array(bytes, at::kByte, device);
+    const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);  // some KB, behind which the norm lies
+    at::Tensor scratch = array(bytes + (int64_t)sizeof(float), at::kByte, device), norm = part_of(scratch, bytes, c10::IntArrayRef(), at::kFloat);
     View v;
     v.device = device;
     launch({&v}, where, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });
