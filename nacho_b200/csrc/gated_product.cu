@@ -185,7 +185,7 @@ struct GradScratch {
 };
 
 // The two products of the gradient, which do not wait for one another: with all pairs of CTAs each, or, where their tiles would leave many of them idle, with a
-// part each (1003 rows of 1100 x 1101 gates and values: 37 us one after the other, 28 beside one another).
+// part each (1003 rows by 1101 hidden units and a width of 1100: 37 us one after the other, 31 beside one another; 64 rows of 4096 x 4096 62 and 39).
 struct GradPlan {
     TileWork::Way x, w;
     int pairs_x, pairs_w;

@@ -358,9 +358,10 @@ struct Stages {
 };
 
 // Pairs of CTAs, one CTA per SM, take tiles of 256 x 256 at most in turn. One warp finds out where they lie, some ahead of the others (half a dozen divisions and
-// the group's offsets: found by every warp for itself at the tile's beginning, the matrix instructions of short sums waited for it), one brings blocks of 128 bytes of both operands into shared memory (the copy
-// engine's tiled form, which turns them as the tensor cores take them and fills up with zeros what lies beyond a matrix), one issues the matrix instructions, and
-// eight read the sums of a whole tile while those of the next one are made: tensor memory holds two.
+// the group's offsets: found by every warp for itself at the tile's beginning, the matrix instructions of short sums waited for it), one brings blocks of 128
+// bytes of both operands into shared memory (the copy engine's tiled form, which turns them as the tensor cores take them and fills up with zeros what lies
+// beyond a matrix), one issues the matrix instructions, and eight read the sums of a whole tile while those of the next one are made: tensor memory holds two.
+// 4096 x 8192 x 4096 gated: 322 us where the clocks hold (tensor cores busy 94 %), 413 under the power cap; 8192^3 in integers 300 us.
 //
 // GATED: 16 rows of gates and 16 of values alternate in the wide operand's tile, so that a gate and its value lie 16 lanes apart in tensor memory and fragments
 // of both land in the same thread.

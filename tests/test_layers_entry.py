@@ -12,7 +12,11 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 def call(body):
     """Runs `body` in a process of its own that sees no GPU, so that nothing is ever launched on the made-up addresses; what it printed."""
-    script = "import ctypes as C\nfrom nacho_b200 import _capi\nfrom nacho_b200._capi import DenseStruct as D, Int8Struct as I, SpanStruct as S, lib, OK, E_BADARG as BAD, E_UNSUPPORTED as UN, E_CAPACITY as CAP, E_CUDA as CUDA\nr = C.byref\n" + body
+    script = """import ctypes as C
+from nacho_b200._capi import DenseStruct as D, Int8Struct as I, SpanStruct as S, lib
+from nacho_b200._capi import OK, E_BADARG as BAD, E_UNSUPPORTED as UN, E_CAPACITY as CAP, E_CUDA as CUDA
+r = C.byref
+""" + body
     r = subprocess.run([sys.executable, "-c", script], cwd=ROOT, env={**os.environ, "CUDA_VISIBLE_DEVICES": ""}, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stderr)
     return r.stdout.split()
