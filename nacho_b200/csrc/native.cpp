@@ -967,6 +967,7 @@ PyObject *clip(PyObject *const *args) {
     }
     const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);  // some KB, behind which the norm lies
     at::Tensor scratch = array(bytes + (int64_t)sizeof(float), at::kByte, device), norm = part_of(scratch, bytes, c10::IntArrayRef(), at::kFloat);
+    for (const at::Tensor &z : to) z.unsafeGetTensorImpl()->bump_version();  // refuses a tensor that must not be written here
     View v;
     v.device = device;
     launch({&v}, where, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });
@@ -978,10 +979,8 @@ PyObject *clip(PyObject *const *args) {
         last = p.get();
     };
     for (const at::Tensor &x : from) record(x);
-    for (const at::Tensor &z : to) {
-        if (!in_place) record(z);
-        z.unsafeGetTensorImpl()->bump_version();
-    }
+    if (!in_place)
+        for (const at::Tensor &z : to) record(z);
     return wrap(norm);
 }
 

@@ -96,9 +96,10 @@ def gpu_int8_product(a: INT8_gpu, w: INT8_gpu, order: ExpertOrder_gpu | None = N
 
 
 def gpu_clip_gradients(gradients, max_norm: float, out=None) -> torch.Tensor:
-    """The root of the sum of all elements' squares (a float32 tensor without dimensions), and every element times ``max_norm / (norm + 1e-6)`` where that is
-    below 1: in place, or into the tensors ``out`` of the same shapes, which may be of other types (32-bit ones that an optimiser reads, say). A norm that is
-    no finite number changes nothing, so that a caller who sees it can leave the step out. The tensors must not overlap in memory."""
+    """The root of the sum of all elements' squares of a list or tuple of tensors (a float32 tensor without dimensions), and every element times
+    ``max_norm / (norm + 1e-6)`` where that is below 1: in place, or into the tensors ``out`` of the same shapes, which may be of other types (32-bit ones
+    that an optimiser reads, say). A norm that is no finite number changes nothing, so that a caller who sees it can leave the step out. The tensors must not
+    overlap in memory."""
     limit = float(max_norm)
     if not limit >= 0:
         raise ValueError("gpu_clip_gradients: max_norm must not be negative")

@@ -680,3 +680,9 @@ def test_clipping_counts_as_a_change_in_place():
     version = t._version
     nacho().gpu_clip_gradients([t], 0.1)
     assert t._version > version
+    with torch.inference_mode():
+        frozen = torch.ones(10, device="cuda")
+        assert abs(float(nacho().gpu_clip_gradients([frozen], 1e9)) - math.sqrt(10)) <= 1e-5
+    with pytest.raises(RuntimeError):  # as any change in place of such a tensor out there
+        nacho().gpu_clip_gradients([frozen], 0.1)
+    assert bool((frozen == 1).all())
