@@ -184,25 +184,31 @@ struct GradScratch {
     }
 };
 
-// The two products of the gradient, which do not wait for one another: with all pairs of CTAs each, or, where their tiles would leave many of them idle, with a
-// part each (1003 rows by 1101 hidden units and a width of 1100: 37 us one after the other, 31 beside one another; 64 rows of 4096 x 4096 62 and 39).
+// The two products of the gradient, which do not wait for one another: with all pairs of CTAs each, or, where their tiles would leave many of them idle, rows' gradient with the pairs
+// that it needs and the weights' with the rest (128 rows of 4096 x 4096: one after the other 48 us, beside one another 40; 1003 rows by 1101 hidden units and a width of 1100: 37 and 27).
+// A tile of the weights' gradient waits for its results to leave where it sums little: 512 tiles of 256 x 256 over 128 rows take 18 us, of which their blocks are 5.
 struct GradPlan {
+    static constexpr int64_t RESULTS = 4, LAUNCH = 4000;  // rows of blocks: for a column of such a tile; for one more kernel in a row
     TileWork::Way x, w;
     int pairs_x, pairs_w;
 
     GradPlan(int64_t rows, int64_t width, int64_t hidden, int64_t groups, const int (&clusters)[2]) {
         const int64_t high = (2 * hidden + TILE_M - 1) / TILE_M, all = all_pairs();
-        const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64}, work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64};
+        const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64};
+        const TileWork work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64, RESULTS};
         x = work_x.best(all, clusters), w = work_w.best(all, clusters);
         pairs_x = pairs_w = (int)all;
-        double least = (x.cost + w.cost) * 7 / 8;  // worth the smaller launches
+        double least = (x.cost + w.cost) * 7 / 8 + LAUNCH;  // parts of the pairs are shared out once: worth it where it gives more than that
         for (int64_t k = 1; k < 16; ++k) {
             const int64_t part = all * k / 16;
             if (part < 1 || part >= all) continue;
             // clusters have to find room beside the other product's CTAs
-            const int half[2] = {clusters[0] * (int)k / 16, clusters[1] * (int)k / 16}, rest[2] = {clusters[0] - half[0] - 1, clusters[1] - half[1] - 1};
-            const TileWork::Way a = work_x.best(part, half), b = work_w.best(all - part, rest);
-            if (std::max(a.cost, b.cost) < least) least = std::max(a.cost, b.cost), x = a, w = b, pairs_x = (int)part, pairs_w = (int)(all - part);
+            const int half[2] = {clusters[0] * (int)k / 16, clusters[1] * (int)k / 16};
+            const TileWork::Way a = work_x.best(part, half);
+            const int64_t mine = std::min(part, work_x.most(a.n) * a.parts), other = all - mine;
+            const int rest[2] = {(int)(clusters[0] * other / all) - 1, (int)(clusters[1] * other / all) - 1};
+            const TileWork::Way b = work_w.best(other, rest);
+            if (std::max(a.cost, b.cost) < least) least = std::max(a.cost, b.cost), x = a, w = b, pairs_x = (int)mine, pairs_w = (int)other;
         }
     }
 };

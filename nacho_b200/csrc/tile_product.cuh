@@ -708,9 +708,10 @@ inline CUtensorMapDataType map_type(int type) { return type == NB200_F16 ? CU_TE
 
 inline int64_t all_pairs() { return std::max(1, sm_count() / 2); }
 
-// A product as tiles: `rows` on the narrow side of all groups together, `wide_tiles` beside one another on the wide one, `blocks` summed for each.
+// A product as tiles: `rows` on the narrow side of all groups together, `wide_tiles` beside one another on the wide one, `blocks` summed for each. `results`: what the products wait
+// for while a column of a tile leaves, in the cost's rows of blocks.
 struct TileWork {
-    int64_t rows, groups, wide_tiles, blocks;
+    int64_t rows, groups, wide_tiles, blocks, results = 0;
 
     // How it goes on so many pairs of CTAs: the narrow side of its tiles, a multiple of 64, the pairs that share a tile's blocks, and what the busiest pair then has to
     // bring, in rows of blocks: 256 of the wide side and n of the narrow one for every tile and block (1330 of them take a microsecond); adding up parts takes as long
@@ -719,17 +720,21 @@ struct TileWork {
         int n, parts;
         double cost;
     };
+    // Tiles at most, however the groups share the rows: each one that has any may leave one tile unfilled.
+    int64_t most(int n) const { return (rows + std::min(groups, rows) * (n - 1)) / n * wide_tiles; }
+
     // Parts: as many pairs as find room for all tiles at once, of at least eight blocks each (`clusters`: of four and eight CTAs that the device holds. A second round
-    // costs more than parts give: 16 tiles of 32 blocks take 19 us in four parts, of which the device holds fewer than 16, and 10 in two).
+    // costs more than parts give: 16 tiles of 32 blocks take 19 us in four parts, of which the device holds fewer than 16, and 10 in two). A launch has a cluster for
+    // every tile that there can be.
     Way best(int64_t pairs, const int (&clusters)[2]) const {
         const int64_t mean = (rows + groups - 1) / groups;
         Way way{0, 1, 0};
         for (int n = TILE_N; n >= 64; n -= 64) {
-            const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, each = TILE_M + std::min<int64_t>(n, mean);
+            const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, all = std::max(tiles, most(n)), each = TILE_M + std::min<int64_t>(n, mean);
             for (int k = 0; k < 3; ++k) {
                 const int parts = 1 << k;
-                if (parts > 1 && (tiles * parts > pairs || tiles > clusters[k - 1] || blocks < 8 * parts)) break;
-                const double cost = (double)((tiles + pairs - 1) / pairs) * (double)each * (double)((blocks + parts - 1) / parts) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
+                if (parts > 1 && (all * parts > pairs || all > clusters[k - 1] || blocks < 8 * parts)) break;
+                const double cost = (double)((tiles + pairs - 1) / pairs) * ((double)each * (double)((blocks + parts - 1) / parts) + (double)(results * std::min<int64_t>(n, mean))) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
                 if (way.n == 0 || cost < way.cost) way = Way{n, parts, cost};
             }
         }
@@ -753,15 +758,15 @@ int launch_tiles(const char *name, TileArgs args, const TileMaps &maps, cudaStre
     if ((st = report_of(stream, &ws))) return st;
     args.report = reinterpret_cast<unsigned long long *>(ws->host) + 32;
     const int64_t per_tile = FORM == Form::GATED ? TILE_M / 2 : TILE_M, wide = (args.wide + per_tile - 1) / per_tile;
-    const int64_t tiles = FORM == Form::WEIGHTS ? (int64_t)args.groups * ((args.across + args.tile_n - 1) / args.tile_n) * wide
-                                                : (args.rows / args.tile_n + (int64_t)args.groups) * wide;
+    const TileWork work = FORM == Form::WEIGHTS ? TileWork{args.across, 1, args.groups * wide, 0} : TileWork{args.rows, args.groups, wide, 0};
+    const int64_t tiles = work.most(args.tile_n);
     if (tiles > INT32_MAX / 64 || args.rows > INT32_MAX - 1024 || args.wide > INT32_MAX / 2 - 1024 || args.across > INT32_MAX - 1024) return NB200_E_UNSUPPORTED;
     args.most = (int)tiles;
     args.patience = args.starve ? SHORT_PATIENCE : PATIENCE;
     args.b_bytes = FORM == Form::WEIGHTS ? (args.tile_n / 2 + 63) / 64 * 8192 : args.tile_n / 2 * 128;
     args.stages = std::min(TileShared::STAGES, TileShared::STAGE_BYTES / (TileShared::A_BYTES + args.b_bytes));
     auto split = k_tiles<SUM, FORM, A_TURNED, true, T>;
-    const int parts = tiles * args.parts <= args.pairs ? args.parts : 1;  // groups may begin and end inside tiles: there may be more than the way counts
+    const int parts = args.parts;
     const int64_t ctas = parts > 1 ? tiles * 2 * parts : 2 * std::max<int64_t>(1, std::min<int64_t>(tiles, args.pairs));
     auto go = [&](auto kernel) -> int {
         if ((st = allow_shared(kernel, TILE_SHARED_BYTES))) return st;

@@ -155,3 +155,51 @@ int main() {
 }""")
     subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "rule"), str(tmp_path / "rule.cpp")], check=True)
     assert subprocess.run([str(tmp_path / "rule")], check=True, capture_output=True, text=True).stdout.split() == ["1"]
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="no host compiler")
+def test_the_tiles_that_a_product_is_launched_for(tmp_path):
+    """One count of tiles for the choice and for the launch: what groups that share the rows in any way have at most, for one group what it has, and with parts no more
+    than find room. 256 rows of 4096 hidden units and a width of 8192, a multiple of every narrow side, are shared by two."""
+    text = open(os.path.join(ROOT, "nacho_b200", "csrc", "tile_product.cuh")).read()
+    rule = text[text.index("struct TileWork {"):]
+    launch = text[text.index("int launch_tiles("):]
+    # the launch takes over what was chosen, for as many tiles as were counted then
+    assert "work.most(args.tile_n)" in launch and re.search(r"parts = args\.parts;", launch)
+    (tmp_path / "count.cpp").write_text("""
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+#include <random>
+constexpr int TILE_M = 256, TILE_N = 256;
+""" + rule[:rule.index("\n};") + 4] + """
+int main() {
+    const int clusters[2] = {33, 14};
+    int shared = 0, bad = 0;
+    for (long long rows = 1; rows <= 1100; ++rows)
+        for (long long wide : {1ll, 6ll, 8ll, 32ll, 64ll}) for (long long blocks : {1ll, 16ll, 128ll, 256ll}) for (long long pairs : {9ll, 37ll, 74ll}) {
+            const TileWork work{rows, 1, wide, blocks};
+            const TileWork::Way way = work.best(pairs, clusters);
+            const long long tiles = (rows + way.n - 1) / way.n * wide;
+            bad += work.most(way.n) != tiles || (way.parts > 1 && (tiles * way.parts > pairs || tiles > clusters[way.parts / 4]));
+            shared += way.parts > 1 && rows % way.n == 0;
+        }
+    std::mt19937 draw(1);
+    for (int i = 0; i < 20000; ++i) {
+        const int groups = 1 + draw() % 40, n = 64 * (1 + draw() % 4);
+        long long rows = draw() % 30, tiles = 0;  // some rows of nobody
+        for (int g = 0; g < groups; ++g) {
+            const long long mine = draw() % 3 ? draw() % 300 : draw() % 2;
+            rows += mine, tiles += (mine + n - 1) / n;
+        }
+        if (rows == 0) continue;
+        const TileWork work{rows, groups, 3, 128};
+        bad += work.most(n) < 3 * tiles;
+        const TileWork::Way way = work.best(74, clusters);
+        bad += way.parts > 1 && (work.most(way.n) * way.parts > 74 || work.most(way.n) > clusters[way.parts / 4]);
+    }
+    const TileWork::Way way = TileWork{256, 1, 32, 128}.best(74, clusters);
+    printf("%d %d %d\\n", bad, shared > 0, (int)(way.parts == 2 && TileWork{256, 1, 32, 128}.most(way.n) == 32));
+}""")
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "count"), str(tmp_path / "count.cpp")], check=True)
+    assert subprocess.run([str(tmp_path / "count")], check=True, capture_output=True, text=True).stdout.split() == ["0", "1", "1"]

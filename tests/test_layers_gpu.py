@@ -686,3 +686,16 @@ def test_clipping_counts_as_a_change_in_place():
     with pytest.raises(RuntimeError):  # as any change in place of such a tensor out there
         nacho().gpu_clip_gradients([frozen], 0.1)
     assert bool((frozen == 1).all())
+
+
+# rows that a tile's narrow side divides, with sums so long that pairs share them
+@pytest.mark.parametrize("rows,hidden,width", [(64, 1024, 2048), (128, 512, 2100), (256, 640, 2048), (512, 256, 1100), (256, 72, 64)])
+def test_whole_tiles_of_long_sums(rows, hidden, width):
+    dtype = torch.bfloat16
+    x, w = normal((rows, width), dtype, 1), normal((2 * hidden, width), dtype, 2, width ** -0.5)
+    check_gated(x, w, None, [0, rows], "silu", dtype)
+    check_grad(normal((rows, hidden), dtype, 5), normal((rows, 2 * hidden), dtype, 6, 2.0), x, w, None, [0, rows], "silu", dtype)
+    order, bounds = order_of([rows // 2, 0, rows // 2])
+    check_gated(x, torch.stack([w, w, w.flip(0)]), order, bounds, "silu", dtype)
+    (qa, sa), (qw, sw) = codes64(x), codes64(w)
+    check_int8(nacho().to_int8_rows(x), nacho().to_int8_rows(w), None, [0, rows], torch.float32, qa, sa, qw[None], sw[None])
