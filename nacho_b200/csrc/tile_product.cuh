@@ -735,7 +735,9 @@ struct TileWork {
                 const int parts = 1 << k;
                 if (parts > 1 && (all * parts > pairs || all > clusters[k - 1] || blocks < 8 * parts)) break;
                 const double cost = (double)((tiles + pairs - 1) / pairs) * ((double)each * (double)((blocks + parts - 1) / parts) + (double)(results * std::min<int64_t>(n, mean))) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
-                if (way.n == 0 || cost < way.cost) way = Way{n, parts, cost};
+                // One group's tiles are no wider than its rows: a stage then has that much more room for others, and a tile comes by one copy. Groups share the rows
+                // unevenly: the wider side is for those that have more.
+                if (way.n == 0 || cost < way.cost || (groups == 1 && cost == way.cost && parts == way.parts)) way = Way{n, parts, cost};
             }
         }
         return way;

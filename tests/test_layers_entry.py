@@ -203,3 +203,25 @@ int main() {
 }""")
     subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "count"), str(tmp_path / "count.cpp")], check=True)
     assert subprocess.run([str(tmp_path / "count")], check=True, capture_output=True, text=True).stdout.split() == ["0", "1", "1"]
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="no host compiler")
+def test_narrow_sides_no_wider_than_the_rows(tmp_path):
+    """Few rows of one group take the narrow side that holds them, with which more stages fit."""
+    text = open(os.path.join(ROOT, "nacho_b200", "csrc", "tile_product.cuh")).read()
+    rule = text[text.index("struct TileWork {"):]
+    (tmp_path / "side.cpp").write_text("""
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+constexpr int TILE_M = 256, TILE_N = 256;
+""" + rule[:rule.index("\n};") + 4] + """
+int main() {
+    const int clusters[2] = {33, 14};
+    for (long long rows = 1; rows <= 256; ++rows) for (long long wide : {1ll, 8ll, 16ll, 32ll, 74ll, 300ll}) for (long long blocks : {1ll, 18ll, 64ll, 128ll}) {
+        const TileWork::Way way = TileWork{rows, 1, wide, blocks}.best(74, clusters);
+        if (way.n - 64 >= rows) printf("%lld %lld %lld: %d\\n", rows, wide, blocks, way.n);
+    }
+}""")
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "side"), str(tmp_path / "side.cpp")], check=True)
+    assert subprocess.run([str(tmp_path / "side")], check=True, capture_output=True, text=True).stdout == ""
