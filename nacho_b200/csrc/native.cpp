@@ -967,7 +967,11 @@ PyObject *clip(PyObject *const *args) {
     }
     const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);  // some KB, behind which the norm lies
     at::Tensor scratch = array(bytes + (int64_t)sizeof(float), at::kByte, device), norm = part_of(scratch, bytes, c10::IntArrayRef(), at::kFloat);
-    for (const at::Tensor &z : to) z.unsafeGetTensorImpl()->bump_version();  // refuses a tensor that must not be written here
+    // A tensor that must not be written here is refused before any of them counts as changed.
+    if (!c10::InferenceMode::is_enabled())
+        for (const at::Tensor &z : to)
+            if (z.is_inference()) refuse(PyExc_RuntimeError, "%s: %s of inference mode cannot be changed outside of it", where, in_place ? "gradients" : "out");
+    for (const at::Tensor &z : to) z.unsafeGetTensorImpl()->bump_version();
     View v;
     v.device = device;
     launch({&v}, where, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });

@@ -699,3 +699,18 @@ def test_whole_tiles_of_long_sums(rows, hidden, width):
     check_gated(x, torch.stack([w, w, w.flip(0)]), order, bounds, "silu", dtype)
     (qa, sa), (qw, sw) = codes64(x), codes64(w)
     check_int8(nacho().to_int8_rows(x), nacho().to_int8_rows(w), None, [0, rows], torch.float32, qa, sa, qw[None], sw[None])
+
+
+@pytest.mark.parametrize("out", [False, True])
+def test_a_refused_clip_changes_nothing(out):
+    """The last tensor must not be written here: those in front do not count as changed."""
+    with torch.inference_mode():
+        frozen = torch.full((9,), 2.0, device="cuda")
+    given = [normal((30, 7), torch.float32, 1), normal((11,), torch.float32, 2)]
+    kept, versions = [t.clone() for t in given], [t._version for t in given]
+    with pytest.raises(RuntimeError, match="inference"):
+        if out:
+            nacho().gpu_clip_gradients([torch.ones_like(t) for t in (*given, frozen)], 0.1, [*given, frozen])
+        else:
+            nacho().gpu_clip_gradients([*given, frozen], 0.1)
+    assert [t._version for t in given] == versions and all(torch.equal(t, k) for t, k in zip(given, kept)) and bool((frozen == 2).all())
