@@ -965,8 +965,8 @@ PyObject *clip(PyObject *const *args) {
         while (next < read.size() && read[next].second <= w.first) ++next;
         if (next < read.size() && read[next].first < w.second) refuse(PyExc_ValueError, "%s: %s overlap one another in memory", where, what);
     }
-    const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);  // some KB, behind which the norm lies
-    at::Tensor scratch = array(bytes + (int64_t)sizeof(float), at::kByte, device), norm = part_of(scratch, bytes, c10::IntArrayRef(), at::kFloat);
+    const int64_t bytes = with_scratch(nb200_clip_scratch(spans.data(), (int64_t)spans.size()), where);
+    at::Tensor scratch = array(bytes, at::kByte, device), norm = at::Tensor(at::detail::empty_cuda({}, at::kFloat, device, std::nullopt));
     // A tensor that must not be written here is refused before any of them counts as changed.
     if (!c10::InferenceMode::is_enabled())
         for (const at::Tensor &z : to)

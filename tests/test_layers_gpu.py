@@ -714,3 +714,10 @@ def test_a_refused_clip_changes_nothing(out):
         else:
             nacho().gpu_clip_gradients([*given, frozen], 0.1)
     assert [t._version for t in given] == versions and all(torch.equal(t, k) for t, k in zip(given, kept)) and bool((frozen == 2).all())
+
+
+def test_a_norm_holds_nothing_else():
+    """Norms that are kept for a log hold four bytes each, however many tensors there were."""
+    for n in (1, 600):
+        norm = nacho().gpu_clip_gradients([normal((5, 3), torch.float32, i) for i in range(n)], 1.0)
+        assert norm.untyped_storage().nbytes() == 4 and norm.storage_offset() == 0
