@@ -825,25 +825,16 @@ nb200_int8 view_int8(PyObject *o, View &v) {
     return nb200_int8{d[0], d[1], d[2], static_cast<int8_t *>(values.data_ptr()), floats(scales)};
 }
 
-// `n` elements of another type `offset` bytes into an array's memory, which both then hold: half of what a second allocation costs a call.
-at::Tensor part_of(const at::Tensor &t, int64_t offset, c10::IntArrayRef sizes, at::ScalarType type) {
-    const caffe2::TypeMeta meta = caffe2::TypeMeta::fromScalarType(type);
-    at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), meta);
-    part.unsafeGetTensorImpl()->set_storage_offset(offset / (int64_t)meta.itemsize());
-    part.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    return part;
-}
-
 struct Int8Result {
     at::Tensor values, scales;
     nb200_int8 m{};
 
     Int8Result(int64_t groups, int64_t rows, int64_t cols, c10::Device dev, const char *where) {
         m = nb200_int8{(int32_t)groups, (int32_t)rows, (int32_t)cols, nullptr, nullptr};
-        const int64_t n = with_scratch(nb200_int8_value_count(&m), where), s = groups * rows;  // n: whole rows of 32 bytes
-        values = array(n + s * (int64_t)sizeof(float), at::kChar, dev), scales = part_of(values, n, s, at::kFloat);
+        const int64_t n = with_scratch(nb200_int8_value_count(&m), where), s = groups * rows;
+        values = array(n, at::kChar, dev), scales = float_array(s, dev);
         m.values = static_cast<int8_t *>(values.data_ptr()), m.scales = floats(scales);
-        used(values, n);
+        used(values, n), used(scales, s);
     }
     PyObject *object() {
         Result r(INT8);

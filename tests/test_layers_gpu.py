@@ -721,3 +721,9 @@ def test_a_norm_holds_nothing_else():
     for n in (1, 600):
         norm = nacho().gpu_clip_gradients([normal((5, 3), torch.float32, i) for i in range(n)], 1.0)
         assert norm.untyped_storage().nbytes() == 4 and norm.storage_offset() == 0
+
+
+@pytest.mark.parametrize("shape", [(40, 200), (1, 33), (3, 5, 64)])
+def test_scales_hold_no_codes(shape):
+    for z in (nacho().to_int8_rows(normal(shape, torch.float32, 1)), nacho().to_int8_rows(torch.ones(shape, dtype=torch.int8, device="cuda"), torch.ones(shape[:-1], device="cuda"))):
+        assert z.scales.untyped_storage().nbytes() == 4 * math.prod(shape[:-1]) and z.scales.storage_offset() == 0
