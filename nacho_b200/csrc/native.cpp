@@ -965,7 +965,7 @@ PyObject *clip(PyObject *const *args) {
     for (const at::Tensor &z : to) z.unsafeGetTensorImpl()->bump_version();
     View v;
     v.device = device;
-    launch({&v}, where, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });
+    const int status = run({&v}, [&](void *stream) { return nb200_clip(spans.data(), (int64_t)spans.size(), (float)max_norm, floats(norm), scratch.data_ptr(), bytes, stream); });
     const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(device.index());
     const void *last = nullptr;  // parts of one long buffer follow one another
     auto record = [&](const at::Tensor &t) {
@@ -976,6 +976,7 @@ PyObject *clip(PyObject *const *args) {
     for (const at::Tensor &x : from) record(x);
     if (!in_place)
         for (const at::Tensor &z : to) record(z);
+    check(status, where);  // behind that: of several launches the first may be under way
     return wrap(norm);
 }
 
