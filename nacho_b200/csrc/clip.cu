@@ -14,7 +14,8 @@ namespace {
 constexpr int NT = 256, TURNS = 4;              // threads; 16-byte chunks that a thread has on its way
 constexpr int CHUNK_BYTES = NT * TURNS * 16;    // what a CTA takes at a time, of the elements' own type
 // CTAs that are at work at once (500 M elements: summed 161 us, with eight per SM 167; scaled 345 us with four, 325 with eight).
-constexpr int SUM_CTAS = 4 * 148, SCALE_CTAS = 8 * 148;
+int sum_ctas() { return 4 * sm_count(); }
+int scale_ctas() { return 8 * sm_count(); }
 
 // A launch's tensors lie in its parameters: a captured graph has them with it.
 template <int N>
@@ -250,7 +251,7 @@ int clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, double
     Spans<N> s;
     for (int64_t l = 0; l < launches; ++l) {
         if ((st = fill(l, s))) return st;
-        const int ctas = std::max(1, std::min(s.first[N], SUM_CTAS));
+        const int ctas = std::max(1, std::min(s.first[N], sum_ctas()));
         double *const at = partial + partials;
         void *args[] = {&s, const_cast<double **>(&at)};
         if ((st = launch_spans("clip_squares", reinterpret_cast<const void *>(k_squares<N>), ctas, args, stream))) return st;
@@ -260,7 +261,7 @@ int clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, double
         if (launches > 1) fill(l, s);
         const double *const sums = partial;
         void *args[] = {&s, const_cast<const double **>(&sums), &partials, &max_norm, &norm};
-        if ((st = launch_spans("clip_scale", reinterpret_cast<const void *>(k_scale<N>), std::max(1, std::min(s.first[N], SCALE_CTAS)), args, stream))) return st;
+        if ((st = launch_spans("clip_scale", reinterpret_cast<const void *>(k_scale<N>), std::max(1, std::min(s.first[N], scale_ctas())), args, stream))) return st;
     }
     return NB200_OK;
 }
@@ -276,7 +277,7 @@ int64_t nb200_clip_scratch(const nb200_span *spans, int64_t n) {
     if (n < 0 || (n > 0 && !spans) || n > INT32_MAX) return -1;
     for (int64_t i = 0; i < n; ++i)
         if (!span_ok(spans[i])) return -1;
-    return std::max<int64_t>(1, launches_of(n)) * SUM_CTAS * (int64_t)sizeof(double);
+    return std::max<int64_t>(1, launches_of(n)) * sum_ctas() * (int64_t)sizeof(double);
 }
 
 int nb200_clip(const nb200_span *spans, int64_t n, float max_norm, float *norm, void *scratch, int64_t scratch_bytes, void *stream_) {
