@@ -272,16 +272,17 @@ __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, int rank) {
             "r"(rank)
             : "memory");
 }
-// A phase of this CTA's barrier that is over, for what arrivals with RELEASE stand for.
-__device__ __forceinline__ void mbar_acquire_cluster(uint64_t *bar, uint32_t parity) {
+// Whether a phase of this CTA's barrier is over; if so, what arrivals with RELEASE stand for is there.
+__device__ __forceinline__ bool mbar_acquire_cluster(uint64_t *bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
+    return done != 0;
 }
 // All threads of all CTAs of the cluster meet.
 __device__ __forceinline__ void cluster_sync() {

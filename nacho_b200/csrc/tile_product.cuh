@@ -587,7 +587,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_tiles(const TileArgs args, 
                 for (int b = begin; b < end; ++b, stage.next()) {
                     if (!(fine = wait_for(&sh.full[stage.at], stage.phase, failed, args.patience))) break;
                     const int rows = FORM == Form::WEIGHTS ? t.last - t.first - b * 64 : 64;
-                    if (tail_rows(b)) mbar_acquire_cluster(&sh.full[stage.at], stage.phase);  // the other CTA's warp has written there too
+                    // The other CTA's warp has written there too. The phase is over: not to see that would be a fault, which ends as a wait that gives up does.
+                    if (tail_rows(b) && !(fine = __all_sync(FULL_MASK, mbar_acquire_cluster(&sh.full[stage.at], stage.phase)))) {
+                        *failed = 1;
+                        break;
+                    }
                     tmem_fence_after();
                     if (elected()) {
                         const uint64_t da = tile_a + (uint64_t)(stage.at * (stage_bytes >> 4)), db = tile_b + (uint64_t)(stage.at * (stage_bytes >> 4));

@@ -53,3 +53,12 @@ def test_fills_of_large_tiles_stay_in_registers():
     found = {name: bytes_ for name, bytes_ in build.spills("csr_merge").items() if re.search(r"csr2_tile(_wide)?ILi31ELi0ELi1ELb0E", name)}
     assert len(found) == 2  # 32- and 64-bit keys
     assert all(max(b) <= 64 for b in found.values()), found
+
+
+def test_the_compiler_warns_of_nothing():
+    build.build()
+    reports = [f for f in os.listdir(build.OBJ_DIR) if f.endswith(".ptxas.txt")]
+    assert len(reports) > 10
+    for name in reports:
+        with open(os.path.join(build.OBJ_DIR, name)) as f:
+            assert not re.search(r"warning", f.read(), re.I), name
