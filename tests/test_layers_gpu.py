@@ -727,3 +727,121 @@ def test_a_norm_holds_nothing_else():
 def test_scales_hold_no_codes(shape):
     for z in (nacho().to_int8_rows(normal(shape, torch.float32, 1)), nacho().to_int8_rows(torch.ones(shape, dtype=torch.int8, device="cuda"), torch.ones(shape[:-1], device="cuda"))):
         assert z.scales.untyped_storage().nbytes() == 4 * math.prod(shape[:-1]) and z.scales.storage_offset() == 0
+
+
+# ---- many tiles, guards, launches beside one another ---------------------------------------------------
+
+# more tiles for each pair of CTAs than it knows ahead, several times over
+@pytest.mark.parametrize("rows,hidden,width", [(5000, 5120, 72), (4900, 5001, 65), (1200, 20000, 136)])
+def test_many_tiles_of_gated_products(rows, hidden, width):
+    dtype = torch.bfloat16
+    check_gated(normal((rows, width), dtype, 1), normal((2 * hidden, width), dtype, 2, width ** -0.5), None, [0, rows], "gelu", dtype)
+
+
+@pytest.mark.parametrize("rows,hidden,width", [(7000, 24, 7040), (7001, 21, 6999), (100, 3600, 7040), (77, 3601, 6999)])
+def test_many_tiles_of_gradients(rows, hidden, width):
+    """Of the rows' gradient, then of the weights'."""
+    dtype = torch.float16
+    x, w = normal((rows, width), dtype, 1), normal((2 * hidden, width), dtype, 2, hidden ** -0.5)
+    check_grad(normal((rows, hidden), dtype, 5), normal((rows, 2 * hidden), dtype, 6, 2.0), x, w, None, [0, rows], "silu", dtype)
+
+
+@pytest.mark.parametrize("rows,n,inner,dtype", [(7000, 7040, 100, torch.bfloat16), (6999, 7001, 33, torch.float16), (7000, 7040, 160, torch.float32)])
+def test_many_tiles_of_integers(rows, n, inner, dtype):
+    x, w = normal((rows, inner), torch.float32, 1), normal((n, inner), torch.float32, 2, 0.05)
+    (qa, sa), (qw, sw) = codes64(x), codes64(w)
+    check_int8(nacho().to_int8_rows(x), nacho().to_int8_rows(w), None, [0, rows], dtype, qa, sa, qw[None], sw[None])
+
+
+@pytest.mark.parametrize("hidden,width", [(1320, 72), (1301, 67)])
+def test_many_tiles_by_expert(hidden, width):
+    dtype = torch.bfloat16
+    counts = [(i * i * 37 + 11 * i) % 400 * (i % 5 > 0) for i in range(60)]
+    order, bounds = order_of(counts, 0, 9)
+    rows = sum(counts) + 9
+    x, w = normal((rows, width), dtype, 3), normal((60, 2 * hidden, width), dtype, 4, width ** -0.5)
+    dh, both = normal((rows, hidden), dtype, 5), normal((rows, 2 * hidden), dtype, 6, 2.0)
+    for t in (x, dh, both):
+        t[bounds[-1]:] = float("nan")
+    check_gated(x, w, order, bounds, "silu", dtype)
+    check_grad(dh, both, x, w, order, bounds, "silu", dtype)
+
+
+def guarded(rows, cols, dtype, pad=0, fill=7.0):
+    """A matrix within a larger array of one value: the array, the matrix, which elements are its own."""
+    stride, lead = cols + pad, 512
+    store = torch.full((lead + rows * stride + 512,), fill, dtype=dtype, device="cuda")
+    view = store[lead:lead + rows * stride].view(rows, stride)[:, :cols]
+    own = torch.zeros(store.shape, dtype=torch.bool, device="cuda")
+    own[lead:lead + rows * stride].view(rows, stride)[:, :cols] = True
+    return store, view, own
+
+
+@pytest.mark.parametrize("rows,groups", [(3000, 300), (500, 300), (900, 7)])
+@pytest.mark.parametrize("hidden,width,pad", [(32, 64, 16), (33, 65, 3)])
+def test_nothing_is_written_around_results(rows, groups, hidden, width, pad):
+    """Offsets that rise and fall, or lie outside the rows: what is written lies in the results' own elements all the same."""
+    import ctypes as C
+    from nacho_b200 import _capi
+    dtype, n = torch.bfloat16, nacho()
+    x, w = normal((rows, width), dtype, 1), normal((groups * 2 * hidden, width), dtype, 2)
+    dh, kept = normal((rows, hidden), dtype, 3), normal((rows, 2 * hidden), dtype, 4)
+    a, b = n.to_int8_rows(x), n.to_int8_rows(w.view(groups, 2 * hidden, width))
+    struct = lambda t: C.byref(_capi.DenseStruct(t.shape[0], t.shape[1], t.stride(0), {torch.float32: 0, torch.bfloat16: 2}[t.dtype], t.data_ptr()))
+    int8 = lambda m: C.byref(_capi.Int8Struct(*m._dims, m._values.data_ptr(), m._scales.data_ptr()))
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    room = lambda bytes_: torch.empty(max(1, bytes_), dtype=torch.uint8, device="cuda")
+    lib, at = _capi.lib, torch.arange(groups + 1, device="cuda", dtype=torch.int32)
+    even = (at * rows // groups).int()
+    for offsets in (even, at % 2 * rows, even.flip(0).contiguous(), ((at * 7919) % (rows + 100) - 50).int()):
+        results = {name: guarded(r, c, t, p) for name, r, c, t, p in (("h", rows, hidden, dtype, pad), ("both", rows, 2 * hidden, dtype, 0), ("dx", rows, width, dtype, pad),
+                                                                        ("dw", groups * 2 * hidden, width, dtype, pad), ("y", rows, 2 * hidden, dtype, pad),
+                                                                        ("y32", rows, 2 * hidden, torch.float32, pad))}
+        r, o = {name: struct(v[1]) for name, v in results.items()}, C.c_void_p(offsets.data_ptr())
+        need = lib.nb200_gated_product_scratch(struct(x), struct(w), groups)
+        some = room(need)
+        assert lib.nb200_gated_product(struct(x), struct(w), groups, o, 0, r["h"], r["both"], some.data_ptr(), need, stream) == _capi.OK
+        need = lib.nb200_gated_product_grad_scratch(struct(x), struct(w), groups)
+        more = room(need)
+        assert lib.nb200_gated_product_grad(struct(dh), struct(kept), struct(x), struct(w), groups, o, 0, r["dx"], r["dw"], more.data_ptr(), need, stream) == _capi.OK
+        assert lib.nb200_int8_product(int8(a), int8(b), o, r["y"], stream) == _capi.OK
+        assert lib.nb200_int8_product(int8(a), int8(b), o, r["y32"], stream) == _capi.OK
+        torch.cuda.synchronize()
+        for name, (store, view, own) in results.items():
+            assert bool((store[~own] == 7.0).all()), name
+        if offsets is even:  # and all of it is written
+            order = n.ExpertOrder_gpu(offsets, torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda"),
+                                      torch.tensor([0, rows], dtype=torch.int32, device="cuda"), (1, groups))
+            three = w.view(groups, 2 * hidden, width)
+            want = dict(zip(("h", "both", "dx", "dw"), (*n.gpu_gated_product(x, three, order, keep=True), *n.gpu_gated_product_grad(dh, kept, x, three, order))))
+            want["y"], want["y32"] = n.gpu_int8_product(a, b, order), n.gpu_int8_product(a, b, order, dtype=torch.float32)
+            assert all(torch.equal(results[name][1], t.view(results[name][1].shape)) for name, t in want.items())
+
+
+@pytest.mark.parametrize("rows,hidden,width,pad", [(300, 96, 200, 0), (1003, 301, 260, 1), (2048, 512, 1024, 0), (128, 1024, 2048, 3), (4000, 1100, 520, 5)])
+def test_gradients_beside_one_another(rows, hidden, width, pad):
+    """Calls that follow at once, on operands that change, in memory that the ones in front have given back: the bits of calls whose kernels run one by one."""
+    from nacho_b200 import _capi
+    n, dtype = nacho(), torch.bfloat16
+    order, _ = order_of([rows // 3, 0, rows - rows // 3 - 5], tail=5)
+    sets = []
+    for i in range(4):
+        x, w, dh, both = some_operands(rows, hidden, width, dtype, 10 * i)
+        if pad:
+            x, w, dh, both = (strided(t, pad, pad) for t in (x, w, dh, both))
+        sets.append(((dh, both, x, w, None), (dh, both, x, torch.stack([w, w.flip(0), w]), order)))
+    want = []
+    _capi.lib.nb200_profile_enable(2)  # an event between any two kernels
+    for pair in sets:
+        for given in pair:
+            want.append(n.gpu_gated_product_grad(*given))
+            torch.cuda.synchronize()
+    _capi.lib.nb200_profile_enable(0)
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for turn in range(25):
+        k = (turn * 5 + turn // 8) % 8
+        got = n.gpu_gated_product_grad(*sets[k // 2][k % 2])
+        for g, t in zip(got, want[k]):
+            off += (g != t).sum()
+        del got
+    assert int(off) == 0
