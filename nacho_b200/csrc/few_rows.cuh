@@ -159,14 +159,18 @@ __global__ void __launch_bounds__(FEW_NT, 2) k_few(const FewArgs args) {
 }
 
 // Whether so few rows go this way, by the rows of a group and the bytes of all weights, of elements of `size` bytes (us on a B200, out of device memory, this way and by tiles of the tensor
-// cores; 16-bit gated products, hidden x width):
-//   - with groups while eight rows are one turn over the weights for nearly all of them (64 experts of 1024 x 2048 with 4 rows 87 and 91, with 6 rows 122
-//     and 92); integers, of which a CTA has half the bytes, never (64 experts of 2048 x 2048 with 3 rows 79 and 47);
-//   - one group of up to 8 rows always (8192 x 8192 45 and 52); more rows, whose own bytes all CTAs read, while the weights are small (16 rows of 4096 x 4096 16 and
-//     18, of 8192 x 8192 60 and 52; 32 rows of 1500 x 1100 9 and 13, of 4096 x 4096 20 and 18).
+// cores; hidden x width or columns x width):
+//   - with groups while there are four rows for each (16 bits: 64 experts of 1024 x 2048 with a row each 82 and 91, with 4 rows 88 and 93, with 8 rows 92 and 93; where one of them
+//     has 64 of 256 rows 92 and 93, 128 of them 98 and 92, and where it has all of them, which eight by eight read its weights again, 85 and 18); integers, of which a CTA has half
+//     the bytes, never (64 experts of 2048 x 2048 with 3 rows 79 and 47);
+//   - one group of up to 8 rows always (16 bits: 8192 x 8192 43 and 48; integers: 4096 x 4096 5.2 and 10, 14336 x 4096 15.2 and 14.9); more rows, whose own bytes all CTAs read, while the
+//     weights are small. 16 bits, 16 rows: 4096 x 4096 16.4 and 17.0, 4094 x 4098 28 and 45, 8192 x 4096 31 and 28; 32 rows: 1100 x 1500 10 and 14, 2048 x 2048 11.7 and 10.5, 2044 x 2052,
+//     whose rows would be copied to boundaries first, 14 and 19. Integers, 16 rows: 6144 x 4096 10.4 and 11.0, 8192 x 4096 11 and 12, 11000 x 4096 15 and 13; 32 rows: 4096 x 4096 8.5 and
+//     10.4, 5000 x 4096 14 and 11.
+// The kernel of 16 rows with gates and values spills 60 bytes a thread where words have 16 bytes, 128 to 384 where they have fewer; those of 8 and 32 rows 40 to 192 with words of 4 and 2.
 inline bool few_rows(int64_t rows, int64_t groups, int64_t bytes, int size) {
     if (groups != 1) return size > 1 && rows <= 4 * groups;
-    return rows <= (bytes <= 24ll << 20 ? 32 : bytes <= 96ll << 20 ? 16 : 8);
+    return rows <= (bytes <= (size > 1 ? 24ll : 18ll) << 20 ? 32 : bytes <= (size > 1 ? 96ll : 34ll) << 20 ? 16 : 8);
 }
 
 template <Sum SUM, bool GATED, int V, typename T>
