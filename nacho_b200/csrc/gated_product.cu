@@ -185,30 +185,38 @@ struct GradScratch {
 };
 
 // The two products of the gradient, which do not wait for one another: with all pairs of CTAs each, or, where their tiles would leave many of them idle, rows' gradient with the pairs
-// that it needs and the weights' with the rest (128 rows of 4096 x 4096: one after the other 48 us, beside one another 40; 1003 rows by 1101 hidden units and a width of 1100: 37 and 27).
-// A tile of the weights' gradient waits for its results to leave where it sums little: 512 tiles of 256 x 256 over 128 rows take 18 us, of which their blocks are 5.
+// that it needs and the weights' with the rest, as far as that keeps up (128 rows of 4096 x 4096: one after the other 48 us, beside one another 39; 1003 rows by 1101 hidden units and a
+// width of 1100: 37 and 27; 14 rows of 4992 x 768: the weights' gradient on all 62 pairs that are left 21.5 us, on 20 to 40 of them, beside which the next kernel's CTAs find room, 18.7).
+// Tiles wait for their results to leave, where they sum little for longer than for their blocks, and longest where warps store them (`words` false). The constants, in rows of blocks, are
+// those by which the plans of 64 products, of 1 to 26000 rows, come nearest to the best of some twenty plans that were measured for each: 2.5 % on the mean.
 struct GradPlan {
-    static constexpr int64_t RESULTS = 4, LAUNCH = 4000;  // rows of blocks: for a column of such a tile; for one more kernel in a row
+    static constexpr int64_t RESULTS = 1280, ODD_RESULTS = 6144, LAUNCH = 8000;  // a tile's results; the same of the weights' gradient without words; a kernel that follows another
     TileWork::Way x, w;
     int pairs_x, pairs_w;
 
-    GradPlan(int64_t rows, int64_t width, int64_t hidden, int64_t groups, const int (&clusters)[2]) {
+    GradPlan(int64_t rows, int64_t width, int64_t hidden, int64_t groups, bool words, const int (&clusters)[2]) {
         const int64_t high = (2 * hidden + TILE_M - 1) / TILE_M, all = all_pairs();
-        const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64};
-        const TileWork work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64, RESULTS};
+        const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64, RESULTS};
+        const TileWork work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64, words ? RESULTS : ODD_RESULTS};
         x = work_x.best(all, clusters), w = work_w.best(all, clusters);
         pairs_x = pairs_w = (int)all;
-        double least = (x.cost + w.cost) * 7 / 8 + LAUNCH;  // parts of the pairs are shared out once: worth it where it gives more than that
-        for (int64_t k = 1; k < 16; ++k) {
-            const int64_t part = all * k / 16;
+        double least = (x.cost + w.cost) * 15 / 16 + LAUNCH;  // the shares of the pairs do not change on the way: they have to give more than a little
+        for (int k = 1; k < 8; ++k) {
+            const int64_t part = all * k / 8;
             if (part < 1 || part >= all) continue;
             // clusters have to find room beside the other product's CTAs
-            const int half[2] = {clusters[0] * (int)k / 16, clusters[1] * (int)k / 16};
+            const int half[2] = {clusters[0] * k / 8, clusters[1] * k / 8};
             const TileWork::Way a = work_x.best(part, half);
             const int64_t mine = std::min(part, work_x.most(a.n) * a.parts), other = all - mine;
             const int rest[2] = {(int)(clusters[0] * other / all) - 1, (int)(clusters[1] * other / all) - 1};
             const TileWork::Way b = work_w.best(other, rest);
-            if (std::max(a.cost, b.cost) < least) least = std::max(a.cost, b.cost), x = a, w = b, pairs_x = (int)mine, pairs_w = (int)other;
+            if (std::max(a.cost, b.cost) >= least) continue;
+            least = std::max(a.cost, b.cost), x = a, w = b, pairs_x = (int)mine, pairs_w = (int)other;
+            if (b.parts == 1 && b.cost < a.cost) {
+                // in as many rounds as three quarters of the other one's time hold
+                const int64_t tiles = work_w.most(b.n), now = (tiles + other - 1) / other, rounds = std::max(now, (int64_t)(a.cost * 3 / 4 * now / b.cost));
+                pairs_w = (int)((tiles + rounds - 1) / rounds);
+            }
         }
     }
 };
@@ -338,7 +346,7 @@ int nb200_gated_product_grad(const nb200_dense *dh, const nb200_dense *both, con
         if ((st = aligned(*x, s.x, *w, s.w, &ax, &aw, true, stream))) return st;
         int clusters[2];
         if ((st = tile_clusters<sum_of<T>, Form::WEIGHTS, true, T>(clusters))) return st;
-        const GradPlan plan(x->rows, x->cols, hidden, groups, clusters);
+        const GradPlan plan(x->rows, x->cols, hidden, groups, word_bytes({dw}) == 16, clusters);
         TileMaps maps{};
         TileArgs args{};
         args.offsets = offsets, args.groups = groups, args.rows = (int)x->rows;

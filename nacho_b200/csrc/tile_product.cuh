@@ -713,7 +713,7 @@ inline CUtensorMapDataType map_type(int type) { return type == NB200_F16 ? CU_TE
 inline int64_t all_pairs() { return std::max(1, sm_count() / 2); }
 
 // A product as tiles: `rows` on the narrow side of all groups together, `wide_tiles` beside one another on the wide one, `blocks` summed for each. `results`: what the products wait
-// for while a column of a tile leaves, in the cost's rows of blocks.
+// for while a tile leaves, in the cost's rows of blocks.
 struct TileWork {
     int64_t rows, groups, wide_tiles, blocks, results = 0;
 
@@ -738,7 +738,7 @@ struct TileWork {
             for (int k = 0; k < 3; ++k) {
                 const int parts = 1 << k;
                 if (parts > 1 && (all * parts > pairs || all > clusters[k - 1] || blocks < 8 * parts)) break;
-                const double cost = (double)((tiles + pairs - 1) / pairs) * ((double)each * (double)((blocks + parts - 1) / parts) + (double)(results * std::min<int64_t>(n, mean))) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
+                const double cost = (double)((tiles + pairs - 1) / pairs) * ((double)each * (double)((blocks + parts - 1) / parts) + (double)results) + (parts > 1 ? 50 * std::min<int64_t>(n, mean) : 0);
                 // One group's tiles are no wider than its rows: a stage then has that much more room for others, and a tile comes by one copy. Groups share the rows
                 // unevenly: the wider side is for those that have more.
                 if (way.n == 0 || cost < way.cost || (groups == 1 && cost == way.cost && parts == way.parts)) way = Way{n, parts, cost};
