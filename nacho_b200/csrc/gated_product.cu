@@ -188,16 +188,16 @@ struct GradScratch {
 // that it needs and the weights' with the rest, as far as that keeps up (128 rows of 4096 x 4096: one after the other 48 us, beside one another 39; 1003 rows by 1101 hidden units and a
 // width of 1100: 37 and 27; 14 rows of 4992 x 768: the weights' gradient on all 62 pairs that are left 21.5 us, on 20 to 40 of them, beside which the next kernel's CTAs find room, 18.7).
 // Tiles wait for their results to leave, where they sum little for longer than for their blocks, and longest where warps store them (`words` false). The constants, in rows of blocks, are
-// those by which the plans of 64 products, of 1 to 26000 rows, come nearest to the best of some twenty plans that were measured for each: 2.5 % on the mean.
+// those by which the plans of 200 products, of one row to some ten thousand, come nearest to the best of some twenty plans that were measured for each: 1.8 % on the mean.
 struct GradPlan {
-    static constexpr int64_t RESULTS = 1280, ODD_RESULTS = 6144, LAUNCH = 8000;  // a tile's results; the same of the weights' gradient without words; a kernel that follows another
+    static constexpr int64_t RESULTS_X = 1280, ODD_RESULTS_X = 4096, RESULTS_W = 1536, ODD_RESULTS_W = 6144, LAUNCH = 8000;  // for a tile; for a kernel that follows another
     TileWork::Way x, w;
     int pairs_x, pairs_w;
 
     GradPlan(int64_t rows, int64_t width, int64_t hidden, int64_t groups, bool words, const int (&clusters)[2]) {
         const int64_t high = (2 * hidden + TILE_M - 1) / TILE_M, all = all_pairs();
-        const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64, RESULTS};
-        const TileWork work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64, words ? RESULTS : ODD_RESULTS};
+        const TileWork work_x{rows, groups, (width + TILE_M - 1) / TILE_M, (2 * hidden + 63) / 64, words ? RESULTS_X : ODD_RESULTS_X};
+        const TileWork work_w{width, 1, groups * high, ((rows + groups - 1) / groups + 63) / 64, words ? RESULTS_W : ODD_RESULTS_W};
         x = work_x.best(all, clusters), w = work_w.best(all, clusters);
         pairs_x = pairs_w = (int)all;
         double least = (x.cost + w.cost) * 15 / 16 + LAUNCH;  // the shares of the pairs do not change on the way: they have to give more than a little
@@ -212,8 +212,8 @@ struct GradPlan {
             const TileWork::Way b = work_w.best(other, rest);
             if (std::max(a.cost, b.cost) >= least) continue;
             least = std::max(a.cost, b.cost), x = a, w = b, pairs_x = (int)mine, pairs_w = (int)other;
-            if (b.parts == 1 && b.cost < a.cost) {
-                // in as many rounds as three quarters of the other one's time hold
+            if (a.parts > 1 && b.parts == 1 && b.cost < a.cost) {
+                // beside clusters in as many rounds as three quarters of their time hold
                 const int64_t tiles = work_w.most(b.n), now = (tiles + other - 1) / other, rounds = std::max(now, (int64_t)(a.cost * 3 / 4 * now / b.cost));
                 pairs_w = (int)((tiles + rounds - 1) / rounds);
             }

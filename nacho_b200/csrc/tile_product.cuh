@@ -734,7 +734,8 @@ struct TileWork {
         const int64_t mean = (rows + groups - 1) / groups;
         Way way{0, 1, 0};
         for (int n = TILE_N; n >= 64; n -= 64) {
-            const int64_t tiles = groups * ((mean + n - 1) / n) * wide_tiles, all = std::max(tiles, most(n)), each = TILE_M + std::min<int64_t>(n, mean);
+            const int64_t each_group = (mean + n - 1) / n * wide_tiles, tiles = std::min(groups, rows) * each_group, all = std::max(groups * each_group, most(n));
+            const int64_t each = TILE_M + std::min<int64_t>(n, mean);
             for (int k = 0; k < 3; ++k) {
                 const int parts = 1 << k;
                 if (parts > 1 && (all * parts > pairs || all > clusters[k - 1] || blocks < 8 * parts)) break;
