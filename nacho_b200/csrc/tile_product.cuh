@@ -361,7 +361,8 @@ struct Stages {
 // the group's offsets: found by every warp for itself at the tile's beginning, the matrix instructions of short sums waited for it), one brings blocks of 128
 // bytes of both operands into shared memory (the copy engine's tiled form, which turns them as the tensor cores take them and fills up with zeros what lies
 // beyond a matrix), one issues the matrix instructions, and eight read the sums of a whole tile while those of the next one are made: tensor memory holds two.
-// 4096 x 8192 x 4096 gated: 322 us where the clocks hold (tensor cores busy 94 %), 413 under the power cap; 8192^3 in integers 300 us.
+// 4096 x 8192 x 4096 gated, both sums kept: 504 K cycles with the tensor cores busy 95 %, which the power cap makes 322 to 345 us alone and 406 to 426 in call after call; without them
+// kept 502 K cycles and 96 %. 8192^3 in integers: 498 K cycles, 300 to 322 us alone.
 //
 // GATED: 16 rows of gates and 16 of values alternate in the wide operand's tile, so that a gate and its value lie 16 lanes apart in tensor memory and fragments
 // of both land in the same thread.
@@ -683,8 +684,8 @@ inline int describe_rows(CUtensorMap *map, CUtensorMapDataType type, void *data,
     const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
     return encode_matrix(map, type, 3, data, extents, pitches, box);
 }
-// The engine takes a copy for every block of an operand, not so much its bytes: with boxes of 16 and 32 rows, 12 copies for a block, 4096 x 8192 x 4096 gated took 368 us
-// (where the clocks hold), with the largest ones 337.
+// The engine takes a copy for every block of an operand, not so much its bytes: with boxes of 16 and 32 rows, 12 copies for a block, 4096 x 8192 x 4096 gated (alone, sums not kept)
+// took 368 us, with the largest ones 337.
 
 // The narrow operand by rows, in boxes for parts of a tile and for half of a whole one.
 inline int describe_narrow(TileMaps *maps, TileArgs *args, CUtensorMapDataType type, void *data, int64_t size, int64_t cols, int64_t rows, int64_t stride) {

@@ -83,7 +83,8 @@ def gpu_gated_product(x: torch.Tensor, w: torch.Tensor, order: ExpertOrder_gpu |
 def gpu_gated_product_grad(dh: torch.Tensor, both: torch.Tensor, x: torch.Tensor, w: torch.Tensor, order: ExpertOrder_gpu | None = None,
                            activation: str = "silu") -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients ``(dx, dw)`` of ``gpu_gated_product``, from the gradient of its result and the products it kept, all of one type. The gradient of both
-    products is rounded to that type before it is multiplied; zeros for what nothing depends on."""
+    products is rounded to that type before it is multiplied, beside the rounding of the results (together 1.4 times as far from exact ones); zeros for
+    what nothing depends on."""
     return _native.gated_product_grad(dh, both, x, w, order, _activation(activation, "gpu_gated_product_grad"))
 
 
